@@ -337,6 +337,72 @@ int32_t kt_rope_attention(float* q, float* k, const float* v, const float* inv_f
                           const int32_t* position, int32_t key_bound, float* cache_k, float* cache_v,
                           int32_t layer, int32_t max_seq, int32_t num_heads, int32_t num_kv_heads,
                           int32_t head_dim, float* context, void* stream);
+/* ---- the KV cache held in 8 bits (kt_kv8.hip) -------------------------------------------
+ * A quarter of the fp32 cache's memory and of what a decode step's attention reads. No
+ * counterpart in the reference, whose cache is fp32 (K/KVCache.kt:9-27).
+ * The rows of a (layer, kv head) are cut into blocks of block_tokens tokens; a block's keys
+ * (and its values, likewise) share one fp32 scale
+ *   s = max(m / QMAX, 2^-120), m = the largest magnitude of the block's rows so far,
+ * QMAX = 127 (int8) or 448 (e4m3: 4 exponent bits, 3 mantissa bits, no infinities), and stand for
+ * code * s, code = the nearest to x * (1 / s), ties to even (the quotients and products rounded
+ * to fp32). A block with a value that is not finite has the scale NaN: what attends to it becomes NaN.
+ * While a block is not full its rows are kept in fp32 too (key_rows, value_rows), and an append
+ * that raises its scale encodes it again from them, so the cache holds the same bits whatever the
+ * calls its rows came in. An append continues the cache where the last one ended, or starts it again
+ * at position 0 or at the first token of a block; after kt_kv8_copy it continues the copy.
+ * The caller owns the memory: kt_kv8_layout's sizes, codes and rows 16-byte aligned. Keys lie as
+ * [layers][kv_heads][slots][head_dim] codes, slots = max_seq rounded up to whole blocks and to
+ * a multiple of 64; values as [layers][kv_heads][slots / 64][head_dim][64], token
+ * 32 h + 16 (p / 2) + 8 u + 4 (p % 2) + i of a chunk at byte 16 p + 8 h + 4 u + i of its dim; int8 codes
+ * are stored + 128; scales as [layers][kv_heads][slots / block_tokens]; rows as
+ * [layers][kv_heads][block_tokens][head_dim]. Memory of tokens that are not held is never used. */
+#define KT_KV8_INT8 0
+#define KT_KV8_E4M3 1
+typedef struct kt_kv8_cache {
+    void* keys;
+    void* values;
+    float* key_scales;
+    float* value_scales;
+    float* key_rows;
+    float* value_rows;
+    int32_t format;        /* KT_KV8_INT8 or KT_KV8_E4M3 */
+    int32_t layers;
+    int32_t kv_heads;
+    int32_t max_seq;
+    int32_t head_dim;      /* 32, 64, 128 or 256 */
+    int32_t block_tokens;  /* 32, 64 or 128 */
+} kt_kv8_cache;
+/* out3: bytes of keys (and of values), scales of keys (and of values), floats of key_rows
+ * (and of value_rows). Reads no pointer of the cache. Host arithmetic. */
+int32_t kt_kv8_layout(const kt_kv8_cache* cache, int64_t* out3);
+/* kt_rope_kv into such a cache: q [tokens x num_heads*head_dim] rotated into q_out (which may
+ * be q; both NULL: only the append), k rotated and v appended at positions *position + t. Rows past
+ * max_seq are not written. k, v and q (unless it is q_out) stay as they are. */
+int32_t kt_rope_kv8(const float* q, const float* k, const float* v, int32_t tokens, int32_t num_heads,
+                    const float* inv_freq, const int32_t* position, const kt_kv8_cache* cache, int32_t layer,
+                    float* q_out, void* stream);
+/* kt_attention over such a cache (K/Attention.kt:277-349 on what its codes stand for): token t's
+ * softmax(q . k_j / sqrt(head_dim)) over j <= *position + t, times v, into context; sums and softmax in
+ * fp32. A token that sees no key (a negative position) gets zeros. q and context are 16-byte
+ * aligned. As kt_attention's, its workspace is sized by one eager call before a recording. */
+int32_t kt_attention_kv8(const float* q, int32_t tokens, const int32_t* position, int32_t key_bound,
+                         const kt_kv8_cache* cache, int32_t layer, int32_t num_heads, float* context, void* stream);
+/* kt_rope_kv8 followed by kt_attention_kv8. For one token q stays as it is; for more it is
+ * rotated in place. */
+int32_t kt_rope_attention_kv8(float* q, const float* k, const float* v, const float* inv_freq, int32_t tokens,
+                              const int32_t* position, int32_t key_bound, const kt_kv8_cache* cache, int32_t layer,
+                              int32_t num_heads, float* context, void* stream);
+/* The rows of tokens first .. first + count - 1 of a layer as fp32 (code * scale), keys and values
+ * [kv_heads x count x head_dim], each of which may be NULL. */
+int32_t kt_kv8_read(const kt_kv8_cache* cache, int32_t layer, int32_t first, int32_t count, float* keys,
+                    float* values, void* stream);
+/* KVCache.copyFrom (K/KVCache.kt:41-55): the first `length` positions of every layer of `source`, which
+ * holds source_length. The codes and scales are the source's; where the copy ends inside a block that the
+ * source has gone past, that block's fp32 rows start from what its codes stand for. The cache may be
+ * the source itself: it is then shortened. */
+int32_t kt_kv8_copy(const kt_kv8_cache* source, int32_t source_length, const kt_kv8_cache* cache, int32_t length,
+                    void* stream);
+
 /* SwiGLU's gate (K/SwiGLU.kt:19-25; K/Tensor.kt:223-237): gate[i] = silu(gate[i]) * up[i]. */
 int32_t kt_silu_mul(float* gate, const float* up, int64_t n, void* stream);
 /* RMSNorm.forward (K/RMSNorm.kt) of x [m x K] with weight, then the grouped projections of
@@ -408,6 +474,35 @@ int32_t kt_argmax(const float* logits, int32_t n, int32_t* index, void* stream);
  * argmax, advance the cache, hand the token out); the argmax does not read the position. */
 int32_t kt_argmax_advance(const float* logits, int32_t n, int32_t* token, int32_t* position,
                           int32_t* generated, int32_t capacity, void* stream);
+/* Control of the next token by the text so far, before kt_argmax: of a row's logits x,
+ *   a token of the row's text:                 x = x > 0 ? x / repetition : x * repetition
+ *   one that occurs o > 0 times from output_start on:  x = x - (o * frequency + presence)
+ *   one with a bias:                           x = x + bias
+ *   one whose bit of `allowed` is 0:           x = -inf
+ * in this order. The text of row r is history[r * history_stride + i] for i < history_length[r] +
+ * length_offset (at most history_capacity entries; ids outside the vocabulary count nothing). It
+ * is read on the device, so a recorded decode step follows its text from replay to replay. */
+typedef struct kt_logits_controls {
+    const int32_t* history;         /* may be NULL without penalties (1, 0, 0) */
+    const int32_t* history_length;  /* device [rows] */
+    const int32_t* output_start;    /* device [rows], or NULL: 0 */
+    int64_t history_stride;         /* 0: one text for all rows */
+    int32_t history_capacity;
+    int32_t length_offset;
+    float repetition;               /* > 0; 1 = none */
+    float frequency;
+    float presence;
+    int32_t bias_count;             /* biases of a row; of a token given twice the later holds */
+    const int32_t* bias_tokens;     /* ids outside the vocabulary are skipped */
+    const float* bias_values;
+    int64_t bias_stride;            /* 0: the same biases for all rows */
+    const uint32_t* allowed;        /* bit i % 32 of word i / 32: token i may follow; or NULL: all may */
+    int64_t allowed_stride;         /* words; 0: one mask for all rows */
+} kt_logits_controls;
+/* logits [rows x n], row r at r * stride, into out (which may be logits, then with its stride).
+ * Allocates nothing. Asynchronous. */
+int32_t kt_process_logits(const float* logits, int32_t rows, int32_t n, int64_t stride, const kt_logits_controls* controls,
+                          float* out, int64_t out_stride, void* stream);
 /* KVCache.advance on the device copy of the length (K/KVCache.kt:29-35): *position += count. */
 int32_t kt_position_add(int32_t* position, int32_t count, void* stream);
 /* generated[*position] = *token when 0 <= *position < capacity: the device-side record of

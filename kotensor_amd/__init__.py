@@ -8,7 +8,8 @@ package is a host-side mirror of the reference's API over that ABI:
 file format (``SafeTensorsFile``, ``save_quantized``, ``load_quantized``) and the
 device-resident decoder around the projections (``Transformer``, ``KVCache``,
 ``InferenceBuffers``, ``RoPEScaling``) and the fused projection + cross-entropy with a
-quantized head (``fused_cross_entropy_loss``).
+quantized head (``fused_cross_entropy_loss``). Beside the reference's API: a KV cache held in 8 bits
+(``QuantizedKVCache``) and penalties, biases and masks on logits (``LogitsControls``).
 """
 from ._lib import IllegalArgumentException, IllegalStateException, LibraryMissingError, LIBRARY_PATH
 from .device import DeviceBuffer, Stream, synchronize, device_count, release_scratch
@@ -17,6 +18,8 @@ from .matmul import MatMul, DeviceTensor
 from .linear import QuantizedLinear, projection, forward_into_group
 from .safetensors import SafeTensorsFile, save_entries, save_quantized, load_quantized
 from .transformer import Transformer, KVCache, InferenceBuffers, RoPEScaling
+from .kv8 import QuantizedKVCache
+from .logits import LogitsControls, process_logits
 from .loss import fused_cross_entropy_loss, FusedLoss, IGNORE_INDEX
 
 __all__ = [
@@ -44,6 +47,9 @@ __all__ = [
     "KVCache",
     "InferenceBuffers",
     "RoPEScaling",
+    "QuantizedKVCache",
+    "LogitsControls",
+    "process_logits",
     "fused_cross_entropy_loss",
     "FusedLoss",
     "IGNORE_INDEX",

@@ -84,6 +84,49 @@ class QMatmulStep(ctypes.Structure):
     ]
 
 
+KT_KV8_INT8 = 0
+KT_KV8_E4M3 = 1
+
+
+class KV8Cache(ctypes.Structure):
+    """kt_kv8_cache: the memory and shape of a KV cache held in 8 bits."""
+    _fields_ = [
+        ("keys", ctypes.c_void_p),
+        ("values", ctypes.c_void_p),
+        ("key_scales", ctypes.c_void_p),
+        ("value_scales", ctypes.c_void_p),
+        ("key_rows", ctypes.c_void_p),
+        ("value_rows", ctypes.c_void_p),
+        ("format", ctypes.c_int32),
+        ("layers", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32),
+        ("max_seq", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("block_tokens", ctypes.c_int32),
+    ]
+
+
+class LogitsControls(ctypes.Structure):
+    """kt_logits_controls: what kt_process_logits takes beside the logits."""
+    _fields_ = [
+        ("history", ctypes.c_void_p),
+        ("history_length", ctypes.c_void_p),
+        ("output_start", ctypes.c_void_p),
+        ("history_stride", ctypes.c_int64),
+        ("history_capacity", ctypes.c_int32),
+        ("length_offset", ctypes.c_int32),
+        ("repetition", ctypes.c_float),
+        ("frequency", ctypes.c_float),
+        ("presence", ctypes.c_float),
+        ("bias_count", ctypes.c_int32),
+        ("bias_tokens", ctypes.c_void_p),
+        ("bias_values", ctypes.c_void_p),
+        ("bias_stride", ctypes.c_int64),
+        ("allowed", ctypes.c_void_p),
+        ("allowed_stride", ctypes.c_int64),
+    ]
+
+
 class _StEntry(ctypes.Structure):
     """kt_st_entry: one tensor of a safetensors header."""
     _fields_ = [
@@ -136,6 +179,12 @@ SIGNATURES = {
     "kt_rmsnorm": [_P, _I, _I, _P, _F, _P, _P],
     "kt_rope_kv": [_P, _P, _P, _I, _I, _I, _I, _P, _P, _P, _P, _I, _I, _P],
     "kt_attention": [_P, _I, _P, _I, _P, _P, _I, _I, _I, _I, _I, _P, _P],
+    "kt_kv8_layout": [ctypes.POINTER(KV8Cache), ctypes.POINTER(ctypes.c_int64)],
+    "kt_rope_kv8": [_P, _P, _P, _I, _I, _P, _P, ctypes.POINTER(KV8Cache), _I, _P, _P],
+    "kt_attention_kv8": [_P, _I, _P, _I, ctypes.POINTER(KV8Cache), _I, _I, _P, _P],
+    "kt_rope_attention_kv8": [_P, _P, _P, _P, _I, _P, _I, ctypes.POINTER(KV8Cache), _I, _I, _P, _P],
+    "kt_kv8_read": [ctypes.POINTER(KV8Cache), _I, _I, _I, _P, _P, _P],
+    "kt_kv8_copy": [ctypes.POINTER(KV8Cache), _I, ctypes.POINTER(KV8Cache), _I, _P],
     "kt_silu_mul": [_P, _P, ctypes.c_int64, _P],
     "kt_swiglu_qmatmul": [_P, _P, _I, ctypes.POINTER(_QWeight), _P, _I, _F, _P, _P],
     "kt_rope_attention": [_P, _P, _P, _P, _I, _P, _I, _P, _P, _I, _I, _I, _I, _I, _P, _P],
@@ -144,6 +193,7 @@ SIGNATURES = {
     "kt_qmatmul_chain": [ctypes.POINTER(QMatmulStep), _I, _P],
     "kt_argmax": [_P, _I, _P, _P],
     "kt_argmax_advance": [_P, _I, _P, _P, _P, _I, _P],
+    "kt_process_logits": [_P, _I, _I, ctypes.c_int64, ctypes.POINTER(LogitsControls), _P, ctypes.c_int64, _P],
     "kt_position_add": [_P, _I, _P],
     "kt_record_token": [_P, _P, _P, _I, _P],
     "kt_graph_begin": [_P],

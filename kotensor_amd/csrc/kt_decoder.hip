@@ -28,6 +28,7 @@
 
 #include "kt_common.h"
 #include "kt_split.h"
+#include "kt_wave.h"
 
 namespace kt {
 namespace {
@@ -38,33 +39,6 @@ constexpr int MAX_SPLITS = 64;  // key splits of one (token, kv head); the merge
 constexpr int MAX_NACC = 4;   // query floats per thread: heads per kv head x head_dim <= 1024
 constexpr int ACC_REGS = 8;   // per lane: query heads of its wave x dims of its lane (head_dim / 64 rounded up)
 constexpr int MAX_HD = 256;
-
-// Sum and maximum over a wave without LDS round trips: inside each row of 16 lanes by DPP
-// exchanges (quad xor 1, quad xor 2, half-row mirror, row mirror: every lane of a row ends
-// with the same row total, the two operands of each add being the same pair), then the
-// four row totals read into scalars and combined in one fixed order, so every lane holds
-// the same bits. Needs every lane of the wave active.
-template <int CTRL>
-__device__ __forceinline__ float dpp_move(float v) {
-    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, false));
-}
-__device__ __forceinline__ float lane_value(float v, int lane) {
-    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
-}
-__device__ __forceinline__ float wave_sum_dpp(float v) {
-    v += dpp_move<0xB1>(v);   // quad_perm [1,0,3,2]
-    v += dpp_move<0x4E>(v);   // quad_perm [2,3,0,1]
-    v += dpp_move<0x141>(v);  // row_half_mirror
-    v += dpp_move<0x140>(v);  // row_mirror
-    return (lane_value(v, 0) + lane_value(v, 16)) + (lane_value(v, 32) + lane_value(v, 48));
-}
-__device__ __forceinline__ float wave_max_dpp(float v) {
-    v = fmaxf(v, dpp_move<0xB1>(v));
-    v = fmaxf(v, dpp_move<0x4E>(v));
-    v = fmaxf(v, dpp_move<0x141>(v));
-    v = fmaxf(v, dpp_move<0x140>(v));
-    return fmaxf(fmaxf(lane_value(v, 0), lane_value(v, 16)), fmaxf(lane_value(v, 32), lane_value(v, 48)));
-}
 
 // ---- RMSNorm ---------------------------------------------------------------------
 // One workgroup per row: out = (x * (1 / sqrt(mean(x^2) + eps))) * weight, the sum of
@@ -115,18 +89,6 @@ __global__ void __launch_bounds__(THREADS) rmsnorm_kernel(const float* __restric
 // Thread (token t, unit u): u < num_heads * half rotates pair i of q head u / half;
 // the next num_kv_heads * half units rotate k and write k and v to the cache.
 #pragma clang fp contract(off)
-// RoPE.applyInPlace's rotation of pair (x1, x2) = (row[i], row[i + half]) at pos:
-// theta = pos * invFreq[i] in fp32, cos and sin in double rounded to float, no
-// contraction (the whole region is compiled with fp contract off).
-__device__ __forceinline__ void rope_cos_sin(int32_t pos, float inv_freq_i, float& c, float& s) {
-    const float theta = static_cast<float>(pos) * inv_freq_i;
-    c = static_cast<float>(cos(static_cast<double>(theta)));
-    s = static_cast<float>(sin(static_cast<double>(theta)));
-}
-__device__ __forceinline__ void rope_apply(float x1, float x2, float c, float s, float& y1, float& y2) {
-    y1 = x1 * c - x2 * s;
-    y2 = x1 * s + x2 * c;
-}
 __device__ __forceinline__ void rope_rotate(float x1, float x2, int32_t pos, float inv_freq_i, float& y1, float& y2) {
     float c, s;
     rope_cos_sin(pos, inv_freq_i, c, s);

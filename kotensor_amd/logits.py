@@ -1,0 +1,112 @@
+"""Control of the next token by the text so far: penalties for its tokens, biases, and a grammar's
+mask on rows of logits (``kt_process_logits``). No counterpart in the reference, whose greedy
+choice takes the logits as they are (Transformer.kt:253-266).
+"""
+from __future__ import annotations
+
+import ctypes
+
+import numpy as np
+
+from . import _lib
+from .device import DeviceBuffer, Stream, default_stream
+from .matmul import DeviceTensor, _nbytes, _ptr
+
+
+class LogitsControls:
+    """Penalties, biases and a mask, in this order on a logit x (oracle: the header's formulas):
+
+    * ``repetition_penalty``: a token of the text has x / penalty (x > 0) or x * penalty;
+    * ``frequency_penalty``, ``presence_penalty``: a token that occurs o > 0 times in the text's
+      output has x - (o * frequency + presence);
+    * ``bias``: {token: value} added to x;
+    * ``allowed``: tokens that may follow, as a boolean array of the vocabulary (one for all rows,
+      or one a row) or, packed, its 32-bit words; the others have minus infinity. A grammar replaces
+      it between steps with ``set_allowed``, which keeps the device address.
+    """
+
+    def __init__(self, repetition_penalty: float = 1.0, frequency_penalty: float = 0.0, presence_penalty: float = 0.0,
+                 bias: dict | None = None, allowed=None, stream: Stream | None = None):
+        if not 0.0 < repetition_penalty < float("inf"):
+            raise _lib.IllegalArgumentException("the repetition penalty must be positive and finite")
+        for name, value in (("frequency", frequency_penalty), ("presence", presence_penalty)):
+            if not abs(value) < float("inf"):
+                raise _lib.IllegalArgumentException(f"the {name} penalty must be finite")
+        self.repetition_penalty, self.frequency_penalty, self.presence_penalty = map(float, (repetition_penalty, frequency_penalty, presence_penalty))
+        self.bias_count = len(bias or {})
+        self._bias_ids = sorted(int(t) for t in bias or {})
+        if self.bias_count:
+            self._bias_tokens = DeviceBuffer.from_numpy(np.array(list(bias.keys()), np.int32), stream)
+            self._bias_values = DeviceBuffer.from_numpy(np.array(list(bias.values()), np.float32), stream)
+        self._allowed, self._words = None, (0, 0)
+        if allowed is not None:
+            self.set_allowed(allowed, stream)
+
+    @property
+    def penalized(self) -> bool:
+        return (self.repetition_penalty, self.frequency_penalty, self.presence_penalty) != (1.0, 0.0, 0.0)
+
+    def set_allowed(self, allowed, stream: Stream | None = None) -> None:
+        """Replaces the mask; one of the same size goes to the same device memory, which a recorded
+        step then reads at its next replay."""
+        a = np.asarray(allowed)
+        if a.ndim not in (1, 2) or a.size == 0:
+            raise _lib.IllegalArgumentException(f"a mask is an array of the vocabulary, or one a row, got {list(a.shape)}")
+        if a.dtype == np.bool_:
+            pad = np.zeros(a.shape[:-1] + (-a.shape[-1] % 32,), np.bool_)
+            a = np.packbits(np.concatenate([a, pad], -1), axis=-1, bitorder="little").view("<u4")
+        elif a.dtype not in (np.dtype("u4"), np.dtype("i4")):
+            raise _lib.IllegalArgumentException(f"a mask is boolean or packed in 32-bit words, got {a.dtype}")
+        words = (a.shape[0] if a.ndim == 2 else 0, a.shape[-1])
+        if self._allowed is None or words != self._words:
+            self._allowed, self._words = DeviceBuffer(a.nbytes), words
+        self._allowed.upload(a, stream)
+
+    def descriptor(self, rows: int, vocabulary: int, history=None, history_length=None, output_start=None, history_stride: int = 0,
+                   history_capacity: int = 0, length_offset: int = 0) -> _lib.LogitsControls:
+        """The kt_logits_controls of a call on ``rows`` rows (device buffers or addresses)."""
+        if self._bias_ids and not 0 <= self._bias_ids[0] <= self._bias_ids[-1] < vocabulary:
+            raise _lib.IllegalArgumentException(f"a biased token is out of vocab bounds {vocabulary}")
+        if self._allowed is not None:
+            if self._words[0] not in (0, rows):
+                raise _lib.IllegalArgumentException(f"a mask of {self._words[0]} rows for {rows} rows of logits")
+            if self._words[1] != (vocabulary + 31) // 32:
+                raise _lib.IllegalArgumentException(f"a mask of {self._words[1]} words does not hold {vocabulary} tokens")
+        c = _lib.LogitsControls()
+        c.history, c.history_length, c.output_start = _ptr(history), _ptr(history_length), _ptr(output_start)
+        c.history_stride, c.history_capacity, c.length_offset = history_stride, history_capacity, length_offset
+        c.repetition, c.frequency, c.presence = self.repetition_penalty, self.frequency_penalty, self.presence_penalty
+        c.bias_count = self.bias_count
+        if self.bias_count:
+            c.bias_tokens, c.bias_values = self._bias_tokens.ptr, self._bias_values.ptr
+        if self._allowed is not None:
+            c.allowed, c.allowed_stride = self._allowed.ptr, self._words[1] if self._words[0] else 0
+        return c
+
+
+def process_logits(logits: DeviceTensor, controls: LogitsControls, history: DeviceBuffer | None = None, history_length: DeviceBuffer | None = None,
+                   output_start: DeviceBuffer | None = None, out: DeviceTensor | None = None, stream: Stream | None = None) -> DeviceTensor:
+    """The controls on logits ``[rows x vocabulary]``, into ``out`` (a new tensor when not given; it may
+    be ``logits``). ``history`` holds int32 tokens ``[rows x capacity]``, ``history_length`` and
+    ``output_start`` one int32 a row."""
+    if len(logits.shape) != 2:
+        raise _lib.IllegalArgumentException("not a matrix")
+    rows, n = logits.shape
+    if out is None:
+        out = DeviceTensor(DeviceBuffer(rows * n * 4), (rows, n))
+    if out.shape != logits.shape:
+        raise _lib.IllegalArgumentException(f"out shape {list(out.shape)} != {list(logits.shape)}")
+    capacity = 0
+    if controls.penalized:
+        if history is None or history_length is None:
+            raise _lib.IllegalArgumentException("penalties need the history and its length")
+        if rows and history.nbytes % (4 * rows):
+            raise _lib.IllegalArgumentException(f"a history of {history.nbytes} bytes does not hold {rows} rows of tokens")
+        capacity = history.nbytes // (4 * max(rows, 1))
+        for name, b in (("history_length", history_length), ("output_start", output_start)):
+            if b is not None and _nbytes(b) < 4 * rows:
+                raise _lib.IllegalArgumentException(f"{name} has {_nbytes(b) // 4} elements, needs {rows}")
+    c = controls.descriptor(rows, n, history, history_length, output_start, capacity, capacity)
+    _lib.call("kt_process_logits", logits.ptr, rows, n, ctypes.c_int64(n), ctypes.byref(c), out.ptr, ctypes.c_int64(n),
+              (stream or default_stream()).handle)
+    return out

@@ -21,6 +21,8 @@ import numpy as np
 
 from . import _lib
 from .device import DeviceBuffer, Stream, default_stream
+from .kv8 import QuantizedKVCache
+from .logits import LogitsControls
 from .quantization import Quantization, QuantizedTensor
 
 TILE_M = 32  # MatMul.TILE_M (MatMul.kt:16), the reference's prefill chunk
@@ -188,6 +190,10 @@ class InferenceBuffers(_Rows):
         self.vocabulary_size, self.max_sequence_length, self.kv_dimension = vocabulary_size, max_sequence_length, kv_dimension
         self.logits = DeviceBuffer(vocabulary_size * 4)
         self.generated = DeviceBuffer(4 * max_sequence_length)  # greedy tokens by position
+        # with LogitsControls: how many leading positions `generated` holds the tokens of (prefill's
+        # record_tokens), and where the output starts
+        self.recorded = 0
+        self.output_start = DeviceBuffer(4)
         self._prefill: dict[int, _Rows] = {}
 
     def prefill_rows(self, rows: int) -> _Rows:
@@ -195,6 +201,10 @@ class InferenceBuffers(_Rows):
             self._prefill.clear()
             self._prefill[rows] = _Rows(rows, self.dimension, self.hidden_dimension, self.kv_dimension)
         return self._prefill[rows]
+
+    def note_recorded(self, position: int) -> None:
+        """A greedy step at `position` recorded the next token."""
+        self.recorded = position + 1 if self.recorded >= position else self.recorded
 
     def logits_numpy(self, stream: Stream | None = None) -> np.ndarray:
         return self.logits.download(np.float32, stream=stream)
@@ -394,7 +404,12 @@ class Transformer:
             return model
 
     # -- caches and buffers -------------------------------------------------------------
-    def new_cache(self, max_sequence_length: int, stream: Stream | None = None) -> KVCache:
+    def new_cache(self, max_sequence_length: int, stream: Stream | None = None, cache_format: str | None = None,
+                  block_tokens: int = 64) -> KVCache | QuantizedKVCache:
+        """A cache for this model: fp32, or with a ``cache_format`` ("int8", "e4m3") held in 8 bits."""
+        if cache_format is not None:
+            return QuantizedKVCache(self.num_layers, self.num_key_value_heads, max_sequence_length, self.head_dim, cache_format,
+                                    block_tokens, stream)
         return KVCache(self.num_layers, self.num_key_value_heads, max_sequence_length, self.head_dim, stream)
 
     def new_inference_buffers(self, max_sequence_length: int) -> InferenceBuffers:
@@ -453,9 +468,13 @@ class Transformer:
                 _lib.call("kt_rmsnorm_qmatmul_group", rows.x.ptr, self.parameters[p + "norm1.weight"].ptr,
                           ctypes.c_float(self.norm_eps), rows.normed.ptr, count, ws, n, os_, bs, 0, ctypes.c_float(1.0),
                           st)
-            _lib.call("kt_rope_attention", rows.q.ptr, rows.k.ptr, rows.v.ptr, self.inv_freq.ptr, count,
-                      cache.position.ptr, key_bound, cache.keys.ptr, cache.values.ptr, l, cache.max_sequence_length,
-                      self.num_heads, self.num_key_value_heads, self.head_dim, rows.context.ptr, st)
+            if isinstance(cache, QuantizedKVCache):
+                _lib.call("kt_rope_attention_kv8", rows.q.ptr, rows.k.ptr, rows.v.ptr, self.inv_freq.ptr, count,
+                          cache.position.ptr, key_bound, ctypes.byref(cache.cache), l, self.num_heads, rows.context.ptr, st)
+            else:
+                _lib.call("kt_rope_attention", rows.q.ptr, rows.k.ptr, rows.v.ptr, self.inv_freq.ptr, count,
+                          cache.position.ptr, key_bound, cache.keys.ptr, cache.values.ptr, l, cache.max_sequence_length,
+                          self.num_heads, self.num_key_value_heads, self.head_dim, rows.context.ptr, st)
             q_ready = False
             if count == 1 and self.chain_one_row and self._zero_bias.get(p + "attention.wOut", True) and \
                     self._zero_bias.get(p + "ffn.wDown", True):
@@ -518,7 +537,25 @@ class Transformer:
         _lib.call("kt_rmsnorm_qmatmul_group", x_row_ptr, self.parameters["finalNorm.weight"].ptr,
                   ctypes.c_float(self.norm_eps), buffers.normed.ptr, 1, ws, n, os_, bs, 0, ctypes.c_float(1.0), st)
 
-    def _decode_step(self, cache: KVCache, buffers: InferenceBuffers, st, argmax: bool) -> None:
+    def _controlled(self, controls: LogitsControls | None, cache: KVCache, buffers: InferenceBuffers, offset: int, st) -> None:
+        """The controls on buffers.logits, in place, for the text in buffers.generated: as many tokens
+        as the cache's device position + offset. (The logits a caller reads are the controlled ones.)"""
+        if controls is None:
+            return
+        n = self.vocabulary_size
+        c = controls.descriptor(1, n, buffers.generated, cache.position, buffers.output_start, buffers.max_sequence_length,
+                                buffers.max_sequence_length, offset)
+        _lib.call("kt_process_logits", buffers.logits.ptr, 1, n, ctypes.c_int64(n), ctypes.byref(c), buffers.logits.ptr,
+                  ctypes.c_int64(n), st)
+
+    @staticmethod
+    def _check_recorded(controls: LogitsControls | None, cache: KVCache, buffers: InferenceBuffers) -> None:
+        if controls is not None and controls.penalized and buffers.recorded < cache.length:
+            raise _lib.IllegalArgumentException(
+                f"penalties need the text's tokens: {buffers.recorded} of {cache.length} are recorded; prefill with record_tokens")
+
+    def _decode_step(self, cache: KVCache, buffers: InferenceBuffers, st, argmax: bool,
+                     controls: LogitsControls | None = None) -> None:
         """One token from buffers.tokens[0] at the device position; the host length is the
         caller's to advance. With argmax the greedy token replaces buffers.tokens[0] and is
         recorded in buffers.generated at its position."""
@@ -527,6 +564,7 @@ class Transformer:
         if not headed:
             self._head(buffers.x.ptr, buffers, st)
         if argmax:
+            self._controlled(controls, cache, buffers, 1, st)  # the text ends with this step's token
             # the head does not read the position: advance it, take the argmax and record
             # the token in one launch after the head
             _lib.call("kt_argmax_advance", buffers.logits.ptr, self.vocabulary_size, buffers.tokens.ptr,
@@ -536,11 +574,12 @@ class Transformer:
 
     # -- the reference's entry points ----------------------------------------------------
     def prefill(self, prompt, cache: KVCache, buffers: InferenceBuffers, stream: Stream | None = None,
-                chunk_rows: int | None = None) -> InferenceBuffers:
+                chunk_rows: int | None = None, record_tokens: bool = False) -> InferenceBuffers:
         """Transformer.prefill (Transformer.kt:99-132): every layer over the prompt in
         chunks (by default one chunk: the GPU takes the whole prompt as one GEMM; the
         reference uses 32 rows), then finalNorm and lmHead on the last row into
-        buffers.logits. Returns the buffers (logits via buffers.logits_numpy())."""
+        buffers.logits. Returns the buffers (logits via buffers.logits_numpy()). With
+        record_tokens the prompt goes to buffers.generated too, for LogitsControls' penalties."""
         prompt = [int(t) for t in prompt]
         if not prompt:
             raise _lib.IllegalArgumentException("Prompt cannot be empty")
@@ -551,6 +590,11 @@ class Transformer:
         st = _stream(stream)
         chunk = chunk_rows or len(prompt)
         rows = None
+        if record_tokens:
+            buffers.generated.upload(np.array(prompt, np.int32), stream, offset=4 * cache.length)
+            buffers.recorded = cache.length + len(prompt) if cache.length <= buffers.recorded else 0
+        else:
+            buffers.recorded = min(buffers.recorded, cache.length)
         for start in range(0, len(prompt), chunk):
             part = prompt[start:start + chunk]
             rows = buffers.prefill_rows(len(part))
@@ -577,12 +621,13 @@ class Transformer:
         return buffers
 
     def greedy_decode(self, cache: KVCache, buffers: InferenceBuffers, steps: int, stream: Stream | None = None,
-                      use_graph: bool = True) -> list[int]:
+                      use_graph: bool = True, controls: LogitsControls | None = None) -> list[int]:
         """The greedy part of streamFrom (Transformer.kt:224-231) after a prefill: takes
         the argmax of buffers.logits, then `steps` decode steps, each feeding the previous
         greedy token (which never leaves the device) and taking the next argmax. Returns
         the steps + 1 greedy tokens. With use_graph (on a created, non-null stream) one
-        decode step is recorded as a HIP graph and replayed."""
+        decode step is recorded as a HIP graph and replayed. With ``controls`` every argmax is
+        that of the controlled logits; what was generated from here on is the output."""
         if cache.remaining < steps:
             raise _lib.IllegalArgumentException(
                 f"KV cache full: {cache.length} + {steps} positions exceed maxSequenceLength {cache.max_sequence_length}")
@@ -592,12 +637,16 @@ class Transformer:
                 f"{cache.length + steps + 1}")
         st = _stream(stream)
         first = cache.length
+        self._check_recorded(controls, cache, buffers)
+        if controls is not None:
+            buffers.output_start.upload(np.array([first], np.int32), stream)
+            self._controlled(controls, cache, buffers, 0, st)
         _lib.call("kt_argmax", buffers.logits.ptr, self.vocabulary_size, buffers.tokens.ptr, st)
         _lib.call("kt_record_token", buffers.tokens.ptr, cache.position.ptr, buffers.generated.ptr,
                   buffers.max_sequence_length, st)
         if use_graph and steps > 1 and st:
-            self.decode_step(cache, buffers, stream)  # the first step also sizes the workspaces
-            graph = self.capture_decode(cache, buffers, stream)
+            self.decode_step(cache, buffers, stream, controls)  # the first step also sizes the workspaces
+            graph = self.capture_decode(cache, buffers, stream, controls)
             try:
                 graph.replay(steps - 1)
             finally:
@@ -605,18 +654,22 @@ class Transformer:
                 graph.destroy()
         else:
             for _ in range(steps):
-                self.decode_step(cache, buffers, stream)
+                self.decode_step(cache, buffers, stream, controls)
         return buffers.generated.download(np.int32, count=steps + 1, stream=stream, offset=4 * first).tolist()
 
-    def decode_step(self, cache: KVCache, buffers: InferenceBuffers, stream: Stream | None = None) -> None:
+    def decode_step(self, cache: KVCache, buffers: InferenceBuffers, stream: Stream | None = None,
+                    controls: LogitsControls | None = None) -> None:
         """One greedy decode step on the device: the token in buffers.tokens (the last
         argmax) in, its logits in buffers.logits, the next argmax in buffers.tokens and in
-        buffers.generated at its position."""
+        buffers.generated at its position. ``controls`` as in greedy_decode, whose first argmax
+        set buffers.output_start."""
         cache.check_room(1)
-        self._decode_step(cache, buffers, _stream(stream), argmax=True)
+        self._decode_step(cache, buffers, _stream(stream), argmax=True, controls=controls)
+        buffers.note_recorded(cache.length)
         cache.length += 1
 
-    def capture_decode(self, cache: KVCache, buffers: InferenceBuffers, stream: Stream) -> "DecodeGraph":
+    def capture_decode(self, cache: KVCache, buffers: InferenceBuffers, stream: Stream,
+                       controls: LogitsControls | None = None) -> "DecodeGraph":
         """decode_step recorded once as a HIP graph on `stream` (a created stream; run one
         decode_step first so the library's workspaces already have their sizes)."""
         st = _stream(stream)
@@ -625,20 +678,23 @@ class Transformer:
         _lib.call("kt_graph_begin", st)
         graph = ctypes.c_void_p()
         try:
-            self._decode_step(cache, buffers, st, argmax=True)
+            self._decode_step(cache, buffers, st, argmax=True, controls=controls)
         except BaseException:
             # end the capture so the stream is usable again, and drop the partial graph
             if _lib.lib().kt_graph_end(st, ctypes.byref(graph)) == _lib.KT_OK and graph:
                 _lib.lib().kt_graph_destroy(graph)
             raise
         _lib.call("kt_graph_end", st, ctypes.byref(graph))
-        return DecodeGraph(graph, cache, stream)
+        return DecodeGraph(graph, cache, stream, buffers, controls)
 
     def generate(self, prompt, max_tokens: int, stop_tokens=(), stream: Stream | None = None,
-                 use_graph: bool = True) -> list[int]:
+                 use_graph: bool = True, cache_format: str | None = None, block_tokens: int = 64,
+                 controls: LogitsControls | None = None) -> list[int]:
         """Greedy generate (Transformer.kt:167-233): prefill, then argmax and decode,
         stopping at a stop token. The greedy token never leaves the device between steps;
-        with use_graph one decode step is recorded as a HIP graph and replayed."""
+        with use_graph one decode step is recorded as a HIP graph and replayed. With a
+        ``cache_format`` the cache is held in 8 bits (new_cache); ``controls`` steer the choice of
+        each token (greedy_decode)."""
         prompt = [int(t) for t in prompt]
         if not prompt:
             raise _lib.IllegalArgumentException("Prompt cannot be empty")
@@ -648,10 +704,10 @@ class Transformer:
         stream = Stream.create() if own else stream
         try:
             max_seq = len(prompt) + max_tokens
-            cache = self.new_cache(max_seq, stream)
+            cache = self.new_cache(max_seq, stream, cache_format, block_tokens)
             buffers = self.new_inference_buffers(max_seq)
-            self.prefill(prompt, cache, buffers, stream)
-            out = self.greedy_decode(cache, buffers, max_tokens - 1, stream, use_graph)
+            self.prefill(prompt, cache, buffers, stream, record_tokens=controls is not None)
+            out = self.greedy_decode(cache, buffers, max_tokens - 1, stream, use_graph, controls)
             tokens = list(prompt)
             stops = set(int(s) for s in stop_tokens)
             for t in out:
@@ -673,13 +729,16 @@ class DecodeGraph:
     """A recorded greedy decode step (Transformer.capture_decode): each replay decodes
     one token at the cache's device position and advances it."""
 
-    def __init__(self, handle: ctypes.c_void_p, cache: KVCache, stream: Stream):
-        self._h, self.cache, self.stream = handle, cache, stream
+    def __init__(self, handle: ctypes.c_void_p, cache: KVCache, stream: Stream, buffers: InferenceBuffers,
+                 controls: LogitsControls | None = None):
+        self._h, self.cache, self.stream, self.buffers = handle, cache, stream, buffers
+        self._controls = controls  # whose device memory the graph addresses
 
     def replay(self, steps: int = 1) -> None:
         self.cache.check_room(steps)
         for _ in range(steps):
             _lib.call("kt_graph_launch", self._h, _stream(self.stream))
+            self.buffers.note_recorded(self.cache.length)
             self.cache.length += 1
 
     def destroy(self) -> None:
