@@ -16,7 +16,9 @@
 // calls they came in.
 #include <math.h>
 
+#include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "kt_common.h"
 #include "kt_wave.h"
@@ -274,6 +276,25 @@ __global__ void __launch_bounds__(THREADS) append_kernel(AppendArgs a) {
 }
 
 // ---- the cached attention -----------------------------------------------------------------
+// Rows: the (token, query head) pairs of a kv head, token t's G heads side by side; a workgroup
+// (kv head, tile of R rows, key split) holds its rows as matrix operands and its waves take the
+// split's chunks of 64 keys in turn. Codes are exact in fp16, and a query is the sum of two fp16
+// numbers to 2^-22 of its row's largest element (the row scaled by a power of two to 2^13 .. 2^14), so
+// two fp16 products with fp32 sums give a score in fp32 precision; likewise a weight for the values.
+//   S^T = K Q^T: a lane ends with scores of one row (its column), so that the running maximum and sum of a
+//     row stay inside the lanes of a column; the exponentials are v_exp_f32 of one multiply-add.
+//   O^T += V^T P^T: the values lie in memory such that the scores' lanes are the operand's.
+// A wave's maximum follows a row's lazily: a larger score moves it only once it is 2^8 above (the weights
+// then stay below 2^15 in fp16, being taken times 2^6), so that the sums are seldom rescaled.
+// A block's value scale 2^e mu joins the exponent as log2(mu) and e less the largest e so far (uniform):
+// weights include it, and the sum of weights takes it out again, with one product a set of 32 keys.
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f16v __attribute__((ext_vector_type(16)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+
 struct AttnArgs {
     KV8View c;
     const float* q;
@@ -281,74 +302,433 @@ struct AttnArgs {
     float* context;
     int32_t tokens, num_heads;
     float scale;
+    // key splits: most of them, and their rows' averages [kv_heads][tiles][splits][R][head_dim], maxima and
+    // sums [..][R][2], and a counter for each (kv head, tile), zero between launches
+    int32_t max_splits;
+    float* averages;
+    float* stats;
+    uint32_t* counters;
 };
 
-// Workgroup (token, query head): a wave takes every fourth key, its lanes the dims. 32 keys' sums join
-// the running ones as one (one by one, the many small weights of a long context would be lost).
+constexpr float LAZY = 8.0f;      // how far a score may pass the maximum, in powers of two
+constexpr float WEIGHT_UP = 6.0f; // weights are taken times 2^6
+constexpr int32_t MOST_QUIET = 40; // how far below the largest a value scale's exponent goes into the exponentials
+
+// Eight codes as fp16.
 template <int FMT>
-__global__ void __launch_bounds__(THREADS) attention_kernel(AttnArgs a) {
-    const KV8View& c = a.c;
-    constexpr int MAXD = 4;
-    __shared__ float part[THREADS / 64][MAXD * 64], pm[THREADS / 64], pl[THREADS / 64];
-    const int32_t HD = c.head_dim, t = blockIdx.y, h = blockIdx.x, g = h / (a.num_heads / c.kv_heads);
-    const int32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int32_t n = min(max(*a.position + t + 1, 0), c.max_seq);
-    const float* q = a.q + (static_cast<size_t>(t) * a.num_heads + h) * HD;
-    float qd[MAXD], acc[MAXD] = {};
-    for (int i = 0; i < MAXD; ++i) qd[i] = lane + 64 * i < HD ? q[lane + 64 * i] : 0.0f;
-    float m = -INFINITY, l = 0.0f, l_part = 0.0f, part_acc[MAXD] = {};
-    int32_t held = 0;
-    for (int32_t j = wave; j < n; j += THREADS / 64) {
-        const uint8_t* key = c.keys + (static_cast<size_t>(g) * c.slots + j) * HD;
-        const uint8_t* value = c.values + (static_cast<size_t>(g) * c.slots / CHUNK + j / CHUNK) * HD * CHUNK + value_byte(j % CHUNK / 4) + j % 4;
-        const size_t block = static_cast<size_t>(g) * (c.slots / c.block) + j / c.block;
-        float d = 0.0f, v[MAXD];
-        for (int i = 0; i < MAXD; ++i) {
-            const int32_t at = lane + 64 * i;
-            float x[4] = {}, y[4] = {};
-            if (at < HD) {
-                decode4<FMT>(key[at], x);
-                decode4<FMT>(value[at * CHUNK], y);
-            }
-            d = fmaf(qd[i], x[0], d);
-            v[i] = y[0];
-        }
-        d = wave_sum_dpp(d) * c.key_scales[block] * a.scale;
-        const float m_new = fmaxf(m, d), alpha = m == -INFINITY ? 0.0f : expf(m - m_new);
-        const float p = expf(d - m_new), pv = p * c.value_scales[block];
-        l *= alpha;
-        l_part = l_part * alpha + p;
-        for (int i = 0; i < MAXD; ++i) {
-            acc[i] *= alpha;
-            part_acc[i] = part_acc[i] * alpha + pv * v[i];
-        }
-        m = m_new;
-        if (++held == 32 || j + THREADS / 64 >= n) {
-            l += l_part;
-            l_part = 0.0f;
-            for (int i = 0; i < MAXD; ++i) {
-                acc[i] += part_acc[i];
-                part_acc[i] = 0.0f;
-            }
-            held = 0;
+__device__ __forceinline__ half8 to_half8(u2 w) {
+    half8 out;
+    half2v* o = reinterpret_cast<half2v*>(&out);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        if constexpr (FMT == KT_KV8_INT8) {  // 0x6400 | byte is 1024 + byte
+            const half2v low = {static_cast<_Float16>(-1152.0f), static_cast<_Float16>(-1152.0f)};
+            o[2 * i] = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(0x64646464u, w[i], 0x04010400u)) + low;
+            o[2 * i + 1] = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(0x64646464u, w[i], 0x04030402u)) + low;
+        } else {
+            o[2 * i] = __builtin_bit_cast(half2v, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(static_cast<int>(w[i]), 1.0f, false));
+            o[2 * i + 1] = __builtin_bit_cast(half2v, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(static_cast<int>(w[i]), 1.0f, true));
         }
     }
-    for (int i = 0; i < MAXD; ++i) part[wave][lane + 64 * i] = acc[i];
-    if (lane == 0) {
-        pm[wave] = m;
-        pl[wave] = l;
+    return out;
+}
+__device__ __forceinline__ u2 half_of(u4 v, int i) { return i ? u2{v[2], v[3]} : u2{v[0], v[1]}; }
+
+// Eight numbers as the sum of two fp16 operands.
+__device__ __forceinline__ void split2(const float (&v)[8], half8& hi, half8& lo) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const half2v h = __builtin_bit_cast(half2v, __builtin_amdgcn_cvt_pkrtz(v[2 * i], v[2 * i + 1]));
+        const half2v l = __builtin_bit_cast(half2v, __builtin_amdgcn_cvt_pkrtz(v[2 * i] - static_cast<float>(h[0]), v[2 * i + 1] - static_cast<float>(h[1])));
+        hi[2 * i] = h[0];
+        hi[2 * i + 1] = h[1];
+        lo[2 * i] = l[0];
+        lo[2 * i + 1] = l[1];
+    }
+}
+
+// The maximum is a rounded product; at sizes where its rounding is a power of two and more, the
+// exponent is the difference of rounded products, so that it stays below LAZY.
+constexpr float HUGE_SCORE = 65536.0f;
+__device__ __forceinline__ float weight_of_huge(float x, float f, float m, float shift) {
+#pragma clang fp contract(off)
+    const float s = x * f;
+    return __builtin_amdgcn_exp2f((s - m) - shift);
+}
+
+// The largest of a value over the lanes of a column (lanes apart by 16 or 32).
+template <int R>
+__device__ __forceinline__ float column_max(float v) {
+    if constexpr (R == 16) v = fmaxf(v, __shfl_xor(v, 16));
+    return fmaxf(v, __shfl_xor(v, 32));
+}
+template <int R>
+__device__ __forceinline__ float column_sum(float v) {
+    if constexpr (R == 16) v += __shfl_xor(v, 16);
+    return v + __shfl_xor(v, 32);
+}
+
+// The shapes of the products: R = 16 rows on 16x16x32, or R = 32 CT on 32x32x16.
+template <int HD, int R>
+struct Shape {
+    static constexpr bool SMALL = R == 16;
+    static constexpr int CT = SMALL ? 1 : R / 32;         // column tiles
+    static constexpr int E = SMALL ? 8 : 16;              // scores of a lane in a set of 32 keys
+    static constexpr int QS = SMALL ? HD / 32 : HD / 16;  // steps of a score
+    static constexpr int KL = SMALL ? (HD + 63) / 64 : HD / 32;  // 16-byte loads of a key's share (HD 32 and R 16: 8 bytes used)
+    static constexpr int KT = SMALL ? 4 : 2;              // groups of keys with loads of their own in a chunk
+    static constexpr int DB = SMALL ? HD / 16 : HD / 32;  // dim blocks of the output
+    static constexpr int VL = SMALL ? 1 : 2;              // 16-byte loads of a dim
+    static constexpr int OE = SMALL ? 4 : 16;
+};
+
+// Splits of a tile's keys, from the number of chunks alone.
+__host__ __device__ __forceinline__ int32_t splits_of(int32_t chunks, int32_t waves, int32_t most) {
+    const int32_t s = (chunks + waves - 1) / waves;
+    return s < 1 ? 1 : s < most ? s : most;
+}
+
+template <int FMT, int HD, int R, int NW>
+__global__ void __launch_bounds__(64 * NW) attention_kernel(AttnArgs a) {
+    using X = Shape<HD, R>;
+    constexpr int LR = HD + 4;  // padded row of the waves' averages
+    extern __shared__ __attribute__((aligned(16))) float attn_lds[];
+    float* avg = attn_lds;               // [NW][R][LR]
+    float* ms = avg + NW * R * LR;       // [NW][R]
+    float* ls = ms + NW * R;             // [NW][R]
+    const KV8View& c = a.c;
+    const int32_t g = blockIdx.x, tile = gridDim.y - 1 - blockIdx.y, split = blockIdx.z;
+    const int32_t G = a.num_heads / c.kv_heads, rows = a.tokens * G;
+    const int32_t tid = threadIdx.x, lane = tid & 63;
+    const int32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int32_t col = X::SMALL ? lane & 15 : lane & 31, grp = X::SMALL ? lane >> 4 : lane >> 5;
+
+    const int32_t P0 = *a.position;
+    const int32_t t_first = tile * R / G, t_last = min((tile * R + R - 1) / G, a.tokens - 1);
+    auto last_key = [&](int32_t t) { return min(P0 + t, c.max_seq - 1); };  // negative: none; never read outside the cache
+    const int32_t n_keys = last_key(t_last) + 1, n_all = last_key(t_first) + 1;  // keys of any row, of every row
+    const int32_t chunks = n_keys > 0 ? (n_keys + CHUNK - 1) / CHUNK : 0;
+    const int32_t splits = splits_of(chunks, NW, a.max_splits);
+    if (split >= splits) return;
+    const int32_t c0 = static_cast<int32_t>(static_cast<int64_t>(chunks) * split / splits);
+    const int32_t c1 = static_cast<int32_t>(static_cast<int64_t>(chunks) * (split + 1) / splits);
+
+    // the rows' parts
+    half8 qh[X::CT][X::QS], ql[X::CT][X::QS];
+    float fr[X::CT];
+    int32_t last[X::CT];
+#pragma unroll
+    for (int ct = 0; ct < X::CT; ++ct) {
+        const int32_t row = tile * R + 32 * ct + col;
+        const int32_t t = min(row, rows - 1) / G, h = min(row, rows - 1) % G;
+        last[ct] = last_key(t);
+        const float* src = a.q + (static_cast<size_t>(t) * a.num_heads + g * G + h) * HD;
+        float v[X::QS][8];
+        uint32_t top = 0;
+#pragma unroll
+        for (int s = 0; s < X::QS; ++s) {
+            const int32_t d = HD == 32 && X::SMALL ? 8 * grp : X::SMALL ? 64 * (s / 2) + 16 * grp + 8 * (s % 2) : 32 * (s / 2) + 16 * grp + 8 * (s % 2);
+            const f4 x = *reinterpret_cast<const f4*>(src + d), y = *reinterpret_cast<const f4*>(src + d + 4);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                v[s][i] = x[i];
+                v[s][4 + i] = y[i];
+                top = max(top, max(magnitude(x[i]), magnitude(y[i])));
+            }
+        }
+        if constexpr (X::SMALL) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 16)));
+        top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 32)));
+        const int32_t up = 13 - max(static_cast<int32_t>(min(top, 0x7F7FFFFFu) >> 23) - 127, -100);
+        const float by = ldexpf(1.0f, up);
+        fr[ct] = ldexpf(a.scale * 1.4426950408889634f, -up);
+#pragma unroll
+        for (int s = 0; s < X::QS; ++s) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[s][i] *= by;
+            split2(v[s], qh[ct][s], ql[ct][s]);
+        }
+    }
+
+    const uint8_t* kbase = c.keys + static_cast<size_t>(g) * c.slots * HD;
+    const uint8_t* vbase = c.values + static_cast<size_t>(g) * c.slots * HD;
+    const float* kscale = c.key_scales + static_cast<size_t>(g) * (c.slots / c.block);
+    const float* vscale = c.value_scales + static_cast<size_t>(g) * (c.slots / c.block);
+    u4 kr[X::KT][X::KL], vr[X::DB][X::VL];
+    float sk[2], sv[2];
+    auto load_keys = [&](int32_t ch) {
+        const uint8_t* p = kbase + static_cast<size_t>(ch) * CHUNK * HD;
+#pragma unroll
+        for (int t = 0; t < X::KT; ++t) {
+            // the key of the operand's row: R 16: set t / 2, its quads 0 1 4 5 or 2 3 6 7
+            const int32_t x = col >> 2;
+            const int32_t key = X::SMALL ? 32 * (t / 2) + 4 * (4 * (x >> 1) + 2 * (t % 2) + (x & 1)) + (col & 3) : 32 * t + col;
+#pragma unroll
+            for (int i = 0; i < X::KL; ++i) {
+                const uint8_t* q = p + key * HD + (X::SMALL ? (HD == 32 ? 8 * grp : 64 * i + 16 * grp) : 32 * i + 16 * grp);
+                if constexpr (HD == 32 && X::SMALL) {
+                    const u2 two = *reinterpret_cast<const u2*>(q);
+                    kr[t][i] = u4{two[0], two[1], 0u, 0u};
+                } else {
+                    kr[t][i] = *reinterpret_cast<const u4*>(q);
+                }
+            }
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int32_t b = (ch * CHUNK + 32 * h) / c.block;
+            sk[h] = kscale[b];
+            sv[h] = vscale[b];
+        }
+    };
+    auto load_values = [&](int32_t ch) {
+        const uint8_t* p = vbase + static_cast<size_t>(ch) * CHUNK * HD;
+#pragma unroll
+        for (int db = 0; db < X::DB; ++db)
+#pragma unroll
+            for (int s = 0; s < X::VL; ++s) {
+                const int32_t d = (X::SMALL ? 16 : 32) * db + col, piece = X::SMALL ? grp : 2 * s + grp;
+                vr[db][s] = *reinterpret_cast<const u4*>(p + d * CHUNK + 16 * piece);
+            }
+    };
+
+    // the key of a lane's score i in its set
+    auto key_of = [&](int i) { return X::SMALL ? 16 * (grp >> 1) + 4 * (grp & 1) + 8 * (i >> 2) + (i & 3) : 8 * (i >> 2) + 4 * grp + (i & 3); };
+
+    typedef typename std::conditional<X::SMALL, f4, f16v>::type acc_t;
+    acc_t o[X::CT][X::DB];
+    float m[X::CT], l[X::CT];
+#pragma unroll
+    for (int ct = 0; ct < X::CT; ++ct) {
+        m[ct] = -INFINITY;
+        l[ct] = 0.0f;
+#pragma unroll
+        for (int db = 0; db < X::DB; ++db)
+#pragma unroll
+            for (int e = 0; e < X::OE; ++e) o[ct][db][e] = 0.0f;
+    }
+    int32_t e_run = -1000;
+
+    if (c0 + wave < c1) {
+        load_keys(c0 + wave);
+        load_values(c0 + wave);
+    }
+    for (int32_t ch = c0 + wave; ch < c1; ch += NW) {
+        const int32_t next = min(ch + NW, c1 - 1);  // (past the end the last chunk again, unused)
+        const float ks[2] = {sk[0], sk[1]}, vs[2] = {sv[0], sv[1]};
+        acc_t sc[2][X::CT][X::SMALL ? 2 : 1];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int t = 0; t < (X::SMALL ? 2 : 1); ++t) {
+#pragma unroll
+                for (int ct = 0; ct < X::CT; ++ct)
+#pragma unroll
+                    for (int e = 0; e < X::OE; ++e) sc[h][ct][t][e] = 0.0f;
+#pragma unroll
+                for (int s = 0; s < X::QS; ++s) {
+                    const half8 k = to_half8<FMT>(half_of(kr[X::SMALL ? 2 * h + t : h][s / 2], s % 2));
+#pragma unroll
+                    for (int ct = 0; ct < X::CT; ++ct) {
+                        if constexpr (X::SMALL) {
+                            sc[h][ct][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql[ct][s], sc[h][ct][t], 0, 0, 0);
+                            sc[h][ct][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh[ct][s], sc[h][ct][t], 0, 0, 0);
+                        } else {
+                            sc[h][ct][t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, ql[ct][s], sc[h][ct][t], 0, 0, 0);
+                            sc[h][ct][t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qh[ct][s], sc[h][ct][t], 0, 0, 0);
+                        }
+                    }
+                }
+            }
+        load_keys(next);
+        const bool masked = ch * CHUNK + CHUNK > n_all;
+        if (FMT == KT_KV8_E4M3 && ch * CHUNK + CHUNK > n_keys) {  // tokens not held: bytes that may be NaNs
+#pragma unroll
+            for (int db = 0; db < X::DB; ++db)
+#pragma unroll
+                for (int s = 0; s < X::VL; ++s)
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        const int32_t piece = X::SMALL ? grp : 2 * s + grp;
+                        const int32_t held = n_keys - (ch * CHUNK + 32 * (w >> 1) + 16 * (piece >> 1) + 8 * (w & 1) + 4 * (piece & 1));
+                        vr[db][s][w] &= held >= 4 ? 0xFFFFFFFFu : held <= 0 ? 0u : (1u << (8 * held)) - 1u;
+                    }
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int32_t key0 = ch * CHUNK + 32 * h;
+            if (key0 >= n_keys) break;
+            // the value scale: 2^e mu
+            const uint32_t vbits = __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, vs[h]));
+            const float vscale_h = __builtin_bit_cast(float, vbits);
+            const bool real = vscale_h == vscale_h;
+            const int32_t e = real ? static_cast<int32_t>(vbits >> 23 & 255) - 127 : max(e_run, 0);
+            if (e > e_run) {
+                const float down = ldexpf(1.0f, max(e_run - e, -200));
+#pragma unroll
+                for (int ct = 0; ct < X::CT; ++ct)
+#pragma unroll
+                    for (int db = 0; db < X::DB; ++db) o[ct][db] *= down;
+                e_run = e;
+            }
+            const float mu = ldexpf(vscale_h, -e);
+            const int32_t quiet = e_run - e, in_exp = quiet <= MOST_QUIET ? quiet : 0;
+            const float shift = static_cast<float>(in_exp) - __builtin_amdgcn_logf(mu) - WEIGHT_UP;
+            const float unscale = ldexpf(1.0f / mu, in_exp);
+            half8 ph[X::CT][X::SMALL ? 1 : 2], pl[X::CT][X::SMALL ? 1 : 2];
+#pragma unroll
+            for (int ct = 0; ct < X::CT; ++ct) {
+                const float f = ks[h] * fr[ct];
+                float x[X::E];
+                float top = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < X::E; ++i) {
+                    x[i] = X::SMALL ? sc[h][ct][X::SMALL ? i >> 2 : 0][X::SMALL ? i & 3 : i] : sc[h][ct][0][i];
+                    if (masked && key0 + key_of(i) > last[ct]) x[i] = -INFINITY;
+                    top = fmaxf(top, x[i]);
+                }
+                if (__ballot(top * f > m[ct] + LAZY)) {
+                    const float m_new = fmaxf(m[ct], column_max<R>(top == -INFINITY ? -INFINITY : top * f));
+                    const float alpha = m[ct] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[ct] - m_new);
+                    l[ct] *= alpha;
+#pragma unroll
+                    for (int db = 0; db < X::DB; ++db) o[ct][db] *= alpha;
+                    m[ct] = m_new;
+                }
+                const float at = m[ct] == -INFINITY ? 0.0f : m[ct];
+                float sum = 0.0f;
+                if (__ballot(fabsf(at) > HUGE_SCORE)) {  // (one-hot rows)
+#pragma unroll
+                    for (int i = 0; i < X::E; ++i) x[i] = weight_of_huge(x[i], f, at, shift);
+                } else {
+                    const float both = at + shift;
+#pragma unroll
+                    for (int i = 0; i < X::E; ++i) x[i] = __builtin_amdgcn_exp2f(fmaf(x[i], f, -both));
+                }
+#pragma unroll
+                for (int i = 0; i < X::E; ++i) {
+                    if (masked && key0 + key_of(i) > last[ct]) x[i] = 0.0f;
+                    sum += x[i];
+                }
+                l[ct] += sum == 0.0f ? 0.0f : sum * unscale;  // (0 * NaN: a row that sees none of the block)
+                if (in_exp != quiet) {
+                    const float down = ldexpf(1.0f, max(in_exp - quiet, -200));
+#pragma unroll
+                    for (int i = 0; i < X::E; ++i) x[i] *= down;
+                }
+#pragma unroll
+                for (int s = 0; s < (X::SMALL ? 1 : 2); ++s) {
+                    float w[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) w[i] = x[8 * s + i];
+                    split2(w, ph[ct][s], pl[ct][s]);
+                }
+            }
+#pragma unroll
+            for (int db = 0; db < X::DB; ++db)
+#pragma unroll
+                for (int s = 0; s < X::VL; ++s) {
+                    const half8 v = to_half8<FMT>(half_of(vr[db][s], h));
+#pragma unroll
+                    for (int ct = 0; ct < X::CT; ++ct) {
+                        if constexpr (X::SMALL) {
+                            o[ct][db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl[ct][s], o[ct][db], 0, 0, 0);
+                            o[ct][db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[ct][s], o[ct][db], 0, 0, 0);
+                        } else {
+                            o[ct][db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl[ct][s], o[ct][db], 0, 0, 0);
+                            o[ct][db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph[ct][s], o[ct][db], 0, 0, 0);
+                        }
+                    }
+                }
+        }
+        load_values(next);
+    }
+
+    // each wave's averages, maxima and sums, then all waves' through LDS
+#pragma unroll
+    for (int ct = 0; ct < X::CT; ++ct) {
+        l[ct] = column_sum<R>(l[ct]);
+        const float inv = l[ct] == 0.0f ? 0.0f : 1.0f / l[ct];
+        float* row = avg + (wave * R + 32 * ct + col) * LR;
+#pragma unroll
+        for (int db = 0; db < X::DB; ++db)
+#pragma unroll
+            for (int e = 0; e < X::OE; e += 4) {
+                f4 v;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = ldexpf(o[ct][db][e + i] * inv, e_run);
+                *reinterpret_cast<f4*>(row + (X::SMALL ? 16 * db + 4 * grp : 32 * db + 2 * e + 4 * grp)) = v;
+            }
+        if (grp == 0) {
+            ms[wave * R + 32 * ct + col] = m[ct];
+            ls[wave * R + 32 * ct + col] = l[ct];
+        }
     }
     __syncthreads();
-    const int32_t d = threadIdx.x;
-    if (d >= HD) return;
-    float mx = -INFINITY, x = 0.0f, sum = 0.0f;
-    for (int w = 0; w < THREADS / 64; ++w) mx = fmaxf(mx, pm[w]);
-    for (int w = 0; w < THREADS / 64; ++w) {
-        const float e = pl[w] == 0.0f ? 0.0f : expf(pm[w] - mx);
-        x += part[w][d] * e;
-        sum += pl[w] * e;
+    const size_t part = ((static_cast<size_t>(g) * gridDim.y + tile) * a.max_splits + split) * R;
+    for (int32_t e = tid; e < R * (HD / 4); e += 64 * NW) {
+        const int32_t r = e / (HD / 4), d = 4 * (e % (HD / 4)), row = tile * R + r;
+        if (row >= rows) break;
+        float mx = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) mx = fmaxf(mx, ms[w * R + r]);
+        f4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+        float sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+            const float lw = ls[w * R + r];
+            const float by = lw == 0.0f ? 0.0f : lw * __builtin_amdgcn_exp2f((ms[w * R + r] == -INFINITY ? mx : ms[w * R + r]) - (mx == -INFINITY ? 0.0f : mx));
+            const f4 v = *reinterpret_cast<const f4*>(avg + (w * R + r) * LR + d);
+            sum += by;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = fmaf(by, v[i], x[i]);
+        }
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] *= inv;
+        if (splits == 1) {
+            *reinterpret_cast<f4*>(a.context + (static_cast<size_t>(row / G) * a.num_heads + g * G + row % G) * HD + d) = x;
+            continue;
+        }
+        // written through to memory: the reader may be on another die
+        float* to = a.averages + (part + r) * HD + d;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) __hip_atomic_store(to + i, x[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (d == 0) {
+            __hip_atomic_store(a.stats + 2 * (part + r), mx, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            __hip_atomic_store(a.stats + 2 * (part + r) + 1, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
     }
-    a.context[(static_cast<size_t>(t) * a.num_heads + h) * HD + d] = n > 0 ? x / sum : 0.0f;
+    if (splits == 1) return;
+    // the last workgroup of the tile to arrive merges the splits, in their order
+    __shared__ uint32_t arrived;
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if (tid == 0) {
+        uint32_t* counter = a.counters + g * gridDim.y + tile;
+        arrived = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (arrived == static_cast<uint32_t>(splits) - 1) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    if (arrived != static_cast<uint32_t>(splits) - 1) return;
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
+    const size_t first = part - static_cast<size_t>(split) * R;
+    for (int32_t e = tid; e < R * HD; e += 64 * NW) {
+        const int32_t r = e / HD, d = e % HD, row = tile * R + r;
+        if (row >= rows) break;
+        float mx = -INFINITY;
+        for (int32_t s = 0; s < splits; ++s)
+            mx = fmaxf(mx, __hip_atomic_load(a.stats + 2 * (first + s * R + r), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+        float x = 0.0f, sum = 0.0f;
+        for (int32_t s = 0; s < splits; ++s) {
+            const float ml = __hip_atomic_load(a.stats + 2 * (first + s * R + r), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            const float ll = __hip_atomic_load(a.stats + 2 * (first + s * R + r) + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            const float by = ll == 0.0f ? 0.0f : ll * __builtin_amdgcn_exp2f((ml == -INFINITY ? mx : ml) - (mx == -INFINITY ? 0.0f : mx));
+            sum += by;
+            x = fmaf(by, __hip_atomic_load(a.averages + (first + s * R + r) * HD + d, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT), x);
+        }
+        a.context[(static_cast<size_t>(row / G) * a.num_heads + g * G + row % G) * HD + d] = sum == 0.0f ? 0.0f : x / sum;
+    }
 }
 
 // ---- rows as fp32, and the copy of a prefix ------------------------------------------------
@@ -496,11 +876,62 @@ int32_t attention_args(const float* q, int32_t tokens, const int32_t* position, 
     return KT_OK;
 }
 
-int32_t launch_attention(const AttnArgs& a, hipStream_t st) {
-    const auto kernel = a.c.fmt == KT_KV8_INT8 ? attention_kernel<KT_KV8_INT8> : attention_kernel<KT_KV8_E4M3>;
-    kernel<<<dim3(static_cast<uint32_t>(a.num_heads), static_cast<uint32_t>(a.tokens)), THREADS, 0, st>>>(a);
+constexpr int WAVES = 4;
+
+template <int FMT, int HD, int R>
+int32_t launch_rows(AttnArgs a, int32_t key_bound, hipStream_t st, AppendArgs* append) {
+    const int32_t tiles = ceil_div(a.tokens * (a.num_heads / a.c.kv_heads), R);
+    const int64_t wgs = static_cast<int64_t>(a.c.kv_heads) * tiles;
+    if (tiles > 65535) return fail(KT_ERR_SHAPE, "too many tokens and heads in one call");
+    // Key splits: two workgroups for each CU where the rows give fewer.
+    const int32_t fill = static_cast<int32_t>(std::min<int64_t>(256, (2 * cu_count() + wgs - 1) / wgs));
+    a.max_splits = splits_of(ceil_div(key_bound, CHUNK), WAVES, wgs < static_cast<int64_t>(MAX_COUNTERS) ? fill : 1);
+    if (a.max_splits > 1 || append) {
+        const size_t rows = static_cast<size_t>(wgs) * a.max_splits * R, q = append ? static_cast<size_t>(a.num_heads) * HD : 0;
+        void* ws = nullptr;
+        if (const int32_t status = workspace_counters(st, (rows * (HD + 2) + q) * sizeof(float), a.max_splits > 1 ? static_cast<size_t>(wgs) : 0, &ws, &a.counters)) return status;
+        a.averages = static_cast<float*>(ws) + q;
+        a.stats = a.averages + rows * HD;
+        if (append) {
+            append->q_out = static_cast<float*>(ws);
+            a.q = append->q_out;
+            if (const int32_t status = launch_append(*append, st)) return status;
+        }
+    }
+    constexpr size_t lds = static_cast<size_t>(WAVES) * R * (HD + 6) * sizeof(float);
+    if constexpr (lds > (64u << 10)) {  // beyond the default dynamic LDS limit (160 KB per CU on gfx950)
+        static std::atomic<bool> raised{false};
+        if (!raised) {
+            KT_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&attention_kernel<FMT, HD, R, WAVES>), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+            raised = true;
+        }
+    }
+    attention_kernel<FMT, HD, R, WAVES><<<dim3(static_cast<uint32_t>(a.c.kv_heads), static_cast<uint32_t>(tiles), static_cast<uint32_t>(a.max_splits)), 64 * WAVES, lds, st>>>(a);
     KT_LAUNCHED("8-bit cache attention kernel");
     return KT_OK;
+}
+
+template <int FMT, int HD>
+int32_t launch_dims(const AttnArgs& a, int32_t key_bound, hipStream_t st, AppendArgs* append) {
+    const int32_t rows = a.tokens * (a.num_heads / a.c.kv_heads);
+    if constexpr (HD < 256) {
+        if (rows > 48) return launch_rows<FMT, HD, 32>(a, key_bound, st, append);
+    }
+    return launch_rows<FMT, HD, 16>(a, key_bound, st, append);
+}
+
+template <int FMT>
+int32_t launch_format(const AttnArgs& a, int32_t key_bound, hipStream_t st, AppendArgs* append) {
+    switch (a.c.head_dim) {
+        case 32: return launch_dims<FMT, 32>(a, key_bound, st, append);
+        case 64: return launch_dims<FMT, 64>(a, key_bound, st, append);
+        case 128: return launch_dims<FMT, 128>(a, key_bound, st, append);
+        default: return launch_dims<FMT, 256>(a, key_bound, st, append);
+    }
+}
+
+int32_t launch_attention(const AttnArgs& a, int32_t key_bound, hipStream_t st, AppendArgs* append = nullptr) {
+    return a.c.fmt == KT_KV8_INT8 ? launch_format<KT_KV8_INT8>(a, key_bound, st, append) : launch_format<KT_KV8_E4M3>(a, key_bound, st, append);
 }
 
 }  // namespace
@@ -531,7 +962,7 @@ int32_t kt_attention_kv8(const float* q, int32_t tokens, const int32_t* position
                          int32_t num_heads, float* context, void* stream) {
     AttnArgs a{};
     if (const int32_t status = attention_args(q, tokens, position, key_bound, cache, layer, num_heads, context, &a)) return status;
-    return tokens == 0 ? KT_OK : launch_attention(a, static_cast<hipStream_t>(stream));
+    return tokens == 0 ? KT_OK : launch_attention(a, key_bound, static_cast<hipStream_t>(stream));
 }
 
 int32_t kt_rope_attention_kv8(float* q, const float* k, const float* v, const float* inv_freq, int32_t tokens, const int32_t* position, int32_t key_bound,
@@ -542,14 +973,9 @@ int32_t kt_rope_attention_kv8(float* q, const float* k, const float* v, const fl
     if (const int32_t status = attention_args(q, tokens, position, key_bound, cache, layer, num_heads, context, &a)) return status;
     if (tokens == 0) return KT_OK;
     hipStream_t st = static_cast<hipStream_t>(stream);
-    if (tokens == 1) {  // q stays as it is
-        void* ws = nullptr;
-        if (const int32_t status = workspace(st, static_cast<size_t>(num_heads) * a.c.head_dim * sizeof(float), &ws)) return status;
-        p.q_out = static_cast<float*>(ws);
-        a.q = p.q_out;
-    }
+    if (tokens == 1) return launch_attention(a, key_bound, st, &p);  // q stays as it is
     if (const int32_t status = launch_append(p, st)) return status;
-    return launch_attention(a, st);
+    return launch_attention(a, key_bound, st);
 }
 
 int32_t kt_kv8_read(const kt_kv8_cache* cache, int32_t layer, int32_t first, int32_t count, float* keys, float* values, void* stream) {
