@@ -368,6 +368,14 @@ __device__ __forceinline__ float column_sum(float v) {
     return v + __shfl_xor(v, 32);
 }
 
+// What a part with the maximum m and the sum l counts beside parts with the maximum mx: a part without keys
+// (l = 0) nothing, one with a NaN a NaN.
+__device__ __forceinline__ float share_of(float m, float l, float mx) {
+    return l == 0.0f ? 0.0f : l * __builtin_amdgcn_exp2f((m == -INFINITY ? mx : m) - (mx == -INFINITY ? 0.0f : mx));
+}
+constexpr int MAX_SPLITS = 128;
+constexpr int THROUGH = 1 | 16;  // buffer cache bits sc0 sc1: past the caches
+
 // The shapes of the products: R = 16 rows on 16x16x32, or R = 32 CT on 32x32x16.
 template <int HD, int R>
 struct Shape {
@@ -665,6 +673,7 @@ __global__ void __launch_bounds__(64 * NW) attention_kernel(AttnArgs a) {
     }
     __syncthreads();
     const size_t part = ((static_cast<size_t>(g) * gridDim.y + tile) * a.max_splits + split) * R;
+    const __amdgpu_buffer_rsrc_t averages = __builtin_amdgcn_make_buffer_rsrc(a.averages + part * HD, 0, R * HD * 4, 0x00020000);
     for (int32_t e = tid; e < R * (HD / 4); e += 64 * NW) {
         const int32_t r = e / (HD / 4), d = 4 * (e % (HD / 4)), row = tile * R + r;
         if (row >= rows) break;
@@ -675,8 +684,7 @@ __global__ void __launch_bounds__(64 * NW) attention_kernel(AttnArgs a) {
         float sum = 0.0f;
 #pragma unroll
         for (int w = 0; w < NW; ++w) {
-            const float lw = ls[w * R + r];
-            const float by = lw == 0.0f ? 0.0f : lw * __builtin_amdgcn_exp2f((ms[w * R + r] == -INFINITY ? mx : ms[w * R + r]) - (mx == -INFINITY ? 0.0f : mx));
+            const float by = share_of(ms[w * R + r], ls[w * R + r], mx);
             const f4 v = *reinterpret_cast<const f4*>(avg + (w * R + r) * LR + d);
             sum += by;
 #pragma unroll
@@ -690,12 +698,11 @@ __global__ void __launch_bounds__(64 * NW) attention_kernel(AttnArgs a) {
             continue;
         }
         // written through to memory: the reader may be on another die
-        float* to = a.averages + (part + r) * HD + d;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) __hip_atomic_store(to + i, x[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const uint32_t at = (static_cast<uint32_t>(r) * HD + d) * 4;
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, x), averages, static_cast<int>(at), 0, THROUGH);
         if (d == 0) {
-            __hip_atomic_store(a.stats + 2 * (part + r), mx, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            __hip_atomic_store(a.stats + 2 * (part + r) + 1, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            const u2 both = {__builtin_bit_cast(uint32_t, mx), __builtin_bit_cast(uint32_t, sum)};
+            __hip_atomic_store(reinterpret_cast<uint64_t*>(a.stats) + part + r, __builtin_bit_cast(uint64_t, both), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
         }
     }
     if (splits == 1) return;
@@ -706,28 +713,73 @@ __global__ void __launch_bounds__(64 * NW) attention_kernel(AttnArgs a) {
     __syncthreads();
     if (tid == 0) {
         uint32_t* counter = a.counters + g * gridDim.y + tile;
-        arrived = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        if (arrived == static_cast<uint32_t>(splits) - 1) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        arrived = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+        if (arrived == static_cast<uint32_t>(splits) - 1) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
     }
     __syncthreads();
     if (arrived != static_cast<uint32_t>(splits) - 1) return;
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
+    const int32_t held = min(R, rows - tile * R);  // rows of this tile
     const size_t first = part - static_cast<size_t>(split) * R;
-    for (int32_t e = tid; e < R * HD; e += 64 * NW) {
-        const int32_t r = e / HD, d = e % HD, row = tile * R + r;
-        if (row >= rows) break;
-        float mx = -INFINITY;
-        for (int32_t s = 0; s < splits; ++s)
-            mx = fmaxf(mx, __hip_atomic_load(a.stats + 2 * (first + s * R + r), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
-        float x = 0.0f, sum = 0.0f;
-        for (int32_t s = 0; s < splits; ++s) {
-            const float ml = __hip_atomic_load(a.stats + 2 * (first + s * R + r), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            const float ll = __hip_atomic_load(a.stats + 2 * (first + s * R + r) + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            const float by = ll == 0.0f ? 0.0f : ll * __builtin_amdgcn_exp2f((ml == -INFINITY ? mx : ml) - (mx == -INFINITY ? 0.0f : mx));
-            sum += by;
-            x = fmaf(by, __hip_atomic_load(a.averages + (first + s * R + r) * HD + d, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT), x);
+    float* weight = attn_lds;                  // [R][MAX_SPLITS]
+    float* total = weight + R * MAX_SPLITS;    // [R]
+    f4* shares = reinterpret_cast<f4*>(total + R);  // [64 NW]
+    for (int32_t r = wave; r < held; r += NW) {  // a row's weights: lane = split
+        float ml[MAX_SPLITS / 64], ll[MAX_SPLITS / 64], mx = -INFINITY, sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < MAX_SPLITS / 64; ++i) {
+            const int32_t s = lane + 64 * i;
+            const uint64_t both = __hip_atomic_load(reinterpret_cast<uint64_t*>(a.stats) + first + static_cast<size_t>(min(s, splits - 1)) * R + r, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+            ml[i] = s < splits ? __builtin_bit_cast(float, static_cast<uint32_t>(both)) : -INFINITY;
+            ll[i] = s < splits ? __builtin_bit_cast(float, static_cast<uint32_t>(both >> 32)) : 0.0f;
         }
-        a.context[(static_cast<size_t>(row / G) * a.num_heads + g * G + row % G) * HD + d] = sum == 0.0f ? 0.0f : x / sum;
+#pragma unroll
+        for (int i = 0; i < MAX_SPLITS / 64; ++i) mx = fmaxf(mx, wave_max_dpp(ml[i]));
+#pragma unroll
+        for (int i = 0; i < MAX_SPLITS / 64; ++i) {
+            const float by = share_of(ml[i], ll[i], mx);
+            weight[r * MAX_SPLITS + lane + 64 * i] = by;
+            sum += wave_sum_dpp(by);
+        }
+        if (lane == 0) total[r] = sum;
+    }
+    __syncthreads();
+    // thread (four dims of a row, phase): every phases-th split, their loads in flight together
+    const __amdgpu_buffer_rsrc_t all = __builtin_amdgcn_make_buffer_rsrc(a.averages + first * HD, 0, splits * R * HD * 4, 0x00020000);
+    const int32_t items = held * (HD / 4), phases = max(1, 64 * NW / items);
+    for (int32_t i0 = 0; i0 < items; i0 += 64 * NW) {
+        const int32_t item = phases > 1 ? tid % items : i0 + tid, phase = phases > 1 ? tid / items : 0;
+        const bool on = item < items && phase < phases;
+        const int32_t r = min(item, items - 1) / (HD / 4), d = 4 * (min(item, items - 1) % (HD / 4));
+        f4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int32_t s0 = phase; on && s0 < splits; s0 += 8 * phases) {
+            u4 v[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+                v[u] = __builtin_amdgcn_raw_buffer_load_b128(all, ((min(s0 + u * phases, splits - 1) * R + r) * HD + d) * 4, 0, THROUGH);
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const int32_t s = s0 + u * phases;
+                const float by = s < splits ? weight[r * MAX_SPLITS + s] : 0.0f;
+                const f4 y = __builtin_bit_cast(f4, v[u]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[i] = s < splits ? fmaf(by, y[i], x[i]) : x[i];
+            }
+        }
+        if (phases > 1) {
+            shares[tid] = x;
+            __syncthreads();
+        }
+        if (on && phase == 0) {
+            for (int32_t p = 1; p < phases; ++p)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[i] += shares[item + p * items][i];
+            const float inv = total[r] == 0.0f ? 0.0f : 1.0f / total[r];
+            const int32_t row = tile * R + r;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] *= inv;
+            *reinterpret_cast<f4*>(a.context + (static_cast<size_t>(row / G) * a.num_heads + g * G + row % G) * HD + d) = x;
+        }
     }
 }
 
@@ -876,15 +928,15 @@ int32_t attention_args(const float* q, int32_t tokens, const int32_t* position, 
     return KT_OK;
 }
 
-constexpr int WAVES = 4;
+constexpr int DIRECT_KEYS = 16 * CHUNK;  // one workgroup of 16 waves, no key splits
 
-template <int FMT, int HD, int R>
+template <int FMT, int HD, int R, int WAVES>
 int32_t launch_rows(AttnArgs a, int32_t key_bound, hipStream_t st, AppendArgs* append) {
     const int32_t tiles = ceil_div(a.tokens * (a.num_heads / a.c.kv_heads), R);
     const int64_t wgs = static_cast<int64_t>(a.c.kv_heads) * tiles;
     if (tiles > 65535) return fail(KT_ERR_SHAPE, "too many tokens and heads in one call");
     // Key splits: two workgroups for each CU where the rows give fewer.
-    const int32_t fill = static_cast<int32_t>(std::min<int64_t>(256, (2 * cu_count() + wgs - 1) / wgs));
+    const int32_t fill = static_cast<int32_t>(std::min<int64_t>(MAX_SPLITS, (2 * cu_count() + wgs - 1) / wgs));
     a.max_splits = splits_of(ceil_div(key_bound, CHUNK), WAVES, wgs < static_cast<int64_t>(MAX_COUNTERS) ? fill : 1);
     if (a.max_splits > 1 || append) {
         const size_t rows = static_cast<size_t>(wgs) * a.max_splits * R, q = append ? static_cast<size_t>(a.num_heads) * HD : 0;
@@ -898,7 +950,7 @@ int32_t launch_rows(AttnArgs a, int32_t key_bound, hipStream_t st, AppendArgs* a
             if (const int32_t status = launch_append(*append, st)) return status;
         }
     }
-    constexpr size_t lds = static_cast<size_t>(WAVES) * R * (HD + 6) * sizeof(float);
+    constexpr size_t lds = sizeof(float) * std::max(static_cast<size_t>(WAVES) * R * (HD + 6), static_cast<size_t>(R) * (MAX_SPLITS + 1) + 4 * 64 * WAVES);
     if constexpr (lds > (64u << 10)) {  // beyond the default dynamic LDS limit (160 KB per CU on gfx950)
         static std::atomic<bool> raised{false};
         if (!raised) {
@@ -915,9 +967,10 @@ template <int FMT, int HD>
 int32_t launch_dims(const AttnArgs& a, int32_t key_bound, hipStream_t st, AppendArgs* append) {
     const int32_t rows = a.tokens * (a.num_heads / a.c.kv_heads);
     if constexpr (HD < 256) {
-        if (rows > 48) return launch_rows<FMT, HD, 32>(a, key_bound, st, append);
+        if (rows > 48) return launch_rows<FMT, HD, 32, 4>(a, key_bound, st, append);
+        if (key_bound <= DIRECT_KEYS) return launch_rows<FMT, HD, 16, 16>(a, key_bound, st, append);
     }
-    return launch_rows<FMT, HD, 16>(a, key_bound, st, append);
+    return launch_rows<FMT, HD, 16, 4>(a, key_bound, st, append);
 }
 
 template <int FMT>
