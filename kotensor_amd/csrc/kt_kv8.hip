@@ -242,11 +242,11 @@ __global__ void __launch_bounds__(THREADS) append_kernel(AppendArgs a) {
     const KV8View& c = a.c;
     const int32_t HD = c.head_dim, B = c.block;
     const int32_t p0 = *a.position;
-    if (p0 < 0 || p0 >= c.max_seq) return;  // the host checks capacity; never write outside the cache
-    const int32_t end = p0 + min(a.tokens, c.max_seq - p0);
     int32_t id = blockIdx.x;
     const int32_t roles = a.blocks * c.kv_heads * 2;
     if (id < roles) {
+        if (p0 < 0 || p0 >= c.max_seq) return;  // the host checks capacity; never write outside the cache
+        const int32_t end = p0 + min(a.tokens, c.max_seq - p0);
         const int32_t g = id / 2 % c.kv_heads, y = id / 2 / c.kv_heads;
         const bool keys = id % 2 == 0;
         const int32_t b0 = p0 / B, b1 = (end - 1) / B;
@@ -263,7 +263,7 @@ __global__ void __launch_bounds__(THREADS) append_kernel(AppendArgs a) {
     // q: a thread's pair of a token, all heads
     const int32_t half = HD >> 1, per = THREADS / half;
     const int32_t i = threadIdx.x % half, t = (id - roles) * per + threadIdx.x / half;
-    if (t >= end - p0) return;
+    if (t >= a.tokens) return;
     float cf, sf;
     rope_cos_sin(p0 + t, a.inv_freq[i], cf, sf);
     const size_t row = static_cast<size_t>(t) * a.num_heads * HD + i;
@@ -308,6 +308,14 @@ struct AttnArgs {
     float* averages;
     float* stats;
     uint32_t* counters;
+    // one token with RoPE and the append inside: its projections before RoPE, the layer, and the decode attention's
+    // cache of cosines and sines (as kt_decoder.hip's: per frequency i words 4 i .. + 3 = position + 1, the
+    // frequency's bits, cos, sin, written by layer 0; or null)
+    const float* k_new;
+    const float* v_new;
+    const float* inv_freq;
+    int32_t layer;
+    uint32_t* rope_cache;
 };
 
 constexpr float LAZY = 8.0f;      // how far a score may pass the maximum, in powers of two
@@ -396,7 +404,85 @@ __host__ __device__ __forceinline__ int32_t splits_of(int32_t chunks, int32_t wa
     return s < 1 ? 1 : s < most ? s : most;
 }
 
-template <int FMT, int HD, int R, int NW>
+// What a workgroup that appends the step's token shares: the rotation, and the token's codes.
+template <int HD, bool STEP>
+struct StepShared {
+    __attribute__((aligned(16))) float cosines[HD / 2], sines[HD / 2];
+    __attribute__((aligned(16))) uint8_t key[HD], value[HD];
+    uint32_t top[4];
+};
+template <int HD>
+struct StepShared<HD, false> {};
+
+// The append of a step's token at pos in the workgroup whose keys end with it: threads 0 .. 127 hold the pairs (i, i + half) of
+// its key, the next 128 those of its value (y1, y2, `on` where there is one); held: the scales of its
+// block. Returns whether earlier rows of the block changed (their codes are in memory when the
+// workgroup's next barrier has passed); the token's codes are in sh, and the block's scales in held.
+template <int FMT, int HD, int NT>
+__device__ bool append_token(const KV8View& c, StepShared<HD, true>& sh, int32_t g, int32_t pos, bool on, float y1, float y2, float (&held)[2]) {
+    constexpr int HALF = HD / 2;
+    const int32_t tid = threadIdx.x, B = c.block, b = pos / B, r = pos % B, i = tid & 127;
+    const bool is_key = tid < 128;
+    uint32_t m = on ? max(magnitude(y1), magnitude(y2)) : 0;
+    if (tid < 256) {
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) m = max(m, static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), o)));
+        if ((tid & 63) == 0) sh.top[tid >> 6] = m;
+    }
+    __syncthreads();
+    const float own[2] = {scale_of<FMT>(max(sh.top[0], sh.top[1])), scale_of<FMT>(max(sh.top[2], sh.top[3]))};
+    bool raised[2];
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+        raised[w] = r > 0 && held[w] < own[w];  // (neither of them NaN)
+        if (r == 0 || raised[w] || own[w] != own[w]) held[w] = own[w];
+    }
+    float* rows[2] = {c.key_rows + static_cast<size_t>(g) * B * HD, c.value_rows + static_cast<size_t>(g) * B * HD};
+    uint8_t* kdst = c.keys + (static_cast<size_t>(g) * c.slots + static_cast<size_t>(b) * B) * HD;
+    uint8_t* vdst = c.values + static_cast<size_t>(g) * c.slots * HD;
+    auto value_to = [&](int32_t tok, int32_t d) { return vdst + (static_cast<size_t>(tok / CHUNK) * HD + d) * CHUNK + value_byte(tok % CHUNK / 4) + tok % 4; };
+    if (on) {
+        const float s = is_key ? held[0] : held[1], inv = s == s ? 1.0f / s : 0.0f;
+        const uint32_t w = encode4<FMT>(s == s ? y1 * inv : 0.0f, s == s ? y2 * inv : 0.0f, 0.0f, 0.0f);
+        const uint8_t c1 = static_cast<uint8_t>(w), c2 = static_cast<uint8_t>(w >> 8);
+        (is_key ? sh.key : sh.value)[i] = c1;
+        (is_key ? sh.key : sh.value)[i + HALF] = c2;
+        if (is_key) {
+            kdst[r * HD + i] = c1;
+            kdst[r * HD + i + HALF] = c2;
+        } else {
+            *value_to(pos, i) = c1;
+            *value_to(pos, i + HALF) = c2;
+        }
+        if (r + 1 < B) {
+            float* row = (is_key ? rows[0] : rows[1]) + r * HD + i;
+            row[0] = y1;
+            row[HALF] = y2;
+        }
+        if (i == 0) (is_key ? c.key_scales : c.value_scales)[static_cast<size_t>(g) * (c.slots / B) + b] = s;
+    }
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+        if (!raised[w]) continue;
+        const float inv = 1.0f / held[w];
+        for (int32_t e = tid; e < r * (HD / 4); e += NT) {
+            const int32_t row = e / (HD / 4), d = 4 * (e % (HD / 4));
+            const f4 x = *reinterpret_cast<const f4*>(rows[w] + row * HD + d);
+            const uint32_t codes = encode4<FMT>(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+            if (w == 0) {
+                reinterpret_cast<uint32_t*>(kdst)[e] = codes;
+            } else {
+#pragma unroll
+                for (int u = 0; u < 4; ++u) *value_to(b * B + row, d + u) = static_cast<uint8_t>(codes >> (8 * u));
+            }
+        }
+    }
+    const bool again = raised[0] || raised[1];
+    if (again) __threadfence();
+    return again;
+}
+
+template <int FMT, int HD, int R, int NW, bool STEP>
 __global__ void __launch_bounds__(64 * NW) attention_kernel(AttnArgs a) {
     using X = Shape<HD, R>;
     constexpr int LR = HD + 4;  // padded row of the waves' averages
@@ -411,6 +497,25 @@ __global__ void __launch_bounds__(64 * NW) attention_kernel(AttnArgs a) {
     const int32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int32_t col = X::SMALL ? lane & 15 : lane & 31, grp = X::SMALL ? lane >> 4 : lane >> 5;
 
+    // a step's token: its loads go out ahead of the position
+    __shared__ StepShared<HD, STEP> sh;
+    constexpr int HALF = HD / 2;
+    const bool on = STEP && tid < 256 && (tid & 127) < HALF;  // threads with a pair of the key or the value
+    float x1 = 0.0f, x2 = 0.0f, ifr = 0.0f;
+    uint32_t ce[4] = {0u, 0u, 0u, 0u};
+    if constexpr (STEP) {
+        if (on) {
+            const float* src = (tid < 128 ? a.k_new : a.v_new) + g * HD + (tid & 127);
+            x1 = src[0];
+            x2 = src[HALF];
+        }
+        if (tid < HALF) {
+            ifr = a.inv_freq[tid];
+            if (a.rope_cache && a.layer != 0)
+#pragma unroll
+                for (int w = 0; w < 4; ++w) ce[w] = __hip_atomic_load(a.rope_cache + 4 * tid + w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+        }
+    }
     const int32_t P0 = *a.position;
     const int32_t t_first = tile * R / G, t_last = min((tile * R + R - 1) / G, a.tokens - 1);
     auto last_key = [&](int32_t t) { return min(P0 + t, c.max_seq - 1); };  // negative: none; never read outside the cache
@@ -418,44 +523,10 @@ __global__ void __launch_bounds__(64 * NW) attention_kernel(AttnArgs a) {
     const int32_t chunks = n_keys > 0 ? (n_keys + CHUNK - 1) / CHUNK : 0;
     const int32_t splits = splits_of(chunks, NW, a.max_splits);
     if (split >= splits) return;
-    const int32_t c0 = static_cast<int32_t>(static_cast<int64_t>(chunks) * split / splits);
-    const int32_t c1 = static_cast<int32_t>(static_cast<int64_t>(chunks) * (split + 1) / splits);
-
-    // the rows' parts
-    half8 qh[X::CT][X::QS], ql[X::CT][X::QS];
-    float fr[X::CT];
-    int32_t last[X::CT];
-#pragma unroll
-    for (int ct = 0; ct < X::CT; ++ct) {
-        const int32_t row = tile * R + 32 * ct + col;
-        const int32_t t = min(row, rows - 1) / G, h = min(row, rows - 1) % G;
-        last[ct] = last_key(t);
-        const float* src = a.q + (static_cast<size_t>(t) * a.num_heads + g * G + h) * HD;
-        float v[X::QS][8];
-        uint32_t top = 0;
-#pragma unroll
-        for (int s = 0; s < X::QS; ++s) {
-            const int32_t d = HD == 32 && X::SMALL ? 8 * grp : X::SMALL ? 64 * (s / 2) + 16 * grp + 8 * (s % 2) : 32 * (s / 2) + 16 * grp + 8 * (s % 2);
-            const f4 x = *reinterpret_cast<const f4*>(src + d), y = *reinterpret_cast<const f4*>(src + d + 4);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                v[s][i] = x[i];
-                v[s][4 + i] = y[i];
-                top = max(top, max(magnitude(x[i]), magnitude(y[i])));
-            }
-        }
-        if constexpr (X::SMALL) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 16)));
-        top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 32)));
-        const int32_t up = 13 - max(static_cast<int32_t>(min(top, 0x7F7FFFFFu) >> 23) - 127, -100);
-        const float by = ldexpf(1.0f, up);
-        fr[ct] = ldexpf(a.scale * 1.4426950408889634f, -up);
-#pragma unroll
-        for (int s = 0; s < X::QS; ++s) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[s][i] *= by;
-            split2(v[s], qh[ct][s], ql[ct][s]);
-        }
-    }
+    // (a block's chunks stay together: a step that changes its codes is the only one to read them)
+    const int32_t per = c.block > CHUNK ? c.block / CHUNK : 1, units = (chunks + per - 1) / per;
+    const int32_t c0 = per * static_cast<int32_t>(static_cast<int64_t>(units) * split / splits);
+    const int32_t c1 = min(per * static_cast<int32_t>(static_cast<int64_t>(units) * (split + 1) / splits), chunks);
 
     const uint8_t* kbase = c.keys + static_cast<size_t>(g) * c.slots * HD;
     const uint8_t* vbase = c.values + static_cast<size_t>(g) * c.slots * HD;
@@ -498,6 +569,152 @@ __global__ void __launch_bounds__(64 * NW) attention_kernel(AttnArgs a) {
                 vr[db][s] = *reinterpret_cast<const u4*>(p + d * CHUNK + 16 * piece);
             }
     };
+    // a step: the scales of the new token's block, where this workgroup's keys end with it
+    const bool holder = STEP && split == splits - 1 && P0 >= 0 && P0 < c.max_seq;
+    float block_scales[2] = {0.0f, 0.0f};
+    if constexpr (STEP) {
+        if (holder && P0 % c.block != 0) {
+            block_scales[0] = kscale[P0 / c.block];
+            block_scales[1] = vscale[P0 / c.block];
+        }
+    }
+    // the new token's codes and its block's scales in the chunk that holds it, whatever the loads saw
+    auto patch = [&]() {
+        if constexpr (STEP) {
+            const int32_t at = P0 % CHUNK;
+#pragma unroll
+            for (int t = 0; t < X::KT; ++t) {
+                const int32_t x = col >> 2, key = 32 * (t / 2) + 4 * (4 * (x >> 1) + 2 * (t % 2) + (x & 1)) + (col & 3);
+                if (key == at) {
+#pragma unroll
+                    for (int i = 0; i < X::KL; ++i) {
+                        if constexpr (HD == 32) {
+                            const u2 two = *reinterpret_cast<const u2*>(sh.key + 8 * grp);
+                            kr[t][i] = u4{two[0], two[1], 0u, 0u};
+                        } else {
+                            kr[t][i] = *reinterpret_cast<const u4*>(sh.key + 64 * i + 16 * grp);
+                        }
+                    }
+                }
+            }
+            const int32_t h = at >> 5, u = at >> 3 & 1, piece = 2 * (at >> 4 & 1) + (at >> 2 & 1), byte = 8 * (at & 3);
+#pragma unroll
+            for (int db = 0; db < X::DB; ++db) {
+                const uint32_t code = static_cast<uint32_t>(sh.value[16 * db + col]) << byte;
+#pragma unroll
+                for (int w = 0; w < 4; ++w)
+                    if (grp == piece && w == 2 * h + u) vr[db][0][w] = (vr[db][0][w] & ~(0xFFu << byte)) | code;
+            }
+#pragma unroll
+            for (int w = 0; w < 2; ++w)
+                if ((P0 / CHUNK * CHUNK + 32 * w) / c.block == P0 / c.block) {
+                    sk[w] = block_scales[0];
+                    sv[w] = block_scales[1];
+                }
+        }
+    };
+    if (c0 + wave < c1) {
+        load_keys(c0 + wave);
+        load_values(c0 + wave);
+    }
+    if constexpr (STEP) {
+        if (tid < HALF) {
+            float cf, sf;
+            if (ce[0] == static_cast<uint32_t>(P0) + 1u && ce[1] == __builtin_bit_cast(uint32_t, ifr)) {
+                cf = __builtin_bit_cast(float, ce[2]);
+                sf = __builtin_bit_cast(float, ce[3]);
+            } else {
+                rope_cos_sin(P0, ifr, cf, sf);
+            }
+            sh.cosines[tid] = cf;
+            sh.sines[tid] = sf;
+            if (a.rope_cache && a.layer == 0 && g == 0 && split == 0) {
+                uint32_t* e = a.rope_cache + 4 * tid;
+                __hip_atomic_store(e, static_cast<uint32_t>(P0) + 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+                __hip_atomic_store(e + 1, __builtin_bit_cast(uint32_t, ifr), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+                __hip_atomic_store(e + 2, __builtin_bit_cast(uint32_t, cf), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+                __hip_atomic_store(e + 3, __builtin_bit_cast(uint32_t, sf), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+            }
+        }
+        __syncthreads();
+    }
+
+    // the rows' parts
+    half8 qh[X::CT][X::QS], ql[X::CT][X::QS];
+    float fr[X::CT];
+    int32_t last[X::CT];
+#pragma unroll
+    for (int ct = 0; ct < X::CT; ++ct) {
+        const int32_t row = tile * R + 32 * ct + col;
+        const int32_t t = min(row, rows - 1) / G, h = min(row, rows - 1) % G;
+        last[ct] = last_key(t);
+        const float* src = a.q + (static_cast<size_t>(t) * a.num_heads + g * G + h) * HD;
+        float v[X::QS][8];
+        uint32_t top = 0;
+#pragma unroll
+        for (int s = 0; s < X::QS; ++s) {
+            const int32_t d = HD == 32 && X::SMALL ? 8 * grp : X::SMALL ? 64 * (s / 2) + 16 * grp + 8 * (s % 2) : 32 * (s / 2) + 16 * grp + 8 * (s % 2);
+            const f4 x = *reinterpret_cast<const f4*>(src + d), y = *reinterpret_cast<const f4*>(src + d + 4);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                v[s][i] = x[i];
+                v[s][4 + i] = y[i];
+                top = max(top, max(magnitude(x[i]), magnitude(y[i])));
+            }
+        }
+        if constexpr (STEP) {  // the rotation leaves the lanes' dims where they are
+            top = 0;
+            float turned[X::QS][8];
+#pragma unroll
+            for (int s = 0; s < X::QS; ++s) {
+                const int32_t i0 = (HD == 32 ? 8 * grp : 64 * (s / 2) + 16 * grp + 8 * (s % 2)) % HALF;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const bool upper = HD <= 64 ? grp >= 2 : s >= X::QS / 2;
+                    const float other = HD <= 64 ? __shfl_xor(v[s][i], 32) : v[s ^ (HD <= 64 ? 0 : X::QS / 2)][i];
+                    float y1, y2;
+                    rope_apply(upper ? other : v[s][i], upper ? v[s][i] : other, sh.cosines[i0 + i], sh.sines[i0 + i], y1, y2);
+                    turned[s][i] = upper ? y2 : y1;
+                    top = max(top, magnitude(turned[s][i]));
+                }
+            }
+#pragma unroll
+            for (int s = 0; s < X::QS; ++s)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[s][i] = turned[s][i];
+        }
+        if constexpr (X::SMALL) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 16)));
+        top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 32)));
+        const int32_t up = 13 - max(static_cast<int32_t>(min(top, 0x7F7FFFFFu) >> 23) - 127, -100);
+        const float by = ldexpf(1.0f, up);
+        fr[ct] = ldexpf(a.scale * 1.4426950408889634f, -up);
+#pragma unroll
+        for (int s = 0; s < X::QS; ++s) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[s][i] *= by;
+            split2(v[s], qh[ct][s], ql[ct][s]);
+        }
+    }
+
+    if constexpr (STEP) {
+        if (holder) {
+            float y1 = x1, y2 = x2;
+            if (on && tid < 128) rope_apply(x1, x2, sh.cosines[tid], sh.sines[tid], y1, y2);
+            const bool again = append_token<FMT, HD, 64 * NW>(c, sh, g, P0, on, y1, y2, block_scales);
+            __syncthreads();
+            // the new token in the chunk that its wave loaded ahead of the append; earlier rows that changed
+            // are loaded again
+            const int32_t mine = chunks - 1 - c0;  // (this workgroup's last chunk)
+            if (c0 + wave < c1) {
+                if (again) {
+                    __threadfence();
+                    load_keys(c0 + wave);
+                    load_values(c0 + wave);
+                }
+                if (wave == mine % NW && mine < NW) patch();
+            }
+        }
+    }
 
     // the key of a lane's score i in its set
     auto key_of = [&](int i) { return X::SMALL ? 16 * (grp >> 1) + 4 * (grp & 1) + 8 * (i >> 2) + (i & 3) : 8 * (i >> 2) + 4 * grp + (i & 3); };
@@ -516,10 +733,6 @@ __global__ void __launch_bounds__(64 * NW) attention_kernel(AttnArgs a) {
     }
     int32_t e_run = -1000;
 
-    if (c0 + wave < c1) {
-        load_keys(c0 + wave);
-        load_values(c0 + wave);
-    }
     for (int32_t ch = c0 + wave; ch < c1; ch += NW) {
         const int32_t next = min(ch + NW, c1 - 1);  // (past the end the last chunk again, unused)
         const float ks[2] = {sk[0], sk[1]}, vs[2] = {sv[0], sv[1]};
@@ -649,6 +862,9 @@ __global__ void __launch_bounds__(64 * NW) attention_kernel(AttnArgs a) {
                 }
         }
         load_values(next);
+        if constexpr (STEP) {
+            if (holder && next == chunks - 1) patch();
+        }
     }
 
     // each wave's averages, maxima and sums, then all waves' through LDS
@@ -930,7 +1146,7 @@ int32_t attention_args(const float* q, int32_t tokens, const int32_t* position, 
 
 constexpr int DIRECT_KEYS = 16 * CHUNK;  // one workgroup of 16 waves, no key splits
 
-template <int FMT, int HD, int R, int WAVES>
+template <int FMT, int HD, int R, int WAVES, bool STEP = false>
 int32_t launch_rows(AttnArgs a, int32_t key_bound, hipStream_t st, AppendArgs* append) {
     const int32_t tiles = ceil_div(a.tokens * (a.num_heads / a.c.kv_heads), R);
     const int64_t wgs = static_cast<int64_t>(a.c.kv_heads) * tiles;
@@ -939,12 +1155,14 @@ int32_t launch_rows(AttnArgs a, int32_t key_bound, hipStream_t st, AppendArgs* a
     const int32_t fill = static_cast<int32_t>(std::min<int64_t>(MAX_SPLITS, (2 * cu_count() + wgs - 1) / wgs));
     a.max_splits = splits_of(ceil_div(key_bound, CHUNK), WAVES, wgs < static_cast<int64_t>(MAX_COUNTERS) ? fill : 1);
     if (a.max_splits > 1 || append) {
-        const size_t rows = static_cast<size_t>(wgs) * a.max_splits * R, q = append ? static_cast<size_t>(a.num_heads) * HD : 0;
+        const size_t rows = static_cast<size_t>(wgs) * a.max_splits * R, q = append && !STEP ? static_cast<size_t>(a.num_heads) * HD : 0;
         void* ws = nullptr;
         if (const int32_t status = workspace_counters(st, (rows * (HD + 2) + q) * sizeof(float), a.max_splits > 1 ? static_cast<size_t>(wgs) : 0, &ws, &a.counters)) return status;
         a.averages = static_cast<float*>(ws) + q;
         a.stats = a.averages + rows * HD;
-        if (append) {
+        if constexpr (STEP) {
+            a.rope_cache = a.counters + ROPE_CACHE_WORD;
+        } else if (append) {
             append->q_out = static_cast<float*>(ws);
             a.q = append->q_out;
             if (const int32_t status = launch_append(*append, st)) return status;
@@ -954,11 +1172,11 @@ int32_t launch_rows(AttnArgs a, int32_t key_bound, hipStream_t st, AppendArgs* a
     if constexpr (lds > (64u << 10)) {  // beyond the default dynamic LDS limit (160 KB per CU on gfx950)
         static std::atomic<bool> raised{false};
         if (!raised) {
-            KT_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&attention_kernel<FMT, HD, R, WAVES>), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+            KT_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&attention_kernel<FMT, HD, R, WAVES, STEP>), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
             raised = true;
         }
     }
-    attention_kernel<FMT, HD, R, WAVES><<<dim3(static_cast<uint32_t>(a.c.kv_heads), static_cast<uint32_t>(tiles), static_cast<uint32_t>(a.max_splits)), 64 * WAVES, lds, st>>>(a);
+    attention_kernel<FMT, HD, R, WAVES, STEP><<<dim3(static_cast<uint32_t>(a.c.kv_heads), static_cast<uint32_t>(tiles), static_cast<uint32_t>(a.max_splits)), 64 * WAVES, lds, st>>>(a);
     KT_LAUNCHED("8-bit cache attention kernel");
     return KT_OK;
 }
@@ -966,6 +1184,12 @@ int32_t launch_rows(AttnArgs a, int32_t key_bound, hipStream_t st, AppendArgs* a
 template <int FMT, int HD>
 int32_t launch_dims(const AttnArgs& a, int32_t key_bound, hipStream_t st, AppendArgs* append) {
     const int32_t rows = a.tokens * (a.num_heads / a.c.kv_heads);
+    if (append && rows <= 16) {  // a step of up to 16 query heads a kv head: one launch
+        if constexpr (HD < 256) {
+            if (key_bound <= DIRECT_KEYS) return launch_rows<FMT, HD, 16, 16, true>(a, key_bound, st, append);
+        }
+        return launch_rows<FMT, HD, 16, 4, true>(a, key_bound, st, append);
+    }
     if constexpr (HD < 256) {
         if (rows > 48) return launch_rows<FMT, HD, 32, 4>(a, key_bound, st, append);
         if (key_bound <= DIRECT_KEYS) return launch_rows<FMT, HD, 16, 16>(a, key_bound, st, append);
@@ -1026,7 +1250,13 @@ int32_t kt_rope_attention_kv8(float* q, const float* k, const float* v, const fl
     if (const int32_t status = attention_args(q, tokens, position, key_bound, cache, layer, num_heads, context, &a)) return status;
     if (tokens == 0) return KT_OK;
     hipStream_t st = static_cast<hipStream_t>(stream);
-    if (tokens == 1) return launch_attention(a, key_bound, st, &p);  // q stays as it is
+    if (tokens == 1) {  // q stays as it is
+        a.k_new = k;
+        a.v_new = v;
+        a.inv_freq = inv_freq;
+        a.layer = layer;
+        return launch_attention(a, key_bound, st, &p);
+    }
     if (const int32_t status = launch_append(p, st)) return status;
     return launch_attention(a, key_bound, st);
 }
