@@ -296,26 +296,27 @@ typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 
 struct AttnArgs {
-    KV8View c;
-    const float* q;
+    // (what the first loads need comes first: it arrives with the wave)
     const int32_t* position;
-    float* context;
-    int32_t tokens, num_heads;
-    float scale;
-    // key splits: most of them, and their rows' averages [kv_heads][tiles][splits][R][head_dim], maxima and
-    // sums [..][R][2], and a counter for each (kv head, tile), zero between launches
-    int32_t max_splits;
-    float* averages;
-    float* stats;
-    uint32_t* counters;
+    const float* q;
     // one token with RoPE and the append inside: its projections before RoPE, the layer, and the decode attention's
     // cache of cosines and sines (as kt_decoder.hip's: per frequency i words 4 i .. + 3 = position + 1, the
     // frequency's bits, cos, sin, written by layer 0; or null)
     const float* k_new;
     const float* v_new;
     const float* inv_freq;
-    int32_t layer;
     uint32_t* rope_cache;
+    int32_t layer;
+    int32_t tokens, num_heads;
+    float scale;
+    KV8View c;
+    float* context;
+    // key splits: most of them, and their rows' averages [kv_heads][tiles][splits][R][head_dim], maxima and
+    // sums [..][R][2], and a counter for each (kv head, tile), zero between launches
+    int32_t max_splits;
+    float* averages;
+    float* stats;
+    uint32_t* counters;
 };
 
 constexpr float LAZY = 8.0f;      // how far a score may pass the maximum, in powers of two
@@ -497,7 +498,25 @@ __global__ void __launch_bounds__(64 * NW) attention_kernel(AttnArgs a) {
     const int32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int32_t col = X::SMALL ? lane & 15 : lane & 31, grp = X::SMALL ? lane >> 4 : lane >> 5;
 
-    // a step's token: its loads go out ahead of the position
+    // the rows' queries; they and a step's token go out ahead of the position
+    float qv[X::CT][X::QS][8];
+    int32_t tok[X::CT];  // the row's token
+#pragma unroll
+    for (int ct = 0; ct < X::CT; ++ct) {
+        const int32_t row = min(tile * R + 32 * ct + col, rows - 1);
+        tok[ct] = STEP ? 0 : row / G;
+        const float* src = a.q + (static_cast<size_t>(tok[ct]) * a.num_heads + g * G + (row - tok[ct] * G)) * HD;
+#pragma unroll
+        for (int s = 0; s < X::QS; ++s) {
+            const int32_t d = HD == 32 && X::SMALL ? 8 * grp : X::SMALL ? 64 * (s / 2) + 16 * grp + 8 * (s % 2) : 32 * (s / 2) + 16 * grp + 8 * (s % 2);
+            const f4 x = *reinterpret_cast<const f4*>(src + d), y = *reinterpret_cast<const f4*>(src + d + 4);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                qv[ct][s][i] = x[i];
+                qv[ct][s][4 + i] = y[i];
+            }
+        }
+    }
     __shared__ StepShared<HD, STEP> sh;
     constexpr int HALF = HD / 2;
     const bool on = STEP && tid < 256 && (tid & 127) < HALF;  // threads with a pair of the key or the value
@@ -509,11 +528,11 @@ __global__ void __launch_bounds__(64 * NW) attention_kernel(AttnArgs a) {
             x1 = src[0];
             x2 = src[HALF];
         }
-        if (tid < HALF) {
-            ifr = a.inv_freq[tid];
+        if (on) {
+            ifr = a.inv_freq[tid & 127];
             if (a.rope_cache && a.layer != 0)
 #pragma unroll
-                for (int w = 0; w < 4; ++w) ce[w] = __hip_atomic_load(a.rope_cache + 4 * tid + w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+                for (int w = 0; w < 4; ++w) ce[w] = __hip_atomic_load(a.rope_cache + 4 * (tid & 127) + w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
         }
     }
     const int32_t P0 = *a.position;
@@ -525,8 +544,9 @@ __global__ void __launch_bounds__(64 * NW) attention_kernel(AttnArgs a) {
     if (split >= splits) return;
     // (a block's chunks stay together: a step that changes its codes is the only one to read them)
     const int32_t per = c.block > CHUNK ? c.block / CHUNK : 1, units = (chunks + per - 1) / per;
-    const int32_t c0 = per * static_cast<int32_t>(static_cast<int64_t>(units) * split / splits);
-    const int32_t c1 = min(per * static_cast<int32_t>(static_cast<int64_t>(units) * (split + 1) / splits), chunks);
+    // (fewer than 2^25 units, at most 2^7 splits)
+    const int32_t c0 = per * static_cast<int32_t>(static_cast<uint32_t>(units) * split / static_cast<uint32_t>(splits));
+    const int32_t c1 = min(per * static_cast<int32_t>(static_cast<uint32_t>(units) * (split + 1) / static_cast<uint32_t>(splits)), chunks);
 
     const uint8_t* kbase = c.keys + static_cast<size_t>(g) * c.slots * HD;
     const uint8_t* vbase = c.values + static_cast<size_t>(g) * c.slots * HD;
@@ -618,22 +638,19 @@ __global__ void __launch_bounds__(64 * NW) attention_kernel(AttnArgs a) {
         load_values(c0 + wave);
     }
     if constexpr (STEP) {
-        if (tid < HALF) {
-            float cf, sf;
-            if (ce[0] == static_cast<uint32_t>(P0) + 1u && ce[1] == __builtin_bit_cast(uint32_t, ifr)) {
-                cf = __builtin_bit_cast(float, ce[2]);
-                sf = __builtin_bit_cast(float, ce[3]);
-            } else {
-                rope_cos_sin(P0, ifr, cf, sf);
-            }
-            sh.cosines[tid] = cf;
-            sh.sines[tid] = sf;
+        if (on) {  // cosines by the key's threads, sines by the value's
+            const bool cosine = tid < 128;
+            const int32_t i = tid & 127;
+            float y = __builtin_bit_cast(float, ce[cosine ? 2 : 3]);
+            if (ce[0] != static_cast<uint32_t>(P0) + 1u || ce[1] != __builtin_bit_cast(uint32_t, ifr)) y = cosine ? rope_cos(P0, ifr) : rope_sin(P0, ifr);
+            (cosine ? sh.cosines : sh.sines)[i] = y;
             if (a.rope_cache && a.layer == 0 && g == 0 && split == 0) {
-                uint32_t* e = a.rope_cache + 4 * tid;
-                __hip_atomic_store(e, static_cast<uint32_t>(P0) + 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
-                __hip_atomic_store(e + 1, __builtin_bit_cast(uint32_t, ifr), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
-                __hip_atomic_store(e + 2, __builtin_bit_cast(uint32_t, cf), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
-                __hip_atomic_store(e + 3, __builtin_bit_cast(uint32_t, sf), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+                uint32_t* e = a.rope_cache + 4 * i;
+                if (cosine) {
+                    __hip_atomic_store(e, static_cast<uint32_t>(P0) + 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+                    __hip_atomic_store(e + 1, __builtin_bit_cast(uint32_t, ifr), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+                }
+                __hip_atomic_store(e + (cosine ? 2 : 3), __builtin_bit_cast(uint32_t, y), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
             }
         }
         __syncthreads();
@@ -645,25 +662,10 @@ __global__ void __launch_bounds__(64 * NW) attention_kernel(AttnArgs a) {
     int32_t last[X::CT];
 #pragma unroll
     for (int ct = 0; ct < X::CT; ++ct) {
-        const int32_t row = tile * R + 32 * ct + col;
-        const int32_t t = min(row, rows - 1) / G, h = min(row, rows - 1) % G;
-        last[ct] = last_key(t);
-        const float* src = a.q + (static_cast<size_t>(t) * a.num_heads + g * G + h) * HD;
-        float v[X::QS][8];
+        last[ct] = last_key(tok[ct]);
+        float (&v)[X::QS][8] = qv[ct];
         uint32_t top = 0;
-#pragma unroll
-        for (int s = 0; s < X::QS; ++s) {
-            const int32_t d = HD == 32 && X::SMALL ? 8 * grp : X::SMALL ? 64 * (s / 2) + 16 * grp + 8 * (s % 2) : 32 * (s / 2) + 16 * grp + 8 * (s % 2);
-            const f4 x = *reinterpret_cast<const f4*>(src + d), y = *reinterpret_cast<const f4*>(src + d + 4);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                v[s][i] = x[i];
-                v[s][4 + i] = y[i];
-                top = max(top, max(magnitude(x[i]), magnitude(y[i])));
-            }
-        }
         if constexpr (STEP) {  // the rotation leaves the lanes' dims where they are
-            top = 0;
             float turned[X::QS][8];
 #pragma unroll
             for (int s = 0; s < X::QS; ++s) {
@@ -675,7 +677,6 @@ __global__ void __launch_bounds__(64 * NW) attention_kernel(AttnArgs a) {
                     float y1, y2;
                     rope_apply(upper ? other : v[s][i], upper ? v[s][i] : other, sh.cosines[i0 + i], sh.sines[i0 + i], y1, y2);
                     turned[s][i] = upper ? y2 : y1;
-                    top = max(top, magnitude(turned[s][i]));
                 }
             }
 #pragma unroll
@@ -683,6 +684,10 @@ __global__ void __launch_bounds__(64 * NW) attention_kernel(AttnArgs a) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) v[s][i] = turned[s][i];
         }
+#pragma unroll
+        for (int s = 0; s < X::QS; ++s)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) top = max(top, magnitude(v[s][i]));
         if constexpr (X::SMALL) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 16)));
         top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 32)));
         const int32_t up = 13 - max(static_cast<int32_t>(min(top, 0x7F7FFFFFu) >> 23) - 127, -100);
@@ -1144,16 +1149,17 @@ int32_t attention_args(const float* q, int32_t tokens, const int32_t* position, 
     return KT_OK;
 }
 
-constexpr int DIRECT_KEYS = 16 * CHUNK;  // one workgroup of 16 waves, no key splits
+constexpr int DIRECT_KEYS = 16 * CHUNK;  // one workgroup of 16 waves (8 of wider heads, whose registers allow no more), no key splits
 
 template <int FMT, int HD, int R, int WAVES, bool STEP = false>
 int32_t launch_rows(AttnArgs a, int32_t key_bound, hipStream_t st, AppendArgs* append) {
+    constexpr bool DIRECT = WAVES > 4;  // no splits
     const int32_t tiles = ceil_div(a.tokens * (a.num_heads / a.c.kv_heads), R);
     const int64_t wgs = static_cast<int64_t>(a.c.kv_heads) * tiles;
     if (tiles > 65535) return fail(KT_ERR_SHAPE, "too many tokens and heads in one call");
     // Key splits: two workgroups for each CU where the rows give fewer.
     const int32_t fill = static_cast<int32_t>(std::min<int64_t>(MAX_SPLITS, (2 * cu_count() + wgs - 1) / wgs));
-    a.max_splits = splits_of(ceil_div(key_bound, CHUNK), WAVES, wgs < static_cast<int64_t>(MAX_COUNTERS) ? fill : 1);
+    a.max_splits = splits_of(ceil_div(key_bound, CHUNK), WAVES, DIRECT ? 1 : wgs < static_cast<int64_t>(MAX_COUNTERS) ? fill : 1);
     if (a.max_splits > 1 || append) {
         const size_t rows = static_cast<size_t>(wgs) * a.max_splits * R, q = append && !STEP ? static_cast<size_t>(a.num_heads) * HD : 0;
         void* ws = nullptr;
@@ -1186,13 +1192,13 @@ int32_t launch_dims(const AttnArgs& a, int32_t key_bound, hipStream_t st, Append
     const int32_t rows = a.tokens * (a.num_heads / a.c.kv_heads);
     if (append && rows <= 16) {  // a step of up to 16 query heads a kv head: one launch
         if constexpr (HD < 256) {
-            if (key_bound <= DIRECT_KEYS) return launch_rows<FMT, HD, 16, 16, true>(a, key_bound, st, append);
+            if (key_bound <= DIRECT_KEYS) return launch_rows<FMT, HD, 16, HD <= 64 ? 16 : 8, true>(a, key_bound, st, append);
         }
         return launch_rows<FMT, HD, 16, 4, true>(a, key_bound, st, append);
     }
     if constexpr (HD < 256) {
         if (rows > 48) return launch_rows<FMT, HD, 32, 4>(a, key_bound, st, append);
-        if (key_bound <= DIRECT_KEYS) return launch_rows<FMT, HD, 16, 16>(a, key_bound, st, append);
+        if (key_bound <= DIRECT_KEYS) return launch_rows<FMT, HD, 16, HD <= 64 ? 16 : 8>(a, key_bound, st, append);
     }
     return launch_rows<FMT, HD, 16, 4>(a, key_bound, st, append);
 }

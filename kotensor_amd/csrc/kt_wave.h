@@ -36,10 +36,15 @@ __device__ __forceinline__ float wave_max_dpp(float v) {
 // RoPE.applyInPlace's rotation of pair (x1, x2) = (row[i], row[i + half]) at pos (K/RoPE.kt:
 // 117-137): theta = pos * invFreq[i] in fp32, cos and sin in double rounded to float, no
 // contraction.
+__device__ __forceinline__ float rope_cos(int32_t pos, float inv_freq_i) {
+    return static_cast<float>(cos(static_cast<double>(static_cast<float>(pos) * inv_freq_i)));
+}
+__device__ __forceinline__ float rope_sin(int32_t pos, float inv_freq_i) {
+    return static_cast<float>(sin(static_cast<double>(static_cast<float>(pos) * inv_freq_i)));
+}
 __device__ __forceinline__ void rope_cos_sin(int32_t pos, float inv_freq_i, float& c, float& s) {
-    const float theta = static_cast<float>(pos) * inv_freq_i;
-    c = static_cast<float>(cos(static_cast<double>(theta)));
-    s = static_cast<float>(sin(static_cast<double>(theta)));
+    c = rope_cos(pos, inv_freq_i);
+    s = rope_sin(pos, inv_freq_i);
 }
 __device__ __forceinline__ void rope_apply(float x1, float x2, float c, float s, float& y1, float& y2) {
 #pragma clang fp contract(off)
