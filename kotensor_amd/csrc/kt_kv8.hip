@@ -416,21 +416,14 @@ template <int HD>
 struct StepShared<HD, false> {};
 
 // The append of a step's token at pos in the workgroup whose keys end with it: threads 0 .. 127 hold the pairs (i, i + half) of
-// its key, the next 128 those of its value (y1, y2, `on` where there is one); held: the scales of its
-// block. Returns whether earlier rows of the block changed (their codes are in memory when the
+// its key, the next 128 those of its value (y1, y2, `on` where there is one; each wave's largest magnitude
+// in sh.top); held: the scales of its block. Returns whether earlier rows of the block changed (their codes are in memory when the
 // workgroup's next barrier has passed); the token's codes are in sh, and the block's scales in held.
 template <int FMT, int HD, int NT>
 __device__ bool append_token(const KV8View& c, StepShared<HD, true>& sh, int32_t g, int32_t pos, bool on, float y1, float y2, float (&held)[2]) {
     constexpr int HALF = HD / 2;
     const int32_t tid = threadIdx.x, B = c.block, b = pos / B, r = pos % B, i = tid & 127;
     const bool is_key = tid < 128;
-    uint32_t m = on ? max(magnitude(y1), magnitude(y2)) : 0;
-    if (tid < 256) {
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) m = max(m, static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), o)));
-        if ((tid & 63) == 0) sh.top[tid >> 6] = m;
-    }
-    __syncthreads();
     const float own[2] = {scale_of<FMT>(max(sh.top[0], sh.top[1])), scale_of<FMT>(max(sh.top[2], sh.top[3]))};
     bool raised[2];
 #pragma unroll
@@ -491,6 +484,7 @@ __global__ void __launch_bounds__(64 * NW) attention_kernel(AttnArgs a) {
     float* avg = attn_lds;               // [NW][R][LR]
     float* ms = avg + NW * R * LR;       // [NW][R]
     float* ls = ms + NW * R;             // [NW][R]
+    __shared__ float fr_s[R];
     const KV8View& c = a.c;
     const int32_t g = blockIdx.x, tile = gridDim.y - 1 - blockIdx.y, split = blockIdx.z;
     const int32_t G = a.num_heads / c.kv_heads, rows = a.tokens * G;
@@ -498,23 +492,20 @@ __global__ void __launch_bounds__(64 * NW) attention_kernel(AttnArgs a) {
     const int32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int32_t col = X::SMALL ? lane & 15 : lane & 31, grp = X::SMALL ? lane >> 4 : lane >> 5;
 
-    // the rows' queries; they and a step's token go out ahead of the position
-    float qv[X::CT][X::QS][8];
-    int32_t tok[X::CT];  // the row's token
+    // The rows' queries, a row at a time to a wave (its dims d, and for the rotation those of d's pair), go out
+    // ahead of the position, as does a step's token.
+    constexpr int RW = R / NW > 0 ? R / NW : 1, DL = (HD + 63) / 64;
+    const int32_t held = min(R, rows - tile * R);  // rows of this tile
+    float qv[RW][DL], qo[STEP ? RW : 1][STEP ? DL : 1];
 #pragma unroll
-    for (int ct = 0; ct < X::CT; ++ct) {
-        const int32_t row = min(tile * R + 32 * ct + col, rows - 1);
-        tok[ct] = STEP ? 0 : row / G;
-        const float* src = a.q + (static_cast<size_t>(tok[ct]) * a.num_heads + g * G + (row - tok[ct] * G)) * HD;
+    for (int i = 0; i < RW; ++i) {
+        const int32_t row = tile * R + min(wave + i * NW, held - 1), t = STEP ? 0 : row / G;
+        const float* src = a.q + (static_cast<size_t>(t) * a.num_heads + g * G + (row - t * G)) * HD;
 #pragma unroll
-        for (int s = 0; s < X::QS; ++s) {
-            const int32_t d = HD == 32 && X::SMALL ? 8 * grp : X::SMALL ? 64 * (s / 2) + 16 * grp + 8 * (s % 2) : 32 * (s / 2) + 16 * grp + 8 * (s % 2);
-            const f4 x = *reinterpret_cast<const f4*>(src + d), y = *reinterpret_cast<const f4*>(src + d + 4);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                qv[ct][s][i] = x[i];
-                qv[ct][s][4 + i] = y[i];
-            }
+        for (int u = 0; u < DL; ++u) {
+            const int32_t d = (lane + 64 * u) % HD;
+            qv[i][u] = src[d];
+            if constexpr (STEP) qo[i][u] = src[(d + HD / 2) % HD];
         }
     }
     __shared__ StepShared<HD, STEP> sh;
@@ -527,8 +518,6 @@ __global__ void __launch_bounds__(64 * NW) attention_kernel(AttnArgs a) {
             const float* src = (tid < 128 ? a.k_new : a.v_new) + g * HD + (tid & 127);
             x1 = src[0];
             x2 = src[HALF];
-        }
-        if (on) {
             ifr = a.inv_freq[tid & 127];
             if (a.rope_cache && a.layer != 0)
 #pragma unroll
@@ -656,56 +645,72 @@ __global__ void __launch_bounds__(64 * NW) attention_kernel(AttnArgs a) {
         __syncthreads();
     }
 
-    // the rows' parts
+    // the rows' parts through LDS
+    _Float16* qs = reinterpret_cast<_Float16*>(attn_lds);  // [2][R][HD + 8]
+    constexpr int QR = HD + 8;
+#pragma unroll
+    for (int i = 0; i < RW; ++i) {
+        const int32_t r = wave + i * NW;
+        if (r >= held) break;
+        uint32_t top = 0;
+#pragma unroll
+        for (int u = 0; u < DL; ++u) {
+            if constexpr (STEP) {
+                const int32_t d = (lane + 64 * u) % HD;
+                const bool upper = d >= HALF;
+                float y1, y2;
+                rope_apply(upper ? qo[i][u] : qv[i][u], upper ? qv[i][u] : qo[i][u], sh.cosines[d % HALF], sh.sines[d % HALF], y1, y2);
+                qv[i][u] = upper ? y2 : y1;
+            }
+            top = max(top, magnitude(qv[i][u]));
+        }
+        // (bits of magnitudes, below an infinity's where they count: their order is the floats')
+        const float top_f = wave_max_dpp(__builtin_bit_cast(float, min(top, 0x7F7FFFFFu)));
+        const int32_t up = 13 - max(static_cast<int32_t>(__builtin_bit_cast(uint32_t, top_f) >> 23) - 127, -100);
+#pragma unroll
+        for (int u = 0; u < DL; ++u) {
+            const float x = ldexpf(qv[i][u], up);
+            const _Float16 hi = static_cast<_Float16>(x), lo = static_cast<_Float16>(x - static_cast<float>(hi));
+            if (lane + 64 * u < HD) {
+                qs[r * QR + lane + 64 * u] = hi;
+                qs[(R + r) * QR + lane + 64 * u] = lo;
+            }
+        }
+        if (lane == 0) fr_s[r] = ldexpf(a.scale * 1.4426950408889634f, -up);
+    }
+    if constexpr (STEP) {
+        if (holder) {
+            if (on && tid < 128) {
+                const float k1 = x1, k2 = x2;
+                rope_apply(k1, k2, sh.cosines[tid], sh.sines[tid], x1, x2);
+            }
+            uint32_t m = on ? max(magnitude(x1), magnitude(x2)) : 0;
+            if (tid < 256) {
+#pragma unroll
+                for (int o = 32; o > 0; o >>= 1) m = max(m, static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), o)));
+                if (lane == 0) sh.top[wave] = m;
+            }
+        }
+    }
+    __syncthreads();
     half8 qh[X::CT][X::QS], ql[X::CT][X::QS];
     float fr[X::CT];
     int32_t last[X::CT];
 #pragma unroll
     for (int ct = 0; ct < X::CT; ++ct) {
-        last[ct] = last_key(tok[ct]);
-        float (&v)[X::QS][8] = qv[ct];
-        uint32_t top = 0;
-        if constexpr (STEP) {  // the rotation leaves the lanes' dims where they are
-            float turned[X::QS][8];
-#pragma unroll
-            for (int s = 0; s < X::QS; ++s) {
-                const int32_t i0 = (HD == 32 ? 8 * grp : 64 * (s / 2) + 16 * grp + 8 * (s % 2)) % HALF;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const bool upper = HD <= 64 ? grp >= 2 : s >= X::QS / 2;
-                    const float other = HD <= 64 ? __shfl_xor(v[s][i], 32) : v[s ^ (HD <= 64 ? 0 : X::QS / 2)][i];
-                    float y1, y2;
-                    rope_apply(upper ? other : v[s][i], upper ? v[s][i] : other, sh.cosines[i0 + i], sh.sines[i0 + i], y1, y2);
-                    turned[s][i] = upper ? y2 : y1;
-                }
-            }
-#pragma unroll
-            for (int s = 0; s < X::QS; ++s)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[s][i] = turned[s][i];
-        }
-#pragma unroll
-        for (int s = 0; s < X::QS; ++s)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) top = max(top, magnitude(v[s][i]));
-        if constexpr (X::SMALL) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 16)));
-        top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 32)));
-        const int32_t up = 13 - max(static_cast<int32_t>(min(top, 0x7F7FFFFFu) >> 23) - 127, -100);
-        const float by = ldexpf(1.0f, up);
-        fr[ct] = ldexpf(a.scale * 1.4426950408889634f, -up);
+        const int32_t r = min(32 * ct + col, held - 1);  // (columns past the rows repeat the last)
+        fr[ct] = fr_s[r];
+        last[ct] = last_key(STEP ? 0 : (tile * R + r) / G);
 #pragma unroll
         for (int s = 0; s < X::QS; ++s) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[s][i] *= by;
-            split2(v[s], qh[ct][s], ql[ct][s]);
+            const int32_t d = HD == 32 && X::SMALL ? 8 * grp : X::SMALL ? 64 * (s / 2) + 16 * grp + 8 * (s % 2) : 32 * (s / 2) + 16 * grp + 8 * (s % 2);
+            qh[ct][s] = *reinterpret_cast<const half8*>(qs + r * QR + d);
+            ql[ct][s] = *reinterpret_cast<const half8*>(qs + (R + r) * QR + d);
         }
     }
-
     if constexpr (STEP) {
         if (holder) {
-            float y1 = x1, y2 = x2;
-            if (on && tid < 128) rope_apply(x1, x2, sh.cosines[tid], sh.sines[tid], y1, y2);
-            const bool again = append_token<FMT, HD, 64 * NW>(c, sh, g, P0, on, y1, y2, block_scales);
+            const bool again = append_token<FMT, HD, 64 * NW>(c, sh, g, P0, on, x1, x2, block_scales);
             __syncthreads();
             // the new token in the chunk that its wave loaded ahead of the append; earlier rows that changed
             // are loaded again
@@ -873,57 +878,68 @@ __global__ void __launch_bounds__(64 * NW) attention_kernel(AttnArgs a) {
     }
 
     // each wave's averages, maxima and sums, then all waves' through LDS
+    const int32_t used = min(NW, c1 - c0);  // waves with keys
+    __syncthreads();                        // (the queries' parts are read)
+    if (wave < used) {
 #pragma unroll
-    for (int ct = 0; ct < X::CT; ++ct) {
-        l[ct] = column_sum<R>(l[ct]);
-        const float inv = l[ct] == 0.0f ? 0.0f : 1.0f / l[ct];
-        float* row = avg + (wave * R + 32 * ct + col) * LR;
+        for (int ct = 0; ct < X::CT; ++ct) {
+            l[ct] = column_sum<R>(l[ct]);
+            const float inv = l[ct] == 0.0f ? 0.0f : 1.0f / l[ct];
+            if (32 * ct + col >= held) continue;
+            float* row = avg + (wave * R + 32 * ct + col) * LR;
 #pragma unroll
-        for (int db = 0; db < X::DB; ++db)
+            for (int db = 0; db < X::DB; ++db)
 #pragma unroll
-            for (int e = 0; e < X::OE; e += 4) {
-                f4 v;
+                for (int e = 0; e < X::OE; e += 4) {
+                    f4 v;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) v[i] = ldexpf(o[ct][db][e + i] * inv, e_run);
-                *reinterpret_cast<f4*>(row + (X::SMALL ? 16 * db + 4 * grp : 32 * db + 2 * e + 4 * grp)) = v;
+                    for (int i = 0; i < 4; ++i) v[i] = ldexpf(o[ct][db][e + i] * inv, e_run);
+                    *reinterpret_cast<f4*>(row + (X::SMALL ? 16 * db + 4 * grp : 32 * db + 2 * e + 4 * grp)) = v;
+                }
+            if (grp == 0) {
+                ms[wave * R + 32 * ct + col] = m[ct];
+                ls[wave * R + 32 * ct + col] = l[ct];
             }
-        if (grp == 0) {
-            ms[wave * R + 32 * ct + col] = m[ct];
-            ls[wave * R + 32 * ct + col] = l[ct];
         }
     }
     __syncthreads();
     const size_t part = ((static_cast<size_t>(g) * gridDim.y + tile) * a.max_splits + split) * R;
     const __amdgpu_buffer_rsrc_t averages = __builtin_amdgcn_make_buffer_rsrc(a.averages + part * HD, 0, R * HD * 4, 0x00020000);
-    for (int32_t e = tid; e < R * (HD / 4); e += 64 * NW) {
+    // thread (wave w's part of row r): its weight among the row's parts, in the place of its sum
+    float by = 0.0f, mx = -INFINITY, sum = 0.0f;
+    const int32_t wr = tid % R, ww = tid / R;
+    static_assert(64 * NW >= R * NW, "a thread for each part of a row");
+    const bool weighs = ww < used && wr < held;
+    if (weighs) {
+        for (int32_t w = 0; w < used; ++w) mx = fmaxf(mx, ms[w * R + wr]);
+        for (int32_t w = 0; w < used; ++w) {
+            const float share = share_of(ms[w * R + wr], ls[w * R + wr], mx);
+            sum += share;
+            by = w == ww ? share : by;
+        }
+        by = sum == 0.0f ? 0.0f : by / sum;
+    }
+    __syncthreads();
+    if (weighs) ls[ww * R + wr] = by;
+    if (splits > 1 && tid < held) {
+        const u2 both = {__builtin_bit_cast(uint32_t, mx), __builtin_bit_cast(uint32_t, sum)};
+        __hip_atomic_store(reinterpret_cast<uint64_t*>(a.stats) + part + tid, __builtin_bit_cast(uint64_t, both), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+    }
+    __syncthreads();
+    for (int32_t e = tid; e < held * (HD / 4); e += 64 * NW) {
         const int32_t r = e / (HD / 4), d = 4 * (e % (HD / 4)), row = tile * R + r;
-        if (row >= rows) break;
-        float mx = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < NW; ++w) mx = fmaxf(mx, ms[w * R + r]);
         f4 x = {0.0f, 0.0f, 0.0f, 0.0f};
-        float sum = 0.0f;
-#pragma unroll
-        for (int w = 0; w < NW; ++w) {
-            const float by = share_of(ms[w * R + r], ls[w * R + r], mx);
+        for (int32_t w = 0; w < used; ++w) {
+            const float y = ls[w * R + r];
             const f4 v = *reinterpret_cast<const f4*>(avg + (w * R + r) * LR + d);
-            sum += by;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = fmaf(by, v[i], x[i]);
+            for (int i = 0; i < 4; ++i) x[i] = fmaf(y, v[i], x[i]);
         }
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] *= inv;
         if (splits == 1) {
-            *reinterpret_cast<f4*>(a.context + (static_cast<size_t>(row / G) * a.num_heads + g * G + row % G) * HD + d) = x;
-            continue;
-        }
-        // written through to memory: the reader may be on another die
-        const uint32_t at = (static_cast<uint32_t>(r) * HD + d) * 4;
-        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, x), averages, static_cast<int>(at), 0, THROUGH);
-        if (d == 0) {
-            const u2 both = {__builtin_bit_cast(uint32_t, mx), __builtin_bit_cast(uint32_t, sum)};
-            __hip_atomic_store(reinterpret_cast<uint64_t*>(a.stats) + part + r, __builtin_bit_cast(uint64_t, both), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+            const int32_t t = STEP ? 0 : row / G;
+            *reinterpret_cast<f4*>(a.context + (static_cast<size_t>(t) * a.num_heads + g * G + (row - t * G)) * HD + d) = x;
+        } else {  // written through to memory: the reader may be on another die
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, x), averages, (r * HD + d) * 4, 0, THROUGH);
         }
     }
     if (splits == 1) return;
@@ -940,7 +956,6 @@ __global__ void __launch_bounds__(64 * NW) attention_kernel(AttnArgs a) {
     __syncthreads();
     if (arrived != static_cast<uint32_t>(splits) - 1) return;
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
-    const int32_t held = min(R, rows - tile * R);  // rows of this tile
     const size_t first = part - static_cast<size_t>(split) * R;
     float* weight = attn_lds;                  // [R][MAX_SPLITS]
     float* total = weight + R * MAX_SPLITS;    // [R]
@@ -1174,7 +1189,7 @@ int32_t launch_rows(AttnArgs a, int32_t key_bound, hipStream_t st, AppendArgs* a
             if (const int32_t status = launch_append(*append, st)) return status;
         }
     }
-    constexpr size_t lds = sizeof(float) * std::max(static_cast<size_t>(WAVES) * R * (HD + 6), static_cast<size_t>(R) * (MAX_SPLITS + 1) + 4 * 64 * WAVES);
+    constexpr size_t lds = sizeof(float) * std::max(std::max(static_cast<size_t>(WAVES) * R * (HD + 6), static_cast<size_t>(R) * (HD + 8)), static_cast<size_t>(R) * (MAX_SPLITS + 1) + 4 * 64 * WAVES);
     if constexpr (lds > (64u << 10)) {  // beyond the default dynamic LDS limit (160 KB per CU on gfx950)
         static std::atomic<bool> raised{false};
         if (!raised) {
