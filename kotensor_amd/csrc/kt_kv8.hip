@@ -366,15 +366,38 @@ __device__ __forceinline__ float weight_of_huge(float x, float f, float m, float
 }
 
 // The largest of a value over the lanes of a column (lanes apart by 16 or 32).
+struct Swapped {
+    float a, b;  // of two lanes apart by 16 (32): the value of the one and of the other, in both
+};
+// (the compiler's builtins for these gave the first result in the place of the second, too; the wait states
+// are those between a vector write and the swap's read)
+__device__ __forceinline__ Swapped swap16(float v) {
+    Swapped s{v, v};
+    asm("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(s.a), "+v"(s.b));
+    return s;
+}
+__device__ __forceinline__ Swapped swap32(float v) {
+    Swapped s{v, v};
+    asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(s.a), "+v"(s.b));
+    return s;
+}
 template <int R>
 __device__ __forceinline__ float column_max(float v) {
-    if constexpr (R == 16) v = fmaxf(v, __shfl_xor(v, 16));
-    return fmaxf(v, __shfl_xor(v, 32));
+    if constexpr (R == 16) {
+        const Swapped s = swap16(v);
+        v = fmaxf(s.a, s.b);
+    }
+    const Swapped s = swap32(v);
+    return fmaxf(s.a, s.b);
 }
 template <int R>
 __device__ __forceinline__ float column_sum(float v) {
-    if constexpr (R == 16) v += __shfl_xor(v, 16);
-    return v + __shfl_xor(v, 32);
+    if constexpr (R == 16) {
+        const Swapped s = swap16(v);
+        v = s.a + s.b;
+    }
+    const Swapped s = swap32(v);
+    return s.a + s.b;
 }
 
 // What a part with the maximum m and the sum l counts beside parts with the maximum mx: a part without keys
@@ -784,93 +807,112 @@ __global__ void __launch_bounds__(64 * NW) attention_kernel(AttnArgs a) {
                         vr[db][s][w] &= held >= 4 ? 0xFFFFFFFFu : held <= 0 ? 0u : (1u << (8 * held)) - 1u;
                     }
         }
+        // the value scales 2^e mu of the two sets of 32 keys (past the last key the first's again)
+        float vs_h[2], ks_h[2], shift[2], unscale[2];
+        int32_t e_h[2], quiet[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const int32_t key0 = ch * CHUNK + 32 * h;
-            if (key0 >= n_keys) break;
-            // the value scale: 2^e mu
-            const uint32_t vbits = __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, vs[h]));
-            const float vscale_h = __builtin_bit_cast(float, vbits);
-            const bool real = vscale_h == vscale_h;
-            const int32_t e = real ? static_cast<int32_t>(vbits >> 23 & 255) - 127 : max(e_run, 0);
-            if (e > e_run) {
-                const float down = ldexpf(1.0f, max(e_run - e, -200));
+            const bool there = h == 0 || ch * CHUNK + 32 < n_keys;
+            ks_h[h] = there ? ks[h] : ks[0];
+            vs_h[h] = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, there ? vs[h] : vs[0])));
+            e_h[h] = static_cast<int32_t>(__builtin_bit_cast(uint32_t, vs_h[h]) >> 23 & 255) - 127;
+        }
 #pragma unroll
-                for (int ct = 0; ct < X::CT; ++ct)
+        for (int h = 0; h < 2; ++h)  // a NaN makes NaNs with any exponent: one that changes nothing for other rows
+            if (vs_h[h] != vs_h[h]) e_h[h] = vs_h[1 - h] == vs_h[1 - h] ? e_h[1 - h] : e_run > -1000 ? e_run : 0;
+        const int32_t e_max = max(e_h[0], e_h[1]);
+        if (e_max > e_run) {
+            const float down = ldexpf(1.0f, max(e_run - e_max, -200));
 #pragma unroll
-                    for (int db = 0; db < X::DB; ++db) o[ct][db] *= down;
-                e_run = e;
-            }
-            const float mu = ldexpf(vscale_h, -e);
-            const int32_t quiet = e_run - e, in_exp = quiet <= MOST_QUIET ? quiet : 0;
-            const float shift = static_cast<float>(in_exp) - __builtin_amdgcn_logf(mu) - WEIGHT_UP;
-            const float unscale = ldexpf(1.0f / mu, in_exp);
-            half8 ph[X::CT][X::SMALL ? 1 : 2], pl[X::CT][X::SMALL ? 1 : 2];
+            for (int ct = 0; ct < X::CT; ++ct)
 #pragma unroll
-            for (int ct = 0; ct < X::CT; ++ct) {
-                const float f = ks[h] * fr[ct];
-                float x[X::E];
-                float top = -INFINITY;
+                for (int db = 0; db < X::DB; ++db) o[ct][db] *= down;
+            e_run = e_max;
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const float mu = ldexpf(vs_h[h], -e_h[h]);
+            quiet[h] = e_run - e_h[h];
+            const int32_t in_exp = quiet[h] <= MOST_QUIET ? quiet[h] : 0;
+            quiet[h] -= in_exp;
+            shift[h] = static_cast<float>(in_exp) - __builtin_amdgcn_logf(mu) - WEIGHT_UP;
+            unscale[h] = ldexpf(1.0f / mu, in_exp);
+        }
+        half8 ph[2][X::CT][X::VL], pl[2][X::CT][X::VL];
+#pragma unroll
+        for (int ct = 0; ct < X::CT; ++ct) {
+            const float f[2] = {ks_h[0] * fr[ct], ks_h[1] * fr[ct]};
+            float x[2][X::E], top = -INFINITY;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float most = -INFINITY;
 #pragma unroll
                 for (int i = 0; i < X::E; ++i) {
-                    x[i] = X::SMALL ? sc[h][ct][X::SMALL ? i >> 2 : 0][X::SMALL ? i & 3 : i] : sc[h][ct][0][i];
-                    if (masked && key0 + key_of(i) > last[ct]) x[i] = -INFINITY;
-                    top = fmaxf(top, x[i]);
+                    x[h][i] = X::SMALL ? sc[h][ct][X::SMALL ? i >> 2 : 0][X::SMALL ? i & 3 : i] : sc[h][ct][0][i];
+                    if (masked && ch * CHUNK + 32 * h + key_of(i) > last[ct]) x[h][i] = -INFINITY;
+                    most = fmaxf(most, x[h][i]);
                 }
-                if (__ballot(top * f > m[ct] + LAZY)) {
-                    const float m_new = fmaxf(m[ct], column_max<R>(top == -INFINITY ? -INFINITY : top * f));
-                    const float alpha = m[ct] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[ct] - m_new);
-                    l[ct] *= alpha;
+                top = fmaxf(top, most * f[h]);
+            }
+            if (__ballot(top > m[ct] + LAZY)) {
+                const float m_new = fmaxf(m[ct], column_max<R>(top));
+                const float alpha = m[ct] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[ct] - m_new);
+                l[ct] *= alpha;
 #pragma unroll
-                    for (int db = 0; db < X::DB; ++db) o[ct][db] *= alpha;
-                    m[ct] = m_new;
-                }
-                const float at = m[ct] == -INFINITY ? 0.0f : m[ct];
-                float sum = 0.0f;
-                if (__ballot(fabsf(at) > HUGE_SCORE)) {  // (one-hot rows)
+                for (int db = 0; db < X::DB; ++db) o[ct][db] *= alpha;
+                m[ct] = m_new;
+            }
+            const float at = m[ct] == -INFINITY ? 0.0f : m[ct];
+            const bool huge = __ballot(fabsf(at) > HUGE_SCORE);  // (one-hot rows)
 #pragma unroll
-                    for (int i = 0; i < X::E; ++i) x[i] = weight_of_huge(x[i], f, at, shift);
+            for (int h = 0; h < 2; ++h) {
+                if (huge) {
+#pragma unroll
+                    for (int i = 0; i < X::E; ++i) x[h][i] = weight_of_huge(x[h][i], f[h], at, shift[h]);
                 } else {
-                    const float both = at + shift;
+                    const float both = at + shift[h];
 #pragma unroll
-                    for (int i = 0; i < X::E; ++i) x[i] = __builtin_amdgcn_exp2f(fmaf(x[i], f, -both));
+                    for (int i = 0; i < X::E; ++i) x[h][i] = __builtin_amdgcn_exp2f(fmaf(x[h][i], f[h], -both));
                 }
+                float sum = 0.0f;
 #pragma unroll
                 for (int i = 0; i < X::E; ++i) {
-                    if (masked && key0 + key_of(i) > last[ct]) x[i] = 0.0f;
-                    sum += x[i];
+                    if (masked && ch * CHUNK + 32 * h + key_of(i) > last[ct]) x[h][i] = 0.0f;
+                    sum += x[h][i];
                 }
-                l[ct] += sum == 0.0f ? 0.0f : sum * unscale;  // (0 * NaN: a row that sees none of the block)
-                if (in_exp != quiet) {
-                    const float down = ldexpf(1.0f, max(in_exp - quiet, -200));
+                l[ct] += sum == 0.0f ? 0.0f : sum * unscale[h];  // (0 * NaN: a row that sees none of the block)
+                if (quiet[h]) {
+                    const float down = ldexpf(1.0f, max(-quiet[h], -200));
 #pragma unroll
-                    for (int i = 0; i < X::E; ++i) x[i] *= down;
+                    for (int i = 0; i < X::E; ++i) x[h][i] *= down;
                 }
-#pragma unroll
-                for (int s = 0; s < (X::SMALL ? 1 : 2); ++s) {
-                    float w[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) w[i] = x[8 * s + i];
-                    split2(w, ph[ct][s], pl[ct][s]);
-                }
-            }
-#pragma unroll
-            for (int db = 0; db < X::DB; ++db)
 #pragma unroll
                 for (int s = 0; s < X::VL; ++s) {
+                    float w[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) w[i] = x[h][8 * s + i];
+                    split2(w, ph[h][ct][s], pl[h][ct][s]);
+                }
+            }
+        }
+#pragma unroll
+        for (int db = 0; db < X::DB; ++db)
+#pragma unroll
+            for (int s = 0; s < X::VL; ++s)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
                     const half8 v = to_half8<FMT>(half_of(vr[db][s], h));
 #pragma unroll
                     for (int ct = 0; ct < X::CT; ++ct) {
                         if constexpr (X::SMALL) {
-                            o[ct][db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl[ct][s], o[ct][db], 0, 0, 0);
-                            o[ct][db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[ct][s], o[ct][db], 0, 0, 0);
+                            o[ct][db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl[h][ct][s], o[ct][db], 0, 0, 0);
+                            o[ct][db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[h][ct][s], o[ct][db], 0, 0, 0);
                         } else {
-                            o[ct][db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl[ct][s], o[ct][db], 0, 0, 0);
-                            o[ct][db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph[ct][s], o[ct][db], 0, 0, 0);
+                            o[ct][db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl[h][ct][s], o[ct][db], 0, 0, 0);
+                            o[ct][db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph[h][ct][s], o[ct][db], 0, 0, 0);
                         }
                     }
                 }
-        }
         load_values(next);
         if constexpr (STEP) {
             if (holder && next == chunks - 1) patch();
@@ -1164,7 +1206,7 @@ int32_t attention_args(const float* q, int32_t tokens, const int32_t* position, 
     return KT_OK;
 }
 
-constexpr int DIRECT_KEYS = 16 * CHUNK;  // one workgroup of 16 waves (8 of wider heads, whose registers allow no more), no key splits
+constexpr int DIRECT_KEYS = 16 * CHUNK;  // one workgroup of 8 waves, no key splits
 
 template <int FMT, int HD, int R, int WAVES, bool STEP = false>
 int32_t launch_rows(AttnArgs a, int32_t key_bound, hipStream_t st, AppendArgs* append) {
@@ -1207,13 +1249,13 @@ int32_t launch_dims(const AttnArgs& a, int32_t key_bound, hipStream_t st, Append
     const int32_t rows = a.tokens * (a.num_heads / a.c.kv_heads);
     if (append && rows <= 16) {  // a step of up to 16 query heads a kv head: one launch
         if constexpr (HD < 256) {
-            if (key_bound <= DIRECT_KEYS) return launch_rows<FMT, HD, 16, HD <= 64 ? 16 : 8, true>(a, key_bound, st, append);
+            if (key_bound <= DIRECT_KEYS) return launch_rows<FMT, HD, 16, 8, true>(a, key_bound, st, append);
         }
         return launch_rows<FMT, HD, 16, 4, true>(a, key_bound, st, append);
     }
     if constexpr (HD < 256) {
         if (rows > 48) return launch_rows<FMT, HD, 32, 4>(a, key_bound, st, append);
-        if (key_bound <= DIRECT_KEYS) return launch_rows<FMT, HD, 16, HD <= 64 ? 16 : 8>(a, key_bound, st, append);
+        if (key_bound <= DIRECT_KEYS) return launch_rows<FMT, HD, 16, 8>(a, key_bound, st, append);
     }
     return launch_rows<FMT, HD, 16, 4>(a, key_bound, st, append);
 }
