@@ -348,7 +348,7 @@ __device__ __forceinline__ void split2(const float (&v)[8], half8& hi, half8& lo
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const half2v h = __builtin_bit_cast(half2v, __builtin_amdgcn_cvt_pkrtz(v[2 * i], v[2 * i + 1]));
-        const half2v l = __builtin_bit_cast(half2v, __builtin_amdgcn_cvt_pkrtz(v[2 * i] - static_cast<float>(h[0]), v[2 * i + 1] - static_cast<float>(h[1])));
+        const half2v l = __builtin_bit_cast(half2v, __builtin_amdgcn_cvt_pkrtz(fmaf(static_cast<float>(h[0]), -1.0f, v[2 * i]), fmaf(static_cast<float>(h[1]), -1.0f, v[2 * i + 1])));
         hi[2 * i] = h[0];
         hi[2 * i + 1] = h[1];
         lo[2 * i] = l[0];
@@ -420,6 +420,7 @@ struct Shape {
     static constexpr int DB = SMALL ? HD / 16 : HD / 32;  // dim blocks of the output
     static constexpr int VL = SMALL ? 1 : 2;              // 16-byte loads of a dim
     static constexpr int OE = SMALL ? 4 : 16;
+    static constexpr int J = SMALL ? 2 : 1;               // sets of 32 keys that share a maximum's check
 };
 
 // Splits of a tile's keys, from the number of chunks alone.
@@ -500,7 +501,7 @@ __device__ bool append_token(const KV8View& c, StepShared<HD, true>& sh, int32_t
 }
 
 template <int FMT, int HD, int R, int NW, bool STEP>
-__global__ void __launch_bounds__(64 * NW) attention_kernel(AttnArgs a) {
+__global__ void __launch_bounds__(64 * NW, R > 16 ? 2 : 1) attention_kernel(AttnArgs a) {
     using X = Shape<HD, R>;
     constexpr int LR = HD + 4;  // padded row of the waves' averages
     extern __shared__ __attribute__((aligned(16))) float attn_lds[];
@@ -716,7 +717,10 @@ __global__ void __launch_bounds__(64 * NW) attention_kernel(AttnArgs a) {
         }
     }
     __syncthreads();
-    half8 qh[X::CT][X::QS], ql[X::CT][X::QS];
+    // A row's operands: in registers for 16 rows, else read from LDS for each set of keys (64 registers
+    // of heads of 128: without them two waves share a SIMD, one's products beside the other's softmax).
+    half8 qh[X::SMALL ? X::QS : 1], ql[X::SMALL ? X::QS : 1];
+    const _Float16* qrow[X::CT];
     float fr[X::CT];
     int32_t last[X::CT];
 #pragma unroll
@@ -724,11 +728,17 @@ __global__ void __launch_bounds__(64 * NW) attention_kernel(AttnArgs a) {
         const int32_t r = min(32 * ct + col, held - 1);  // (columns past the rows repeat the last)
         fr[ct] = fr_s[r];
         last[ct] = last_key(STEP ? 0 : (tile * R + r) / G);
+        qrow[ct] = qs + r * QR + (HD == 32 && X::SMALL ? 8 : 16) * grp;
+    }
+    auto query = [&](int ct, int s, int part) {  // step s of column tile ct's operand
+        const int32_t d = HD == 32 && X::SMALL ? 0 : (X::SMALL ? 64 : 32) * (s / 2) + 8 * (s % 2);
+        return *reinterpret_cast<const half8*>(qrow[ct] + part * R * QR + d);
+    };
+    if constexpr (X::SMALL) {
 #pragma unroll
         for (int s = 0; s < X::QS; ++s) {
-            const int32_t d = HD == 32 && X::SMALL ? 8 * grp : X::SMALL ? 64 * (s / 2) + 16 * grp + 8 * (s % 2) : 32 * (s / 2) + 16 * grp + 8 * (s % 2);
-            qh[ct][s] = *reinterpret_cast<const half8*>(qs + r * QR + d);
-            ql[ct][s] = *reinterpret_cast<const half8*>(qs + (R + r) * QR + d);
+            qh[s] = query(0, s, 0);
+            ql[s] = query(0, s, 1);
         }
     }
     if constexpr (STEP) {
@@ -769,31 +779,6 @@ __global__ void __launch_bounds__(64 * NW) attention_kernel(AttnArgs a) {
     for (int32_t ch = c0 + wave; ch < c1; ch += NW) {
         const int32_t next = min(ch + NW, c1 - 1);  // (past the end the last chunk again, unused)
         const float ks[2] = {sk[0], sk[1]}, vs[2] = {sv[0], sv[1]};
-        acc_t sc[2][X::CT][X::SMALL ? 2 : 1];
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int t = 0; t < (X::SMALL ? 2 : 1); ++t) {
-#pragma unroll
-                for (int ct = 0; ct < X::CT; ++ct)
-#pragma unroll
-                    for (int e = 0; e < X::OE; ++e) sc[h][ct][t][e] = 0.0f;
-#pragma unroll
-                for (int s = 0; s < X::QS; ++s) {
-                    const half8 k = to_half8<FMT>(half_of(kr[X::SMALL ? 2 * h + t : h][s / 2], s % 2));
-#pragma unroll
-                    for (int ct = 0; ct < X::CT; ++ct) {
-                        if constexpr (X::SMALL) {
-                            sc[h][ct][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql[ct][s], sc[h][ct][t], 0, 0, 0);
-                            sc[h][ct][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh[ct][s], sc[h][ct][t], 0, 0, 0);
-                        } else {
-                            sc[h][ct][t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, ql[ct][s], sc[h][ct][t], 0, 0, 0);
-                            sc[h][ct][t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qh[ct][s], sc[h][ct][t], 0, 0, 0);
-                        }
-                    }
-                }
-            }
-        load_keys(next);
         const bool masked = ch * CHUNK + CHUNK > n_all;
         if (FMT == KT_KV8_E4M3 && ch * CHUNK + CHUNK > n_keys) {  // tokens not held: bytes that may be NaNs
 #pragma unroll
@@ -807,20 +792,48 @@ __global__ void __launch_bounds__(64 * NW) attention_kernel(AttnArgs a) {
                         vr[db][s][w] &= held >= 4 ? 0xFFFFFFFFu : held <= 0 ? 0u : (1u << (8 * held)) - 1u;
                     }
         }
-        // the value scales 2^e mu of the two sets of 32 keys (past the last key the first's again)
-        float vs_h[2], ks_h[2], shift[2], unscale[2];
-        int32_t e_h[2], quiet[2];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h0 = 0; h0 < 2; h0 += X::J) {  // J sets of 32 keys at a time
+        if (X::J == 1 && ch * CHUNK + 32 * h0 >= n_keys) break;
+        acc_t sc[X::J][X::CT][X::SMALL ? 2 : 1];
+#pragma unroll
+        for (int j = 0; j < X::J; ++j)
+#pragma unroll
+            for (int t = 0; t < (X::SMALL ? 2 : 1); ++t) {
+#pragma unroll
+                for (int ct = 0; ct < X::CT; ++ct)
+#pragma unroll
+                    for (int e = 0; e < X::OE; ++e) sc[j][ct][t][e] = 0.0f;
+#pragma unroll
+                for (int s = 0; s < X::QS; ++s) {
+                    const half8 k = to_half8<FMT>(half_of(kr[X::SMALL ? 2 * (h0 + j) + t : h0 + j][s / 2], s % 2));
+#pragma unroll
+                    for (int ct = 0; ct < X::CT; ++ct) {
+                        if constexpr (X::SMALL) {
+                            sc[j][ct][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql[s], sc[j][ct][t], 0, 0, 0);
+                            sc[j][ct][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh[s], sc[j][ct][t], 0, 0, 0);
+                        } else {
+                            sc[j][ct][t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, query(ct, s, 1), sc[j][ct][t], 0, 0, 0);
+                            sc[j][ct][t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, query(ct, s, 0), sc[j][ct][t], 0, 0, 0);
+                        }
+                    }
+                }
+            }
+        if (h0 + X::J == 2) load_keys(next);
+        // the sets' value scales 2^e mu (past the last key the first's again)
+        float vs_h[X::J], ks_h[X::J], shift[X::J], unscale[X::J];
+        int32_t e_h[X::J], quiet[X::J];
+#pragma unroll
+        for (int h = 0; h < X::J; ++h) {
             const bool there = h == 0 || ch * CHUNK + 32 < n_keys;
-            ks_h[h] = there ? ks[h] : ks[0];
-            vs_h[h] = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, there ? vs[h] : vs[0])));
+            ks_h[h] = there ? ks[h0 + h] : ks[0];
+            vs_h[h] = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, there ? vs[h0 + h] : vs[0])));
             e_h[h] = static_cast<int32_t>(__builtin_bit_cast(uint32_t, vs_h[h]) >> 23 & 255) - 127;
         }
 #pragma unroll
-        for (int h = 0; h < 2; ++h)  // a NaN makes NaNs with any exponent: one that changes nothing for other rows
-            if (vs_h[h] != vs_h[h]) e_h[h] = vs_h[1 - h] == vs_h[1 - h] ? e_h[1 - h] : e_run > -1000 ? e_run : 0;
-        const int32_t e_max = max(e_h[0], e_h[1]);
+        for (int h = 0; h < X::J; ++h)  // a NaN makes NaNs with any exponent: one that changes nothing for other rows
+            if (vs_h[h] != vs_h[h]) e_h[h] = vs_h[X::J - 1 - h] == vs_h[X::J - 1 - h] ? e_h[X::J - 1 - h] : e_run > -1000 ? e_run : 0;
+        const int32_t e_max = max(e_h[0], e_h[X::J - 1]);
         if (e_max > e_run) {
             const float down = ldexpf(1.0f, max(e_run - e_max, -200));
 #pragma unroll
@@ -830,7 +843,7 @@ __global__ void __launch_bounds__(64 * NW) attention_kernel(AttnArgs a) {
             e_run = e_max;
         }
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < X::J; ++h) {
             const float mu = ldexpf(vs_h[h], -e_h[h]);
             quiet[h] = e_run - e_h[h];
             const int32_t in_exp = quiet[h] <= MOST_QUIET ? quiet[h] : 0;
@@ -838,18 +851,18 @@ __global__ void __launch_bounds__(64 * NW) attention_kernel(AttnArgs a) {
             shift[h] = static_cast<float>(in_exp) - __builtin_amdgcn_logf(mu) - WEIGHT_UP;
             unscale[h] = ldexpf(1.0f / mu, in_exp);
         }
-        half8 ph[2][X::CT][X::VL], pl[2][X::CT][X::VL];
+        half8 ph[X::J][X::CT][X::VL], pl[X::J][X::CT][X::VL];
 #pragma unroll
         for (int ct = 0; ct < X::CT; ++ct) {
-            const float f[2] = {ks_h[0] * fr[ct], ks_h[1] * fr[ct]};
-            float x[2][X::E], top = -INFINITY;
+            float x[X::J][X::E], f[X::J], top = -INFINITY;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
+            for (int h = 0; h < X::J; ++h) {
+                f[h] = ks_h[h] * fr[ct];
                 float most = -INFINITY;
 #pragma unroll
                 for (int i = 0; i < X::E; ++i) {
                     x[h][i] = X::SMALL ? sc[h][ct][X::SMALL ? i >> 2 : 0][X::SMALL ? i & 3 : i] : sc[h][ct][0][i];
-                    if (masked && ch * CHUNK + 32 * h + key_of(i) > last[ct]) x[h][i] = -INFINITY;
+                    if (masked && ch * CHUNK + 32 * (h0 + h) + key_of(i) > last[ct]) x[h][i] = -INFINITY;
                     most = fmaxf(most, x[h][i]);
                 }
                 top = fmaxf(top, most * f[h]);
@@ -865,7 +878,7 @@ __global__ void __launch_bounds__(64 * NW) attention_kernel(AttnArgs a) {
             const float at = m[ct] == -INFINITY ? 0.0f : m[ct];
             const bool huge = __ballot(fabsf(at) > HUGE_SCORE);  // (one-hot rows)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
+            for (int h = 0; h < X::J; ++h) {
                 if (huge) {
 #pragma unroll
                     for (int i = 0; i < X::E; ++i) x[h][i] = weight_of_huge(x[h][i], f[h], at, shift[h]);
@@ -877,7 +890,7 @@ __global__ void __launch_bounds__(64 * NW) attention_kernel(AttnArgs a) {
                 float sum = 0.0f;
 #pragma unroll
                 for (int i = 0; i < X::E; ++i) {
-                    if (masked && ch * CHUNK + 32 * h + key_of(i) > last[ct]) x[h][i] = 0.0f;
+                    if (masked && ch * CHUNK + 32 * (h0 + h) + key_of(i) > last[ct]) x[h][i] = 0.0f;
                     sum += x[h][i];
                 }
                 l[ct] += sum == 0.0f ? 0.0f : sum * unscale[h];  // (0 * NaN: a row that sees none of the block)
@@ -900,8 +913,8 @@ __global__ void __launch_bounds__(64 * NW) attention_kernel(AttnArgs a) {
 #pragma unroll
             for (int s = 0; s < X::VL; ++s)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const half8 v = to_half8<FMT>(half_of(vr[db][s], h));
+                for (int h = 0; h < X::J; ++h) {
+                    const half8 v = to_half8<FMT>(half_of(vr[db][s], h0 + h));
 #pragma unroll
                     for (int ct = 0; ct < X::CT; ++ct) {
                         if constexpr (X::SMALL) {
@@ -913,6 +926,7 @@ __global__ void __launch_bounds__(64 * NW) attention_kernel(AttnArgs a) {
                         }
                     }
                 }
+        }
         load_values(next);
         if constexpr (STEP) {
             if (holder && next == chunks - 1) patch();
