@@ -348,7 +348,10 @@ __device__ __forceinline__ void split2(const float (&v)[8], half8& hi, half8& lo
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const half2v h = __builtin_bit_cast(half2v, __builtin_amdgcn_cvt_pkrtz(v[2 * i], v[2 * i + 1]));
-        const half2v l = __builtin_bit_cast(half2v, __builtin_amdgcn_cvt_pkrtz(fmaf(static_cast<float>(h[0]), -1.0f, v[2 * i]), fmaf(static_cast<float>(h[1]), -1.0f, v[2 * i + 1])));
+        float a, b;  // what is left of the two: one mixed multiply-add each (the compiler converts and subtracts)
+        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(a) : "v"(h), "v"(v[2 * i]));
+        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(b) : "v"(h), "v"(v[2 * i + 1]));
+        const half2v l = __builtin_bit_cast(half2v, __builtin_amdgcn_cvt_pkrtz(a, b));
         hi[2 * i] = h[0];
         hi[2 * i + 1] = h[1];
         lo[2 * i] = l[0];
@@ -776,11 +779,12 @@ __global__ void __launch_bounds__(64 * NW, R > 16 ? 2 : 1) attention_kernel(Attn
     }
     int32_t e_run = -1000;
 
-    for (int32_t ch = c0 + wave; ch < c1; ch += NW) {
+    // (two forms of the loop's body: only chunks that not every row sees whole compare keys with rows)
+    auto attend_chunk = [&](auto masked_form, const int32_t ch) {
+        constexpr bool masked = decltype(masked_form)::value;
         const int32_t next = min(ch + NW, c1 - 1);  // (past the end the last chunk again, unused)
         const float ks[2] = {sk[0], sk[1]}, vs[2] = {sv[0], sv[1]};
-        const bool masked = ch * CHUNK + CHUNK > n_all;
-        if (FMT == KT_KV8_E4M3 && ch * CHUNK + CHUNK > n_keys) {  // tokens not held: bytes that may be NaNs
+        if (masked && FMT == KT_KV8_E4M3 && ch * CHUNK + CHUNK > n_keys) {  // tokens not held: bytes that may be NaNs
 #pragma unroll
             for (int db = 0; db < X::DB; ++db)
 #pragma unroll
@@ -794,7 +798,7 @@ __global__ void __launch_bounds__(64 * NW, R > 16 ? 2 : 1) attention_kernel(Attn
         }
 #pragma unroll
         for (int h0 = 0; h0 < 2; h0 += X::J) {  // J sets of 32 keys at a time
-        if (X::J == 1 && ch * CHUNK + 32 * h0 >= n_keys) break;
+        if (masked && X::J == 1 && ch * CHUNK + 32 * h0 >= n_keys) break;
         acc_t sc[X::J][X::CT][X::SMALL ? 2 : 1];
 #pragma unroll
         for (int j = 0; j < X::J; ++j)
@@ -825,7 +829,7 @@ __global__ void __launch_bounds__(64 * NW, R > 16 ? 2 : 1) attention_kernel(Attn
         int32_t e_h[X::J], quiet[X::J];
 #pragma unroll
         for (int h = 0; h < X::J; ++h) {
-            const bool there = h == 0 || ch * CHUNK + 32 < n_keys;
+            const bool there = !masked || h == 0 || ch * CHUNK + 32 < n_keys;
             ks_h[h] = there ? ks[h0 + h] : ks[0];
             vs_h[h] = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, there ? vs[h0 + h] : vs[0])));
             e_h[h] = static_cast<int32_t>(__builtin_bit_cast(uint32_t, vs_h[h]) >> 23 & 255) - 127;
@@ -931,7 +935,10 @@ __global__ void __launch_bounds__(64 * NW, R > 16 ? 2 : 1) attention_kernel(Attn
         if constexpr (STEP) {
             if (holder && next == chunks - 1) patch();
         }
-    }
+    };
+    int32_t ch = c0 + wave;
+    for (; ch < c1 && ch * CHUNK + CHUNK <= n_all; ch += NW) attend_chunk(std::false_type{}, ch);
+    for (; ch < c1; ch += NW) attend_chunk(std::true_type{}, ch);
 
     // each wave's averages, maxima and sums, then all waves' through LDS
     const int32_t used = min(NW, c1 - c0);  // waves with keys
