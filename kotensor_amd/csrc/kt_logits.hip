@@ -16,8 +16,9 @@ namespace kt {
 namespace {
 
 constexpr int THREADS = 256;
-constexpr int SEGMENT = 4096;  // logits of a workgroup
 typedef float f4 __attribute__((ext_vector_type(4)));
+typedef int32_t i4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
 struct LogitsArgs {
     const float* logits;
@@ -27,50 +28,109 @@ struct LogitsArgs {
     kt_logits_controls c;
 };
 
-// Workgroup (segment, row): counts the text's tokens of its segment in LDS, by integer
-// atomics, whose order changes nothing, then reads, changes and writes its logits once. Of a token
-// biased twice the later entry holds (the largest entry index).
+// Workgroup (segment of 1024 VECS logits, row): its logits go into registers first; meanwhile it counts the text's
+// tokens of its segment in LDS, by integer atomics, whose order changes nothing; then it changes and writes
+// each logit once. Every workgroup of a row reads the row's whole text, from L2 after the first.
+// Of a token biased twice the later entry holds (the largest entry index).
+template <int VECS>
 __global__ void __launch_bounds__(THREADS) process_kernel(LogitsArgs a) {
-    __shared__ uint32_t marks[SEGMENT];  // occurrences from output_start on; the top bit: any
-    __shared__ int32_t entry[SEGMENT];   // the token's bias, or -1
+    constexpr int SEGMENT = 4 * THREADS * VECS;
+    __shared__ __attribute__((aligned(16))) uint32_t marks[SEGMENT];  // occurrences from output_start on; the top bit: any
+    extern __shared__ __attribute__((aligned(16))) int32_t entry[];   // [SEGMENT] with biases: the token's, or -1
     const kt_logits_controls& c = a.c;
     const int32_t r = blockIdx.y, first = blockIdx.x * SEGMENT, count = min(SEGMENT, a.n - first), tid = threadIdx.x;
     const bool biased = c.bias_count > 0;
-    if (a.text) for (int32_t i = tid; i < count; i += THREADS) marks[i] = 0;
-    if (biased) for (int32_t i = tid; i < count; i += THREADS) entry[i] = -1;
-    __syncthreads();
-    if (a.text) {
-        const int32_t* text = c.history + r * c.history_stride;
-        const int64_t length = min(max(static_cast<int64_t>(c.history_length[r]) + c.length_offset, int64_t{0}), static_cast<int64_t>(c.history_capacity));
-        const int32_t start = c.output_start ? c.output_start[r] : 0;
-        for (int64_t i = tid; i < length; i += THREADS) {
-            const uint32_t at = static_cast<uint32_t>(text[i]) - static_cast<uint32_t>(first);
-            if (text[i] < 0 || at >= static_cast<uint32_t>(count)) continue;
-            atomicOr(&marks[at], 0x80000000u);
-            if (i >= start) atomicAdd(&marks[at], 1u);
-        }
-    }
-    if (biased) {
-        const int32_t* tokens = c.bias_tokens + r * c.bias_stride;
-        for (int64_t i = tid; i < c.bias_count; i += THREADS) {
-            const uint32_t at = static_cast<uint32_t>(tokens[i]) - static_cast<uint32_t>(first);
-            if (tokens[i] >= 0 && at < static_cast<uint32_t>(count)) atomicMax(&entry[at], static_cast<int32_t>(i));
-        }
-    }
-    __syncthreads();
     const float* x = a.logits + r * a.stride + first;
     float* y = a.out + r * a.out_stride + first;
-    for (int32_t i = tid; i < count; i += THREADS) {
-        float v = x[i];
-        if (a.text && marks[i]) {
-            v = v > 0.0f ? v / c.repetition : v * c.repetition;
-            const uint32_t o = marks[i] & 0x7FFFFFFFu;
-            if (o) v -= static_cast<float>(o) * c.frequency + c.presence;
+    // (four logits at 4 (tid + 256 u); rows may begin at any float. A group that the row ends in goes one by one.)
+    f4 v[VECS];
+#pragma unroll
+    for (int u = 0; u < VECS; ++u) {
+        const int32_t at = 4 * (tid + u * THREADS);
+        v[u] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (at + 4 <= count) {
+            v[u] = load_any<f4>(x + at);
+        } else {
+            for (int i = 0; i < 4; ++i)
+                if (at + i < count) v[u][i] = x[at + i];
         }
-        if (biased && entry[i] >= 0) v += c.bias_values[r * c.bias_stride + entry[i]];
-        if (a.mask && !(c.allowed[r * c.allowed_stride + ((first + i) >> 5)] >> ((first + i) & 31) & 1u)) v = -INFINITY;
-        y[i] = v;
     }
+    if (a.text || biased) {
+#pragma unroll
+        for (int u = 0; u < VECS; ++u) {
+            reinterpret_cast<u4*>(marks)[tid + u * THREADS] = u4{0u, 0u, 0u, 0u};
+            if (biased) reinterpret_cast<i4*>(entry)[tid + u * THREADS] = i4{-1, -1, -1, -1};
+        }
+        __syncthreads();
+        if (a.text) {
+            const int32_t* text = c.history + r * c.history_stride;
+            const int64_t length = min(max(static_cast<int64_t>(c.history_length[r]) + c.length_offset, int64_t{0}), static_cast<int64_t>(c.history_capacity));
+            const int32_t start = c.output_start ? c.output_start[r] : 0;
+            auto mark = [&](int32_t token, int64_t i) {
+                const uint32_t at = static_cast<uint32_t>(token) - static_cast<uint32_t>(first);
+                if (token < 0 || at >= static_cast<uint32_t>(count)) return;
+                atomicOr(&marks[at], 0x80000000u);
+                if (i >= start) atomicAdd(&marks[at], 1u);
+            };
+            const int64_t whole = length / 4;
+            for (int64_t i = tid; i < whole; i += THREADS) {
+                const i4 t = load_any<i4>(text + 4 * i);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) mark(t[e], 4 * i + e);
+            }
+            if (tid < length - 4 * whole) mark(text[4 * whole + tid], 4 * whole + tid);
+        }
+        if (biased) {
+            const int32_t* tokens = c.bias_tokens + r * c.bias_stride;
+            for (int64_t i = tid; i < c.bias_count; i += THREADS) {
+                const uint32_t at = static_cast<uint32_t>(tokens[i]) - static_cast<uint32_t>(first);
+                if (tokens[i] >= 0 && at < static_cast<uint32_t>(count)) atomicMax(&entry[at], static_cast<int32_t>(i));
+            }
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int u = 0; u < VECS; ++u) {
+        const int32_t at = 4 * (tid + u * THREADS);
+        if (at >= count) break;
+        if (a.text) {
+            const u4 m = reinterpret_cast<const u4*>(marks)[tid + u * THREADS];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (!m[e]) continue;
+                v[u][e] = v[u][e] > 0.0f ? v[u][e] / c.repetition : v[u][e] * c.repetition;
+                const uint32_t o = m[e] & 0x7FFFFFFFu;
+                if (o) v[u][e] -= static_cast<float>(o) * c.frequency + c.presence;
+            }
+        }
+        if (biased) {
+            const i4 b = reinterpret_cast<const i4*>(entry)[tid + u * THREADS];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (b[e] >= 0) v[u][e] += c.bias_values[r * c.bias_stride + b[e]];
+        }
+        if (a.mask) {
+            const uint32_t bits = c.allowed[r * c.allowed_stride + ((first + at) >> 5)] >> ((first + at) & 31);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (!(bits >> e & 1u)) v[u][e] = -INFINITY;
+        }
+        if (at + 4 <= count) {
+            __builtin_memcpy(y + at, &v[u], sizeof(f4));
+        } else {
+            for (int i = 0; i < 4; ++i)
+                if (at + i < count) y[at + i] = v[u][i];
+        }
+    }
+}
+
+template <int VECS>
+int32_t launch(const LogitsArgs& a, int32_t rows, hipStream_t st) {
+    constexpr int SEGMENT = 4 * THREADS * VECS;
+    process_kernel<VECS><<<dim3(static_cast<uint32_t>((a.n - 1) / SEGMENT + 1), static_cast<uint32_t>(rows)), THREADS,
+                           a.c.bias_count > 0 ? SEGMENT * sizeof(int32_t) : 0, st>>>(a);
+    KT_LAUNCHED("logits kernel");
+    return KT_OK;
 }
 
 }  // namespace
@@ -104,9 +164,11 @@ int32_t kt_process_logits(const float* logits, int32_t rows, int32_t n, int64_t 
         return fail(KT_ERR_SHAPE, "a mask of %d tokens does not fit its stride", n);
     if (rows == 0) return KT_OK;
     LogitsArgs a{logits, out, stride, out_stride, n, text, c.allowed != nullptr, c};
-    process_kernel<<<dim3(static_cast<uint32_t>((n - 1) / SEGMENT + 1), static_cast<uint32_t>(rows)), THREADS, 0, static_cast<hipStream_t>(stream)>>>(a);
-    KT_LAUNCHED("logits kernel");
-    return KT_OK;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    // short segments while they fit the card at once, long ones (fewer readings of the text) beyond
+    const int64_t short_ones = (static_cast<int64_t>(n - 1) / 1024 + 1) * rows;
+    if (short_ones <= 2 * cu_count()) return launch<1>(a, rows, st);
+    return launch<2>(a, rows, st);
 }
 
 }  // extern "C"
