@@ -21,10 +21,15 @@
 #include <type_traits>
 
 #include "kt_common.h"
+#include "kt_split.h"
 #include "kt_wave.h"
 
 namespace kt {
 namespace {
+
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 
 constexpr int THREADS = 256;
 constexpr int CHUNK = 64;  // tokens whose values lie together
@@ -133,6 +138,7 @@ __device__ __forceinline__ int32_t value_byte(int32_t quad) {
 // The first block's earlier rows come from the fp32 rows of the open block, which the last
 // block's rows replace: where the first block has earlier rows, one workgroup does both, in
 // that order.
+constexpr int Q_HEADS = 8;
 struct AppendArgs {
     KV8View c;
     const float* q;
@@ -165,38 +171,64 @@ __device__ void append_block(const AppendArgs& a, float* lds, uint32_t (&part)[T
     float* rows = (KEYS ? c.key_rows : c.value_rows) + static_cast<size_t>(g) * B * HD;
     const int32_t t0 = b * B - p0;  // token of row 0 in this call
     const bool open = n < B;
+    float* scale = (KEYS ? c.key_scales : c.value_scales) + static_cast<size_t>(g) * (c.slots / B) + b;
+    const float held = lo > 0 ? *scale : 0.0f;
     uint32_t m = 0;
+    constexpr int AHEAD = 4;  // pairs, or groups of four values, a thread loads at a time
     if constexpr (KEYS) {
-        const int32_t half = HD >> 1;
-        for (int32_t e = tid; e < (n - lo) * half; e += THREADS) {
-            const int32_t r = lo + e / half, i = e % half;
-            const float* src = a.k + (static_cast<size_t>(t0 + r) * c.kv_heads + g) * HD + i;
-            float cf, sf, y1, y2;
-            rope_cos_sin(b * B + r, a.inv_freq[i], cf, sf);
-            rope_apply(src[0], src[half], cf, sf, y1, y2);
-            lds[r * LR + i] = y1;
-            lds[r * LR + i + half] = y2;
-            m = max(m, max(magnitude(y1), magnitude(y2)));
-            if (open) {
-                rows[r * HD + i] = y1;
-                rows[r * HD + i + half] = y2;
+        const int32_t half = HD >> 1, pairs = (n - lo) * half;
+        for (int32_t e0 = tid; e0 < pairs; e0 += AHEAD * THREADS) {
+            float x1[AHEAD], x2[AHEAD], f[AHEAD];
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) {
+                const int32_t e = min(e0 + u * THREADS, pairs - 1), r = lo + e / half, i = e % half;
+                const float* src = a.k + (static_cast<size_t>(t0 + r) * c.kv_heads + g) * HD + i;
+                x1[u] = src[0];
+                x2[u] = src[half];
+                f[u] = a.inv_freq[i];
+            }
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) {
+                const int32_t e = e0 + u * THREADS, r = lo + e / half, i = e % half;
+                if (e >= pairs) break;
+                float cf, sf, y1, y2;
+                rope_sin_cos(b * B + r, f[u], cf, sf);
+                rope_apply(x1[u], x2[u], cf, sf, y1, y2);
+                lds[r * LR + i] = y1;
+                lds[r * LR + i + half] = y2;
+                m = max(m, max(magnitude(y1), magnitude(y2)));
+                if (open) {
+                    rows[r * HD + i] = y1;
+                    rows[r * HD + i + half] = y2;
+                }
             }
         }
     } else {
-        for (int32_t e = tid; e < (n - lo) * HD; e += THREADS) {
-            const int32_t r = lo + e / HD, d = e % HD;
-            const float y = a.v[(static_cast<size_t>(t0 + r) * c.kv_heads + g) * HD + d];
-            lds[r * LR + d] = y;
-            m = max(m, magnitude(y));
-            if (open) rows[r * HD + d] = y;
+        const int32_t quads = (n - lo) * (HD / 4);
+        for (int32_t e0 = tid; e0 < quads; e0 += AHEAD * THREADS) {
+            f4 y[AHEAD];
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) {
+                const int32_t e = min(e0 + u * THREADS, quads - 1), r = lo + e / (HD / 4), d = 4 * (e % (HD / 4));
+                y[u] = load_any<f4>(a.v + (static_cast<size_t>(t0 + r) * c.kv_heads + g) * HD + d);
+            }
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) {
+                const int32_t e = e0 + u * THREADS, r = lo + e / (HD / 4), d = 4 * (e % (HD / 4));
+                if (e >= quads) break;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    lds[r * LR + d + i] = y[u][i];
+                    m = max(m, magnitude(y[u][i]));
+                }
+                if (open) *reinterpret_cast<f4*>(rows + r * HD + d) = y[u];
+            }
         }
     }
     m = block_max(m, part);
-    float* scale = (KEYS ? c.key_scales : c.value_scales) + static_cast<size_t>(g) * (c.slots / B) + b;
     float s = scale_of<FMT>(m);
     int32_t from = lo;
     if (lo > 0) {
-        const float held = *scale;
         if (held != held || held >= s) {
             s = held;
         } else if (s == s) {  // raised: the earlier rows again
@@ -204,7 +236,7 @@ __device__ void append_block(const AppendArgs& a, float* lds, uint32_t (&part)[T
             for (int32_t e = tid; e < lo * HD; e += THREADS) lds[e / HD * LR + e % HD] = rows[e];
         }
     }
-    __syncthreads();  // the rows are in LDS, the held scale is read
+    __syncthreads();  // the rows are in LDS, every thread has read the held scale
     if (tid == 0) *scale = s;
     const float inv = s == s ? 1.0f / s : 0.0f;
     auto at = [&](int32_t r, int32_t d) { return s == s ? lds[r * LR + d] * inv : 0.0f; };
@@ -260,18 +292,27 @@ __global__ void __launch_bounds__(THREADS) append_kernel(AppendArgs a) {
             __syncthreads();  // the first block's rows are read
         }
     }
-    // q: a thread's pair of a token, all heads
-    const int32_t half = HD >> 1, per = THREADS / half;
-    const int32_t i = threadIdx.x % half, t = (id - roles) * per + threadIdx.x / half;
+    // q: a thread's pair of a token, Q_HEADS heads whose loads go out together
+    const int32_t half = HD >> 1, per = THREADS / half, groups = (a.num_heads + Q_HEADS - 1) / Q_HEADS;
+    id -= roles;
+    const int32_t i = threadIdx.x % half, t = id / groups * per + threadIdx.x / half, h0 = id % groups * Q_HEADS;
     if (t >= a.tokens) return;
-    float cf, sf;
-    rope_cos_sin(p0 + t, a.inv_freq[i], cf, sf);
     const size_t row = static_cast<size_t>(t) * a.num_heads * HD + i;
-    for (int32_t h = 0; h < a.num_heads; ++h) {
+    float x1[Q_HEADS], x2[Q_HEADS], cf, sf;
+#pragma unroll
+    for (int u = 0; u < Q_HEADS; ++u) {
+        const size_t at = row + static_cast<size_t>(min(h0 + u, a.num_heads - 1)) * HD;
+        x1[u] = a.q[at];
+        x2[u] = a.q[at + half];
+    }
+    rope_sin_cos(p0 + t, a.inv_freq[i], cf, sf);
+#pragma unroll
+    for (int u = 0; u < Q_HEADS; ++u) {
+        if (h0 + u >= a.num_heads) break;
         float y1, y2;
-        rope_apply(a.q[row + h * HD], a.q[row + h * HD + half], cf, sf, y1, y2);
-        a.q_out[row + h * HD] = y1;
-        a.q_out[row + h * HD + half] = y2;
+        rope_apply(x1[u], x2[u], cf, sf, y1, y2);
+        a.q_out[row + (h0 + u) * HD] = y1;
+        a.q_out[row + (h0 + u) * HD + half] = y2;
     }
 }
 
@@ -290,10 +331,7 @@ __global__ void __launch_bounds__(THREADS) append_kernel(AppendArgs a) {
 // weights include it, and the sum of weights takes it out again, with one product a set of 32 keys.
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
-typedef float f4 __attribute__((ext_vector_type(4)));
 typedef float f16v __attribute__((ext_vector_type(16)));
-typedef uint32_t u4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 
 struct AttnArgs {
     // (what the first loads need comes first: it arrives with the wave)
@@ -1083,46 +1121,62 @@ __global__ void __launch_bounds__(64 * NW, R > 16 ? 2 : 1) attention_kernel(Attn
 }
 
 // ---- rows as fp32, and the copy of a prefix ------------------------------------------------
-// Workgroup (chunk, kv head, keys or values): the chunk's rows in [first, first + count) as
-// code * scale; the values turn through LDS.
+// Workgroup (chunk, kv head, 64 dims of the keys or of the values): the chunk's rows in [first, first + count) as code *
+// scale, sixteen codes a thread; the values turn through LDS. One memory round trip and the stores.
 template <int FMT>
 __global__ void __launch_bounds__(THREADS) read_kernel(KV8View c, int32_t first, int32_t count, float* keys, float* values) {
     __shared__ float turned[CHUNK][65];
-    const int32_t HD = c.head_dim, g = blockIdx.y, tid = threadIdx.x;
+    const int32_t HD = c.head_dim, g = blockIdx.y, tid = threadIdx.x, d0 = blockIdx.z / 2 * 64, nd = min(64, HD - d0);
     const int32_t tok0 = (first / CHUNK + static_cast<int32_t>(blockIdx.x)) * CHUNK;
-    const bool is_key = blockIdx.z == 0;
+    const bool is_key = blockIdx.z % 2 == 0;
     float* out = is_key ? keys : values;
     if (!out) return;
-    out += static_cast<size_t>(g) * count * HD;
+    out += static_cast<size_t>(g) * count * HD + d0;
     const float* scales = (is_key ? c.key_scales : c.value_scales) + static_cast<size_t>(g) * (c.slots / c.block);
     const uint8_t* src = (is_key ? c.keys : c.values) + (static_cast<size_t>(g) * c.slots + tok0) * HD;
     auto inside = [&](int32_t tok) { return tok >= first && tok < first + count; };
     if (is_key) {
-        for (int32_t e = tid; e < CHUNK * HD / 4; e += THREADS) {
-            const int32_t r = e / (HD / 4), d = 4 * (e % (HD / 4)), tok = tok0 + r;
-            if (!inside(tok)) continue;
+        const int32_t per = nd / 16, r = tid / per, d = 16 * (tid % per), tok = tok0 + r;
+        if (r >= CHUNK || !inside(tok)) return;
+        const u4 w = *reinterpret_cast<const u4*>(src + r * HD + d0 + d);
+        const float s = scales[tok / c.block];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
             float x[4];
-            decode4<FMT>(reinterpret_cast<const uint32_t*>(src)[e], x);
-            const float s = scales[tok / c.block];
-            *reinterpret_cast<float4*>(out + static_cast<size_t>(tok - first) * HD + d) = make_float4(x[0] * s, x[1] * s, x[2] * s, x[3] * s);
+            decode4<FMT>(w[i], x);
+            *reinterpret_cast<float4*>(out + static_cast<size_t>(tok - first) * HD + d + 4 * i) = make_float4(x[0] * s, x[1] * s, x[2] * s, x[3] * s);
         }
         return;
     }
-    for (int32_t d0 = 0; d0 < HD; d0 += 64) {  // 64 dims at a time
-        const int32_t nd = min(64, HD - d0);
-        for (int32_t e = tid; e < nd * 16; e += THREADS) {
-            const int32_t quad = e % 16, d = e / 16;
-            float x[4];
-            decode4<FMT>(*reinterpret_cast<const uint32_t*>(src + (d0 + d) * CHUNK + value_byte(quad)), x);
+    constexpr int OUT = 4;  // groups of four dims a thread writes: 64 x 16 of them
+    const int32_t groups = nd / 4;
+    float s[OUT];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) turned[4 * quad + i][d] = x[i];
+    for (int u = 0; u < OUT; ++u) {
+        const int32_t tok = tok0 + min((tid + u * THREADS) / groups, CHUNK - 1);
+        s[u] = inside(tok) ? scales[tok / c.block] : 0.0f;
+    }
+    if (tid < 4 * nd) {  // (dim, piece)
+        const int32_t d = tid / 4, piece = tid % 4;
+        const u4 w = *reinterpret_cast<const u4*>(src + (d0 + d) * CHUNK + 16 * piece);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {  // four tokens from 32 (i / 2) + 16 (piece / 2) + 8 (i % 2) + 4 (piece % 2)
+            float x[4];
+            decode4<FMT>(w[i], x);
+            const int32_t t = 32 * (i >> 1) + 16 * (piece >> 1) + 8 * (i & 1) + 4 * (piece & 1);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) turned[t + e][d] = x[e];
         }
-        __syncthreads();
-        for (int32_t e = tid; e < CHUNK * nd; e += THREADS) {
-            const int32_t tok = tok0 + e / nd, d = e % nd;
-            if (inside(tok)) out[static_cast<size_t>(tok - first) * HD + d0 + d] = turned[e / nd][d] * scales[tok / c.block];
-        }
-        __syncthreads();
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < OUT; ++u) {
+        const int32_t e = tid + u * THREADS, r = e / groups, d = 4 * (e % groups), tok = tok0 + r;
+        if (r >= CHUNK || !inside(tok)) continue;
+        f4 x;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = turned[r][d + i] * s[u];
+        __builtin_memcpy(out + static_cast<size_t>(tok - first) * HD + d, &x, sizeof(x));
     }
 }
 
@@ -1192,7 +1246,8 @@ int32_t append_args(const float* q, const float* k, const float* v, int32_t toke
 
 int32_t launch_append(const AppendArgs& a, hipStream_t st) {
     const int32_t per = THREADS / (a.c.head_dim / 2);
-    const int64_t grid = static_cast<int64_t>(a.blocks) * a.c.kv_heads * 2 + (a.q ? (a.tokens + per - 1) / per : 0);
+    const int64_t grid = static_cast<int64_t>(a.blocks) * a.c.kv_heads * 2 +
+                         (a.q ? static_cast<int64_t>((a.tokens + per - 1) / per) * ((a.num_heads + Q_HEADS - 1) / Q_HEADS) : 0);
     if (grid > INT32_MAX) return fail(KT_ERR_SHAPE, "too many tokens and heads in one call");
     const size_t lds = static_cast<size_t>(a.c.block) * (a.c.head_dim + 1) * sizeof(float);
     if (lds > (64u << 10)) {  // beyond the default dynamic LDS limit (160 KB per CU on gfx950)
@@ -1351,7 +1406,7 @@ int32_t kt_kv8_read(const kt_kv8_cache* cache, int32_t layer, int32_t first, int
     if (first < 0 || count < 0 || count > c.max_seq - first) return fail(KT_ERR_RANGE, "tokens %d + %d out of bounds %d", first, count, c.max_seq);
     if (!aligned(keys, 16)) return fail(KT_ERR_ARGUMENT, "keys must be 16-byte aligned");
     if (count == 0 || (!keys && !values)) return KT_OK;
-    const dim3 grid(static_cast<uint32_t>((first + count - 1) / CHUNK - first / CHUNK + 1), static_cast<uint32_t>(c.kv_heads), 2);
+    const dim3 grid(static_cast<uint32_t>((first + count - 1) / CHUNK - first / CHUNK + 1), static_cast<uint32_t>(c.kv_heads), 2u * static_cast<uint32_t>(ceil_div(c.head_dim, 64)));
     const auto kernel = c.fmt == KT_KV8_INT8 ? read_kernel<KT_KV8_INT8> : read_kernel<KT_KV8_E4M3>;
     kernel<<<grid, THREADS, 0, static_cast<hipStream_t>(stream)>>>(c, first, count, keys, values);
     KT_LAUNCHED("8-bit cache read kernel");

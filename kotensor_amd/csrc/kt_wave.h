@@ -46,6 +46,13 @@ __device__ __forceinline__ void rope_cos_sin(int32_t pos, float inv_freq_i, floa
     c = rope_cos(pos, inv_freq_i);
     s = rope_sin(pos, inv_freq_i);
 }
+// The same by one argument reduction for both.
+__device__ __forceinline__ void rope_sin_cos(int32_t pos, float inv_freq_i, float& c, float& s) {
+    double cd, sd;
+    sincos(static_cast<double>(static_cast<float>(pos) * inv_freq_i), &sd, &cd);
+    c = static_cast<float>(cd);
+    s = static_cast<float>(sd);
+}
 __device__ __forceinline__ void rope_apply(float x1, float x2, float c, float s, float& y1, float& y2) {
 #pragma clang fp contract(off)
     y1 = x1 * c - x2 * s;
