@@ -461,6 +461,7 @@ struct Shape {
     static constexpr int DB = SMALL ? HD / 16 : HD / 32;  // dim blocks of the output
     static constexpr int VL = SMALL ? 1 : 2;              // 16-byte loads of a dim
     static constexpr int OE = SMALL ? 4 : 16;
+    static constexpr bool QREG = SMALL && HD < 256;       // a row's operands stay in registers
     static constexpr int J = SMALL ? 2 : 1;               // sets of 32 keys that share a maximum's check
 };
 
@@ -758,9 +759,9 @@ __global__ void __launch_bounds__(64 * NW, R > 16 ? 2 : 1) attention_kernel(Attn
         }
     }
     __syncthreads();
-    // A row's operands: in registers for 16 rows, else read from LDS for each set of keys (64 registers
+    // A row's operands: in registers for 16 rows of up to 128 dims, else read from LDS for each set of keys (64 registers
     // of heads of 128: without them two waves share a SIMD, one's products beside the other's softmax).
-    half8 qh[X::SMALL ? X::QS : 1], ql[X::SMALL ? X::QS : 1];
+    half8 qh[X::QREG ? X::QS : 1], ql[X::QREG ? X::QS : 1];
     const _Float16* qrow[X::CT];
     float fr[X::CT];
     int32_t last[X::CT];
@@ -775,7 +776,7 @@ __global__ void __launch_bounds__(64 * NW, R > 16 ? 2 : 1) attention_kernel(Attn
         const int32_t d = HD == 32 && X::SMALL ? 0 : (X::SMALL ? 64 : 32) * (s / 2) + 8 * (s % 2);
         return *reinterpret_cast<const half8*>(qrow[ct] + part * R * QR + d);
     };
-    if constexpr (X::SMALL) {
+    if constexpr (X::QREG) {
 #pragma unroll
         for (int s = 0; s < X::QS; ++s) {
             qh[s] = query(0, s, 0);
@@ -852,8 +853,8 @@ __global__ void __launch_bounds__(64 * NW, R > 16 ? 2 : 1) attention_kernel(Attn
 #pragma unroll
                     for (int ct = 0; ct < X::CT; ++ct) {
                         if constexpr (X::SMALL) {
-                            sc[j][ct][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql[s], sc[j][ct][t], 0, 0, 0);
-                            sc[j][ct][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh[s], sc[j][ct][t], 0, 0, 0);
+                            sc[j][ct][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, X::QREG ? ql[X::QREG ? s : 0] : query(ct, s, 1), sc[j][ct][t], 0, 0, 0);
+                            sc[j][ct][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, X::QREG ? qh[X::QREG ? s : 0] : query(ct, s, 0), sc[j][ct][t], 0, 0, 0);
                         } else {
                             sc[j][ct][t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, query(ct, s, 1), sc[j][ct][t], 0, 0, 0);
                             sc[j][ct][t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, query(ct, s, 0), sc[j][ct][t], 0, 0, 0);
@@ -1006,41 +1007,30 @@ __global__ void __launch_bounds__(64 * NW, R > 16 ? 2 : 1) attention_kernel(Attn
     __syncthreads();
     const size_t part = ((static_cast<size_t>(g) * gridDim.y + tile) * a.max_splits + split) * R;
     const __amdgpu_buffer_rsrc_t averages = __builtin_amdgcn_make_buffer_rsrc(a.averages + part * HD, 0, R * HD * 4, 0x00020000);
-    // thread (wave w's part of row r): its weight among the row's parts, in the place of its sum
-    float by = 0.0f, mx = -INFINITY, sum = 0.0f;
-    const int32_t wr = tid % R, ww = tid / R;
-    static_assert(64 * NW >= R * NW, "a thread for each part of a row");
-    const bool weighs = ww < used && wr < held;
-    if (weighs) {
-        for (int32_t w = 0; w < used; ++w) mx = fmaxf(mx, ms[w * R + wr]);
-        for (int32_t w = 0; w < used; ++w) {
-            const float share = share_of(ms[w * R + wr], ls[w * R + wr], mx);
-            sum += share;
-            by = w == ww ? share : by;
-        }
-        by = sum == 0.0f ? 0.0f : by / sum;
-    }
-    __syncthreads();
-    if (weighs) ls[ww * R + wr] = by;
-    if (splits > 1 && tid < held) {
-        const u2 both = {__builtin_bit_cast(uint32_t, mx), __builtin_bit_cast(uint32_t, sum)};
-        __hip_atomic_store(reinterpret_cast<uint64_t*>(a.stats) + part + tid, __builtin_bit_cast(uint64_t, both), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
-    }
-    __syncthreads();
-    for (int32_t e = tid; e < held * (HD / 4); e += 64 * NW) {
+    for (int32_t e = tid; e < held * (HD / 4); e += 64 * NW) {  // (every thread weighs its row's parts itself: no further barrier)
         const int32_t r = e / (HD / 4), d = 4 * (e % (HD / 4)), row = tile * R + r;
+        float mx = -INFINITY, sum = 0.0f;
         f4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int32_t w = 0; w < used; ++w) mx = fmaxf(mx, ms[w * R + r]);
         for (int32_t w = 0; w < used; ++w) {
-            const float y = ls[w * R + r];
+            const float by = share_of(ms[w * R + r], ls[w * R + r], mx);
             const f4 v = *reinterpret_cast<const f4*>(avg + (w * R + r) * LR + d);
+            sum += by;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = fmaf(y, v[i], x[i]);
+            for (int i = 0; i < 4; ++i) x[i] = fmaf(by, v[i], x[i]);
         }
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] *= inv;
         if (splits == 1) {
             const int32_t t = STEP ? 0 : row / G;
             *reinterpret_cast<f4*>(a.context + (static_cast<size_t>(t) * a.num_heads + g * G + (row - t * G)) * HD + d) = x;
         } else {  // written through to memory: the reader may be on another die
             __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, x), averages, (r * HD + d) * 4, 0, THROUGH);
+            if (d == 0) {
+                const u2 both = {__builtin_bit_cast(uint32_t, mx), __builtin_bit_cast(uint32_t, sum)};
+                __hip_atomic_store(reinterpret_cast<uint64_t*>(a.stats) + part + r, __builtin_bit_cast(uint64_t, both), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+            }
         }
     }
     if (splits == 1) return;
@@ -1061,6 +1051,19 @@ __global__ void __launch_bounds__(64 * NW, R > 16 ? 2 : 1) attention_kernel(Attn
     float* weight = attn_lds;                  // [R][MAX_SPLITS]
     float* total = weight + R * MAX_SPLITS;    // [R]
     f4* shares = reinterpret_cast<f4*>(total + R);  // [64 NW]
+    // thread (four dims of a row, phase): every phases-th split, eight loads in flight together, the first eight with the
+    // maxima and sums
+    constexpr int BATCH = 8;
+    const __amdgpu_buffer_rsrc_t all = __builtin_amdgcn_make_buffer_rsrc(a.averages + first * HD, 0, splits * R * HD * 4, 0x00020000);
+    const int32_t items = held * (HD / 4), phases = max(1, 64 * NW / items);
+    const int32_t phase = phases > 1 ? tid / items : 0;
+    u4 v[BATCH];
+    auto load_batch = [&](int32_t item, int32_t s0) {
+        const int32_t at = (min(item, items - 1) / (HD / 4)) * HD + 4 * (min(item, items - 1) % (HD / 4));
+#pragma unroll
+        for (int u = 0; u < BATCH; ++u) v[u] = __builtin_amdgcn_raw_buffer_load_b128(all, (min(s0 + u * phases, splits - 1) * R * HD + at) * 4, 0, THROUGH);
+    };
+    load_batch(phases > 1 ? tid % items : tid, phase);
     for (int32_t r = wave; r < held; r += NW) {  // a row's weights: lane = split
         float ml[MAX_SPLITS / 64], ll[MAX_SPLITS / 64], mx = -INFINITY, sum = 0.0f;
 #pragma unroll
@@ -1081,21 +1084,15 @@ __global__ void __launch_bounds__(64 * NW, R > 16 ? 2 : 1) attention_kernel(Attn
         if (lane == 0) total[r] = sum;
     }
     __syncthreads();
-    // thread (four dims of a row, phase): every phases-th split, their loads in flight together
-    const __amdgpu_buffer_rsrc_t all = __builtin_amdgcn_make_buffer_rsrc(a.averages + first * HD, 0, splits * R * HD * 4, 0x00020000);
-    const int32_t items = held * (HD / 4), phases = max(1, 64 * NW / items);
     for (int32_t i0 = 0; i0 < items; i0 += 64 * NW) {
-        const int32_t item = phases > 1 ? tid % items : i0 + tid, phase = phases > 1 ? tid / items : 0;
+        const int32_t item = phases > 1 ? tid % items : i0 + tid;
         const bool on = item < items && phase < phases;
         const int32_t r = min(item, items - 1) / (HD / 4), d = 4 * (min(item, items - 1) % (HD / 4));
         f4 x = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int32_t s0 = phase; on && s0 < splits; s0 += 8 * phases) {
-            u4 v[8];
+        for (int32_t s0 = phase; on && s0 < splits; s0 += BATCH * phases) {
+            if (i0 > 0 || s0 > phase) load_batch(item, s0);
 #pragma unroll
-            for (int u = 0; u < 8; ++u)
-                v[u] = __builtin_amdgcn_raw_buffer_load_b128(all, ((min(s0 + u * phases, splits - 1) * R + r) * HD + d) * 4, 0, THROUGH);
-#pragma unroll
-            for (int u = 0; u < 8; ++u) {
+            for (int u = 0; u < BATCH; ++u) {
                 const int32_t s = s0 + u * phases;
                 const float by = s < splits ? weight[r * MAX_SPLITS + s] : 0.0f;
                 const f4 y = __builtin_bit_cast(f4, v[u]);
@@ -1112,10 +1109,10 @@ __global__ void __launch_bounds__(64 * NW, R > 16 ? 2 : 1) attention_kernel(Attn
 #pragma unroll
                 for (int i = 0; i < 4; ++i) x[i] += shares[item + p * items][i];
             const float inv = total[r] == 0.0f ? 0.0f : 1.0f / total[r];
-            const int32_t row = tile * R + r;
+            const int32_t row = tile * R + r, t = STEP ? 0 : row / G;
 #pragma unroll
             for (int i = 0; i < 4; ++i) x[i] *= inv;
-            *reinterpret_cast<f4*>(a.context + (static_cast<size_t>(row / G) * a.num_heads + g * G + row % G) * HD + d) = x;
+            *reinterpret_cast<f4*>(a.context + (static_cast<size_t>(t) * a.num_heads + g * G + (row - t * G)) * HD + d) = x;
         }
     }
 }
@@ -1323,13 +1320,11 @@ int32_t launch_rows(AttnArgs a, int32_t key_bound, hipStream_t st, AppendArgs* a
 template <int FMT, int HD>
 int32_t launch_dims(const AttnArgs& a, int32_t key_bound, hipStream_t st, AppendArgs* append) {
     const int32_t rows = a.tokens * (a.num_heads / a.c.kv_heads);
-    if (append && rows <= 16) {  // a step of up to 16 query heads a kv head: one launch
-        if constexpr (HD < 256) {
+    if constexpr (HD < 256) {  // (of 256 dims the step's form would not fit the registers)
+        if (append && rows <= 16) {  // a step of up to 16 query heads a kv head: one launch
             if (key_bound <= DIRECT_KEYS) return launch_rows<FMT, HD, 16, 8, true>(a, key_bound, st, append);
+            return launch_rows<FMT, HD, 16, 4, true>(a, key_bound, st, append);
         }
-        return launch_rows<FMT, HD, 16, 4, true>(a, key_bound, st, append);
-    }
-    if constexpr (HD < 256) {
         if (rows > 48) return launch_rows<FMT, HD, 32, 4>(a, key_bound, st, append);
         if (key_bound <= DIRECT_KEYS) return launch_rows<FMT, HD, 16, 8>(a, key_bound, st, append);
     }
