@@ -330,6 +330,7 @@ __global__ void __launch_bounds__(THREADS) append_kernel(AppendArgs a) {
 // A block's value scale 2^e mu joins the exponent as log2(mu) and e less the largest e so far (uniform):
 // weights include it, and the sum of weights takes it out again, with one product a set of 32 keys.
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef float f16v __attribute__((ext_vector_type(16)));
 
@@ -558,20 +559,21 @@ __global__ void __launch_bounds__(64 * NW, R > 16 ? 2 : 1) attention_kernel(Attn
     const int32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int32_t col = X::SMALL ? lane & 15 : lane & 31, grp = X::SMALL ? lane >> 4 : lane >> 5;
 
-    // The rows' queries, a row at a time to a wave (its dims d, and for the rotation those of d's pair), go out
-    // ahead of the position, as does a step's token.
-    constexpr int RW = R / NW > 0 ? R / NW : 1, DL = (HD + 63) / 64;
+    // The rows' queries, sixteen lanes to a row (four dims each, or 64 apart; for the rotation those of the dims'
+    // pairs, too), go out ahead of the position, as does a step's token.
+    constexpr int RW = R / (4 * NW) > 0 ? R / (4 * NW) : 1, DL = HD / 64 > 0 ? HD / 64 : 1;
     const int32_t held = min(R, rows - tile * R);  // rows of this tile
-    float qv[RW][DL], qo[STEP ? RW : 1][STEP ? DL : 1];
+    const int32_t lr = lane >> 4, lc = lane & 15;
+    f4 qv[RW][DL], qo[STEP ? RW : 1][STEP ? DL : 1];
 #pragma unroll
     for (int i = 0; i < RW; ++i) {
-        const int32_t row = tile * R + min(wave + i * NW, held - 1), t = STEP ? 0 : row / G;
+        const int32_t row = tile * R + min(4 * (wave + i * NW) + lr, held - 1), t = STEP ? 0 : row / G;
         const float* src = a.q + (static_cast<size_t>(t) * a.num_heads + g * G + (row - t * G)) * HD;
 #pragma unroll
         for (int u = 0; u < DL; ++u) {
-            const int32_t d = (lane + 64 * u) % HD;
-            qv[i][u] = src[d];
-            if constexpr (STEP) qo[i][u] = src[(d + HD / 2) % HD];
+            const int32_t d = (4 * lc + 64 * u) % HD;
+            qv[i][u] = *reinterpret_cast<const f4*>(src + d);
+            if constexpr (STEP) qo[i][u] = *reinterpret_cast<const f4*>(src + (d + HD / 2) % HD);
         }
     }
     __shared__ StepShared<HD, STEP> sh;
@@ -716,33 +718,50 @@ __global__ void __launch_bounds__(64 * NW, R > 16 ? 2 : 1) attention_kernel(Attn
     constexpr int QR = HD + 8;
 #pragma unroll
     for (int i = 0; i < RW; ++i) {
-        const int32_t r = wave + i * NW;
-        if (r >= held) break;
+        if (4 * (wave + i * NW) >= held) break;
+        const int32_t r = 4 * (wave + i * NW) + lr;
         uint32_t top = 0;
 #pragma unroll
         for (int u = 0; u < DL; ++u) {
             if constexpr (STEP) {
-                const int32_t d = (lane + 64 * u) % HD;
+                const int32_t d = (4 * lc + 64 * u) % HD;
                 const bool upper = d >= HALF;
-                float y1, y2;
-                rope_apply(upper ? qo[i][u] : qv[i][u], upper ? qv[i][u] : qo[i][u], sh.cosines[d % HALF], sh.sines[d % HALF], y1, y2);
-                qv[i][u] = upper ? y2 : y1;
-            }
-            top = max(top, magnitude(qv[i][u]));
-        }
-        // (bits of magnitudes, below an infinity's where they count: their order is the floats')
-        const float top_f = wave_max_dpp(__builtin_bit_cast(float, min(top, 0x7F7FFFFFu)));
-        const int32_t up = 13 - max(static_cast<int32_t>(__builtin_bit_cast(uint32_t, top_f) >> 23) - 127, -100);
+                const f4 cf = *reinterpret_cast<const f4*>(&sh.cosines[d % HALF]), sf = *reinterpret_cast<const f4*>(&sh.sines[d % HALF]);
 #pragma unroll
-        for (int u = 0; u < DL; ++u) {
-            const float x = ldexpf(qv[i][u], up);
-            const _Float16 hi = static_cast<_Float16>(x), lo = static_cast<_Float16>(x - static_cast<float>(hi));
-            if (lane + 64 * u < HD) {
-                qs[r * QR + lane + 64 * u] = hi;
-                qs[(R + r) * QR + lane + 64 * u] = lo;
+                for (int e = 0; e < 4; ++e) {
+                    float y1, y2;
+                    rope_apply(upper ? qo[i][u][e] : qv[i][u][e], upper ? qv[i][u][e] : qo[i][u][e], cf[e], sf[e], y1, y2);
+                    qv[i][u][e] = upper ? y2 : y1;
+                }
             }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) top = max(top, magnitude(qv[i][u][e]));
         }
-        if (lane == 0) fr_s[r] = ldexpf(a.scale * 1.4426950408889634f, -up);
+        // the row's largest magnitude (bits below an infinity's, whose order is the floats')
+        float most = __builtin_bit_cast(float, min(top, 0x7F7FFFFFu));
+        most = fmaxf(most, dpp_move<0xB1>(most));
+        most = fmaxf(most, dpp_move<0x4E>(most));
+        most = fmaxf(most, dpp_move<0x141>(most));
+        most = fmaxf(most, dpp_move<0x140>(most));
+        const int32_t up = 13 - max(static_cast<int32_t>(__builtin_bit_cast(uint32_t, most) >> 23) - 127, -100);
+        const float by = ldexpf(1.0f, up);
+        if (r < held) {
+#pragma unroll
+            for (int u = 0; u < DL; ++u) {
+                half4 hi, lo;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float x = qv[i][u][e] * by;
+                    hi[e] = static_cast<_Float16>(x);
+                    lo[e] = static_cast<_Float16>(x - static_cast<float>(hi[e]));
+                }
+                if (4 * lc + 64 * u < HD) {
+                    *reinterpret_cast<half4*>(qs + r * QR + 4 * lc + 64 * u) = hi;
+                    *reinterpret_cast<half4*>(qs + (R + r) * QR + 4 * lc + 64 * u) = lo;
+                }
+            }
+            if (lc == 0) fr_s[r] = ldexpf(a.scale * 1.4426950408889634f, -up);
+        }
     }
     if constexpr (STEP) {
         if (holder) {
