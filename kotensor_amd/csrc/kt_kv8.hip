@@ -911,7 +911,7 @@ __global__ void __launch_bounds__(64 * NW, R > 16 ? 2 : 1) attention_kernel(Attn
             const int32_t in_exp = quiet[h] <= MOST_QUIET ? quiet[h] : 0;
             quiet[h] -= in_exp;
             shift[h] = static_cast<float>(in_exp) - __builtin_amdgcn_logf(mu) - WEIGHT_UP;
-            unscale[h] = ldexpf(1.0f / mu, in_exp);
+            unscale[h] = ldexpf(__builtin_amdgcn_rcpf(mu), in_exp);  // (off by one unit at most, as a weight's rounding)
         }
         half8 ph[X::J][X::CT][X::VL], pl[X::J][X::CT][X::VL];
 #pragma unroll
@@ -1298,7 +1298,9 @@ int32_t attention_args(const float* q, int32_t tokens, const int32_t* position, 
     return KT_OK;
 }
 
-constexpr int DIRECT_KEYS = 16 * CHUNK;  // one workgroup of 8 waves, no key splits
+// Up to so many keys one workgroup of 8 waves takes them without splits. A step of 32 heads, with the call, and with
+// splits: heads of 64 after 500 keys 8.8 us (10.6), 1000 10.2 (10.4), 1500 11.8 (10.5); of 128 500 11.9 (12.6), 760 13.0 (12.5).
+constexpr int direct_keys(int hd) { return hd <= 64 ? 16 * CHUNK : 10 * CHUNK; }
 
 template <int FMT, int HD, int R, int WAVES, bool STEP = false>
 int32_t launch_rows(AttnArgs a, int32_t key_bound, hipStream_t st, AppendArgs* append) {
@@ -1306,13 +1308,15 @@ int32_t launch_rows(AttnArgs a, int32_t key_bound, hipStream_t st, AppendArgs* a
     const int32_t tiles = ceil_div(a.tokens * (a.num_heads / a.c.kv_heads), R);
     const int64_t wgs = static_cast<int64_t>(a.c.kv_heads) * tiles;
     if (tiles > 65535) return fail(KT_ERR_SHAPE, "too many tokens and heads in one call");
-    // Key splits: two workgroups for each CU where the rows give fewer.
-    const int32_t fill = static_cast<int32_t>(std::min<int64_t>(MAX_SPLITS, (2 * cu_count() + wgs - 1) / wgs));
+    // Key splits: as many as two workgroups for each CU hold, which is what fits at once (24 tokens of 32 heads after
+    // 4000, rounded up to 528 workgroups: 16.9 us for 12.6).
+    const int32_t fill = static_cast<int32_t>(std::min<int64_t>(MAX_SPLITS, std::max<int64_t>(1, 2 * cu_count() / wgs)));
     a.max_splits = splits_of(ceil_div(key_bound, CHUNK), WAVES, DIRECT ? 1 : wgs < static_cast<int64_t>(MAX_COUNTERS) ? fill : 1);
     if (a.max_splits > 1 || append) {
         const size_t rows = static_cast<size_t>(wgs) * a.max_splits * R, q = append && !STEP ? static_cast<size_t>(a.num_heads) * HD : 0;
         void* ws = nullptr;
-        if (const int32_t status = workspace_counters(st, (rows * (HD + 2) + q) * sizeof(float), a.max_splits > 1 ? static_cast<size_t>(wgs) : 0, &ws, &a.counters)) return status;
+        if (const int32_t status = workspace_counters(st, (rows * (HD + 2) + q) * sizeof(float) + 16, a.max_splits > 1 ? static_cast<size_t>(wgs) : 0, &ws, &a.counters)) return status;
+        ws = reinterpret_cast<void*>((reinterpret_cast<uintptr_t>(ws) + 15) & ~uintptr_t{15});  // (it begins at any dword)
         a.averages = static_cast<float*>(ws) + q;
         a.stats = a.averages + rows * HD;
         if constexpr (STEP) {
@@ -1341,11 +1345,14 @@ int32_t launch_dims(const AttnArgs& a, int32_t key_bound, hipStream_t st, Append
     const int32_t rows = a.tokens * (a.num_heads / a.c.kv_heads);
     if constexpr (HD < 256) {  // (of 256 dims the step's form would not fit the registers)
         if (append && rows <= 16) {  // a step of up to 16 query heads a kv head: one launch
-            if (key_bound <= DIRECT_KEYS) return launch_rows<FMT, HD, 16, 8, true>(a, key_bound, st, append);
+            if (key_bound <= direct_keys(HD)) return launch_rows<FMT, HD, 16, 8, true>(a, key_bound, st, append);
             return launch_rows<FMT, HD, 16, 4, true>(a, key_bound, st, append);
         }
-        if (rows > 48) return launch_rows<FMT, HD, 32, 4>(a, key_bound, st, append);
-        if (key_bound <= DIRECT_KEYS) return launch_rows<FMT, HD, 16, 8>(a, key_bound, st, append);
+        // Tiles of 16 rows while two workgroups for each CU hold them, of 32 beyond. 32 heads of 64, 8 kv heads, with the call,
+        // 16 (32): 16 tokens after 1000 8.0 us (12.6), 256 after 1000 13.4 (18.6), after 4000 32.4 (32.6), 512 after 4000 61
+        // (48), a prompt of 1024 28.5 (19.3); heads of 128, 64 tokens after 4000 23.0 (25.1), 300 76 (66).
+        if (static_cast<int64_t>(a.c.kv_heads) * ceil_div(rows, 16) > 2 * cu_count()) return launch_rows<FMT, HD, 32, 4>(a, key_bound, st, append);
+        if (key_bound <= direct_keys(HD)) return launch_rows<FMT, HD, 16, 8>(a, key_bound, st, append);
     }
     return launch_rows<FMT, HD, 16, 4>(a, key_bound, st, append);
 }

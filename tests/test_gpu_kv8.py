@@ -219,8 +219,9 @@ def _filled(kt, rng, fmt, block, d, kv, n, max_seq, layers=1, layer=0, loud=None
 def _attend(kt, cache, layer, q, start, heads, bound=None, stream=None):
     from kotensor_amd import _lib
     dq, pos, out = _dev(kt, q), _dev(kt, np.array([start], np.int32)), _dev(kt, np.full(q.shape, 7.0, np.float32))
-    _lib.call("kt_attention_kv8", dq.ptr, q.shape[0], pos.ptr, bound or start + q.shape[0], ctypes.byref(cache.cache), layer, heads, out.ptr, stream)
     kt.synchronize()
+    _lib.call("kt_attention_kv8", dq.ptr, q.shape[0], pos.ptr, bound or start + q.shape[0], ctypes.byref(cache.cache), layer, heads, out.ptr, stream)
+    _lib.call("kt_stream_sync", stream)
     return out.download(np.float32).reshape(q.shape)
 
 
@@ -388,6 +389,23 @@ def test_step_equals_its_parts(kt, oracle_lib, fmt, block, start, heads, kv, d):
         tol = _tolerance(turned, held[0], heads)
         assert normwise_rel(out.download(np.float32), want.reshape(-1)) <= tol
         assert normwise_rel(want, kv8_ref.attend(turned, *held, start + t, heads)) <= tol
+
+
+def test_after_a_call_that_leaves_the_workspace_at_an_odd_place(kt):
+    """The fp32 cache's attention of an odd number of heads and splits sizes the stream's zeroed words, behind which
+    the general area begins at any dword: the splits' pairs of words are placed at their own alignment."""
+    from kotensor_amd import _lib
+    banner("kv8-workspace")
+    rng = np.random.default_rng(17)
+    stream = kt.Stream.create()
+    q, k = rng.standard_normal((1, 3 * 64)).astype(np.float32), rng.standard_normal((1, 700, 64)).astype(np.float32)
+    dq, dk, pos, out = _dev(kt, q), _dev(kt, k), _dev(kt, np.array([699], np.int32)), kt.DeviceBuffer(q.nbytes)
+    _lib.call("kt_attention", dq.ptr, 1, pos.ptr, 700, dk.ptr, dk.ptr, 0, 700, 3, 1, 64, out.ptr, stream.handle)
+    stream.synchronize()
+    cache, keys, values = _filled(kt, rng, "int8", 64, 64, 1, 3000, 3000)
+    got = _attend(kt, cache, 0, q, 2999, 3, stream=stream.handle)
+    assert normwise_rel(got, kv8_ref.attend(q, keys, values, 2999, 3)) <= _tolerance(q, keys, 3)
+    stream.destroy()
 
 
 def test_steps_of_two_streams_and_threads(kt):
