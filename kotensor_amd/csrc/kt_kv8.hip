@@ -1287,7 +1287,8 @@ int32_t attention_args(const float* q, int32_t tokens, const int32_t* position, 
     if (const int32_t status = check_heads(num_heads, a->c.kv_heads)) return status;
     if (tokens < 0 || key_bound < tokens || key_bound > a->c.max_seq)
         return fail(KT_ERR_ARGUMENT, "key bound %d must cover the %d tokens and fit maxSequenceLength %d", key_bound, tokens, a->c.max_seq);
-    if (tokens > 65535) return fail(KT_ERR_ARGUMENT, "%d tokens in one call: at most 65535", tokens);
+    if (static_cast<int64_t>(tokens) * (num_heads / a->c.kv_heads) > 65535 * 16)
+        return fail(KT_ERR_SHAPE, "%d tokens of %d query heads a key/value head in one call: at most %d rows", tokens, num_heads / a->c.kv_heads, 65535 * 16);
     if (!aligned(q, 16) || !aligned(context, 16)) return fail(KT_ERR_ARGUMENT, "attention: q and the context must be 16-byte aligned");
     a->q = q;
     a->position = position;
@@ -1307,25 +1308,30 @@ int32_t launch_rows(AttnArgs a, int32_t key_bound, hipStream_t st, AppendArgs* a
     constexpr bool DIRECT = WAVES > 4;  // no splits
     const int32_t tiles = ceil_div(a.tokens * (a.num_heads / a.c.kv_heads), R);
     const int64_t wgs = static_cast<int64_t>(a.c.kv_heads) * tiles;
-    if (tiles > 65535) return fail(KT_ERR_SHAPE, "too many tokens and heads in one call");
     // Key splits: as many as two workgroups for each CU hold, which is what fits at once (24 tokens of 32 heads after
     // 4000, rounded up to 528 workgroups: 16.9 us for 12.6).
     const int32_t fill = static_cast<int32_t>(std::min<int64_t>(MAX_SPLITS, std::max<int64_t>(1, 2 * cu_count() / wgs)));
     a.max_splits = splits_of(ceil_div(key_bound, CHUNK), WAVES, DIRECT ? 1 : wgs < static_cast<int64_t>(MAX_COUNTERS) ? fill : 1);
-    if (a.max_splits > 1 || append) {
-        const size_t rows = static_cast<size_t>(wgs) * a.max_splits * R, q = append && !STEP ? static_cast<size_t>(a.num_heads) * HD : 0;
+    CallScratch turned;  // the rotated query of a step whose append is a launch of its own
+    if (append && !STEP) {
+        const size_t bytes = static_cast<size_t>(a.num_heads) * HD * sizeof(float);
+        if (const int32_t status = turned.take(CALL_SLICES, st, bytes)) return status;
+        append->q_out = static_cast<float*>(turned.ptr);
+    }
+    const bool in_workspace = append && !STEP && !turned.ptr;  // (a capture begun by other means)
+    if (a.max_splits > 1 || STEP || in_workspace) {
+        const size_t rows = static_cast<size_t>(wgs) * a.max_splits * R, q = in_workspace ? static_cast<size_t>(a.num_heads) * HD : 0;
         void* ws = nullptr;
         if (const int32_t status = workspace_counters(st, (rows * (HD + 2) + q) * sizeof(float) + 16, a.max_splits > 1 ? static_cast<size_t>(wgs) : 0, &ws, &a.counters)) return status;
         ws = reinterpret_cast<void*>((reinterpret_cast<uintptr_t>(ws) + 15) & ~uintptr_t{15});  // (it begins at any dword)
         a.averages = static_cast<float*>(ws) + q;
         a.stats = a.averages + rows * HD;
-        if constexpr (STEP) {
-            a.rope_cache = a.counters + ROPE_CACHE_WORD;
-        } else if (append) {
-            append->q_out = static_cast<float*>(ws);
-            a.q = append->q_out;
-            if (const int32_t status = launch_append(*append, st)) return status;
-        }
+        if constexpr (STEP) a.rope_cache = a.counters + ROPE_CACHE_WORD;
+        if (in_workspace) append->q_out = static_cast<float*>(ws);
+    }
+    if (append && !STEP) {
+        a.q = append->q_out;
+        if (const int32_t status = launch_append(*append, st)) return status;
     }
     constexpr size_t lds = sizeof(float) * std::max(std::max(static_cast<size_t>(WAVES) * R * (HD + 6), static_cast<size_t>(R) * (HD + 8)), static_cast<size_t>(R) * (MAX_SPLITS + 1) + 4 * 64 * WAVES);
     if constexpr (lds > (64u << 10)) {  // beyond the default dynamic LDS limit (160 KB per CU on gfx950)

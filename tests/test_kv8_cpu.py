@@ -85,6 +85,9 @@ def test_calls_refused():
     refused(lib.kt_attention_kv8(20, 1, 16, 1, good, 0, 4, 16, None), arg, "16-byte aligned")
     refused(lib.kt_attention_kv8(16, 1, 16, 1, good, 0, 4, 24, None), arg, "16-byte aligned")
     refused(lib.kt_attention_kv8(16, 1, 16, 1, good, -1, 4, 16, None), rng, "layer -1")
+    wide = ctypes.byref(_cache(max_seq=2_000_000))
+    refused(lib.kt_attention_kv8(16, 524_281, 16, 524_281, wide, 0, 4, 16, None), shape, "at most 1048560 rows")
+    refused(lib.kt_rope_attention_kv8(16, 16, 16, 16, 2_000_000, 16, 2_000_000, wide, 0, 4000, 16, None), shape, "at most 1048560 rows")
     assert lib.kt_attention_kv8(16, 0, 16, 0, good, 0, 4, 16, None) == _lib.KT_OK
     refused(lib.kt_rope_attention_kv8(None, 16, 16, 16, 1, 16, 1, good, 0, 4, 16, None), arg, "NULL")
     refused(lib.kt_rope_attention_kv8(16, 16, 16, None, 1, 16, 1, good, 0, 4, 16, None), arg, "NULL")
