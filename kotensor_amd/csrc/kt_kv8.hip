@@ -133,8 +133,10 @@ __device__ __forceinline__ int32_t value_byte(int32_t quad) {
 
 // ---- RoPE and the append ---------------------------------------------------------------
 // Workgroup (block y of those the new tokens touch, kv head, keys or values) rotates and
-// encodes its block through LDS; further workgroups rotate q. Bound by the launch for one
-// token, by reading the rows and (keys, q) the double-precision cosines for a prompt.
+// encodes its block through LDS; further workgroups rotate q. Traced, 32 query and 8 kv heads: one token 4.2 us, the
+// launch and three memory round trips; 1024 tokens of heads of 64 9.4 us (22 MB moved: 4.3 at a copy's rate), 1501 of
+// heads of 128 16.0 (65 MB, 13), bound by the double-precision cosines of the keys' workgroups, each of which makes
+// its block's anew (a table of them would be another launch).
 // The first block's earlier rows come from the fp32 rows of the open block, which the last
 // block's rows replace: where the first block has earlier rows, one workgroup does both, in
 // that order.
@@ -329,6 +331,15 @@ __global__ void __launch_bounds__(THREADS) append_kernel(AppendArgs a) {
 // then stay below 2^15 in fp16, being taken times 2^6), so that the sums are seldom rescaled.
 // A block's value scale 2^e mu joins the exponent as log2(mu) and e less the largest e so far (uniform):
 // weights include it, and the sum of weights takes it out again, with one product a set of 32 keys.
+// Waves' sums meet in LDS; key splits' through memory, where the last workgroup of a tile to arrive (a counter,
+// which it returns to zero) merges all in their order: no workgroup waits for another, and the bits do not depend on
+// who is last.
+// Traced, 32 query and 8 kv heads: a step with its append at 131072 keys of 128 dims (e4m3) 54.8 us, 269 MB at
+// 4.9 TB/s, the rate of a large copy; at 8192 keys of 64 (int8) 12.5 us, of which the cache's 8.4 MB are 1.7: latencies
+// of the launch, the position, the keys (3.6 us to the end of the scores' work), the append in the last split (1.4) and
+// the splits' meeting (4); at 544 keys of 2 kv heads 8.9. Seven tokens after 4000 (e4m3) 12.2. A prompt of 1024 tokens
+// 21.4 us; 301 tokens after 7000 (heads of 128, int8) 118: 300 Tflop/s, 600 in the products of two parts, bound by the
+// vector work beside them (580 instructions a wave and 64 keys, 256 of them the codes' conversion, for 64 products).
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
@@ -1138,7 +1149,8 @@ __global__ void __launch_bounds__(64 * NW, R > 16 ? 2 : 1) attention_kernel(Attn
 
 // ---- rows as fp32, and the copy of a prefix ------------------------------------------------
 // Workgroup (chunk, kv head, 64 dims of the keys or of the values): the chunk's rows in [first, first + count) as code *
-// scale, sixteen codes a thread; the values turn through LDS. One memory round trip and the stores.
+// scale, sixteen codes a thread; the values turn through LDS. One memory round trip and the stores: a block of 64 tokens
+// of 8 heads of 64 3.2 us traced, 1501 tokens of heads of 128 6.6 (12.3 MB written and 3.1 read: 2.3 TB/s).
 template <int FMT>
 __global__ void __launch_bounds__(THREADS) read_kernel(KV8View c, int32_t first, int32_t count, float* keys, float* values) {
     __shared__ float turned[CHUNK][65];

@@ -32,6 +32,9 @@ struct LogitsArgs {
 // tokens of its segment in LDS, by integer atomics, whose order changes nothing; then it changes and writes
 // each logit once. Every workgroup of a row reads the row's whole text, from L2 after the first.
 // Of a token biased twice the later entry holds (the largest entry index).
+// Traced: 64 rows of 151936 with texts of up to 4096, 100 biases and masks 21.4 us, 80 MB at 3.7 TB/s (scalar
+// accesses after the text, segments of 4096: 48.7); one row of 32000 3.0, 5 of 49157 3.7 (5.1, 9.6): the launch and two
+// memory round trips.
 template <int VECS>
 __global__ void __launch_bounds__(THREADS) process_kernel(LogitsArgs a) {
     constexpr int SEGMENT = 4 * THREADS * VECS;
@@ -165,7 +168,8 @@ int32_t kt_process_logits(const float* logits, int32_t rows, int32_t n, int64_t 
     if (rows == 0) return KT_OK;
     LogitsArgs a{logits, out, stride, out_stride, n, text, c.allowed != nullptr, c};
     hipStream_t st = static_cast<hipStream_t>(stream);
-    // short segments while they fit the card at once, long ones (fewer readings of the text) beyond
+    // Segments of 1024 while they fit the card at once, of 2048 (fewer readings of the text) beyond. With 1024, 2048 and
+    // 4096: 64 rows of 151936 24.1, 21.5, 25.3 us; 5 of 49157 3.8, 4.7; one of 32000 3.1, 3.5.
     const int64_t short_ones = (static_cast<int64_t>(n - 1) / 1024 + 1) * rows;
     if (short_ones <= 2 * cu_count()) return launch<1>(a, rows, st);
     return launch<2>(a, rows, st);
