@@ -349,14 +349,10 @@ struct AttnArgs {
     // (what the first loads need comes first: it arrives with the wave)
     const int32_t* position;
     const float* q;
-    // one token with RoPE and the append inside: its projections before RoPE, the layer, and the decode attention's
-    // cache of cosines and sines (as kt_decoder.hip's: per frequency i words 4 i .. + 3 = position + 1, the
-    // frequency's bits, cos, sin, written by layer 0; or null)
+    // one token with RoPE and the append inside: its projections before RoPE
     const float* k_new;
     const float* v_new;
     const float* inv_freq;
-    uint32_t* rope_cache;
-    int32_t layer;
     int32_t tokens, num_heads;
     float scale;
     KV8View c;
@@ -591,16 +587,12 @@ __global__ void __launch_bounds__(64 * NW, R > 16 ? 2 : 1) attention_kernel(Attn
     constexpr int HALF = HD / 2;
     const bool on = STEP && tid < 256 && (tid & 127) < HALF;  // threads with a pair of the key or the value
     float x1 = 0.0f, x2 = 0.0f, ifr = 0.0f;
-    uint32_t ce[4] = {0u, 0u, 0u, 0u};
     if constexpr (STEP) {
         if (on) {
             const float* src = (tid < 128 ? a.k_new : a.v_new) + g * HD + (tid & 127);
             x1 = src[0];
             x2 = src[HALF];
             ifr = a.inv_freq[tid & 127];
-            if (a.rope_cache && a.layer != 0)
-#pragma unroll
-                for (int w = 0; w < 4; ++w) ce[w] = __hip_atomic_load(a.rope_cache + 4 * (tid & 127) + w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
         }
     }
     const int32_t P0 = *a.position;
@@ -707,19 +699,8 @@ __global__ void __launch_bounds__(64 * NW, R > 16 ? 2 : 1) attention_kernel(Attn
     }
     if constexpr (STEP) {
         if (on) {  // cosines by the key's threads, sines by the value's
-            const bool cosine = tid < 128;
-            const int32_t i = tid & 127;
-            float y = __builtin_bit_cast(float, ce[cosine ? 2 : 3]);
-            if (ce[0] != static_cast<uint32_t>(P0) + 1u || ce[1] != __builtin_bit_cast(uint32_t, ifr)) y = cosine ? rope_cos(P0, ifr) : rope_sin(P0, ifr);
-            (cosine ? sh.cosines : sh.sines)[i] = y;
-            if (a.rope_cache && a.layer == 0 && g == 0 && split == 0) {
-                uint32_t* e = a.rope_cache + 4 * i;
-                if (cosine) {
-                    __hip_atomic_store(e, static_cast<uint32_t>(P0) + 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
-                    __hip_atomic_store(e + 1, __builtin_bit_cast(uint32_t, ifr), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
-                }
-                __hip_atomic_store(e + (cosine ? 2 : 3), __builtin_bit_cast(uint32_t, y), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
-            }
+            if (tid < 128) sh.cosines[tid] = rope_cos(P0, ifr);
+            else sh.sines[tid - 128] = rope_sin(P0, ifr);
         }
         __syncthreads();
     }
@@ -1331,14 +1312,13 @@ int32_t launch_rows(AttnArgs a, int32_t key_bound, hipStream_t st, AppendArgs* a
         append->q_out = static_cast<float*>(turned.ptr);
     }
     const bool in_workspace = append && !STEP && !turned.ptr;  // (a capture begun by other means)
-    if (a.max_splits > 1 || STEP || in_workspace) {
+    if (a.max_splits > 1 || in_workspace) {
         const size_t rows = static_cast<size_t>(wgs) * a.max_splits * R, q = in_workspace ? static_cast<size_t>(a.num_heads) * HD : 0;
         void* ws = nullptr;
         if (const int32_t status = workspace_counters(st, (rows * (HD + 2) + q) * sizeof(float) + 16, a.max_splits > 1 ? static_cast<size_t>(wgs) : 0, &ws, &a.counters)) return status;
         ws = reinterpret_cast<void*>((reinterpret_cast<uintptr_t>(ws) + 15) & ~uintptr_t{15});  // (it begins at any dword)
         a.averages = static_cast<float*>(ws) + q;
         a.stats = a.averages + rows * HD;
-        if constexpr (STEP) a.rope_cache = a.counters + ROPE_CACHE_WORD;
         if (in_workspace) append->q_out = static_cast<float*>(ws);
     }
     if (append && !STEP) {
@@ -1432,7 +1412,6 @@ int32_t kt_rope_attention_kv8(float* q, const float* k, const float* v, const fl
         a.k_new = k;
         a.v_new = v;
         a.inv_freq = inv_freq;
-        a.layer = layer;
         return launch_attention(a, key_bound, st, &p);
     }
     if (const int32_t status = launch_append(p, st)) return status;
