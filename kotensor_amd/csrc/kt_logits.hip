@@ -15,7 +15,6 @@
 namespace kt {
 namespace {
 
-constexpr int THREADS = 256;
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef int32_t i4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
@@ -28,14 +27,13 @@ struct LogitsArgs {
     kt_logits_controls c;
 };
 
-// Workgroup (segment of 1024 VECS logits, row): its logits go into registers first; meanwhile it counts the text's
+// Workgroup (segment of 4 THREADS VECS logits, row): its logits go into registers first; meanwhile it counts the text's
 // tokens of its segment in LDS, by integer atomics, whose order changes nothing; then it changes and writes
 // each logit once. Every workgroup of a row reads the row's whole text, from L2 after the first.
 // Of a token biased twice the later entry holds (the largest entry index).
-// Traced: 64 rows of 151936 with texts of up to 4096, 100 biases and masks 21.4 us, 80 MB at 3.7 TB/s (scalar
-// accesses after the text, segments of 4096: 48.7); one row of 32000 3.0, 5 of 49157 3.7 (5.1, 9.6): the launch and two
-// memory round trips.
-template <int VECS>
+// Traced: 64 rows of 151936 with texts of up to 4096, 100 biases and masks 19.9 us, 80 MB at 4.0 TB/s (scalar
+// accesses after the text: 48.7); one row of 32000 3.0, 5 of 49157 3.7: the launch and two memory round trips.
+template <int THREADS, int VECS>
 __global__ void __launch_bounds__(THREADS) process_kernel(LogitsArgs a) {
     constexpr int SEGMENT = 4 * THREADS * VECS;
     __shared__ __attribute__((aligned(16))) uint32_t marks[SEGMENT];  // occurrences from output_start on; the top bit: any
@@ -127,10 +125,10 @@ __global__ void __launch_bounds__(THREADS) process_kernel(LogitsArgs a) {
     }
 }
 
-template <int VECS>
+template <int THREADS, int VECS>
 int32_t launch(const LogitsArgs& a, int32_t rows, hipStream_t st) {
     constexpr int SEGMENT = 4 * THREADS * VECS;
-    process_kernel<VECS><<<dim3(static_cast<uint32_t>((a.n - 1) / SEGMENT + 1), static_cast<uint32_t>(rows)), THREADS,
+    process_kernel<THREADS, VECS><<<dim3(static_cast<uint32_t>((a.n - 1) / SEGMENT + 1), static_cast<uint32_t>(rows)), THREADS,
                            a.c.bias_count > 0 ? SEGMENT * sizeof(int32_t) : 0, st>>>(a);
     KT_LAUNCHED("logits kernel");
     return KT_OK;
@@ -168,11 +166,12 @@ int32_t kt_process_logits(const float* logits, int32_t rows, int32_t n, int64_t 
     if (rows == 0) return KT_OK;
     LogitsArgs a{logits, out, stride, out_stride, n, text, c.allowed != nullptr, c};
     hipStream_t st = static_cast<hipStream_t>(stream);
-    // Segments of 1024 while they fit the card at once, of 2048 (fewer readings of the text) beyond. With 1024, 2048 and
-    // 4096: 64 rows of 151936 24.1, 21.5, 25.3 us; 5 of 49157 3.8, 4.7; one of 32000 3.1, 3.5.
+    // Segments of 1024 logits on 256 threads up to four for each CU, of 4096 on 512 (fewer readings of the text) beyond. Rows of
+    // 151936, texts of 4096, short and long: 2 rows 4.8 and 5.3 us, 4 5.1 and 5.4, 8 6.2 and 6.2, 16 9.8 and 7.9, 64 25.2 and 20.3
+    // (2048 on 256 threads 22.3, 8192 on 1024 19.8, and 16 rows 8.2).
     const int64_t short_ones = (static_cast<int64_t>(n - 1) / 1024 + 1) * rows;
-    if (short_ones <= 2 * cu_count()) return launch<1>(a, rows, st);
-    return launch<2>(a, rows, st);
+    if (short_ones <= 4 * cu_count()) return launch<256, 1>(a, rows, st);
+    return launch<512, 2>(a, rows, st);
 }
 
 }  // extern "C"

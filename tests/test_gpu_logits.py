@@ -51,6 +51,11 @@ def test_controls_against_64_bits(kt, rows, n, length, bias, mask):
     assert same_bits(dl.numpy(), got)
 
 
+@pytest.mark.parametrize("rows,n,length", [(1100, 33, 9), (205, 4097, 100), (1025, 1000, 5)])
+def test_segments_of_many_rows(kt, rows, n, length):
+    test_controls_against_64_bits(kt, rows, n, length, 5, True)
+
+
 @pytest.mark.parametrize("repetition,frequency,presence", [(1.0, 0.0, 0.0), (2.0, 0.0, 0.0), (1.0, 0.7, 0.0), (1.0, 0.0, -0.4), (0.5, -0.1, 0.3)])
 def test_each_penalty(kt, repetition, frequency, presence):
     banner("logits-penalty", repetition, frequency, presence)
