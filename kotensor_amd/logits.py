@@ -47,8 +47,8 @@ class LogitsControls:
         return (self.repetition_penalty, self.frequency_penalty, self.presence_penalty) != (1.0, 0.0, 0.0)
 
     def set_allowed(self, allowed, stream: Stream | None = None) -> None:
-        """Replaces the mask; one of the same size goes to the same device memory, which a recorded
-        step then reads at its next replay."""
+        """Sets the mask. Another one of the same shape replaces it in the same device memory, which a
+        recorded step then reads at its next replay; one of another shape is refused."""
         a = np.asarray(allowed)
         if a.ndim not in (1, 2) or a.size == 0:
             raise _lib.IllegalArgumentException(f"a mask is an array of the vocabulary, or one a row, got {list(a.shape)}")
@@ -58,8 +58,11 @@ class LogitsControls:
         elif a.dtype not in (np.dtype("u4"), np.dtype("i4")):
             raise _lib.IllegalArgumentException(f"a mask is boolean or packed in 32-bit words, got {a.dtype}")
         words = (a.shape[0] if a.ndim == 2 else 0, a.shape[-1])
-        if self._allowed is None or words != self._words:
+        if self._allowed is None:
             self._allowed, self._words = DeviceBuffer(a.nbytes), words
+        elif words != self._words:  # (a recorded step may address the memory)
+            raise _lib.IllegalArgumentException(
+                f"a mask of {words[0]} rows, {words[1]} words cannot replace one of {self._words[0]} rows, {self._words[1]} words")
         self._allowed.upload(a, stream)
 
     def descriptor(self, rows: int, vocabulary: int, history=None, history_length=None, output_start=None, history_stride: int = 0,

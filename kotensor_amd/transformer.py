@@ -616,6 +616,7 @@ class Transformer:
         if not 0 <= int(token) < self.vocabulary_size:
             raise _lib.IllegalArgumentException(f"{token} out of vocab bounds {self.vocabulary_size}")
         buffers.tokens.upload(np.array([int(token)], np.int32), stream)
+        buffers.recorded = min(buffers.recorded, cache.length)
         self._decode_step(cache, buffers, _stream(stream), argmax=False)
         cache.length += 1
         return buffers
@@ -664,6 +665,7 @@ class Transformer:
         buffers.generated at its position. ``controls`` as in greedy_decode, whose first argmax
         set buffers.output_start."""
         cache.check_room(1)
+        self._check_recorded(controls, cache, buffers)
         self._decode_step(cache, buffers, _stream(stream), argmax=True, controls=controls)
         buffers.note_recorded(cache.length)
         cache.length += 1
@@ -736,6 +738,7 @@ class DecodeGraph:
 
     def replay(self, steps: int = 1) -> None:
         self.cache.check_room(steps)
+        Transformer._check_recorded(self._controls, self.cache, self.buffers)
         for _ in range(steps):
             _lib.call("kt_graph_launch", self._h, _stream(self.stream))
             self.buffers.note_recorded(self.cache.length)

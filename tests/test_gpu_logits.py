@@ -194,3 +194,29 @@ def test_penalties_need_the_text(kt):
         kt.LogitsControls(allowed=np.ones((2, 100), bool)).descriptor(1, 100)
     with pytest.raises(kt.IllegalArgumentException, match="history"):
         kt.process_logits(kt.DeviceTensor.zeros((1, 100)), controls)
+
+
+def test_text_of_an_earlier_sequence_does_not_count(kt):
+    model = kt.Transformer(100, 128, 1, 2, 128, 1, quantization=kt.Quantization(8, 32))
+    cache, buffers, controls, stream = model.new_cache(60), model.new_inference_buffers(60), kt.LogitsControls(1.2), kt.Stream.create()
+    model.prefill(list(range(20)), cache, buffers, stream, record_tokens=True)
+    model.greedy_decode(cache, buffers, 4, stream, controls=controls)
+    graph = model.capture_decode(cache, buffers, stream, controls)
+    graph.replay(2)
+    cache.reset(stream)
+    for token in (7, 8, 9):
+        model.decode(token, cache, buffers, stream)
+    for call in (lambda: model.greedy_decode(cache, buffers, 4, stream, controls=controls), lambda: model.decode_step(cache, buffers, stream, controls), graph.replay):
+        with pytest.raises(kt.IllegalArgumentException, match="record_tokens"):
+            call()
+    stream.synchronize()
+    graph.destroy()
+    stream.destroy()
+
+
+def test_a_mask_keeps_its_shape(kt):
+    controls = kt.LogitsControls(allowed=np.ones(100, bool))
+    for shape in ((1, 100), (129,), (4, 100)):
+        with pytest.raises(kt.IllegalArgumentException, match="cannot replace"):
+            controls.set_allowed(np.ones(shape, bool))
+    controls.set_allowed(np.zeros(128, bool))  # as many words
