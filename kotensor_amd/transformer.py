@@ -189,6 +189,7 @@ class InferenceBuffers(_Rows):
         self.dimension, self.hidden_dimension = dimension, hidden_dimension
         self.vocabulary_size, self.max_sequence_length, self.kv_dimension = vocabulary_size, max_sequence_length, kv_dimension
         self.logits = DeviceBuffer(vocabulary_size * 4)
+        self.controlled = DeviceBuffer(vocabulary_size * 4)  # LogitsControls' result, of which a step takes the argmax
         self.generated = DeviceBuffer(4 * max_sequence_length)  # greedy tokens by position
         # with LogitsControls: how many leading positions `generated` holds the tokens of (prefill's
         # record_tokens), and where the output starts
@@ -537,16 +538,18 @@ class Transformer:
         _lib.call("kt_rmsnorm_qmatmul_group", x_row_ptr, self.parameters["finalNorm.weight"].ptr,
                   ctypes.c_float(self.norm_eps), buffers.normed.ptr, 1, ws, n, os_, bs, 0, ctypes.c_float(1.0), st)
 
-    def _controlled(self, controls: LogitsControls | None, cache: KVCache, buffers: InferenceBuffers, offset: int, st) -> None:
-        """The controls on buffers.logits, in place, for the text in buffers.generated: as many tokens
-        as the cache's device position + offset. (The logits a caller reads are the controlled ones.)"""
+    def _controlled(self, controls: LogitsControls | None, cache: KVCache, buffers: InferenceBuffers, offset: int, st) -> DeviceBuffer:
+        """The logits of which the next token is the argmax: buffers.logits, or with controls what they make of
+        them for the text in buffers.generated, as many tokens as the cache's device position + offset.
+        buffers.logits stay the model's, so that a call that goes on applies the controls to them anew."""
         if controls is None:
-            return
+            return buffers.logits
         n = self.vocabulary_size
         c = controls.descriptor(1, n, buffers.generated, cache.position, buffers.output_start, buffers.max_sequence_length,
                                 buffers.max_sequence_length, offset)
-        _lib.call("kt_process_logits", buffers.logits.ptr, 1, n, ctypes.c_int64(n), ctypes.byref(c), buffers.logits.ptr,
+        _lib.call("kt_process_logits", buffers.logits.ptr, 1, n, ctypes.c_int64(n), ctypes.byref(c), buffers.controlled.ptr,
                   ctypes.c_int64(n), st)
+        return buffers.controlled
 
     @staticmethod
     def _check_recorded(controls: LogitsControls | None, cache: KVCache, buffers: InferenceBuffers) -> None:
@@ -564,10 +567,10 @@ class Transformer:
         if not headed:
             self._head(buffers.x.ptr, buffers, st)
         if argmax:
-            self._controlled(controls, cache, buffers, 1, st)  # the text ends with this step's token
+            logits = self._controlled(controls, cache, buffers, 1, st)  # the text ends with this step's token
             # the head does not read the position: advance it, take the argmax and record
             # the token in one launch after the head
-            _lib.call("kt_argmax_advance", buffers.logits.ptr, self.vocabulary_size, buffers.tokens.ptr,
+            _lib.call("kt_argmax_advance", logits.ptr, self.vocabulary_size, buffers.tokens.ptr,
                       cache.position.ptr, buffers.generated.ptr, buffers.max_sequence_length, st)
         else:
             _lib.call("kt_position_add", cache.position.ptr, 1, st)
@@ -628,7 +631,10 @@ class Transformer:
         greedy token (which never leaves the device) and taking the next argmax. Returns
         the steps + 1 greedy tokens. With use_graph (on a created, non-null stream) one
         decode step is recorded as a HIP graph and replayed. With ``controls`` every argmax is
-        that of the controlled logits; what was generated from here on is the output."""
+        that of the controlled logits (buffers.logits stay the model's own); what was generated from here on
+        is the output. A call that goes on where another ended chooses that one's last token again, first: the
+        same one while controls and mask are the same. To change the mask from token to token, go on with
+        decode_step or replays."""
         if cache.remaining < steps:
             raise _lib.IllegalArgumentException(
                 f"KV cache full: {cache.length} + {steps} positions exceed maxSequenceLength {cache.max_sequence_length}")
@@ -641,8 +647,8 @@ class Transformer:
         self._check_recorded(controls, cache, buffers)
         if controls is not None:
             buffers.output_start.upload(np.array([first], np.int32), stream)
-            self._controlled(controls, cache, buffers, 0, st)
-        _lib.call("kt_argmax", buffers.logits.ptr, self.vocabulary_size, buffers.tokens.ptr, st)
+        logits = self._controlled(controls, cache, buffers, 0, st)
+        _lib.call("kt_argmax", logits.ptr, self.vocabulary_size, buffers.tokens.ptr, st)
         _lib.call("kt_record_token", buffers.tokens.ptr, cache.position.ptr, buffers.generated.ptr,
                   buffers.max_sequence_length, st)
         if use_graph and steps > 1 and st:
