@@ -192,9 +192,12 @@ class InferenceBuffers(_Rows):
         self.controlled = DeviceBuffer(vocabulary_size * 4)  # LogitsControls' result, of which a step takes the argmax
         self.generated = DeviceBuffer(4 * max_sequence_length)  # greedy tokens by position
         # with LogitsControls: how many leading positions `generated` holds the tokens of (prefill's
-        # record_tokens), and where the output starts
+        # record_tokens), and the position at which the output starts, the last prefill's end: on the host,
+        # and on the device as far as controlled calls have read it
         self.recorded = 0
+        self.output_from = 0
         self.output_start = DeviceBuffer(4)
+        self._output_uploaded = None
         self._prefill: dict[int, _Rows] = {}
 
     def prefill_rows(self, rows: int) -> _Rows:
@@ -202,6 +205,12 @@ class InferenceBuffers(_Rows):
             self._prefill.clear()
             self._prefill[rows] = _Rows(rows, self.dimension, self.hidden_dimension, self.kv_dimension)
         return self._prefill[rows]
+
+    def upload_output_start(self, stream: Stream | None = None) -> None:
+        """Brings the device's output_start to output_from, ahead of a controlled call."""
+        if self._output_uploaded != self.output_from:
+            self.output_start.upload(np.array([self.output_from], np.int32), stream)
+            self._output_uploaded = self.output_from
 
     def note_recorded(self, position: int) -> None:
         """A greedy step at `position` recorded the next token."""
@@ -605,6 +614,7 @@ class Transformer:
             self._embed(rows, len(part), st)
             self._layers(rows, len(part), cache, cache.length + len(part), st)
             cache.advance(len(part), stream)
+        buffers.output_from = cache.length
         self._head(rows.x.ptr + (rows.rows - 1) * self.dimension * 4, buffers, st)
         return buffers
 
@@ -631,10 +641,10 @@ class Transformer:
         greedy token (which never leaves the device) and taking the next argmax. Returns
         the steps + 1 greedy tokens. With use_graph (on a created, non-null stream) one
         decode step is recorded as a HIP graph and replayed. With ``controls`` every argmax is
-        that of the controlled logits (buffers.logits stay the model's own); what was generated from here on
-        is the output. A call that goes on where another ended chooses that one's last token again, first: the
-        same one while controls and mask are the same. To change the mask from token to token, go on with
-        decode_step or replays."""
+        that of the controlled logits (buffers.logits stay the model's own); the output is what
+        follows the last prefill, whichever calls it came from. A call that goes on where another
+        ended first chooses that one's last token again: the same one while controls and mask are the
+        same. To change the mask from token to token, go on with decode_step or replays."""
         if cache.remaining < steps:
             raise _lib.IllegalArgumentException(
                 f"KV cache full: {cache.length} + {steps} positions exceed maxSequenceLength {cache.max_sequence_length}")
@@ -646,7 +656,7 @@ class Transformer:
         first = cache.length
         self._check_recorded(controls, cache, buffers)
         if controls is not None:
-            buffers.output_start.upload(np.array([first], np.int32), stream)
+            buffers.upload_output_start(stream)
         logits = self._controlled(controls, cache, buffers, 0, st)
         _lib.call("kt_argmax", logits.ptr, self.vocabulary_size, buffers.tokens.ptr, st)
         _lib.call("kt_record_token", buffers.tokens.ptr, cache.position.ptr, buffers.generated.ptr,
@@ -668,10 +678,11 @@ class Transformer:
                     controls: LogitsControls | None = None) -> None:
         """One greedy decode step on the device: the token in buffers.tokens (the last
         argmax) in, its logits in buffers.logits, the next argmax in buffers.tokens and in
-        buffers.generated at its position. ``controls`` as in greedy_decode, whose first argmax
-        set buffers.output_start."""
+        buffers.generated at its position. ``controls`` as in greedy_decode."""
         cache.check_room(1)
         self._check_recorded(controls, cache, buffers)
+        if controls is not None:
+            buffers.upload_output_start(stream)
         self._decode_step(cache, buffers, _stream(stream), argmax=True, controls=controls)
         buffers.note_recorded(cache.length)
         cache.length += 1
@@ -745,6 +756,8 @@ class DecodeGraph:
     def replay(self, steps: int = 1) -> None:
         self.cache.check_room(steps)
         Transformer._check_recorded(self._controls, self.cache, self.buffers)
+        if self._controls is not None:
+            self.buffers.upload_output_start(self.stream)
         for _ in range(steps):
             _lib.call("kt_graph_launch", self._h, _stream(self.stream))
             self.buffers.note_recorded(self.cache.length)
