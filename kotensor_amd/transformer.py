@@ -561,10 +561,15 @@ class Transformer:
         return buffers.controlled
 
     @staticmethod
-    def _check_recorded(controls: LogitsControls | None, cache: KVCache, buffers: InferenceBuffers) -> None:
-        if controls is not None and controls.penalized and buffers.recorded < cache.length:
+    def _check_recorded(controls: LogitsControls | None, cache: KVCache, buffers: InferenceBuffers, steps: int = 0) -> None:
+        if controls is None or not controls.penalized:
+            return
+        if buffers.recorded < cache.length:
             raise _lib.IllegalArgumentException(
                 f"penalties need the text's tokens: {buffers.recorded} of {cache.length} are recorded; prefill with record_tokens")
+        if cache.length + steps > buffers.max_sequence_length:
+            raise _lib.IllegalArgumentException(
+                f"InferenceBuffers sized for {buffers.max_sequence_length} positions, the text ends at {cache.length + steps}")
 
     def _decode_step(self, cache: KVCache, buffers: InferenceBuffers, st, argmax: bool,
                      controls: LogitsControls | None = None) -> None:
@@ -680,7 +685,7 @@ class Transformer:
         argmax) in, its logits in buffers.logits, the next argmax in buffers.tokens and in
         buffers.generated at its position. ``controls`` as in greedy_decode."""
         cache.check_room(1)
-        self._check_recorded(controls, cache, buffers)
+        self._check_recorded(controls, cache, buffers, 1)
         if controls is not None:
             buffers.upload_output_start(stream)
         self._decode_step(cache, buffers, _stream(stream), argmax=True, controls=controls)
@@ -755,7 +760,7 @@ class DecodeGraph:
 
     def replay(self, steps: int = 1) -> None:
         self.cache.check_room(steps)
-        Transformer._check_recorded(self._controls, self.cache, self.buffers)
+        Transformer._check_recorded(self._controls, self.cache, self.buffers, steps)
         if self._controls is not None:
             self.buffers.upload_output_start(self.stream)
         for _ in range(steps):

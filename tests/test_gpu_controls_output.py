@@ -80,3 +80,25 @@ def test_a_later_prompt_starts_a_new_output(kt):
     assert got == _plain_steps(model, text, len(text), 5, args)
     graph.destroy()
     stream.destroy()
+
+
+def test_text_behind_the_buffers_end(kt):
+    """A step whose own token has no place in the buffers' record is refused where penalties count it."""
+    banner("controls-output-end")
+    model, controls, stream = _model(kt), kt.LogitsControls(1.2), kt.Stream.create()
+    cache, buffers = model.new_cache(20), model.new_inference_buffers(14)
+    model.prefill(_prompt()[:10], cache, buffers, stream, record_tokens=True)
+    model.greedy_decode(cache, buffers, 2, stream, controls=controls)
+    graph = model.capture_decode(cache, buffers, stream, controls)
+    with pytest.raises(kt.IllegalArgumentException, match="InferenceBuffers sized for 14"):
+        graph.replay(3)
+    graph.replay(1)
+    model.decode_step(cache, buffers, stream, controls)  # takes the token at position 13; its own choice has no place
+    for call in (lambda: model.decode_step(cache, buffers, stream, controls), graph.replay):
+        with pytest.raises(kt.IllegalArgumentException, match="InferenceBuffers sized for 14"):
+            call()
+    assert cache.length == 14
+    model.decode_step(cache, buffers, stream)  # without penalties as before
+    stream.synchronize()
+    graph.destroy()
+    stream.destroy()
