@@ -39,6 +39,8 @@ class LogitsControls:
             self._bias_tokens = DeviceBuffer.from_numpy(np.array(list(bias.keys()), np.int32), stream)
             self._bias_values = DeviceBuffer.from_numpy(np.array(list(bias.values()), np.float32), stream)
         self._allowed, self._words = None, (0, 0)
+        self._entries: int | None = None  # tokens of a boolean mask; packed words hold no length
+        self._vocabulary: int | None = None  # of the calls that the mask was described for
         if allowed is not None:
             self.set_allowed(allowed, stream)
 
@@ -48,8 +50,10 @@ class LogitsControls:
 
     def set_allowed(self, allowed, stream: Stream | None = None) -> None:
         """Sets the mask. Another one of the same shape replaces it in the same device memory, which a
-        recorded step then reads at its next replay; one of another shape is refused."""
+        recorded step then reads at its next replay; one of another shape is refused. A boolean mask has
+        one entry for each token of the vocabulary, packed words as many as hold them."""
         a = np.asarray(allowed)
+        entries = a.shape[-1] if a.ndim and a.dtype == np.bool_ else None
         if a.ndim not in (1, 2) or a.size == 0:
             raise _lib.IllegalArgumentException(f"a mask is an array of the vocabulary, or one a row, got {list(a.shape)}")
         if a.dtype == np.bool_:
@@ -58,12 +62,20 @@ class LogitsControls:
         elif a.dtype not in (np.dtype("u4"), np.dtype("i4")):
             raise _lib.IllegalArgumentException(f"a mask is boolean or packed in 32-bit words, got {a.dtype}")
         words = (a.shape[0] if a.ndim == 2 else 0, a.shape[-1])
+        if self._vocabulary is not None and words == self._words:
+            self._check_entries(entries, self._vocabulary)
         if self._allowed is None:
             self._allowed, self._words = DeviceBuffer(a.nbytes), words
         elif words != self._words:  # (a recorded step may address the memory)
             raise _lib.IllegalArgumentException(
                 f"a mask of {words[0]} rows, {words[1]} words cannot replace one of {self._words[0]} rows, {self._words[1]} words")
         self._allowed.upload(a, stream)
+        self._entries = entries
+
+    @staticmethod
+    def _check_entries(entries: int | None, vocabulary: int) -> None:
+        if entries not in (None, vocabulary):
+            raise _lib.IllegalArgumentException(f"a mask of {entries} tokens for a vocabulary of {vocabulary}")
 
     def descriptor(self, rows: int, vocabulary: int, history=None, history_length=None, output_start=None, history_stride: int = 0,
                    history_capacity: int = 0, length_offset: int = 0) -> _lib.LogitsControls:
@@ -75,6 +87,8 @@ class LogitsControls:
                 raise _lib.IllegalArgumentException(f"a mask of {self._words[0]} rows for {rows} rows of logits")
             if self._words[1] != (vocabulary + 31) // 32:
                 raise _lib.IllegalArgumentException(f"a mask of {self._words[1]} words does not hold {vocabulary} tokens")
+            self._check_entries(self._entries, vocabulary)
+            self._vocabulary = vocabulary
         c = _lib.LogitsControls()
         c.history, c.history_length, c.output_start = _ptr(history), _ptr(history_length), _ptr(output_start)
         c.history_stride, c.history_capacity, c.length_offset = history_stride, history_capacity, length_offset
