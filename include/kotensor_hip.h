@@ -500,8 +500,9 @@ typedef struct kt_logits_controls {
     const uint32_t* allowed;        /* bit i % 32 of word i / 32: token i may follow; or NULL: all may */
     int64_t allowed_stride;         /* words; 0: one mask for all rows */
 } kt_logits_controls;
-/* logits [rows x n], row r at r * stride, into out (which may be logits, then with its stride).
- * Allocates nothing. Asynchronous. */
+/* logits [rows x n], row r at r * stride, into out (which may be logits, then with its stride). kt_argmax
+ * takes logits above -1e9 only: of a row whose mask or biases leave none it gives token 0, so a caller
+ * that chooses by it checks that they leave one. Allocates nothing. Asynchronous. */
 int32_t kt_process_logits(const float* logits, int32_t rows, int32_t n, int64_t stride, const kt_logits_controls* controls,
                           float* out, int64_t out_stride, void* stream);
 /* KVCache.advance on the device copy of the length (K/KVCache.kt:29-35): *position += count. */

@@ -12,6 +12,8 @@ from . import _lib
 from .device import DeviceBuffer, Stream, default_stream
 from .matmul import DeviceTensor, _nbytes, _ptr
 
+NO_CANDIDATE = -1e9  # kt_argmax takes logits above this only
+
 
 class LogitsControls:
     """Penalties, biases and a mask, in this order on a logit x (oracle: the header's formulas):
@@ -23,6 +25,10 @@ class LogitsControls:
     * ``allowed``: tokens that may follow, as a boolean array of the vocabulary (one for all rows,
       or one a row) or, packed, its 32-bit words; the others have minus infinity. A grammar replaces
       it between steps with ``set_allowed``, which keeps the device address.
+
+    The argmax takes no logit at or below -1e9: a bias of that size bans its token, as minus infinity does, and so
+    does such a penalty. Where the mask and the biases leave no token, ``greedy_decode``, ``decode_step`` and replays
+    refuse; where penalties of 1e9 leave none, the argmax gives token 0.
     """
 
     def __init__(self, repetition_penalty: float = 1.0, frequency_penalty: float = 0.0, presence_penalty: float = 0.0,
@@ -35,12 +41,15 @@ class LogitsControls:
         self.repetition_penalty, self.frequency_penalty, self.presence_penalty = map(float, (repetition_penalty, frequency_penalty, presence_penalty))
         self.bias_count = len(bias or {})
         self._bias_ids = sorted(int(t) for t in bias or {})
+        self._banned = [int(t) for t, v in (bias or {}).items() if not v > NO_CANDIDATE]
         if self.bias_count:
             self._bias_tokens = DeviceBuffer.from_numpy(np.array(list(bias.keys()), np.int32), stream)
             self._bias_values = DeviceBuffer.from_numpy(np.array(list(bias.values()), np.float32), stream)
         self._allowed, self._words = None, (0, 0)
         self._entries: int | None = None  # tokens of a boolean mask; packed words hold no length
         self._vocabulary: int | None = None  # of the calls that the mask was described for
+        self._host_words: np.ndarray | None = None
+        self._may_follow: int | None = None  # the vocabulary of which the present mask and biases leave a token
         if allowed is not None:
             self.set_allowed(allowed, stream)
 
@@ -70,16 +79,15 @@ class LogitsControls:
             raise _lib.IllegalArgumentException(
                 f"a mask of {words[0]} rows, {words[1]} words cannot replace one of {self._words[0]} rows, {self._words[1]} words")
         self._allowed.upload(a, stream)
-        self._entries = entries
+        self._entries, self._host_words, self._may_follow = entries, a.view(np.uint32).copy(), None
 
     @staticmethod
     def _check_entries(entries: int | None, vocabulary: int) -> None:
         if entries not in (None, vocabulary):
             raise _lib.IllegalArgumentException(f"a mask of {entries} tokens for a vocabulary of {vocabulary}")
 
-    def descriptor(self, rows: int, vocabulary: int, history=None, history_length=None, output_start=None, history_stride: int = 0,
-                   history_capacity: int = 0, length_offset: int = 0) -> _lib.LogitsControls:
-        """The kt_logits_controls of a call on ``rows`` rows (device buffers or addresses)."""
+    def check(self, rows: int, vocabulary: int) -> None:
+        """Refuses rows of logits that the biases or the mask do not fit."""
         if self._bias_ids and not 0 <= self._bias_ids[0] <= self._bias_ids[-1] < vocabulary:
             raise _lib.IllegalArgumentException(f"a biased token is out of vocab bounds {vocabulary}")
         if self._allowed is not None:
@@ -89,6 +97,26 @@ class LogitsControls:
                 raise _lib.IllegalArgumentException(f"a mask of {self._words[1]} words does not hold {vocabulary} tokens")
             self._check_entries(self._entries, vocabulary)
             self._vocabulary = vocabulary
+
+    def check_choice(self, vocabulary: int) -> None:
+        """Refuses a choice where the mask and the biases leave no token of the vocabulary, which the argmax would
+        answer with token 0."""
+        self.check(1, vocabulary)
+        if self._may_follow == vocabulary:
+            return
+        words = np.full((vocabulary + 31) // 32, 0xFFFFFFFF, np.uint32) if self._host_words is None else self._host_words.reshape(-1).copy()
+        if vocabulary % 32:
+            words[vocabulary // 32] &= np.uint32((1 << vocabulary % 32) - 1)
+        for t in self._banned:
+            words[t // 32] &= np.uint32(~(1 << t % 32) & 0xFFFFFFFF)
+        if not words[:(vocabulary + 31) // 32].any():
+            raise _lib.IllegalArgumentException("no token may follow: the mask and the biases leave none of the vocabulary")
+        self._may_follow = vocabulary
+
+    def descriptor(self, rows: int, vocabulary: int, history=None, history_length=None, output_start=None, history_stride: int = 0,
+                   history_capacity: int = 0, length_offset: int = 0) -> _lib.LogitsControls:
+        """The kt_logits_controls of a call on ``rows`` rows (device buffers or addresses)."""
+        self.check(rows, vocabulary)
         c = _lib.LogitsControls()
         c.history, c.history_length, c.output_start = _ptr(history), _ptr(history_length), _ptr(output_start)
         c.history_stride, c.history_capacity, c.length_offset = history_stride, history_capacity, length_offset

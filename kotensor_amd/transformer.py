@@ -561,8 +561,11 @@ class Transformer:
         return buffers.controlled
 
     @staticmethod
-    def _check_recorded(controls: LogitsControls | None, cache: KVCache, buffers: InferenceBuffers, steps: int = 0) -> None:
-        if controls is None or not controls.penalized:
+    def _check_controls(controls: LogitsControls | None, cache: KVCache, buffers: InferenceBuffers, steps: int = 0) -> None:
+        if controls is None:
+            return
+        controls.check_choice(buffers.vocabulary_size)
+        if not controls.penalized:
             return
         if buffers.recorded < cache.length:
             raise _lib.IllegalArgumentException(
@@ -659,7 +662,7 @@ class Transformer:
                 f"{cache.length + steps + 1}")
         st = _stream(stream)
         first = cache.length
-        self._check_recorded(controls, cache, buffers)
+        self._check_controls(controls, cache, buffers)
         if controls is not None:
             buffers.upload_output_start(stream)
         logits = self._controlled(controls, cache, buffers, 0, st)
@@ -685,7 +688,7 @@ class Transformer:
         argmax) in, its logits in buffers.logits, the next argmax in buffers.tokens and in
         buffers.generated at its position. ``controls`` as in greedy_decode."""
         cache.check_room(1)
-        self._check_recorded(controls, cache, buffers, 1)
+        self._check_controls(controls, cache, buffers, 1)
         if controls is not None:
             buffers.upload_output_start(stream)
         self._decode_step(cache, buffers, _stream(stream), argmax=True, controls=controls)
@@ -760,7 +763,7 @@ class DecodeGraph:
 
     def replay(self, steps: int = 1) -> None:
         self.cache.check_room(steps)
-        Transformer._check_recorded(self._controls, self.cache, self.buffers, steps)
+        Transformer._check_controls(self._controls, self.cache, self.buffers, steps)
         if self._controls is not None:
             self.buffers.upload_output_start(self.stream)
         for _ in range(steps):

@@ -43,3 +43,58 @@ def test_a_mask_replaced_by_one_of_another_length(kt):
         controls.set_allowed(mask)
         want = mask if mask.dtype == bool else np.unpackbits(mask.view(np.uint8), bitorder="little")[:100] > 0
         assert np.array_equal(np.isfinite(kt.process_logits(logits, controls).numpy()[0]), want)
+
+
+def _words_behind(count):
+    words = np.zeros((count + 31) // 32, np.uint32)
+    words[-1] = 0xFFFFFFFF << (count % 32) & 0xFFFFFFFF
+    return words
+
+
+DEAD = {"none": lambda: {"allowed": np.zeros(100, bool)}, "behind the vocabulary": lambda: {"allowed": _words_behind(100)},
+        "all banned": lambda: {"bias": {t: -np.inf for t in range(100)}},
+        "the allowed banned": lambda: {"allowed": np.arange(100) % 50 == 7, "bias": {7: -1e9, 57: -np.inf, 3: 2.0}}}
+
+
+@pytest.mark.parametrize("kind", list(DEAD))
+def test_nothing_may_follow(kt, kind):
+    """A grammar at its end leaves no token to choose: every call that would choose one refuses."""
+    banner("controls-mask-dead", kind)
+    model, controls, stream = _model(kt), kt.LogitsControls(**DEAD[kind]()), kt.Stream.create()
+    cache, buffers = model.new_cache(20), model.new_inference_buffers(20)
+    model.prefill([1, 2, 3], cache, buffers, stream)
+    for call in (lambda: model.greedy_decode(cache, buffers, 4, stream, controls=controls), lambda: model.generate([1, 2, 3], 4, controls=controls),
+                 lambda: model.decode_step(cache, buffers, stream, controls)):
+        with pytest.raises(kt.IllegalArgumentException, match="no token may follow"):
+            call()
+    assert cache.length == 3
+    model.greedy_decode(cache, buffers, 0, stream)
+    model.decode_step(cache, buffers, stream)
+    graph = model.capture_decode(cache, buffers, stream, controls)  # (its mask may be another one when it is replayed)
+    with pytest.raises(kt.IllegalArgumentException, match="no token may follow"):
+        graph.replay()
+    stream.synchronize()
+    graph.destroy()
+    logits = kt.DeviceTensor.zeros((1, 100))  # the logits themselves may be asked for
+    assert np.all(kt.process_logits(logits, controls).numpy()[0] <= -1e9)
+    stream.destroy()
+
+
+def test_a_grammar_that_ends_between_replays(kt):
+    banner("controls-mask-ends")
+    model, stream = _model(kt), kt.Stream.create()
+    controls = kt.LogitsControls(bias={40: 5.0}, allowed=np.ones(100, bool))
+    cache, buffers = model.new_cache(20), model.new_inference_buffers(20)
+    model.prefill([1, 2, 3], cache, buffers, stream)
+    model.greedy_decode(cache, buffers, 2, stream, controls=controls)
+    graph = model.capture_decode(cache, buffers, stream, controls)
+    controls.set_allowed(np.zeros(100, bool), stream)
+    with pytest.raises(kt.IllegalArgumentException, match="no token may follow"):
+        graph.replay()
+    for only in (61, 40):
+        controls.set_allowed(np.arange(100) == only, stream)
+        graph.replay()
+        stream.synchronize()
+        assert buffers.tokens.download(np.int32, count=1)[0] == only
+    graph.destroy()
+    stream.destroy()
