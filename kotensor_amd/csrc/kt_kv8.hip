@@ -329,8 +329,10 @@ __global__ void __launch_bounds__(THREADS) append_kernel(AppendArgs a) {
 //   O^T += V^T P^T: the values lie in memory such that the scores' lanes are the operand's.
 // A wave's maximum follows a row's lazily: a larger score moves it only once it is 2^8 above (the weights
 // then stay below 2^15 in fp16, being taken times 2^6), so that the sums are seldom rescaled.
-// A block's value scale 2^e mu joins the exponent as log2(mu) and e less the largest e so far (uniform):
-// weights include it, and the sum of weights takes it out again, with one product a set of 32 keys.
+// A block's value scale 2^e mu joins the exponent as log2(mu) and e less the row's own exponent, that of its largest
+// contribution (weight times scale) so far, likewise moved lazily: weights include it, and the sum of weights takes it out
+// again, with one product a set of 32 keys. So a weight's parts end 2^-30 below the row's largest contribution, whatever
+// the loudness of blocks that the row hardly attends to or does not see.
 // Waves' sums meet in LDS; key splits' through memory, where the last workgroup of a tile to arrive (a counter,
 // which it returns to zero) merges all in their order: no workgroup waits for another, and the bits do not depend on
 // who is last.
@@ -343,6 +345,7 @@ __global__ void __launch_bounds__(THREADS) append_kernel(AppendArgs a) {
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+typedef float f2v __attribute__((ext_vector_type(2)));
 typedef float f16v __attribute__((ext_vector_type(16)));
 
 struct AttnArgs {
@@ -367,7 +370,8 @@ struct AttnArgs {
 
 constexpr float LAZY = 8.0f;      // how far a score may pass the maximum, in powers of two
 constexpr float WEIGHT_UP = 6.0f; // weights are taken times 2^6
-constexpr int32_t MOST_QUIET = 40; // how far below the largest a value scale's exponent goes into the exponentials
+constexpr float MOST_QUIET = 40.0f; // how far below the row's a value scale's exponent goes into the exponentials
+constexpr float NO_EXPONENT = -1000.0f; // of a row without a contribution so far
 
 // Eight codes as fp16.
 template <int FMT>
@@ -397,7 +401,8 @@ __device__ __forceinline__ void split2(const float (&v)[8], half8& hi, half8& lo
         float a, b;  // what is left of the two: one mixed multiply-add each (the compiler converts and subtracts)
         asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(a) : "v"(h), "v"(v[2 * i]));
         asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(b) : "v"(h), "v"(v[2 * i + 1]));
-        const half2v l = __builtin_bit_cast(half2v, __builtin_amdgcn_cvt_pkrtz(a, b));
+        // (to the nearest, so that what weights below fp16's normal numbers lose has no sign)
+        const half2v l = __builtin_convertvector((f2v{a, b}), half2v);
         hi[2 * i] = h[0];
         hi[2 * i + 1] = h[1];
         lo[2 * i] = l[0];
@@ -412,6 +417,11 @@ __device__ __forceinline__ float weight_of_huge(float x, float f, float m, float
 #pragma clang fp contract(off)
     const float s = x * f;
     return __builtin_amdgcn_exp2f((s - m) - shift);
+}
+// A score as the maxima hold it: rounded, also where the next step subtracts one.
+__device__ __forceinline__ float rounded_score(float x, float f) {
+#pragma clang fp contract(off)
+    return x * f;
 }
 
 // The largest of a value over the lanes of a column (lanes apart by 16 or 32).
@@ -817,18 +827,19 @@ __global__ void __launch_bounds__(64 * NW, R > 16 ? 2 : 1) attention_kernel(Attn
 
     typedef typename std::conditional<X::SMALL, f4, f16v>::type acc_t;
     acc_t o[X::CT][X::DB];
-    float m[X::CT], l[X::CT];
+    // a row's maximum, sum of weights, largest contribution (its exponent, relative to the maximum) and that exponent as a
+    // whole number, whose power of two o is held in
+    float m[X::CT], l[X::CT], reach[X::CT], ex[X::CT];
 #pragma unroll
     for (int ct = 0; ct < X::CT; ++ct) {
         m[ct] = -INFINITY;
         l[ct] = 0.0f;
+        reach[ct] = ex[ct] = NO_EXPONENT;
 #pragma unroll
         for (int db = 0; db < X::DB; ++db)
 #pragma unroll
             for (int e = 0; e < X::OE; ++e) o[ct][db][e] = 0.0f;
     }
-    int32_t e_run = -1000;
-
     // (two forms of the loop's body: only chunks that not every row sees whole compare keys with rows)
     auto attend_chunk = [&](auto masked_form, const int32_t ch) {
         constexpr bool masked = decltype(masked_form)::value;
@@ -875,69 +886,64 @@ __global__ void __launch_bounds__(64 * NW, R > 16 ? 2 : 1) attention_kernel(Attn
             }
         if (h0 + X::J == 2) load_keys(next);
         // the sets' value scales 2^e mu (past the last key the first's again)
-        float vs_h[X::J], ks_h[X::J], shift[X::J], unscale[X::J];
-        int32_t e_h[X::J], quiet[X::J];
+        float ks_h[X::J], e_h[X::J], shift_h[X::J], unscale_h[X::J];
 #pragma unroll
         for (int h = 0; h < X::J; ++h) {
             const bool there = !masked || h == 0 || ch * CHUNK + 32 < n_keys;
             ks_h[h] = there ? ks[h0 + h] : ks[0];
-            vs_h[h] = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, there ? vs[h0 + h] : vs[0])));
-            e_h[h] = static_cast<int32_t>(__builtin_bit_cast(uint32_t, vs_h[h]) >> 23 & 255) - 127;
-        }
-#pragma unroll
-        for (int h = 0; h < X::J; ++h)  // a NaN makes NaNs with any exponent: one that changes nothing for other rows
-            if (vs_h[h] != vs_h[h]) e_h[h] = vs_h[X::J - 1 - h] == vs_h[X::J - 1 - h] ? e_h[X::J - 1 - h] : e_run > -1000 ? e_run : 0;
-        const int32_t e_max = max(e_h[0], e_h[X::J - 1]);
-        if (e_max > e_run) {
-            const float down = ldexpf(1.0f, max(e_run - e_max, -200));
-#pragma unroll
-            for (int ct = 0; ct < X::CT; ++ct)
-#pragma unroll
-                for (int db = 0; db < X::DB; ++db) o[ct][db] *= down;
-            e_run = e_max;
-        }
-#pragma unroll
-        for (int h = 0; h < X::J; ++h) {
-            const float mu = ldexpf(vs_h[h], -e_h[h]);
-            quiet[h] = e_run - e_h[h];
-            const int32_t in_exp = quiet[h] <= MOST_QUIET ? quiet[h] : 0;
-            quiet[h] -= in_exp;
-            shift[h] = static_cast<float>(in_exp) - __builtin_amdgcn_logf(mu) - WEIGHT_UP;
-            unscale[h] = ldexpf(__builtin_amdgcn_rcpf(mu), in_exp);  // (off by one unit at most, as a weight's rounding)
+            const float vs_h = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, there ? vs[h0 + h] : vs[0])));
+            const int32_t e = static_cast<int32_t>(__builtin_bit_cast(uint32_t, vs_h) >> 23 & 255) - 127;  // (of a NaN any)
+            const float mu = ldexpf(vs_h, -e);
+            e_h[h] = static_cast<float>(e);
+            shift_h[h] = -__builtin_amdgcn_logf(mu) - WEIGHT_UP;
+            unscale_h[h] = __builtin_amdgcn_rcpf(mu);  // (off by one unit at most, as a weight's rounding)
         }
         half8 ph[X::J][X::CT][X::VL], pl[X::J][X::CT][X::VL];
 #pragma unroll
         for (int ct = 0; ct < X::CT; ++ct) {
-            float x[X::J][X::E], f[X::J], top = -INFINITY;
+            // a set's scores, the largest, and how far above the row's exponent (where it is) its value scale's is
+            float x[X::J][X::E], f[X::J], most[X::J], above = -INFINITY;
 #pragma unroll
             for (int h = 0; h < X::J; ++h) {
                 f[h] = ks_h[h] * fr[ct];
-                float most = -INFINITY;
+                most[h] = -INFINITY;
 #pragma unroll
                 for (int i = 0; i < X::E; ++i) {
                     x[h][i] = X::SMALL ? sc[h][ct][X::SMALL ? i >> 2 : 0][X::SMALL ? i & 3 : i] : sc[h][ct][0][i];
                     if (masked && ch * CHUNK + 32 * (h0 + h) + key_of(i) > last[ct]) x[h][i] = -INFINITY;
-                    most = fmaxf(most, x[h][i]);
+                    most[h] = fmaxf(most[h], x[h][i]);
                 }
-                top = fmaxf(top, most * f[h]);
+                most[h] = rounded_score(most[h], f[h]);
+                above = fmaxf(above, (most[h] - m[ct]) + fmaxf(e_h[h] - ex[ct], 0.0f));
             }
-            if (__ballot(top > m[ct] + LAZY)) {
-                const float m_new = fmaxf(m[ct], column_max<R>(top));
-                const float alpha = m[ct] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[ct] - m_new);
+            if (__ballot(above > LAZY)) {
+                const float m_new = fmaxf(m[ct], column_max<R>(fmaxf(most[0], most[X::J - 1])));
+                float r = NO_EXPONENT;
+#pragma unroll
+                for (int h = 0; h < X::J; ++h) r = fmaxf(r, (most[h] - m_new) + e_h[h]);
+                const bool first = m[ct] == -INFINITY;
+                const float fall = first ? 0.0f : m[ct] - m_new, alpha = first ? 0.0f : __builtin_amdgcn_exp2f(fall);
+                reach[ct] = fmaxf(reach[ct] + fall, column_max<R>(r));
+                const float ex_new = rintf(fmaxf(reach[ct], NO_EXPONENT));
+                const float beta = first ? 0.0f : __builtin_amdgcn_exp2f(fall + (ex[ct] - ex_new));
                 l[ct] *= alpha;
 #pragma unroll
-                for (int db = 0; db < X::DB; ++db) o[ct][db] *= alpha;
+                for (int db = 0; db < X::DB; ++db) o[ct][db] *= beta;
                 m[ct] = m_new;
+                ex[ct] = ex_new;
             }
             const float at = m[ct] == -INFINITY ? 0.0f : m[ct];
             const bool huge = __ballot(fabsf(at) > HUGE_SCORE);  // (one-hot rows)
 #pragma unroll
             for (int h = 0; h < X::J; ++h) {
+                float quiet = ex[ct] - e_h[h];
+                const float in_exp = quiet <= MOST_QUIET ? quiet : 0.0f, shift = in_exp + shift_h[h];
+                quiet -= in_exp;
                 if (huge) {
 #pragma unroll
-                    for (int i = 0; i < X::E; ++i) x[h][i] = weight_of_huge(x[h][i], f[h], at, shift[h]);
+                    for (int i = 0; i < X::E; ++i) x[h][i] = weight_of_huge(x[h][i], f[h], at, shift);
                 } else {
-                    const float both = at + shift[h];
+                    const float both = at + shift;
 #pragma unroll
                     for (int i = 0; i < X::E; ++i) x[h][i] = __builtin_amdgcn_exp2f(fmaf(x[h][i], f[h], -both));
                 }
@@ -947,9 +953,10 @@ __global__ void __launch_bounds__(64 * NW, R > 16 ? 2 : 1) attention_kernel(Attn
                     if (masked && ch * CHUNK + 32 * (h0 + h) + key_of(i) > last[ct]) x[h][i] = 0.0f;
                     sum += x[h][i];
                 }
-                l[ct] += sum == 0.0f ? 0.0f : sum * unscale[h];  // (0 * NaN: a row that sees none of the block)
-                if (quiet[h]) {
-                    const float down = ldexpf(1.0f, max(-quiet[h], -200));
+                // (0 * NaN: a row that sees none of the block)
+                l[ct] += sum == 0.0f ? 0.0f : sum * ldexpf(unscale_h[h], static_cast<int32_t>(in_exp));
+                if (quiet != 0.0f) {
+                    const float down = ldexpf(1.0f, static_cast<int32_t>(fmaxf(-quiet, -200.0f)));
 #pragma unroll
                     for (int i = 0; i < X::E; ++i) x[h][i] *= down;
                 }
@@ -1006,7 +1013,7 @@ __global__ void __launch_bounds__(64 * NW, R > 16 ? 2 : 1) attention_kernel(Attn
                 for (int e = 0; e < X::OE; e += 4) {
                     f4 v;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) v[i] = ldexpf(o[ct][db][e + i] * inv, e_run);
+                    for (int i = 0; i < 4; ++i) v[i] = ldexpf(o[ct][db][e + i] * inv, static_cast<int32_t>(ex[ct]));
                     *reinterpret_cast<f4*>(row + (X::SMALL ? 16 * db + 4 * grp : 32 * db + 2 * e + 4 * grp)) = v;
                 }
             if (grp == 0) {
