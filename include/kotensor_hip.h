@@ -349,7 +349,9 @@ int32_t kt_rope_attention(float* q, float* k, const float* v, const float* inv_f
  * While a block is not full its rows are kept in fp32 too (key_rows, value_rows), and an append
  * that raises its scale encodes it again from them, so the cache holds the same bits whatever the
  * calls its rows came in. An append continues the cache where the last one ended, or starts it again
- * at position 0 or at the first token of a block; after kt_kv8_copy it continues the copy.
+ * at position 0 or at the first token of a block; after kt_kv8_copy it continues the copy. A scale
+ * with its sign bit set (kt_kv8_copy) stands for its magnitude; the next append into its block makes
+ * the block's scale and codes anew from the fp32 rows.
  * The caller owns the memory: kt_kv8_layout's sizes, codes and rows 16-byte aligned. Keys lie as
  * [layers][kv_heads][slots][head_dim] codes, slots = max_seq rounded up to whole blocks and to
  * a multiple of 64; values as [layers][kv_heads][slots / 64][head_dim][64], token
@@ -398,9 +400,12 @@ int32_t kt_rope_attention_kv8(float* q, const float* k, const float* v, const fl
 int32_t kt_kv8_read(const kt_kv8_cache* cache, int32_t layer, int32_t first, int32_t count, float* keys,
                     float* values, void* stream);
 /* KVCache.copyFrom (K/KVCache.kt:41-55): the first `length` positions of every layer of `source`, which
- * holds source_length. The codes and scales are the source's; where the copy ends inside a block that the
- * source has gone past, that block's fp32 rows start from what its codes stand for. The cache may be
- * the source itself: it is then shortened. */
+ * holds source_length. The codes and scales are the source's. Where the copy drops rows of the source's open
+ * block, the next append encodes that block as if they had never been there (until then its tokens
+ * are read as the source holds them). Where it ends inside a block that the source has gone past, that
+ * block's fp32 rows are gone: they start from what its codes stand for, under the scale that the dropped
+ * rows had a part in (NaN if one of them was not finite). The cache may be the source itself: it is
+ * then shortened. */
 int32_t kt_kv8_copy(const kt_kv8_cache* source, int32_t source_length, const kt_kv8_cache* cache, int32_t length,
                     void* stream);
 

@@ -13,7 +13,9 @@
 // 127 for int8, 448 for e4m3), its codes the nearest to x * (1 / s), ties to even; a value that is
 // not finite makes the scale NaN. An append that raises the scale of the open block encodes the
 // block again from its fp32 rows, so what the cache holds depends on the rows alone, not on the
-// calls they came in.
+// calls they came in. A copy that ends inside the source's open block drops rows that the block's scale may
+// come from: it sets the scale's sign bit (readers take the magnitude), and the next append makes the scale and
+// the codes anew from the rows that stayed.
 #include <math.h>
 
 #include <algorithm>
@@ -164,6 +166,8 @@ __device__ __forceinline__ uint32_t block_max(uint32_t m, uint32_t (&part)[THREA
 }
 
 __device__ __forceinline__ uint32_t magnitude(float x) { return __builtin_bit_cast(uint32_t, x) & 0x7FFFFFFFu; }
+// Whether a block's scale says that rows of it were dropped (a NaN may say so, too).
+__device__ __forceinline__ bool shortened(float scale) { return __builtin_bit_cast(uint32_t, scale) >> 31; }
 
 // The block b of a head, of whose rows 0 .. n - 1 those from lo on are new.
 template <int FMT, bool KEYS>
@@ -228,9 +232,17 @@ __device__ void append_block(const AppendArgs& a, float* lds, uint32_t (&part)[T
         }
     }
     m = block_max(m, part);
-    float s = scale_of<FMT>(m);
     int32_t from = lo;
-    if (lo > 0) {
+    if (lo > 0 && shortened(held)) {  // the earlier rows that stayed, and the scale of all
+        from = 0;
+        for (int32_t e = tid; e < lo * HD; e += THREADS) {
+            lds[e / HD * LR + e % HD] = rows[e];
+            m = max(m, magnitude(rows[e]));
+        }
+        m = block_max(m, part);
+    }
+    float s = scale_of<FMT>(m);
+    if (from > 0) {
         if (held != held || held >= s) {
             s = held;
         } else if (s == s) {  // raised: the earlier rows again
@@ -495,6 +507,7 @@ struct StepShared {
     __attribute__((aligned(16))) float cosines[HD / 2], sines[HD / 2];
     __attribute__((aligned(16))) uint8_t key[HD], value[HD];
     uint32_t top[4];
+    uint32_t rest[2][8];
 };
 template <int HD>
 struct StepShared<HD, false> {};
@@ -508,14 +521,32 @@ __device__ bool append_token(const KV8View& c, StepShared<HD, true>& sh, int32_t
     constexpr int HALF = HD / 2;
     const int32_t tid = threadIdx.x, B = c.block, b = pos / B, r = pos % B, i = tid & 127;
     const bool is_key = tid < 128;
-    const float own[2] = {scale_of<FMT>(max(sh.top[0], sh.top[1])), scale_of<FMT>(max(sh.top[2], sh.top[3]))};
+    uint32_t most[2] = {max(sh.top[0], sh.top[1]), max(sh.top[2], sh.top[3])};
+    float* rows[2] = {c.key_rows + static_cast<size_t>(g) * B * HD, c.value_rows + static_cast<size_t>(g) * B * HD};
+    const bool remake[2] = {r > 0 && shortened(held[0]), r > 0 && shortened(held[1])};
+    if (remake[0] || remake[1]) {  // the earlier rows that stayed count for the scale
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+            uint32_t m = 0;
+            for (int32_t e = tid; e < r * (HD / 4); e += NT) {
+                const f4 x = *reinterpret_cast<const f4*>(rows[w] + 4 * e);
+                m = max(max(m, max(magnitude(x[0]), magnitude(x[1]))), max(magnitude(x[2]), magnitude(x[3])));
+            }
+            for (int o = 32; o > 0; o >>= 1) m = max(m, static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), o)));
+            if ((tid & 63) == 0) sh.rest[w][tid >> 6] = m;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < 2; ++w)
+            for (int i = 0; remake[w] && i < NT / 64; ++i) most[w] = max(most[w], sh.rest[w][i]);
+    }
     bool raised[2];
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
-        raised[w] = r > 0 && held[w] < own[w];  // (neither of them NaN)
-        if (r == 0 || raised[w] || own[w] != own[w]) held[w] = own[w];
+        const float own = scale_of<FMT>(most[w]);
+        raised[w] = r > 0 && (remake[w] ? own == own : held[w] < own);  // (below: neither of them NaN)
+        if (r == 0 || raised[w] || remake[w] || own != own) held[w] = own;
     }
-    float* rows[2] = {c.key_rows + static_cast<size_t>(g) * B * HD, c.value_rows + static_cast<size_t>(g) * B * HD};
     uint8_t* kdst = c.keys + (static_cast<size_t>(g) * c.slots + static_cast<size_t>(b) * B) * HD;
     uint8_t* vdst = c.values + static_cast<size_t>(g) * c.slots * HD;
     auto value_to = [&](int32_t tok, int32_t d) { return vdst + (static_cast<size_t>(tok / CHUNK) * HD + d) * CHUNK + value_byte(tok % CHUNK / 4) + tok % 4; };
@@ -890,10 +921,10 @@ __global__ void __launch_bounds__(64 * NW, R > 16 ? 2 : 1) attention_kernel(Attn
 #pragma unroll
         for (int h = 0; h < X::J; ++h) {
             const bool there = !masked || h == 0 || ch * CHUNK + 32 < n_keys;
-            ks_h[h] = there ? ks[h0 + h] : ks[0];
-            const float vs_h = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, there ? vs[h0 + h] : vs[0])));
-            const int32_t e = static_cast<int32_t>(__builtin_bit_cast(uint32_t, vs_h) >> 23 & 255) - 127;  // (of a NaN any)
-            const float mu = ldexpf(vs_h, -e);
+            ks_h[h] = fabsf(there ? ks[h0 + h] : ks[0]);
+            const uint32_t vs_h = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(magnitude(there ? vs[h0 + h] : vs[0]))));
+            const int32_t e = static_cast<int32_t>(vs_h >> 23) - 127;  // (of a NaN any)
+            const float mu = ldexpf(__builtin_bit_cast(float, vs_h), -e);
             e_h[h] = static_cast<float>(e);
             shift_h[h] = -__builtin_amdgcn_logf(mu) - WEIGHT_UP;
             unscale_h[h] = __builtin_amdgcn_rcpf(mu);  // (off by one unit at most, as a weight's rounding)
@@ -1155,7 +1186,7 @@ __global__ void __launch_bounds__(THREADS) read_kernel(KV8View c, int32_t first,
         const int32_t per = nd / 16, r = tid / per, d = 16 * (tid % per), tok = tok0 + r;
         if (r >= CHUNK || !inside(tok)) return;
         const u4 w = *reinterpret_cast<const u4*>(src + r * HD + d0 + d);
-        const float s = scales[tok / c.block];
+        const float s = fabsf(scales[tok / c.block]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             float x[4];
@@ -1170,7 +1201,7 @@ __global__ void __launch_bounds__(THREADS) read_kernel(KV8View c, int32_t first,
 #pragma unroll
     for (int u = 0; u < OUT; ++u) {
         const int32_t tok = tok0 + min((tid + u * THREADS) / groups, CHUNK - 1);
-        s[u] = inside(tok) ? scales[tok / c.block] : 0.0f;
+        s[u] = inside(tok) ? fabsf(scales[tok / c.block]) : 0.0f;
     }
     if (tid < 4 * nd) {  // (dim, piece)
         const int32_t d = tid / 4, piece = tid % 4;
@@ -1197,7 +1228,9 @@ __global__ void __launch_bounds__(THREADS) read_kernel(KV8View c, int32_t first,
 }
 
 // Workgroup (chunk, kv head): the chunk's codes and scales; the workgroups of chunk 0 also the open block's
-// rows, from the source's rows where it is the source's open block too, else from its codes.
+// rows, from the source's rows where it is the source's open block too, else from its codes. Where the source's
+// open block loses rows, its scale says so. (The cache may be the source: a thread writes a scale that
+// it alone has read, and codes and rows as they are.)
 template <int FMT>
 __global__ void __launch_bounds__(THREADS) copy_kernel(KV8View to, KV8View from, int32_t length, int32_t source_length) {
     const int32_t HD = to.head_dim, B = to.block, g = blockIdx.y, tid = threadIdx.x;
@@ -1213,14 +1246,15 @@ __global__ void __launch_bounds__(THREADS) copy_kernel(KV8View to, KV8View from,
     const float* vs = from.value_scales + head_to * (from.slots / B);
     const int32_t per = max(1, CHUNK / B), blocks = (length + B - 1) / B;
     const int32_t b = B > CHUNK ? (blockIdx.x % 2 == 0 ? blockIdx.x / 2 : blocks) : blockIdx.x * per + tid;
+    const int32_t open = length / B;
+    const bool same = open == source_length / B;
     if (tid < per && b < blocks) {
-        to.key_scales[head_to * (to.slots / B) + b] = ks[b];
-        to.value_scales[head_to * (to.slots / B) + b] = vs[b];
+        const bool drops = same && b == open && length < source_length;
+        to.key_scales[head_to * (to.slots / B) + b] = drops ? -fabsf(ks[b]) : ks[b];
+        to.value_scales[head_to * (to.slots / B) + b] = drops ? -fabsf(vs[b]) : vs[b];
     }
     if (blockIdx.x != 0 || length % B == 0) return;
-    const int32_t open = length / B;
     const size_t rows = head_to * B * HD;
-    const bool same = open == source_length / B;
     for (int32_t e = tid; e < length % B * HD; e += THREADS) {
         if (same) {
             to.key_rows[rows + e] = from.key_rows[rows + e];
