@@ -1352,15 +1352,22 @@ int32_t launch_rows(AttnArgs a, int32_t key_bound, hipStream_t st, AppendArgs* a
         if (const int32_t status = turned.take(CALL_SLICES, st, bytes)) return status;
         append->q_out = static_cast<float*>(turned.ptr);
     }
-    const bool in_workspace = append && !STEP && !turned.ptr;  // (a capture begun by other means)
-    if (a.max_splits > 1 || in_workspace) {
-        const size_t rows = static_cast<size_t>(wgs) * a.max_splits * R, q = in_workspace ? static_cast<size_t>(a.num_heads) * HD : 0;
+    // The workspace: the splits' averages and sums, behind room for that query, which a capture begun by other means takes
+    // (no scratch to have there) and an eager call reserves: it sizes what a recording of its shapes needs.
+    size_t q = 0;
+    if (append && !STEP) {
+        hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+        if (turned.ptr) KT_HIP(hipStreamIsCapturing(st, &capture));
+        if (capture == hipStreamCaptureStatusNone) q = static_cast<size_t>(a.num_heads) * HD;
+    }
+    if (a.max_splits > 1 || q > 0) {
+        const size_t rows = a.max_splits > 1 ? static_cast<size_t>(wgs) * a.max_splits * R : 0;
         void* ws = nullptr;
         if (const int32_t status = workspace_counters(st, (rows * (HD + 2) + q) * sizeof(float) + 16, a.max_splits > 1 ? static_cast<size_t>(wgs) : 0, &ws, &a.counters)) return status;
         ws = reinterpret_cast<void*>((reinterpret_cast<uintptr_t>(ws) + 15) & ~uintptr_t{15});  // (it begins at any dword)
         a.averages = static_cast<float*>(ws) + q;
         a.stats = a.averages + rows * HD;
-        if (in_workspace) append->q_out = static_cast<float*>(ws);
+        if (append && !STEP && !turned.ptr) append->q_out = static_cast<float*>(ws);
     }
     if (append && !STEP) {
         a.q = append->q_out;

@@ -1,0 +1,94 @@
+"""How calls on an 8-bit cache are launched: captures that the library did not begin."""
+import ctypes
+
+import numpy as np
+import pytest
+
+from gpu_helpers import banner, same_bits
+from test_gpu_kv8 import _append, _dev, _inv_freq, _rows
+from test_gpu_recorded_scratch import _hip
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("heads,kv,d", [(2, 1, 256), (8, 4, 256), (20, 1, 64), (34, 2, 128)])
+@pytest.mark.parametrize("start,bound", [(10, 64), (700, 4000)])
+def test_a_callers_own_capture_of_a_step(kt, heads, kv, d, start, bound):
+    """Steps whose append is a launch of its own: one eager call of the same shapes on the stream has sized what
+    a capture begun with HIP itself needs, with and without key splits."""
+    from kotensor_amd import _lib
+    banner("kv8-own-capture", heads, kv, d, start, bound)
+    rng = np.random.default_rng(heads + d)
+    k, v = _rows(rng, start + 4, kv, d), _rows(rng, start + 4, kv, d)
+    one, two = (kt.QuantizedKVCache(1, kv, bound, d, "int8", 64) for _ in range(2))
+    for c in (one, two):
+        _append(kt, c, 0, k[:start], v[:start], 0)
+        c.advance(start)
+    freq, stream, out = _dev(kt, _inv_freq(d)), kt.Stream.create(), kt.DeviceBuffer(4 * heads * d)
+    dq, dk, dv = kt.DeviceBuffer(4 * heads * d), kt.DeviceBuffer(4 * kv * d), kt.DeviceBuffer(4 * kv * d)
+    q = rng.standard_normal((4, heads * d)).astype(np.float32)
+
+    def run(cache):
+        _lib.call("kt_rope_attention_kv8", dq.ptr, dk.ptr, dv.ptr, freq.ptr, 1, cache.position.ptr, bound, ctypes.byref(cache.cache), 0, heads, out.ptr, stream.handle)
+        _lib.call("kt_position_add", cache.position.ptr, 1, stream.handle)
+
+    def load(i):
+        dq.upload(q[i])
+        dk.upload(k[start + i])
+        dv.upload(v[start + i])
+        out.fill_zero()
+        kt.synchronize()
+    want = []
+    for i in range(4):
+        load(i)
+        run(one)
+        stream.synchronize()
+        want.append(out.download(np.float32))
+    hip, handle, graph, exe = _hip(), ctypes.c_void_p(stream.handle), ctypes.c_void_p(), ctypes.c_void_p()
+    assert hip.hipStreamBeginCapture(handle, 1) == 0  # thread-local
+    try:
+        run(two)
+    finally:
+        assert hip.hipStreamEndCapture(handle, ctypes.byref(graph)) == 0
+    assert hip.hipGraphInstantiate(ctypes.byref(exe), graph, None, None, ctypes.c_size_t(0)) == 0
+    assert hip.hipGraphDestroy(graph) == 0
+    for i in range(4):
+        load(i)
+        _lib.call("kt_graph_launch", exe, stream.handle)
+        stream.synchronize()
+        assert same_bits(out.download(np.float32), want[i]), i
+    for a, b in zip(one.rows_numpy(0, 0, start + 4), two.rows_numpy(0, 0, start + 4)):
+        assert same_bits(a, b)
+    assert hip.hipGraphExecDestroy(exe) == 0
+    stream.destroy()
+
+
+def test_a_recording_without_an_eager_call(kt):
+    """A step of 256 dims without key splits needs nothing of its stream: it is recorded on a new one."""
+    from kotensor_amd import _lib
+    banner("kv8-record-first")
+    rng = np.random.default_rng(3)
+    heads, kv, d = 4, 2, 256
+    k, v, q = _rows(rng, 11, kv, d), _rows(rng, 11, kv, d), rng.standard_normal(heads * d).astype(np.float32)
+    one, two = (kt.QuantizedKVCache(1, kv, 64, d, "e4m3", 32) for _ in range(2))
+    for c in (one, two):
+        _append(kt, c, 0, k[:10], v[:10], 0)
+        c.advance(10)
+    dq, dk, dv, freq, out = _dev(kt, q), _dev(kt, k[10]), _dev(kt, v[10]), _dev(kt, _inv_freq(d)), [kt.DeviceBuffer(q.nbytes) for _ in range(2)]
+    stream, graph = kt.Stream.create(), ctypes.c_void_p()
+
+    def run(cache, out, st):
+        _lib.call("kt_rope_attention_kv8", dq.ptr, dk.ptr, dv.ptr, freq.ptr, 1, cache.position.ptr, 64, ctypes.byref(cache.cache), 0, heads, out.ptr, st)
+    kt.synchronize()
+    _lib.call("kt_graph_begin", stream.handle)
+    try:
+        run(one, out[0], stream.handle)
+    finally:
+        _lib.call("kt_graph_end", stream.handle, ctypes.byref(graph))
+    _lib.call("kt_graph_launch", graph, stream.handle)
+    stream.synchronize()
+    run(two, out[1], None)
+    kt.synchronize()
+    assert same_bits(out[0].download(np.float32), out[1].download(np.float32))
+    _lib.call("kt_graph_destroy", graph)
+    stream.destroy()
