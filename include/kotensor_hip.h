@@ -385,9 +385,12 @@ int32_t kt_rope_kv8(const float* q, const float* k, const float* v, int32_t toke
                     float* q_out, void* stream);
 /* kt_attention over such a cache (K/Attention.kt:277-349 on what its codes stand for): token t's
  * softmax(q . k_j / sqrt(head_dim)) over j <= *position + t, times v, into context; sums and softmax in
- * fp32, a key's weight times its block's value scale to 2^-30 of the row's largest. A token that sees no key (a negative position) gets zeros; scores are taken to lie in
- * fp32's range. q and context are 16-byte aligned and apart; tokens * num_heads / kv_heads is at most
- * 1048560. As kt_attention's, its workspace is sized by one eager call before a recording. */
+ * fp32, a key's weight times its block's value scale to 2^-30 of the row's largest. A token that sees no
+ * key (a negative position) gets zeros; scores are taken to lie in fp32's range. q and context are 16-byte
+ * aligned and apart; tokens * num_heads / kv_heads is at most 1048560. key_bound sizes the launch: up to 1024
+ * keys (640 of 128 dims) another form runs than beyond, whose sums have another order, so calls with bounds on both
+ * sides agree to rounding and not in every bit. As kt_attention's, its workspace is sized by one eager
+ * call before a recording. */
 int32_t kt_attention_kv8(const float* q, int32_t tokens, const int32_t* position, int32_t key_bound,
                          const kt_kv8_cache* cache, int32_t layer, int32_t num_heads, float* context, void* stream);
 /* kt_rope_kv8 followed by kt_attention_kv8. For one token q stays as it is; for more it is

@@ -1333,8 +1333,12 @@ int32_t attention_args(const float* q, int32_t tokens, const int32_t* position, 
     return KT_OK;
 }
 
-// Up to so many keys one workgroup of 8 waves takes them without splits. A step of 32 heads, with the call, and with
-// splits: heads of 64 after 500 keys 8.8 us (10.6), 1000 10.2 (10.4), 1500 11.8 (10.5); of 128 500 11.9 (12.6), 760 13.0 (12.5).
+// Up to so many keys one workgroup of 8 waves takes them without splits. The rule reads key_bound, for a recorded step
+// all that the host knows: in Transformer the cache's capacity, so a short text in a long cache takes the splits' form, and the
+// same text in caches on both sides of the limit has sums in another order. Steps of 32 heads of 64 traced, bound 1024 (8192):
+// 200 keys 7.8 us (8.0), 500 8.9 (10.6), 1000 11.2 (10.9); 14 heads, 2 kv heads, 543 8.6 (10.6). With the call, and a bound
+// at the length: heads of 64 after 500 keys 8.8 us (with splits 10.6), 1000 10.2 (10.4), 1500 11.8 (10.5); of 128 500 11.9
+// (12.6), 760 13.0 (12.5).
 constexpr int direct_keys(int hd) { return hd <= 64 ? 16 * CHUNK : 10 * CHUNK; }
 
 template <int FMT, int HD, int R, int WAVES, bool STEP = false>

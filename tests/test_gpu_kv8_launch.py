@@ -1,11 +1,14 @@
-"""How calls on an 8-bit cache are launched: captures that the library did not begin."""
+"""How calls on an 8-bit cache are launched: captures that the library did not begin, and bounds on both sides of the
+length at which the form of the attention changes."""
 import ctypes
 
 import numpy as np
 import pytest
 
+from conftest import normwise_rel
 from gpu_helpers import banner, same_bits
-from test_gpu_kv8 import _append, _dev, _inv_freq, _rows
+from oracle import kv8_ref
+from test_gpu_kv8 import _append, _attend, _dev, _filled, _inv_freq, _rows, _tolerance
 from test_gpu_recorded_scratch import _hip
 
 pytestmark = pytest.mark.gpu
@@ -92,3 +95,18 @@ def test_a_recording_without_an_eager_call(kt):
     assert same_bits(out[0].download(np.float32), out[1].download(np.float32))
     _lib.call("kt_graph_destroy", graph)
     stream.destroy()
+
+
+@pytest.mark.parametrize("fmt,block", [("int8", 64), ("e4m3", 128)])
+@pytest.mark.parametrize("tokens,start,heads,kv,d,wide", [(1, 980, 32, 8, 64, 1060), (1, 600, 32, 8, 128, 700), (7, 1000, 14, 2, 64, 9000), (16, 500, 6, 6, 32, 1100), (3, 630, 8, 1, 128, 5000)])
+def test_bounds_on_both_sides_of_a_form(kt, fmt, block, tokens, start, heads, kv, d, wide):
+    """A bound of up to 1024 keys (640 of 128 dims) takes the keys in one workgroup, a larger one in splits: the
+    sums' order differs, so the bits may; each is within the tolerance."""
+    banner("kv8-bounds", fmt, block, tokens, start, heads, kv, d, wide)
+    rng = np.random.default_rng(start)
+    n = start + tokens
+    cache, keys, values = _filled(kt, rng, fmt, block, d, kv, n, wide)
+    q = (1.5 * rng.standard_normal((tokens, heads * d))).astype(np.float32)
+    want = kv8_ref.attend(q, keys, values, start, heads)
+    for bound in (n, wide):
+        assert normwise_rel(_attend(kt, cache, 0, q, start, heads, bound), want) <= _tolerance(q, keys, heads)
