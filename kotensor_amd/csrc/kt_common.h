@@ -4,6 +4,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <memory>
 
 #include "../../include/kotensor_hip.h"
@@ -27,6 +28,24 @@ int32_t hip_fail(hipError_t err, const char* what);
         hipError_t kt_err_ = hipGetLastError();                  \
         if (kt_err_ != hipSuccess) return ::kt::hip_fail(kt_err_, name); \
     } while (0)
+
+// gfx950 gives a workgroup up to 160 KB of LDS; a kernel asks for more than 64 KB of dynamic LDS by
+// raising its attribute first. allow_lds raises kernel KERN's to BYTES (where the kernel has static
+// LDS beside it, to exactly what its launches need) when a launch needs more than the default, once for
+// each device: the attribute is the current device's.
+constexpr size_t LDS_DEFAULT = 64 << 10, LDS_MAX = 160 << 10;
+template <auto KERN, size_t BYTES = LDS_MAX>
+int32_t allow_lds(size_t lds) {
+    static std::atomic<uint64_t> raised{0};  // a bit for each of 64 devices; further ones raise it every time
+    if (lds <= LDS_DEFAULT) return KT_OK;
+    int device = 0;
+    KT_HIP(hipGetDevice(&device));
+    const uint64_t bit = device >= 0 && device < 64 ? uint64_t{1} << device : 0;
+    if (raised.load(std::memory_order_acquire) & bit) return KT_OK;
+    KT_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(KERN), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(BYTES)));
+    raised.fetch_or(bit, std::memory_order_release);
+    return KT_OK;
+}
 
 // Device workspace owned by the library, one per (device, stream). Calls on one
 // stream are ordered by that stream, so they may reuse the same bytes. Growing it

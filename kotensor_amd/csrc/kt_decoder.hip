@@ -24,7 +24,6 @@
 // differ from the reference's sequential sums by fp32 rounding only.
 #include <math.h>
 
-#include <atomic>
 
 #include "kt_common.h"
 #include "kt_split.h"
@@ -1606,12 +1605,7 @@ static int32_t attention_launch(const float* q, int32_t tokens, const int32_t* p
         if (head_dim == 64) {
             attention_prefill_kernel<64><<<grid, THREADS, sizeof(PrefillShared<64>), st>>>(a, tokens, qb_tokens, nqb, paired);
         } else {
-            static std::atomic<bool> raised{false};
-            if (!raised) {  // beyond the default dynamic LDS limit (160 KB per CU on gfx950)
-                KT_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&attention_prefill_kernel<128>),
-                                           hipFuncAttributeMaxDynamicSharedMemorySize, sizeof(PrefillShared<128>)));
-                raised = true;
-            }
+            if (const int32_t ls = allow_lds<&attention_prefill_kernel<128>, sizeof(PrefillShared<128>)>(sizeof(PrefillShared<128>))) return ls;
             attention_prefill_kernel<128><<<grid, THREADS, sizeof(PrefillShared<128>), st>>>(a, tokens, qb_tokens, nqb,
                                                                                           paired);
         }
@@ -1696,16 +1690,8 @@ static int32_t attention_launch(const float* q, int32_t tokens, const int32_t* p
     }
     const dim3 grid(static_cast<uint32_t>(num_kv_heads), static_cast<uint32_t>(a.splits), static_cast<uint32_t>(tokens));
     const size_t lds = attention_lds(G, head_dim);
-    if (lds > (64u << 10)) {  // beyond the default dynamic LDS limit (160 KB per CU on gfx950)
-        static bool raised = false;
-        if (!raised) {
-            KT_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&attention_kernel<8>),
-                                       hipFuncAttributeMaxDynamicSharedMemorySize, 160 << 10));
-            KT_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&attention_kernel<16>),
-                                       hipFuncAttributeMaxDynamicSharedMemorySize, 160 << 10));
-            raised = true;
-        }
-    }
+    if (head_dim > 64)
+        if (const int32_t ls = head_dim <= 128 ? allow_lds<&attention_kernel<8>>(lds) : allow_lds<&attention_kernel<16>>(lds)) return ls;
     if (head_dim <= 64) attention_kernel<4><<<grid, THREADS, lds, st>>>(a);
     else if (head_dim <= 128) attention_kernel<8><<<grid, THREADS, lds, st>>>(a);
     else attention_kernel<16><<<grid, THREADS, lds, st>>>(a);

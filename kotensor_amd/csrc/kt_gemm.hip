@@ -1204,17 +1204,9 @@ static int32_t launch_gemm_packed_tiles(const float* a, int32_t m, const WeightV
     }
     KT_LAUNCHED("qmatmul: tiled gemm prep");
     constexpr size_t lds = plds_bytes(TN);
-    static bool raised = false;
-    if (!raised && lds > LDS_DEFAULT) {  // the meet is beyond the default dynamic LDS limit (exactly
-        // what it needs: the kernel's static LDS comes on top)
-        KT_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&gemm_packed_kernel<4, true, TM, TN, PD>),
-                                   hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds)));
-        KT_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&gemm_packed_kernel<8, true, TM, TN, PD>),
-                                   hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds)));
-        KT_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&gemm_packed_kernel<8, false, TM, TN, PD>),
-                                   hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds)));
-        raised = true;
-    }
+    if (const int32_t ls = w.bits == 4 ? allow_lds<&gemm_packed_kernel<4, true, TM, TN, PD>, lds>(lds)
+                           : w.z       ? allow_lds<&gemm_packed_kernel<8, true, TM, TN, PD>, lds>(lds)
+                                       : allow_lds<&gemm_packed_kernel<8, false, TM, TN, PD>, lds>(lds)) return ls;
     const uint32_t blocks = static_cast<uint32_t>(ceil_div(tiles_n, XCDS) * XCDS * tiles_m * splits);
 #define KT_GEMM_ARGS a16t, er, jobs, m, w.K, S, w.g, tiles_m, tiles_n, splits, chunks_per_split * 4, alpha, accumulate
     if (w.bits == 4) gemm_packed_kernel<4, true, TM, TN, PD><<<blocks, PTHREADS, lds, st>>>(KT_GEMM_ARGS);

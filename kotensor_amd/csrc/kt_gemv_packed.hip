@@ -46,7 +46,6 @@
 #include "kt_common.h"
 #include "kt_packed.h"
 #include <algorithm>
-#include <atomic>
 #include <type_traits>
 
 namespace kt {

@@ -19,7 +19,6 @@
 #include <math.h>
 
 #include <algorithm>
-#include <atomic>
 #include <type_traits>
 
 #include "kt_common.h"
@@ -1300,14 +1299,7 @@ int32_t launch_append(const AppendArgs& a, hipStream_t st) {
                          (a.q ? static_cast<int64_t>((a.tokens + per - 1) / per) * ((a.num_heads + Q_HEADS - 1) / Q_HEADS) : 0);
     if (grid > INT32_MAX) return fail(KT_ERR_SHAPE, "too many tokens and heads in one call");
     const size_t lds = static_cast<size_t>(a.c.block) * (a.c.head_dim + 1) * sizeof(float);
-    if (lds > (64u << 10)) {  // beyond the default dynamic LDS limit (160 KB per CU on gfx950)
-        static std::atomic<bool> raised{false};
-        if (!raised) {
-            KT_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&append_kernel<KT_KV8_INT8>), hipFuncAttributeMaxDynamicSharedMemorySize, 144 << 10));
-            KT_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&append_kernel<KT_KV8_E4M3>), hipFuncAttributeMaxDynamicSharedMemorySize, 144 << 10));
-            raised = true;
-        }
-    }
+    if (const int32_t ls = a.c.fmt == KT_KV8_INT8 ? allow_lds<&append_kernel<KT_KV8_INT8>, 144 << 10>(lds) : allow_lds<&append_kernel<KT_KV8_E4M3>, 144 << 10>(lds)) return ls;
     const auto kernel = a.c.fmt == KT_KV8_INT8 ? append_kernel<KT_KV8_INT8> : append_kernel<KT_KV8_E4M3>;
     kernel<<<static_cast<uint32_t>(grid), THREADS, lds, st>>>(a);
     KT_LAUNCHED("8-bit cache append kernel");
@@ -1378,13 +1370,7 @@ int32_t launch_rows(AttnArgs a, int32_t key_bound, hipStream_t st, AppendArgs* a
         if (const int32_t status = launch_append(*append, st)) return status;
     }
     constexpr size_t lds = sizeof(float) * std::max(std::max(static_cast<size_t>(WAVES) * R * (HD + 6), static_cast<size_t>(R) * (HD + 8)), static_cast<size_t>(R) * (MAX_SPLITS + 1) + 4 * 64 * WAVES);
-    if constexpr (lds > (64u << 10)) {  // beyond the default dynamic LDS limit (160 KB per CU on gfx950)
-        static std::atomic<bool> raised{false};
-        if (!raised) {
-            KT_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&attention_kernel<FMT, HD, R, WAVES, STEP>), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
-            raised = true;
-        }
-    }
+    if (const int32_t ls = allow_lds<&attention_kernel<FMT, HD, R, WAVES, STEP>, lds>(lds)) return ls;
     attention_kernel<FMT, HD, R, WAVES, STEP><<<dim3(static_cast<uint32_t>(a.c.kv_heads), static_cast<uint32_t>(tiles), static_cast<uint32_t>(a.max_splits)), 64 * WAVES, lds, st>>>(a);
     KT_LAUNCHED("8-bit cache attention kernel");
     return KT_OK;

@@ -6,7 +6,6 @@
 // [set][group][16] (fp32, then bytes).
 #pragma once
 
-#include <atomic>
 #include <type_traits>
 
 #include "kt_common.h"
@@ -114,21 +113,6 @@ __host__ __device__ constexpr int32_t stage_rows(int32_t nmax, int32_t gshift) {
     return gshift <= 2 ? nmax << (2 - gshift) : (((nmax << 2) + (1 << gshift) - 1) >> gshift) + 1;
 }
 constexpr int32_t STAGE_ROW_BYTES = SET * 4 + SET;  // scales and zero points of one group row
-
-// gfx950 gives a workgroup up to 160 KB of LDS; a kernel asks for more than 64 KB of
-// dynamic LDS by raising its attribute first (allow_lds).
-constexpr size_t LDS_DEFAULT = 64 << 10, LDS_MAX = 160 << 10;
-// Raises the dynamic-LDS attribute of kernel KERN to LDS_MAX once, when a launch needs
-// more than the default.
-template <auto KERN>
-int32_t allow_lds(size_t lds) {
-    static std::atomic<bool> raised{false};
-    if (lds <= LDS_DEFAULT || raised.load(std::memory_order_acquire)) return KT_OK;
-    KT_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(KERN), hipFuncAttributeMaxDynamicSharedMemorySize,
-                               static_cast<int>(LDS_MAX)));
-    raised.store(true, std::memory_order_release);
-    return KT_OK;
-}
 
 inline int32_t log2_exact(int32_t v) {
     int32_t s = 0;
