@@ -399,7 +399,8 @@ int32_t kt_rope_attention_kv8(float* q, const float* k, const float* v, const fl
                               const int32_t* position, int32_t key_bound, const kt_kv8_cache* cache, int32_t layer,
                               int32_t num_heads, float* context, void* stream);
 /* The rows of tokens first .. first + count - 1 of a layer as fp32 (code * scale), keys and values
- * [kv_heads x count x head_dim], each of which may be NULL. */
+ * [kv_heads x count x head_dim], each of which may be NULL; keys are 16-byte aligned, values may begin at
+ * any float. */
 int32_t kt_kv8_read(const kt_kv8_cache* cache, int32_t layer, int32_t first, int32_t count, float* keys,
                     float* values, void* stream);
 /* KVCache.copyFrom (K/KVCache.kt:41-55): the first `length` positions of every layer of `source`, which

@@ -1,5 +1,5 @@
 """How calls on an 8-bit cache are launched: captures that the library did not begin, and bounds on both sides of the
-length at which the form of the attention changes."""
+length at which the form of the attention changes; and where reads may go."""
 import ctypes
 
 import numpy as np
@@ -110,3 +110,23 @@ def test_bounds_on_both_sides_of_a_form(kt, fmt, block, tokens, start, heads, kv
     want = kv8_ref.attend(q, keys, values, start, heads)
     for bound in (n, wide):
         assert normwise_rel(_attend(kt, cache, 0, q, start, heads, bound), want) <= _tolerance(q, keys, heads)
+
+
+@pytest.mark.parametrize("fmt,block,d", [("int8", 64, 64), ("e4m3", 32, 256), ("int8", 128, 32)])
+def test_values_are_read_to_any_float(kt, fmt, block, d):
+    """Keys at 16 bytes, values at any float; the floats around them stay."""
+    from kotensor_amd import _lib
+    rng = np.random.default_rng(d)
+    cache = kt.QuantizedKVCache(1, 2, 150, d, fmt, block)
+    k, v = _rows(rng, 140, 2, d), _rows(rng, 140, 2, d)
+    _append(kt, cache, 0, k, v, 0)
+    want, count = cache.rows_numpy(0, 3, 130), 2 * 130 * d
+    for offset in (1, 2, 3):
+        banner("kv8-read-offset", fmt, d, offset)
+        keys, values = (_dev(kt, np.full(count + 8, 7.0, np.float32)) for _ in range(2))
+        _lib.call("kt_kv8_read", ctypes.byref(cache.cache), 0, 3, 130, keys.ptr + 16, values.ptr + 4 * offset, None)
+        kt.synchronize()
+        for buffer, first, rows in ((keys, 4, want[0]), (values, offset, want[1])):
+            got = buffer.download(np.float32)
+            assert same_bits(got[first:first + count].reshape(rows.shape), rows)
+            assert np.all(got[:first] == 7.0) and np.all(got[first + count:] == 7.0)
