@@ -57,6 +57,10 @@ class LogitsControls:
     def penalized(self) -> bool:
         return (self.repetition_penalty, self.frequency_penalty, self.presence_penalty) != (1.0, 0.0, 0.0)
 
+    @property
+    def masked(self) -> bool:
+        return self._allowed is not None
+
     def set_allowed(self, allowed, stream: Stream | None = None) -> None:
         """Sets the mask. Another one of the same shape replaces it in the same device memory, which a
         recorded step then reads at its next replay; one of another shape is refused. A boolean mask has

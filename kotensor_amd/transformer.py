@@ -192,8 +192,9 @@ class InferenceBuffers(_Rows):
         self.controlled = DeviceBuffer(vocabulary_size * 4)  # LogitsControls' result, of which a step takes the argmax
         self.generated = DeviceBuffer(4 * max_sequence_length)  # greedy tokens by position
         # with LogitsControls: how many leading positions `generated` holds the tokens of (prefill's
-        # record_tokens), and the position at which the output starts, the last prefill's end: on the host,
-        # and on the device as far as controlled calls have read it
+        # record_tokens), and the position at which the output starts, the last prefill's end (a caller that
+        # prefills tokens of the output sets it back): on the host, and on the device as far as controlled
+        # calls have read it
         self.recorded = 0
         self.output_from = 0
         self.output_start = DeviceBuffer(4)
@@ -760,11 +761,14 @@ class DecodeGraph:
                  controls: LogitsControls | None = None):
         self._h, self.cache, self.stream, self.buffers = handle, cache, stream, buffers
         self._controls = controls  # whose device memory the graph addresses
+        self._masked = controls is not None and controls.masked
 
     def replay(self, steps: int = 1) -> None:
         self.cache.check_room(steps)
         Transformer._check_controls(self._controls, self.cache, self.buffers, steps)
         if self._controls is not None:
+            if self._controls.masked and not self._masked:
+                raise _lib.IllegalStateException("the step was recorded without a mask, and one was set since: record it again")
             self.buffers.upload_output_start(self.stream)
         for _ in range(steps):
             _lib.call("kt_graph_launch", self._h, _stream(self.stream))

@@ -98,3 +98,27 @@ def test_a_grammar_that_ends_between_replays(kt):
         assert buffers.tokens.download(np.int32, count=1)[0] == only
     graph.destroy()
     stream.destroy()
+
+
+def test_a_first_mask_after_the_recording(kt):
+    """A step recorded without a mask addresses none: a replay does not pass over one that was set since."""
+    banner("controls-mask-first")
+    model, stream = _model(kt), kt.Stream.create()
+    controls = kt.LogitsControls(bias={40: 5.0})
+    cache, buffers = model.new_cache(20), model.new_inference_buffers(20)
+    model.prefill([1, 2, 3], cache, buffers, stream)
+    model.greedy_decode(cache, buffers, 2, stream, controls=controls)
+    graph = model.capture_decode(cache, buffers, stream, controls)
+    graph.replay()
+    controls.set_allowed(np.arange(100) == 61, stream)
+    length = cache.length
+    with pytest.raises(kt.IllegalStateException, match="recorded without a mask"):
+        graph.replay()
+    assert cache.length == length
+    again = model.capture_decode(cache, buffers, stream, controls)
+    again.replay()
+    stream.synchronize()
+    assert buffers.tokens.download(np.int32, count=1)[0] == 61
+    graph.destroy()
+    again.destroy()
+    stream.destroy()
