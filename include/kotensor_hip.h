@@ -413,6 +413,94 @@ int32_t kt_kv8_read(const kt_kv8_cache* cache, int32_t layer, int32_t first, int
 int32_t kt_kv8_copy(const kt_kv8_cache* source, int32_t source_length, const kt_kv8_cache* cache, int32_t length,
                     void* stream);
 
+/* ---- the cache in pages that several sequences share, and trees of drafted tokens --------
+ * (kt_paged.hip, kt_paged_attention.hip). No counterpart in the reference, whose cache holds one
+ * sequence (K/KVCache.kt:3-59).
+ * The pool: keys and values [layers][pages][kv_heads][page_tokens][head_dim] in fp32, fp16 or bf16
+ * (rounded to the nearest, ties to even; fp16 takes magnitudes from 65520 on as infinities), 16-byte
+ * aligned, of kt_paged_layout's size each; the caller owns it and hands out its pages. Sequences may share
+ * pages that none of them appends to. */
+#define KT_PAGED_F32 0
+#define KT_PAGED_F16 1
+#define KT_PAGED_BF16 2
+typedef struct kt_paged_cache {
+    void* keys;
+    void* values;
+    int32_t format;        /* KT_PAGED_F32, KT_PAGED_F16 or KT_PAGED_BF16 */
+    int32_t layers;
+    int32_t pages;
+    int32_t kv_heads;
+    int32_t page_tokens;   /* 16, 32, 64, 128 or 256 */
+    int32_t head_dim;      /* 32, 64, 128 or 256 */
+} kt_paged_cache;
+/* The sequences of a call. Sequence s holds lengths[s] tokens; rows starts[s] .. starts[s + 1] - 1 of
+ * the call's q, k, v and context are its next ones (none: starts[s] == starts[s + 1]), row i of them
+ * token lengths[s] + i, which lies in page tables[s * table_stride + token / page_tokens]. Rows before starts[0] and from
+ * starts[sequences] on belong to no sequence: what a call writes for rows leaves them as they are.
+ * In a text (masks and depths NULL) row i sees the tokens up to its own, and its rotary position is its
+ * token's number. In a tree its position is lengths[s] + depths[row], and it sees the tokens below lengths[s] and
+ * token lengths[s] + j where bit j % 32 of word j / 32 of masks[row * mask_words ..] is set, for the
+ * sequence's own rows j (kt_tree_masks; other masks do as well). A tree's rows without children are
+ * rows of a text for whoever comes later only after kt_paged_keep.
+ * All arrays are device memory that the kernels read, so a recorded step follows them from replay to replay:
+ * nothing in them is refused, and nothing in them makes a call read or write outside the pool. A page number outside
+ * the pool holds nothing: its tokens are neither written nor seen. Tokens below 0 and past the table are not there.
+ * starts that do not ascend within 0 .. rows, or a sequence of more than most_rows rows, are the caller's mistake: the
+ * call's outputs are then unspecified. */
+typedef struct kt_paged_batch {
+    const int32_t* tables;    /* [sequences][table_stride] page numbers */
+    const int32_t* lengths;   /* [sequences] */
+    const int32_t* starts;    /* [sequences + 1] */
+    const int32_t* depths;    /* [rows], or NULL */
+    const uint32_t* masks;    /* [rows][mask_words], or NULL */
+    int32_t table_stride;
+    int32_t sequences;        /* at most 65535 */
+    int32_t rows;             /* rows of q, k, v and context */
+    int32_t most_rows;        /* at least every sequence's rows */
+    int32_t key_bound;        /* at least every lengths[s] + its rows: it sizes the launch, and tokens from it on are not seen */
+    int32_t mask_words;       /* 32 * mask_words >= most_rows */
+} kt_paged_batch;
+/* Bytes of the keys, and of the values. Reads no pointer of the cache. Host arithmetic. */
+int32_t kt_paged_layout(const kt_paged_cache* cache, int64_t* bytes);
+/* kt_rope_kv for a batch: q [rows x num_heads*head_dim] rotated into q_out (which may be q; both NULL: only
+ * the append), k rotated and k and v [rows x kv_heads*head_dim] appended at their tokens' places. k, v and q
+ * (unless it is q_out) stay as they are; lengths too (kt_paged_advance, kt_paged_keep). */
+int32_t kt_rope_paged(const float* q, const float* k, const float* v, int32_t num_heads, const float* inv_freq,
+                      const kt_paged_cache* cache, int32_t layer, const kt_paged_batch* batch, float* q_out, void* stream);
+/* kt_attention for a batch whose keys and values the pool holds already: softmax(q . k_j / sqrt(head_dim)) over the
+ * tokens a row sees, times v, into context [rows x num_heads*head_dim]; products in fp32 precision, sums and softmax
+ * in fp32. A row that sees no token gets zeros. Values that are not finite stay with the rows that see them. Scores
+ * are taken to lie in fp32's range. q and context are 16-byte aligned and apart. The stream's workspace is sized by one eager call of the
+ * same bounds before a recording. */
+int32_t kt_attention_paged(const float* q, int32_t num_heads, const kt_paged_cache* cache, int32_t layer,
+                           const kt_paged_batch* batch, float* context, void* stream);
+/* kt_rope_paged, then kt_attention_paged on the rotated queries. q, k and v stay as they are. */
+int32_t kt_rope_attention_paged(const float* q, const float* k, const float* v, const float* inv_freq, int32_t num_heads,
+                                const kt_paged_cache* cache, int32_t layer, const kt_paged_batch* batch, float* context,
+                                void* stream);
+/* The depths (of a root 0) and masks (a row and what is above it) of each sequence's rows as trees: parents[row] is the
+ * index of its parent among its sequence's rows; a root's is -1 (as is any that is not below the row's own index).
+ * Writes depths and masks, which may be the batch's own; of the batch reads starts, sequences, rows and mask_words. */
+int32_t kt_tree_masks(const int32_t* parents, const kt_paged_batch* batch, int32_t* depths, uint32_t* masks, void* stream);
+/* The greedy check of each sequence's tree: tokens[row] is its token, chosen[row] the token the model chose after it
+ * (kt_argmax of the row's logits). Row 0 is kept; then, as long as there is one, the first row whose parent is the
+ * last one kept and whose token is the one chosen after that. kept[s * kept_stride ..] receives the kept rows'
+ * indices, ascending, and -1 behind them, counts[s] their number, next[s] the token chosen after the last (of a
+ * sequence without rows: 0 kept, next left as it is). kept_stride >= most_rows. */
+int32_t kt_tree_accept(const int32_t* tokens, const int32_t* chosen, const int32_t* parents, const kt_paged_batch* batch,
+                       int32_t* kept, int32_t kept_stride, int32_t* counts, int32_t* next, void* stream);
+/* What stays of a tree: in every layer the keys and values of row kept[s * kept_stride + m] move to token lengths[s] + m, for
+ * m < counts[s] (up to the first entry that does not ascend or is none of the sequence's rows), and
+ * new_lengths[s] = lengths[s] + that count. new_lengths may be the batch's lengths, or lies apart from them. */
+int32_t kt_paged_keep(const kt_paged_cache* cache, const kt_paged_batch* batch, const int32_t* kept, int32_t kept_stride,
+                      const int32_t* counts, int32_t* new_lengths, void* stream);
+/* lengths[s] += the sequence's rows of the batch: what a text's rows have become once every layer has them. */
+int32_t kt_paged_advance(int32_t* lengths, const kt_paged_batch* batch, void* stream);
+/* The rows of tokens first .. first + count - 1 of a sequence as fp32, keys and values [kv_heads x count x head_dim],
+ * each of which may be NULL; table: its row of the tables, of `entries` page numbers. Tokens that have no place give NaN. */
+int32_t kt_paged_read(const kt_paged_cache* cache, int32_t layer, const int32_t* table, int32_t entries, int32_t first,
+                      int32_t count, float* keys, float* values, void* stream);
+
 /* SwiGLU's gate (K/SwiGLU.kt:19-25; K/Tensor.kt:223-237): gate[i] = silu(gate[i]) * up[i]. */
 int32_t kt_silu_mul(float* gate, const float* up, int64_t n, void* stream);
 /* RMSNorm.forward (K/RMSNorm.kt) of x [m x K] with weight, then the grouped projections of

@@ -106,6 +106,24 @@ class KV8Cache(ctypes.Structure):
     ]
 
 
+KT_PAGED_F32 = 0
+KT_PAGED_F16 = 1
+KT_PAGED_BF16 = 2
+
+
+class PagedCache(ctypes.Structure):
+    """kt_paged_cache: the memory and shape of a cache in pages."""
+    _fields_ = [("keys", ctypes.c_void_p), ("values", ctypes.c_void_p), ("format", ctypes.c_int32), ("layers", ctypes.c_int32),
+                ("pages", ctypes.c_int32), ("kv_heads", ctypes.c_int32), ("page_tokens", ctypes.c_int32), ("head_dim", ctypes.c_int32)]
+
+
+class PagedBatch(ctypes.Structure):
+    """kt_paged_batch: the sequences of a call on such a cache."""
+    _fields_ = [("tables", ctypes.c_void_p), ("lengths", ctypes.c_void_p), ("starts", ctypes.c_void_p), ("depths", ctypes.c_void_p),
+                ("masks", ctypes.c_void_p), ("table_stride", ctypes.c_int32), ("sequences", ctypes.c_int32), ("rows", ctypes.c_int32),
+                ("most_rows", ctypes.c_int32), ("key_bound", ctypes.c_int32), ("mask_words", ctypes.c_int32)]
+
+
 class LogitsControls(ctypes.Structure):
     """kt_logits_controls: what kt_process_logits takes beside the logits."""
     _fields_ = [
@@ -185,6 +203,15 @@ SIGNATURES = {
     "kt_rope_attention_kv8": [_P, _P, _P, _P, _I, _P, _I, ctypes.POINTER(KV8Cache), _I, _I, _P, _P],
     "kt_kv8_read": [ctypes.POINTER(KV8Cache), _I, _I, _I, _P, _P, _P],
     "kt_kv8_copy": [ctypes.POINTER(KV8Cache), _I, ctypes.POINTER(KV8Cache), _I, _P],
+    "kt_paged_layout": [ctypes.POINTER(PagedCache), ctypes.POINTER(ctypes.c_int64)],
+    "kt_rope_paged": [_P, _P, _P, _I, _P, ctypes.POINTER(PagedCache), _I, ctypes.POINTER(PagedBatch), _P, _P],
+    "kt_attention_paged": [_P, _I, ctypes.POINTER(PagedCache), _I, ctypes.POINTER(PagedBatch), _P, _P],
+    "kt_rope_attention_paged": [_P, _P, _P, _P, _I, ctypes.POINTER(PagedCache), _I, ctypes.POINTER(PagedBatch), _P, _P],
+    "kt_tree_masks": [_P, ctypes.POINTER(PagedBatch), _P, _P, _P],
+    "kt_tree_accept": [_P, _P, _P, ctypes.POINTER(PagedBatch), _P, _I, _P, _P, _P],
+    "kt_paged_keep": [ctypes.POINTER(PagedCache), ctypes.POINTER(PagedBatch), _P, _I, _P, _P, _P],
+    "kt_paged_advance": [_P, ctypes.POINTER(PagedBatch), _P],
+    "kt_paged_read": [ctypes.POINTER(PagedCache), _I, _P, _I, _I, _I, _P, _P, _P],
     "kt_silu_mul": [_P, _P, ctypes.c_int64, _P],
     "kt_swiglu_qmatmul": [_P, _P, _I, ctypes.POINTER(_QWeight), _P, _I, _F, _P, _P],
     "kt_rope_attention": [_P, _P, _P, _P, _I, _P, _I, _P, _P, _I, _I, _I, _I, _I, _P, _P],
