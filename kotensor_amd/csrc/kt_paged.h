@@ -62,7 +62,8 @@ __device__ __forceinline__ void store_element(uint8_t* p, int64_t at, float x) {
 int32_t view_paged(const kt_paged_cache* cache, int32_t layer, PagedView* v);
 int32_t view_batch(const kt_paged_batch* batch, const kt_paged_cache* cache, BatchView* v);
 
-// The attention of a batch. inv_freq: NULL, or q is rotated on the way (kt_rope_attention_paged).
+// The attention of a batch (kt_paged_attention.h). k and v: NULL, or the projections of a step's tokens (at most one a
+// sequence), which the launch rotates, as the queries, appends and attends to.
 struct PagedAttnArgs {
     const float* q;
     const float* inv_freq;
@@ -72,6 +73,8 @@ struct PagedAttnArgs {
     int32_t num_heads;
     float scale;
 };
-int32_t launch_paged_attention(const PagedAttnArgs& a, hipStream_t st);
+int32_t launch_paged_attention_f32(const PagedAttnArgs& a, const float* k, const float* v, hipStream_t st);
+int32_t launch_paged_attention_f16(const PagedAttnArgs& a, const float* k, const float* v, hipStream_t st);
+int32_t launch_paged_attention_bf16(const PagedAttnArgs& a, const float* k, const float* v, hipStream_t st);
 
 }  // namespace kt

@@ -322,6 +322,11 @@ int32_t append_args(const float* q, const float* k, const float* v, int32_t num_
     return KT_OK;
 }
 
+int32_t launch_attention(const PagedAttnArgs& a, hipStream_t st, const float* k = nullptr, const float* v = nullptr) {
+    const auto launch = a.c.fmt == KT_PAGED_F32 ? launch_paged_attention_f32 : a.c.fmt == KT_PAGED_F16 ? launch_paged_attention_f16 : launch_paged_attention_bf16;
+    return launch(a, k, v, st);
+}
+
 int32_t attention_args(const float* q, int32_t num_heads, const kt_paged_cache* cache, int32_t layer, const kt_paged_batch* batch, float* context,
                        PagedAttnArgs* a) {
     if (const int32_t status = view_paged(cache, layer, &a->c)) return status;
@@ -358,19 +363,27 @@ int32_t kt_attention_paged(const float* q, int32_t num_heads, const kt_paged_cac
                            void* stream) {
     PagedAttnArgs a{};
     if (const int32_t status = attention_args(q, num_heads, cache, layer, batch, context, &a)) return status;
-    return a.b.rows == 0 || a.b.sequences == 0 ? KT_OK : launch_paged_attention(a, static_cast<hipStream_t>(stream));
+    return a.b.rows == 0 || a.b.sequences == 0 ? KT_OK : launch_attention(a, static_cast<hipStream_t>(stream));
 }
 
 int32_t kt_rope_attention_paged(const float* q, const float* k, const float* v, const float* inv_freq, int32_t num_heads, const kt_paged_cache* cache,
                                 int32_t layer, const kt_paged_batch* batch, float* context, void* stream) {
     AppendArgs p{};
     PagedAttnArgs a{};
-    if (const int32_t status = append_args(nullptr, k, v, num_heads, inv_freq, cache, layer, batch, nullptr, &p)) return status;
+    if (const int32_t status = append_args(q, k, v, num_heads, inv_freq, cache, layer, batch, context, &p)) return status;
     if (const int32_t status = attention_args(q, num_heads, cache, layer, batch, context, &a)) return status;
     if (a.b.rows == 0 || a.b.sequences == 0) return KT_OK;
-    if (const int32_t status = launch_append(p, static_cast<hipStream_t>(stream))) return status;
-    a.inv_freq = inv_freq;
-    return launch_paged_attention(a, static_cast<hipStream_t>(stream));
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    // A step of up to 16 query heads a kv head: one launch (of 256 dims its form would not fit the registers).
+    if (a.b.most_rows == 1 && num_heads / a.c.kv_heads <= 16 && a.c.head_dim < 256) {
+        a.inv_freq = inv_freq;
+        return launch_attention(a, st, k, v);
+    }
+    // Otherwise the rotated queries wait in the context: a tile's are read by its own parts alone, all of them before
+    // the last writes what becomes of them there.
+    if (const int32_t status = launch_append(p, st)) return status;
+    a.q = context;
+    return launch_attention(a, st);
 }
 
 int32_t kt_tree_masks(const int32_t* parents, const kt_paged_batch* batch, int32_t* depths, uint32_t* masks, void* stream) {

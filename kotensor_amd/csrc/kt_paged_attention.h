@@ -1,0 +1,943 @@
+// kt_paged_attention.h -- attention over the cache in pages (kt_paged.h): decode steps, prompts and
+// trees of drafted tokens of several sequences in one launch. No counterpart in the reference
+// (K/Attention.kt:277-349 attends in one sequence's cache). One translation unit a format includes it.
+//
+// Rows: the (row, query head) pairs of a sequence and kv head, a row's G heads side by side, in tiles of R. A
+// tile's keys are cut into parts of about the same number of chunks for all sequences of the launch, whatever
+// their lengths: every workgroup reads the sequences' rows and lengths, from which follow the parts'
+// size and its own place among them, so that one long sequence beside short ones fills the card. A workgroup holds
+// its rows' queries as matrix operands, its waves take the part's chunks of 32 keys in turn, straight from memory into
+// registers: no LDS and no barrier in the loop.
+//   S^T = K Q^T: a lane ends with scores of one row (its column), so that the running maximum and sum of a
+//     row stay inside the lanes of a column.
+//   O^T += V^T P^T: a lane loads its dims of the tokens whose weights it holds, and turns them in registers.
+// Products in fp32 precision: numbers held in fp16 are one operand and queries and weights two fp16 ones (to
+// 2^-22 of a row's largest query, 2^-30 of its largest weight); held in bf16 one operand and three bf16 ones (exact);
+// fp32 three each, of whose nine products the six down to 2^-17 are formed (kt_split.h).
+// A wave's maximum follows a row's lazily: a larger score moves it only once it is 2^8 above, so that the sums are
+// seldom rescaled. Waves' sums meet in LDS; parts' through memory, where the last workgroup of a tile to
+// arrive (a counter, which it returns to zero) merges all in their order: no workgroup waits for
+// another, and the bits do not depend on who is last.
+#pragma once
+
+#include <algorithm>
+#include <type_traits>
+
+#include "kt_paged.h"
+#include "kt_split.h"
+
+namespace kt {
+namespace paged {
+
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f16v __attribute__((ext_vector_type(16)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+
+constexpr int CHUNK = 32;        // keys a wave takes at a time
+constexpr float LAZY = 8.0f;     // how far a score may pass the maximum, in powers of two
+constexpr int MAX_SPLITS = 128;  // parts of a tile
+constexpr int THROUGH = 1 | 16;  // buffer cache bits sc0 sc1: past the caches
+
+// ---- operands ------------------------------------------------------------------------------
+// QP parts of a query or weight, KP of a key or value; weights are taken times 2^UP.
+template <int FMT>
+struct Format {
+    typedef bf16x8 op;
+    static constexpr int QP = 3, KP = FMT == KT_PAGED_F32 ? 3 : 1, E = element_bytes(FMT);
+    static constexpr float UP = 0.0f;
+};
+template <>
+struct Format<KT_PAGED_F16> {
+    typedef half8 op;
+    static constexpr int QP = 2, KP = 1, E = 2;
+    static constexpr float UP = 6.0f;  // (so that their second parts are normal numbers down to 2^-20)
+};
+
+template <bool SMALL, typename A>
+__device__ __forceinline__ A product(bf16x8 a, bf16x8 b, A c) {
+    if constexpr (SMALL) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+template <bool SMALL, typename A>
+__device__ __forceinline__ A product(half8 a, half8 b, A c) {
+    if constexpr (SMALL) return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+// The sum of the parts' products down to 2^-17 of the largest, the small ones first.
+template <bool SMALL, int KP, int QP, typename OP, typename A>
+__device__ __forceinline__ A products(const OP (&k)[KP], const OP (&q)[QP], A c) {
+#pragma unroll
+    for (int w = QP - 1; w >= 0; --w)
+#pragma unroll
+        for (int i = KP - 1; i >= 0; --i)
+            if (w - i >= 0) c = product<SMALL>(k[i], q[w - i], c);
+    return c;
+}
+
+__device__ __forceinline__ void split_weights(const float (&v)[8], bf16x8 (&part)[3]) { split3_nearest(v, part); }
+__device__ __forceinline__ void split_weights(const float (&v)[8], half8 (&part)[2]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const half2v h = __builtin_bit_cast(half2v, __builtin_amdgcn_cvt_pkrtz(v[2 * i], v[2 * i + 1]));
+        // (to the nearest, so that what weights below fp16's normal numbers lose has no sign)
+        const half2v l = __builtin_convertvector((f32x2{v[2 * i] - static_cast<float>(h[0]), v[2 * i + 1] - static_cast<float>(h[1])}), half2v);
+        part[0][2 * i] = h[0];
+        part[0][2 * i + 1] = h[1];
+        part[1][2 * i] = l[0];
+        part[1][2 * i + 1] = l[1];
+    }
+}
+
+// Eight consecutive elements (registers of a row) as operands.
+template <int FMT>
+__device__ __forceinline__ void to_operands(const uint32_t* w, typename Format<FMT>::op (&part)[Format<FMT>::KP]) {
+    if constexpr (FMT == KT_PAGED_F32) {
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = __builtin_bit_cast(float, w[i]);
+        split3_nearest(v, part);
+    } else {
+        part[0] = __builtin_bit_cast(typename Format<FMT>::op, u4{w[0], w[1], w[2], w[3]});
+    }
+}
+
+__device__ __forceinline__ uint32_t magnitude(float x) { return __builtin_bit_cast(uint32_t, x) & 0x7FFFFFFFu; }
+
+// ---- exchanges over the lanes of a column (apart by 16 or 32) --------------------------------
+struct Swapped {
+    float a, b;  // of two lanes apart by 16 (32): the value of the one and of the other, in both
+};
+// (the wait states are those between a vector write and the swap's read)
+__device__ __forceinline__ Swapped swap16(float v) {
+    Swapped s{v, v};
+    asm("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(s.a), "+v"(s.b));
+    return s;
+}
+__device__ __forceinline__ Swapped swap32(float v) {
+    Swapped s{v, v};
+    asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(s.a), "+v"(s.b));
+    return s;
+}
+template <bool SMALL>
+__device__ __forceinline__ float column_max(float v) {
+    if constexpr (SMALL) {
+        const Swapped s = swap16(v);
+        v = fmaxf(s.a, s.b);
+    }
+    const Swapped s = swap32(v);
+    return fmaxf(s.a, s.b);
+}
+template <bool SMALL>
+__device__ __forceinline__ float column_sum(float v) {
+    if constexpr (SMALL) {
+        const Swapped s = swap16(v);
+        v = s.a + s.b;
+    }
+    const Swapped s = swap32(v);
+    return s.a + s.b;
+}
+
+// The maximum is a rounded product; at sizes where its rounding is a power of two and more, the
+// exponent is the difference of rounded products, so that it stays below LAZY.
+constexpr float HUGE_SCORE = 65536.0f;
+__device__ __forceinline__ float weight_of_huge(float x, float f, float m, float up) {
+#pragma clang fp contract(off)
+    const float s = x * f;
+    return __builtin_amdgcn_exp2f((s - m) + up);
+}
+// A score as the maxima hold it: rounded, also where the next step subtracts one.
+__device__ __forceinline__ float rounded_score(float x, float f) {
+#pragma clang fp contract(off)
+    return x * f;
+}
+// What a part with the maximum m and the sum l counts beside parts with the maximum mx: a part without keys
+// (l = 0) nothing, one with a NaN a NaN.
+__device__ __forceinline__ float share_of(float m, float l, float mx) {
+    return l == 0.0f ? 0.0f : l * __builtin_amdgcn_exp2f((m == -INFINITY ? mx : m) - (mx == -INFINITY ? 0.0f : mx));
+}
+
+// ---- the parts of a launch ---------------------------------------------------------------------
+struct Args {
+    PagedAttnArgs p;
+    const float* k_new;  // STEP: the step's projections before RoPE
+    const float* v_new;
+    int32_t target;      // workgroups among which the launch's chunks are shared out
+    float* averages;     // [slots][R][head_dim]: the parts' averages
+    float* stats;        // [slots][R][2]: their maxima and sums
+    uint32_t* counters;  // [slots], zero between launches
+};
+
+struct Part {
+    int32_t sequence, first, n, length;  // its rows and tokens
+    int32_t tile, head, split, splits;
+    int32_t keys;   // tokens that rows of the sequence may see
+    int32_t per;    // chunks a part may have
+    int32_t slot;   // of the tile's first part
+};
+
+__device__ __forceinline__ int32_t held_keys(const PagedView& c, const BatchView& b, int32_t length, int32_t n) {
+    const int64_t most = min(room_of(c, b), static_cast<int64_t>(b.key_bound));
+    return static_cast<int32_t>(min(max(static_cast<int64_t>(length) + n, int64_t{0}), most));
+}
+__device__ __forceinline__ int64_t wave_total(int64_t v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+    return v;
+}
+__device__ __forceinline__ int32_t lane_int(int32_t v, int32_t lane) { return __builtin_amdgcn_readlane(v, lane); }
+
+// Which part of the launch workgroup `at` has; false: none. Every lane is a sequence. A launch has at most target + (its tiles
+// of all kv heads) parts, and at most 2 target that share a tile: a part's size is at least the chunks over target.
+template <int R, int NW>
+__device__ __forceinline__ bool find_part(const Args& a, int32_t at, Part& out) {
+    const PagedView& c = a.p.c;
+    const BatchView& b = a.p.b;
+    const int32_t lane = threadIdx.x & 63, G = a.p.num_heads / c.kv_heads;
+    int32_t first = 0, n = 0, length = 0;
+    auto load = [&](int32_t s0) {
+        const int32_t s = min(s0 + lane, b.sequences - 1);
+        first = start_of(b, s);
+        n = start_of(b, s + 1) - first;
+        length = b.lengths[s];
+        if (s0 + lane >= b.sequences) n = 0;
+        n = min(max(n, 0), b.most_rows);
+    };
+    auto tiles_of = [&]() { return static_cast<int32_t>((static_cast<int64_t>(n) * G + R - 1) / R); };
+    auto chunks_of = [&]() { return (held_keys(c, b, length, n) + CHUNK - 1) / CHUNK; };
+    int64_t total = 0, rows = 0;
+    for (int32_t s0 = 0; s0 < b.sequences; s0 += 64) {
+        load(s0);
+        total += static_cast<int64_t>(tiles_of()) * c.kv_heads * max(chunks_of(), 1);
+        rows += n;
+    }
+    total = wave_total(total);
+    if (wave_total(rows) > b.rows) return false;  // starts that do not ascend
+    int64_t per = (total + a.target - 1) / a.target;
+    per = (per + NW - 1) / NW * NW;
+    if (per < NW) per = NW;
+    int32_t before = 0, slots = 0;
+    for (int32_t s0 = 0; s0 < b.sequences; s0 += 64) {
+        if (b.sequences > 64) load(s0);
+        const int32_t tiles = tiles_of(), chunks = chunks_of();
+        const int32_t size = static_cast<int32_t>(max(per, static_cast<int64_t>((chunks + MAX_SPLITS - 1) / MAX_SPLITS)));
+        const int32_t splits = max((chunks + size - 1) / size, 1), parts = tiles * c.kv_heads * splits;
+        const int32_t mine = splits > 1 ? parts : 0;
+        int32_t upto = parts, slots_upto = mine;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int32_t x = __shfl_up(upto, o), y = __shfl_up(slots_upto, o);
+            if (lane >= o) {
+                upto += x;
+                slots_upto += y;
+            }
+        }
+        const int32_t passed = __popcll(__ballot(before + upto <= at));
+        if (passed < 64) {
+            const int32_t local = at - before - (lane_int(upto, passed) - lane_int(parts, passed));
+            out.sequence = s0 + passed;
+            out.first = lane_int(first, passed);
+            out.n = lane_int(n, passed);
+            out.length = lane_int(length, passed);
+            out.splits = lane_int(splits, passed);
+            out.per = lane_int(size, passed);
+            out.head = local % c.kv_heads;  // (workgroups go round the eight dies: a head's stay on few of them)
+            const int32_t rest = local / c.kv_heads;
+            out.split = rest % out.splits;
+            out.tile = lane_int(tiles, passed) - 1 - rest / out.splits;  // (a text's last tiles see the most)
+            out.keys = held_keys(c, b, out.length, out.n);
+            out.slot = slots + lane_int(slots_upto, passed) - lane_int(mine, passed) + (out.tile * c.kv_heads + out.head) * out.splits;
+            return true;
+        }
+        before += lane_int(upto, 63);
+        slots += lane_int(slots_upto, 63);
+    }
+    return false;
+}
+
+// ---- the kernel ----------------------------------------------------------------------------------
+// R = 16 rows on 16x16x32, or R = 32 CT on 32x32x16.
+template <int FMT, int HD, int R>
+struct Shape {
+    static constexpr bool SMALL = R == 16;
+    static constexpr int CT = SMALL ? 1 : R / 32;         // column tiles
+    static constexpr int LANES = SMALL ? 16 : 32;         // columns of a tile
+    static constexpr int KT = SMALL ? 2 : 1;              // key tiles of a chunk
+    static constexpr int QS = SMALL ? HD / 32 : HD / 16;  // steps of a score
+    static constexpr int E = SMALL ? 8 : 16;              // scores of a lane
+    static constexpr int VS = SMALL ? 1 : 2;              // steps of an output
+    static constexpr int DB = HD / LANES;                 // dim blocks of the output: consecutive dims of a lane
+    static constexpr int OE = SMALL ? 4 : 16;
+    static constexpr int KW = 8 * Format<FMT>::E / 4;     // dwords of a key tile's step
+    static constexpr int VW = (DB * Format<FMT>::E + 3) / 4;  // dwords of a token's dims (of one dim in 16 bits: half of one)
+    static constexpr bool QREG = SMALL && HD < 256;       // a row's operands stay in registers
+};
+
+// What a step's workgroups share: the rotation, and the new token as the cache holds it.
+template <int HD, bool STEP>
+struct StepShared {
+    __attribute__((aligned(16))) float cosines[HD / 2], sines[HD / 2];
+    __attribute__((aligned(16))) uint8_t key[4 * HD], value[4 * HD];
+};
+template <int HD>
+struct StepShared<HD, false> {};
+
+template <int N>
+__device__ __forceinline__ void load_words(const uint8_t* p, uint32_t (&w)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+        if constexpr (N >= 4) {
+            const u4 v = *reinterpret_cast<const u4*>(p + 4 * i);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[i + e] = v[e];
+        } else if constexpr (N == 2) {
+            const uint2 v = *reinterpret_cast<const uint2*>(p);
+            w[0] = v.x;
+            w[1] = v.y;
+        } else {
+            w[0] = *reinterpret_cast<const uint32_t*>(p);
+        }
+    }
+}
+
+template <int FMT>
+__device__ __forceinline__ bool any_not_finite(uint32_t w) {
+    if constexpr (FMT == KT_PAGED_F32) return (w & 0x7F800000u) == 0x7F800000u;
+    constexpr uint32_t x = FMT == KT_PAGED_F16 ? 0x7C00u : 0x7F80u;
+    return (w & x) == x || (w >> 16 & x) == x;
+}
+template <int FMT>
+__device__ __forceinline__ uint32_t finite_only(uint32_t w) {
+    if constexpr (FMT == KT_PAGED_F32) return (w & 0x7F800000u) == 0x7F800000u ? 0u : w;
+    constexpr uint32_t x = FMT == KT_PAGED_F16 ? 0x7C00u : 0x7F80u;
+    return ((w & x) == x ? 0u : w & 0xFFFFu) | ((w >> 16 & x) == x ? 0u : w & 0xFFFF0000u);
+}
+
+template <int FMT, int HD, int R, int NW, bool STEP>
+__global__ void __launch_bounds__(64 * NW, HD == 256 || (FMT == KT_PAGED_F32 && HD == 128) ? 1 : 2) attention_kernel(Args a) {
+    using F = Format<FMT>;
+    using X = Shape<FMT, HD, R>;
+    using op = typename F::op;
+    constexpr int LR = HD + 4;  // padded row of the waves' averages
+    constexpr int QR = HD + 8;  // padded row of a query's parts
+    extern __shared__ __attribute__((aligned(16))) float lds[];
+    float* avg = lds;               // [NW][R][LR]
+    float* ms = avg + NW * R * LR;  // [NW][R]
+    float* ls = ms + NW * R;        // [NW][R]
+    __shared__ float fr_s[R];
+    __shared__ StepShared<HD, STEP> sh;
+    const PagedView& c = a.p.c;
+    const BatchView& b = a.p.b;
+    const int32_t tid = threadIdx.x, lane = tid & 63;
+    const int32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int32_t col = lane % X::LANES, grp = lane / X::LANES;
+    const int32_t H = a.p.num_heads, G = H / c.kv_heads;
+    Part part;
+    if (!find_part<R, NW>(a, blockIdx.x, part)) return;
+    const int32_t g = part.head, row0 = part.tile * R, held = min(R, part.n * G - row0);  // rows of this tile
+    // where row r of the tile lies in q and context
+    auto row_at = [&](int32_t r) {
+        const int32_t t = (row0 + r) / G;
+        return (static_cast<size_t>(part.first + t) * H + g * G + (row0 + r - t * G)) * HD;
+    };
+
+    // The rows' queries, sixteen lanes to a row (four dims each, or 64 apart; for the rotation those of the dims'
+    // pairs, too).
+    constexpr int RW = R / (4 * NW) > 0 ? R / (4 * NW) : 1, DL = HD / 64 > 0 ? HD / 64 : 1, HALF = HD / 2;
+    const int32_t lr = lane >> 4, lc = lane & 15;
+    f4 qv[RW][DL], qo[STEP ? RW : 1][STEP ? DL : 1];
+#pragma unroll
+    for (int i = 0; i < RW; ++i) {
+        const float* src = a.p.q + row_at(min(4 * (wave + i * NW) + lr, held - 1));
+#pragma unroll
+        for (int u = 0; u < DL; ++u) {
+            const int32_t d = (4 * lc + 64 * u) % HD;
+            qv[i][u] = *reinterpret_cast<const f4*>(src + d);
+            if constexpr (STEP) qo[i][u] = *reinterpret_cast<const f4*>(src + (d + HALF) % HD);
+        }
+    }
+    // a step: the new token's pairs, those of the key in threads 0 .. 127, of the value in the next 128
+    const bool on = STEP && tid < 256 && (tid & 127) < HALF;
+    float x1 = 0.0f, x2 = 0.0f, ifr = 0.0f;
+    int32_t pos = 0;
+    if constexpr (STEP) {
+        pos = part.length + (b.depths ? b.depths[part.first] : 0);
+        if (on) {
+            const float* src = (tid < 128 ? a.k_new : a.v_new) + (static_cast<size_t>(part.first) * c.kv_heads + g) * HD + (tid & 127);
+            x1 = src[0];
+            x2 = src[HALF];
+            ifr = a.p.inv_freq[tid & 127];
+        }
+    }
+
+    // The tile's keys: tokens below n_keys that some row sees, below n_all that all see.
+    const int32_t t_first = row0 / G, t_last = (row0 + held - 1) / G;
+    const int64_t new_first = part.length;
+    const bool tree = b.masks != nullptr;
+    const int32_t n_keys = tree ? part.keys : static_cast<int32_t>(min(static_cast<int64_t>(part.keys), max(new_first + t_last + 1, int64_t{0})));
+    const int32_t n_all = static_cast<int32_t>(min(static_cast<int64_t>(n_keys), max(new_first + (tree ? 0 : t_first + 1), int64_t{0})));
+    const int32_t chunks = (n_keys + CHUNK - 1) / CHUNK;
+    const int32_t splits = max(1, min(part.splits, (chunks + part.per - 1) / part.per));
+    if (part.split >= splits) return;
+    const int32_t c0 = static_cast<int32_t>(static_cast<int64_t>(chunks) * part.split / splits);
+    const int32_t c1 = static_cast<int32_t>(static_cast<int64_t>(chunks) * (part.split + 1) / splits);
+
+    // A chunk's halves of 16 tokens, each in one page: where they begin, and which there are.
+    typedef const __attribute__((address_space(4))) int32_t* table_t;  // (read-only, by uniform indexes)
+    const table_t table = (table_t)(b.tables + static_cast<size_t>(part.sequence) * b.table_stride);
+    const int32_t last_entry = n_keys > 0 ? (n_keys - 1) >> c.page_shift : 0;
+    struct Pages {
+        int32_t page[2];
+    };
+    auto pages_of = [&](int32_t ch) {
+        Pages p;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) p.page[h] = table[min((ch * CHUNK + 16 * h) >> c.page_shift, last_entry)];
+        return p;
+    };
+    const int32_t in_page = (1 << c.page_shift) - 1;
+    struct Where {
+        size_t base[2];
+        uint32_t there;  // bit: a token that the sequence holds
+    };
+    auto where_of = [&](int32_t ch, const Pages& p) {
+        Where w;
+        w.there = 0;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int32_t x = ch * CHUNK + 16 * h;
+            const bool fine = p.page[h] >= 0 && p.page[h] < c.pages;
+            const size_t page = fine ? p.page[h] : 0;
+            w.base[h] = (((page * c.kv_heads + g) << c.page_shift) + (x & in_page)) * (HD * F::E);
+            const int32_t m = min(max(n_keys - x, 0), 16);
+            w.there |= (fine ? (1u << m) - 1u : 0u) << (16 * h);
+        }
+        return w;
+    };
+
+    uint32_t kr[X::KT][X::QS][X::KW], vr[X::VS][8][X::VW];
+    auto load_keys = [&](const Where& w) {
+#pragma unroll
+        for (int t = 0; t < X::KT; ++t) {
+            const size_t base = X::SMALL ? w.base[t] : col < 16 ? w.base[0] : w.base[1];
+            const uint8_t* p = c.keys + base + ((col & 15) * HD + 8 * grp) * F::E;
+#pragma unroll
+            for (int s = 0; s < X::QS; ++s) load_words(p + (X::SMALL ? 32 : 16) * s * F::E, kr[t][s]);
+        }
+    };
+    // the token of a lane's value (or weight) e of step s
+    auto token_of = [&](int s, int e) { return X::SMALL ? 16 * (e >> 2) + 4 * grp + (e & 3) : 16 * s + 8 * (e >> 2) + 4 * grp + (e & 3); };
+    auto load_values = [&](const Where& w) {
+#pragma unroll
+        for (int s = 0; s < X::VS; ++s)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const uint8_t* p = c.values + w.base[X::SMALL ? e >> 2 : s] + ((token_of(s, e) & 15) * HD + col * X::DB) * F::E;
+                if constexpr (X::DB * F::E == 2) vr[s][e][0] = *reinterpret_cast<const uint16_t*>(p);
+                else load_words(p, vr[s][e]);
+            }
+    };
+    // a step's token in its chunk's registers, whatever the loads saw
+    const bool holder = STEP && part.split == splits - 1;
+    auto patch = [&]() {
+        if constexpr (STEP) {
+            const int32_t at = part.length & (CHUNK - 1);
+#pragma unroll
+            for (int t = 0; t < X::KT; ++t)
+                if (16 * t + col == at)
+#pragma unroll
+                    for (int s = 0; s < X::QS; ++s) load_words(sh.key + (32 * s + 8 * grp) * F::E, kr[t][s]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (token_of(0, e) == at) load_words(sh.value + col * X::DB * F::E, vr[0][e]);
+        }
+    };
+    int32_t ch = c0 + wave;
+    Where here{};
+    Pages pages{};
+    if (ch < c1) {
+        here = where_of(ch, pages_of(ch));
+        load_keys(here);
+        load_values(here);
+        pages = pages_of(min(ch + NW, c1 - 1));
+    }
+    if constexpr (STEP) {
+        if (on) {  // cosines by the key's threads, sines by the value's
+            if (tid < 128) sh.cosines[tid] = rope_cos(pos, ifr);
+            else sh.sines[tid - 128] = rope_sin(pos, ifr);
+        }
+        __syncthreads();
+    }
+
+    // the rows' parts through LDS
+    typedef typename std::conditional<FMT == KT_PAGED_F16, _Float16, __bf16>::type element;
+    element* qs = reinterpret_cast<element*>(lds);  // [QP][R][QR]
+#pragma unroll
+    for (int i = 0; i < RW; ++i) {
+        if (4 * (wave + i * NW) >= held) break;
+        const int32_t r = 4 * (wave + i * NW) + lr;
+        uint32_t top = 0;
+#pragma unroll
+        for (int u = 0; u < DL; ++u) {
+            if constexpr (STEP) {
+                const int32_t d = (4 * lc + 64 * u) % HD;
+                const bool upper = d >= HALF;
+                const f4 cf = *reinterpret_cast<const f4*>(&sh.cosines[d % HALF]), sf = *reinterpret_cast<const f4*>(&sh.sines[d % HALF]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float y1, y2;
+                    rope_apply(upper ? qo[i][u][e] : qv[i][u][e], upper ? qv[i][u][e] : qo[i][u][e], cf[e], sf[e], y1, y2);
+                    qv[i][u][e] = upper ? y2 : y1;
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) top = max(top, magnitude(qv[i][u][e]));
+        }
+        int32_t up = 0;
+        if constexpr (FMT == KT_PAGED_F16) {
+            // the row scaled by a power of two to 2^13 .. 2^14 (bits below an infinity's, whose order is the floats')
+            float most = __builtin_bit_cast(float, min(top, 0x7F7FFFFFu));
+            most = fmaxf(most, dpp_move<0xB1>(most));
+            most = fmaxf(most, dpp_move<0x4E>(most));
+            most = fmaxf(most, dpp_move<0x141>(most));
+            most = fmaxf(most, dpp_move<0x140>(most));
+            up = 13 - max(static_cast<int32_t>(__builtin_bit_cast(uint32_t, most) >> 23) - 127, -100);
+        }
+        if (r < held) {
+#pragma unroll
+            for (int u = 0; u < DL; ++u) {
+                if (4 * lc + 64 * u >= HD) continue;
+                float rest[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) rest[e] = FMT == KT_PAGED_F16 ? ldexpf(qv[i][u][e], up) : qv[i][u][e];
+#pragma unroll
+                for (int w = 0; w < F::QP; ++w) {
+                    element part4[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        part4[e] = static_cast<element>(rest[e]);
+                        rest[e] -= static_cast<float>(part4[e]);
+                    }
+                    __builtin_memcpy(__builtin_assume_aligned(qs + (w * R + r) * QR + 4 * lc + 64 * u, 8), part4, sizeof(part4));
+                }
+            }
+            if (lc == 0) fr_s[r] = ldexpf(a.p.scale * 1.4426950408889634f, -up);
+        }
+    }
+    if constexpr (STEP) {
+        if (on) {  // the new token as the cache holds it
+            const int32_t i = tid & 127;
+            if (tid < 128) {
+                const float k1 = x1, k2 = x2;
+                rope_apply(k1, k2, sh.cosines[i], sh.sines[i], x1, x2);
+            }
+            uint8_t* mine = tid < 128 ? sh.key : sh.value;
+            store_element<FMT>(mine, i, x1);
+            store_element<FMT>(mine, i + HALF, x2);
+            if (holder) {
+                const int64_t at = place_of(c, b, part.sequence, part.length, g);
+                if (at >= 0) {
+                    store_element<FMT>(tid < 128 ? c.keys : c.values, at + i, x1);
+                    store_element<FMT>(tid < 128 ? c.keys : c.values, at + i + HALF, x2);
+                }
+            }
+        }
+    }
+    __syncthreads();
+    op qreg[X::QREG ? X::QS : 1][F::QP];
+    const element* qrow[X::CT];
+    float fr[X::CT];
+    int32_t token[X::CT];  // of the column's row, among the sequence's new ones
+#pragma unroll
+    for (int ct = 0; ct < X::CT; ++ct) {
+        const int32_t r = min(32 * ct + col, held - 1);  // (columns past the rows repeat the last)
+        fr[ct] = fr_s[r];
+        token[ct] = (row0 + r) / G;
+        qrow[ct] = qs + r * QR + 8 * grp;
+    }
+    auto query = [&](int ct, int s, op (&q)[F::QP]) {  // step s of column tile ct's operands
+#pragma unroll
+        for (int w = 0; w < F::QP; ++w) q[w] = *reinterpret_cast<const op*>(qrow[ct] + w * R * QR + (X::SMALL ? 32 : 16) * s);
+    };
+    if constexpr (X::QREG) {
+#pragma unroll
+        for (int s = 0; s < X::QS; ++s) query(0, s, qreg[s]);
+    }
+    if constexpr (STEP) {
+        if (holder && ch < c1 && ch == part.length / CHUNK) patch();
+    }
+
+    // the tokens of a chunk that a column's row sees, a bit each
+    auto seen = [&](int ct, int32_t x0, uint32_t there) {
+        const int64_t below = new_first - x0;  // tokens of the chunk before the new ones
+        uint32_t bits = below >= 32 ? 0xFFFFFFFFu : below <= 0 ? 0u : (1u << below) - 1u;
+        if (tree) {
+            const uint32_t* mask = b.masks + static_cast<size_t>(part.first + token[ct]) * b.mask_words;
+            auto word = [&](int64_t w) { return w >= 0 && w < b.mask_words ? mask[w] : 0u; };
+            if (below < 32) {  // the mask's bits from -below on
+                const int64_t from = -below, w = from >> 5;
+                const int32_t by = static_cast<int32_t>(from & 31);
+                bits |= word(w) >> by | (by ? word(w + 1) << (32 - by) : 0u);
+            }
+        } else {
+            const int64_t upto = below + token[ct] + 1;
+            bits = upto >= 32 ? 0xFFFFFFFFu : upto <= 0 ? 0u : (1u << upto) - 1u;
+        }
+        return bits & there;
+    };
+
+    typedef typename std::conditional<X::SMALL, f4, f16v>::type acc_t;
+    acc_t o[X::CT][X::DB];
+    float m[X::CT], l[X::CT];
+#pragma unroll
+    for (int ct = 0; ct < X::CT; ++ct) {
+        m[ct] = -INFINITY;
+        l[ct] = 0.0f;
+#pragma unroll
+        for (int db = 0; db < X::DB; ++db)
+#pragma unroll
+            for (int e = 0; e < X::OE; ++e) o[ct][db][e] = 0.0f;
+    }
+    // the operands of dim block db, step s: the tokens' elements of the lane's dim
+    auto value_operand = [&](int s, int db, op (&v)[F::KP]) {
+        if constexpr (FMT == KT_PAGED_F32) {
+            uint32_t w[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[e] = vr[s][e][db];
+            to_operands<FMT>(w, v);
+        } else {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = __builtin_amdgcn_perm(vr[s][2 * i + 1][db / 2], vr[s][2 * i][db / 2], db % 2 ? 0x07060302u : 0x05040100u);
+            to_operands<FMT>(w, v);
+        }
+    };
+    // (two forms of the loop's body: only chunks that not every row sees whole compare keys with rows)
+    auto attend_chunk = [&](auto masked_form) {
+        constexpr bool masked = decltype(masked_form)::value;
+        const Where now = here;
+        acc_t sc[X::CT][X::KT];
+#pragma unroll
+        for (int ct = 0; ct < X::CT; ++ct)
+#pragma unroll
+            for (int t = 0; t < X::KT; ++t)
+#pragma unroll
+                for (int e = 0; e < X::OE; ++e) sc[ct][t][e] = 0.0f;
+#pragma unroll
+        for (int s = 0; s < X::QS; ++s) {
+            op k[X::KT][F::KP];
+#pragma unroll
+            for (int t = 0; t < X::KT; ++t) to_operands<FMT>(kr[t][s], k[t]);
+#pragma unroll
+            for (int ct = 0; ct < X::CT; ++ct) {
+                if constexpr (X::QREG) {
+#pragma unroll
+                    for (int t = 0; t < X::KT; ++t) sc[ct][t] = products<X::SMALL>(k[t], qreg[s], sc[ct][t]);
+                } else {
+                    op q[F::QP];
+                    query(ct, s, q);
+#pragma unroll
+                    for (int t = 0; t < X::KT; ++t) sc[ct][t] = products<X::SMALL>(k[t], q, sc[ct][t]);
+                }
+            }
+        }
+        const int32_t next = min(ch + NW, c1 - 1);  // (past the end the last chunk again, unused)
+        here = where_of(next, pages);
+        load_keys(here);
+        pages = pages_of(min(ch + 2 * NW, c1 - 1));
+        op p[X::CT][X::VS][F::QP];
+        float x[X::CT][X::E];
+        uint32_t vis[X::CT];
+#pragma unroll
+        for (int ct = 0; ct < X::CT; ++ct) {
+            if constexpr (masked) vis[ct] = seen(ct, ch * CHUNK, now.there);
+            auto hidden = [&](int i) { return masked && !(vis[ct] >> token_of(i >> 3, i & 7) & 1); };
+            float most = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < X::E; ++i) {
+                x[ct][i] = X::SMALL ? sc[ct][X::SMALL ? i >> 2 : 0][X::SMALL ? i & 3 : i] : sc[ct][0][i];
+                if (hidden(i)) x[ct][i] = -INFINITY;
+                most = fmaxf(most, x[ct][i]);
+            }
+            most = rounded_score(most, fr[ct]);
+            if (__ballot(most - m[ct] > LAZY)) {
+                const float m_new = fmaxf(m[ct], column_max<X::SMALL>(most));
+                const float alpha = m[ct] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[ct] - m_new);
+                l[ct] *= alpha;
+#pragma unroll
+                for (int db = 0; db < X::DB; ++db) o[ct][db] *= alpha;
+                m[ct] = m_new;
+            }
+            const float at = m[ct] == -INFINITY ? 0.0f : m[ct];
+            if (__ballot(fabsf(at) > HUGE_SCORE)) {  // (one-hot rows)
+#pragma unroll
+                for (int i = 0; i < X::E; ++i) x[ct][i] = weight_of_huge(x[ct][i], fr[ct], at, F::UP);
+            } else {
+#pragma unroll
+                for (int i = 0; i < X::E; ++i) x[ct][i] = __builtin_amdgcn_exp2f(fmaf(x[ct][i], fr[ct], F::UP - at));
+            }
+#pragma unroll
+            for (int i = 0; i < X::E; ++i) {
+                if (hidden(i)) x[ct][i] = 0.0f;  // (of a row with an infinite maximum)
+                l[ct] += x[ct][i];
+            }
+#pragma unroll
+            for (int s = 0; s < X::VS; ++s) {
+                float w[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) w[e] = x[ct][8 * s + e];
+                split_weights(w, p[ct][s]);
+            }
+        }
+        if constexpr (masked) {
+            // values of tokens that are not there count for nothing; what is not finite goes to the rows that see it alone
+            bool odd = false;
+#pragma unroll
+            for (int s = 0; s < X::VS; ++s)
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+#pragma unroll
+                    for (int w = 0; w < X::VW; ++w) {
+                        if (!(now.there >> token_of(s, e) & 1)) vr[s][e][w] = 0;
+                        odd |= any_not_finite<FMT>(vr[s][e][w]);
+                    }
+            if (__ballot(odd)) {
+                const bool own = STEP && holder && ch == part.length / CHUNK;  // (the new token is in LDS)
+                for (int32_t tok = 0; tok < CHUNK; ++tok) {
+                    if (!(now.there >> tok & 1)) continue;
+                    const int32_t from = X::SMALL ? tok >> 2 & 3 : tok >> 2 & 1, i = X::SMALL ? 4 * (tok >> 4) + (tok & 3) : 4 * (tok >> 3) + (tok & 3);
+                    const uint8_t* row = c.values + (tok < 16 ? now.base[0] : now.base[1]) + (tok & 15) * HD * F::E;
+                    if constexpr (STEP) {
+                        if (own && tok == (part.length & (CHUNK - 1))) row = sh.value;
+                    }
+#pragma unroll
+                    for (int ct = 0; ct < X::CT; ++ct) {
+                        float weight = 0.0f;
+#pragma unroll
+                        for (int e = 0; e < X::E; ++e)
+                            if (e == i) weight = x[ct][e];
+                        weight = __shfl(weight, from * X::LANES + col);
+                        if (!(vis[ct] >> tok & 1)) continue;
+#pragma unroll
+                        for (int e = 0; e < X::OE; ++e) {
+                            const int32_t d = (X::SMALL ? 4 * grp + e : 8 * (e >> 2) + 4 * grp + (e & 3)) * X::DB;
+#pragma unroll
+                            for (int db = 0; db < X::DB; ++db) {
+                                const float v = load_element<FMT>(row, d + db);
+                                if (!(fabsf(v) < INFINITY)) o[ct][db][e] += weight * v;
+                            }
+                        }
+                    }
+                }
+#pragma unroll
+                for (int s = 0; s < X::VS; ++s)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+#pragma unroll
+                        for (int w = 0; w < X::VW; ++w) vr[s][e][w] = finite_only<FMT>(vr[s][e][w]);
+            }
+        }
+#pragma unroll
+        for (int db = 0; db < X::DB; ++db)
+#pragma unroll
+            for (int s = 0; s < X::VS; ++s) {
+                op v[F::KP];
+                value_operand(s, db, v);
+#pragma unroll
+                for (int ct = 0; ct < X::CT; ++ct) o[ct][db] = products<X::SMALL>(v, p[ct][s], o[ct][db]);
+            }
+        load_values(here);
+        if constexpr (STEP) {
+            if (holder && next == part.length / CHUNK) patch();
+        }
+    };
+    for (; ch < c1; ch += NW) {
+        if (ch * CHUNK + CHUNK <= n_all && here.there == 0xFFFFFFFFu) attend_chunk(std::false_type{});
+        else attend_chunk(std::true_type{});
+    }
+
+    // each wave's averages, maxima and sums, then all waves' through LDS
+    const int32_t used = min(NW, c1 - c0);  // waves with keys
+    __syncthreads();                        // (the queries' parts are read)
+    if (wave < used) {
+#pragma unroll
+        for (int ct = 0; ct < X::CT; ++ct) {
+            l[ct] = column_sum<X::SMALL>(l[ct]);
+            const float inv = l[ct] == 0.0f ? 0.0f : 1.0f / l[ct];
+            if (32 * ct + col >= held) continue;
+            float* row = avg + (wave * R + 32 * ct + col) * LR;
+#pragma unroll
+            for (int e = 0; e < X::OE; ++e) {
+                const int32_t d = (X::SMALL ? 4 * grp + e : 8 * (e >> 2) + 4 * grp + (e & 3)) * X::DB;
+#pragma unroll
+                for (int db = 0; db < X::DB; ++db) row[d + db] = o[ct][db][e] * inv;
+            }
+            if (grp == 0) {
+                ms[wave * R + 32 * ct + col] = m[ct];
+                ls[wave * R + 32 * ct + col] = l[ct];
+            }
+        }
+    }
+    __syncthreads();
+    const size_t at_slot = static_cast<size_t>(part.slot + part.split) * R;
+    const __amdgpu_buffer_rsrc_t averages = __builtin_amdgcn_make_buffer_rsrc(a.averages + at_slot * HD, 0, R * HD * 4, 0x00020000);
+    for (int32_t e = tid; e < held * (HD / 4); e += 64 * NW) {  // (every thread weighs its row's parts itself: no further barrier)
+        const int32_t r = e / (HD / 4), d = 4 * (e % (HD / 4));
+        float mx = -INFINITY, sum = 0.0f;
+        f4 y = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int32_t w = 0; w < used; ++w) mx = fmaxf(mx, ms[w * R + r]);
+        for (int32_t w = 0; w < used; ++w) {
+            const float by = share_of(ms[w * R + r], ls[w * R + r], mx);
+            const f4 v = *reinterpret_cast<const f4*>(avg + (w * R + r) * LR + d);
+            sum += by;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y[i] = fmaf(by, v[i], y[i]);
+        }
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] *= inv;
+        if (splits == 1) {
+            *reinterpret_cast<f4*>(a.p.context + row_at(r) + d) = y;
+        } else {  // written through to memory: the reader may be on another die
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, y), averages, (r * HD + d) * 4, 0, THROUGH);
+            if (d == 0) {
+                const uint64_t both = __builtin_bit_cast(uint32_t, mx) | static_cast<uint64_t>(__builtin_bit_cast(uint32_t, sum)) << 32;
+                __hip_atomic_store(reinterpret_cast<uint64_t*>(a.stats) + at_slot + r, both, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+            }
+        }
+    }
+    if (splits == 1) return;
+    // the last workgroup of the tile to arrive merges the parts, in their order
+    __shared__ uint32_t arrived;
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if (tid == 0) {
+        uint32_t* counter = a.counters + part.slot;
+        arrived = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+        if (arrived == static_cast<uint32_t>(splits) - 1) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+    }
+    __syncthreads();
+    if (arrived != static_cast<uint32_t>(splits) - 1) return;
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
+    const size_t slot0 = static_cast<size_t>(part.slot) * R;
+    float* weight = lds;                       // [R][MAX_SPLITS]
+    float* total = weight + R * MAX_SPLITS;    // [R]
+    f4* shares = reinterpret_cast<f4*>(total + R);  // [64 NW]
+    // thread (four dims of a row, phase): every phases-th part, eight loads in flight together, the first eight with the
+    // maxima and sums
+    constexpr int BATCH = 8;
+    const __amdgpu_buffer_rsrc_t all = __builtin_amdgcn_make_buffer_rsrc(a.averages + slot0 * HD, 0, splits * R * HD * 4, 0x00020000);
+    const int32_t items = held * (HD / 4), phases = max(1, 64 * NW / items);
+    const int32_t phase = phases > 1 ? tid / items : 0;
+    u4 v[BATCH];
+    auto load_batch = [&](int32_t item, int32_t s0) {
+        const int32_t at = (min(item, items - 1) / (HD / 4)) * HD + 4 * (min(item, items - 1) % (HD / 4));
+#pragma unroll
+        for (int u = 0; u < BATCH; ++u) v[u] = __builtin_amdgcn_raw_buffer_load_b128(all, (min(s0 + u * phases, splits - 1) * R * HD + at) * 4, 0, THROUGH);
+    };
+    load_batch(phases > 1 ? tid % items : tid, phase);
+    for (int32_t r = wave; r < held; r += NW) {  // a row's weights: lane = part
+        float ml[MAX_SPLITS / 64], ll[MAX_SPLITS / 64], mx = -INFINITY, sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < MAX_SPLITS / 64; ++i) {
+            const int32_t s = lane + 64 * i;
+            const uint64_t both = __hip_atomic_load(reinterpret_cast<uint64_t*>(a.stats) + slot0 + static_cast<size_t>(min(s, splits - 1)) * R + r, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+            ml[i] = s < splits ? __builtin_bit_cast(float, static_cast<uint32_t>(both)) : -INFINITY;
+            ll[i] = s < splits ? __builtin_bit_cast(float, static_cast<uint32_t>(both >> 32)) : 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < MAX_SPLITS / 64; ++i) mx = fmaxf(mx, wave_max_dpp(ml[i]));
+#pragma unroll
+        for (int i = 0; i < MAX_SPLITS / 64; ++i) {
+            const float by = share_of(ml[i], ll[i], mx);
+            weight[r * MAX_SPLITS + lane + 64 * i] = by;
+            sum += wave_sum_dpp(by);
+        }
+        if (lane == 0) total[r] = sum;
+    }
+    __syncthreads();
+    for (int32_t i0 = 0; i0 < items; i0 += 64 * NW) {
+        const int32_t item = phases > 1 ? tid % items : i0 + tid;
+        const bool mine = item < items && phase < phases;
+        const int32_t r = min(item, items - 1) / (HD / 4), d = 4 * (min(item, items - 1) % (HD / 4));
+        f4 y = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int32_t s0 = phase; mine && s0 < splits; s0 += BATCH * phases) {
+            if (i0 > 0 || s0 > phase) load_batch(item, s0);
+#pragma unroll
+            for (int u = 0; u < BATCH; ++u) {
+                const int32_t s = s0 + u * phases;
+                const float by = s < splits ? weight[r * MAX_SPLITS + s] : 0.0f;
+                const f4 z = __builtin_bit_cast(f4, v[u]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) y[i] = s < splits ? fmaf(by, z[i], y[i]) : y[i];
+            }
+        }
+        if (phases > 1) {
+            shares[tid] = y;
+            __syncthreads();
+        }
+        if (mine && phase == 0) {
+            for (int32_t p = 1; p < phases; ++p)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) y[i] += shares[item + p * items][i];
+            const float inv = total[r] == 0.0f ? 0.0f : 1.0f / total[r];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y[i] *= inv;
+            *reinterpret_cast<f4*>(a.p.context + row_at(r) + d) = y;
+        }
+    }
+}
+
+// ---- launches ---------------------------------------------------------------------------------------
+template <int FMT, int HD, int R, int NW, bool STEP>
+int32_t launch_rows(Args a, hipStream_t st) {
+    const BatchView& b = a.p.b;
+    const int64_t G = a.p.num_heads / a.p.c.kv_heads;
+    const int64_t tiles = std::min(b.sequences * ((b.most_rows * G + R - 1) / R), b.rows * G / R + b.sequences) * a.p.c.kv_heads;
+    const int64_t chunks = (static_cast<int64_t>(b.key_bound) + CHUNK - 1) / CHUNK, most_splits = std::min<int64_t>(MAX_SPLITS, (chunks + NW - 1) / NW);
+    a.target = 2 * cu_count();
+    const int64_t grid = std::min(tiles + a.target, tiles * most_splits);
+    if (grid > INT32_MAX / 64) return fail(KT_ERR_SHAPE, "too many rows and heads in one call");
+    if (most_splits > 1) {
+        const size_t slots = static_cast<size_t>(std::min<int64_t>(2 * a.target, grid));
+        void* ws = nullptr;
+        if (const int32_t status = workspace_counters(st, slots * R * (HD + 2) * sizeof(float) + 16, slots, &ws, &a.counters)) return status;
+        ws = reinterpret_cast<void*>((reinterpret_cast<uintptr_t>(ws) + 15) & ~uintptr_t{15});  // (it begins at any dword)
+        a.averages = static_cast<float*>(ws);
+        a.stats = a.averages + slots * R * HD;
+    }
+    constexpr size_t lds = std::max(std::max(sizeof(float) * NW * R * (HD + 6), size_t{2} * Format<FMT>::QP * R * (HD + 8)), sizeof(float) * (R * (MAX_SPLITS + 1) + 4 * 64 * NW));
+    if (const int32_t ls = allow_lds<&attention_kernel<FMT, HD, R, NW, STEP>, lds>(lds)) return ls;
+    attention_kernel<FMT, HD, R, NW, STEP><<<static_cast<uint32_t>(grid), 64 * NW, lds, st>>>(a);
+    KT_LAUNCHED("paged attention kernel");
+    return KT_OK;
+}
+
+template <int FMT, int HD>
+int32_t launch_dims(const Args& a, hipStream_t st) {
+    const int64_t G = a.p.num_heads / a.p.c.kv_heads;
+    if constexpr (HD < 256) {
+        if (a.k_new) return launch_rows<FMT, HD, 16, 4, true>(a, st);
+        if (a.p.b.most_rows * G > 16) return launch_rows<FMT, HD, 32, 4, false>(a, st);
+    }
+    return launch_rows<FMT, HD, 16, 4, false>(a, st);
+}
+
+template <int FMT>
+int32_t launch(const PagedAttnArgs& p, const float* k, const float* v, hipStream_t st) {
+    Args a{};
+    a.p = p;
+    a.k_new = k;
+    a.v_new = v;
+    switch (p.c.head_dim) {
+        case 32: return launch_dims<FMT, 32>(a, st);
+        case 64: return launch_dims<FMT, 64>(a, st);
+        case 128: return launch_dims<FMT, 128>(a, st);
+        default: return launch_dims<FMT, 256>(a, st);
+    }
+}
+
+}  // namespace paged
+}  // namespace kt
