@@ -90,6 +90,15 @@ __device__ __forceinline__ void split_weights(const float (&v)[8], half8 (&part)
     }
 }
 
+__device__ __forceinline__ void split_query(const float (&v)[8], bf16x8 (&part)[3]) { split3_nearest(v, part); }
+__device__ __forceinline__ void split_query(const float (&v)[8], half8 (&part)[2]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        part[0][i] = static_cast<_Float16>(v[i]);
+        part[1][i] = static_cast<_Float16>(v[i] - static_cast<float>(part[0][i]));
+    }
+}
+
 // Eight consecutive elements (registers of a row) as operands.
 template <int FMT>
 __device__ __forceinline__ void to_operands(const uint32_t* w, typename Format<FMT>::op (&part)[Format<FMT>::KP]) {
@@ -158,6 +167,60 @@ __device__ __forceinline__ float share_of(float m, float l, float mx) {
     return l == 0.0f ? 0.0f : l * __builtin_amdgcn_exp2f((m == -INFINITY ? mx : m) - (mx == -INFINITY ? 0.0f : mx));
 }
 
+// A chunk's scores x of one row (a lane's share of them) into weights; m and l: the row's running maximum and the sum of this
+// lane's weights; rescale: what the maximum's move does to the sums. vis: the tokens that the row sees, a bit each.
+template <int FMT, bool SMALL, bool masked, int E, typename TOKEN, typename RESCALE>
+__device__ __forceinline__ void to_weights(float (&x)[E], uint32_t vis, float f, float& m, float& l, TOKEN token_of, RESCALE rescale) {
+    constexpr float UP = Format<FMT>::UP;
+    auto hidden = [&](int i) { return masked && !(vis >> token_of(i) & 1); };
+    float most = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        if (hidden(i)) x[i] = -INFINITY;
+        most = fmaxf(most, x[i]);
+    }
+    most = rounded_score(most, f);
+    if (__ballot(most - m > LAZY)) {
+        const float m_new = fmaxf(m, column_max<SMALL>(most));
+        const float alpha = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - m_new);
+        l *= alpha;
+        rescale(alpha);
+        m = m_new;
+    }
+    const float at = m == -INFINITY ? 0.0f : m;
+    if (__ballot(fabsf(at) > HUGE_SCORE)) {  // (one-hot rows)
+#pragma unroll
+        for (int i = 0; i < E; ++i) x[i] = weight_of_huge(x[i], f, at, UP);
+    } else {
+#pragma unroll
+        for (int i = 0; i < E; ++i) x[i] = __builtin_amdgcn_exp2f(fmaf(x[i], f, UP - at));
+    }
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        if (hidden(i)) x[i] = 0.0f;  // (of a row with an infinite maximum)
+        l += x[i];
+    }
+}
+
+// The tokens x0 .. x0 + 31 that row `index` of a sequence's rows sees, a bit each.
+__device__ __forceinline__ uint32_t seen_bits(const BatchView& b, int32_t first, int32_t index, int64_t length, int32_t x0, uint32_t there) {
+    const int64_t below = length - x0;  // tokens of the chunk before the new ones
+    uint32_t bits = below >= 32 ? 0xFFFFFFFFu : below <= 0 ? 0u : (1u << below) - 1u;
+    if (b.masks) {
+        const uint32_t* mask = b.masks + static_cast<size_t>(first + index) * b.mask_words;
+        auto word = [&](int64_t w) { return w >= 0 && w < b.mask_words ? mask[w] : 0u; };
+        if (below < 32) {  // the mask's bits from -below on
+            const int64_t from = -below, w = from >> 5;
+            const int32_t by = static_cast<int32_t>(from & 31);
+            bits |= word(w) >> by | (by ? word(w + 1) << (32 - by) : 0u);
+        }
+    } else {
+        const int64_t upto = below + index + 1;
+        bits = upto >= 32 ? 0xFFFFFFFFu : upto <= 0 ? 0u : (1u << upto) - 1u;
+    }
+    return bits & there;
+}
+
 // ---- the parts of a launch ---------------------------------------------------------------------
 struct Args {
     PagedAttnArgs p;
@@ -190,7 +253,7 @@ __device__ __forceinline__ int32_t lane_int(int32_t v, int32_t lane) { return __
 
 // Which part of the launch workgroup `at` has; false: none. Every lane is a sequence. A launch has at most target + (its tiles
 // of all kv heads) parts, and at most 2 target that share a tile: a part's size is at least the chunks over target.
-template <int R, int NW>
+template <int R, int LEAST>
 __device__ __forceinline__ bool find_part(const Args& a, int32_t at, Part& out) {
     const PagedView& c = a.p.c;
     const BatchView& b = a.p.b;
@@ -215,8 +278,7 @@ __device__ __forceinline__ bool find_part(const Args& a, int32_t at, Part& out) 
     total = wave_total(total);
     if (wave_total(rows) > b.rows) return false;  // starts that do not ascend
     int64_t per = (total + a.target - 1) / a.target;
-    per = (per + NW - 1) / NW * NW;
-    if (per < NW) per = NW;
+    per = (max(per, int64_t{1}) + LEAST - 1) / LEAST * LEAST;
     int32_t before = 0, slots = 0;
     for (int32_t s0 = 0; s0 < b.sequences; s0 += 64) {
         if (b.sequences > 64) load(s0);
@@ -254,6 +316,165 @@ __device__ __forceinline__ bool find_part(const Args& a, int32_t at, Part& out) 
         slots += lane_int(slots_upto, 63);
     }
     return false;
+}
+
+// A tile's keys: tokens below n_keys that some row sees, below n_all that all see; the part's chunks c0 .. c1 - 1.
+struct Keys {
+    int32_t n_keys, n_all, splits, c0, c1;
+};
+template <int R>
+__device__ __forceinline__ Keys keys_of(const Args& a, const Part& part, int32_t held) {
+    const int32_t G = a.p.num_heads / a.p.c.kv_heads, t_first = part.tile * R / G, t_last = (part.tile * R + held - 1) / G;
+    const int64_t length = part.length;
+    const bool tree = a.p.b.masks != nullptr;
+    Keys k;
+    k.n_keys = tree ? part.keys : static_cast<int32_t>(min(static_cast<int64_t>(part.keys), max(length + t_last + 1, int64_t{0})));
+    k.n_all = static_cast<int32_t>(min(static_cast<int64_t>(k.n_keys), max(length + (tree ? 0 : t_first + 1), int64_t{0})));
+    const int32_t chunks = (k.n_keys + CHUNK - 1) / CHUNK;
+    k.splits = max(1, min(part.splits, (chunks + part.per - 1) / part.per));
+    k.c0 = static_cast<int32_t>(static_cast<int64_t>(chunks) * part.split / k.splits);
+    k.c1 = static_cast<int32_t>(static_cast<int64_t>(chunks) * (part.split + 1) / k.splits);
+    return k;
+}
+
+// A chunk's halves of 16 tokens, each in one page: their pages, then where they begin (bytes from the layer's keys or values)
+// and which tokens there are, a bit each.
+struct Pages {
+    int32_t page[2];
+};
+struct Where {
+    size_t base[2];
+    uint32_t there;
+};
+struct PageReader {
+    typedef const __attribute__((address_space(4))) int32_t* table_t;  // (read-only, by uniform indexes)
+    const PagedView& c;
+    table_t table;
+    int32_t head, n_keys, last_entry, row_bytes;
+    __device__ __forceinline__ PageReader(const PagedView& view, const BatchView& b, const Part& part, int32_t keys, int32_t element)
+        : c(view), table((table_t)(b.tables + static_cast<size_t>(part.sequence) * b.table_stride)), head(part.head), n_keys(keys),
+          last_entry(keys > 0 ? (keys - 1) >> view.page_shift : 0), row_bytes(view.head_dim * element) {}
+    __device__ __forceinline__ Pages pages_of(int32_t ch) const {
+        Pages p;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) p.page[h] = table[min((ch * CHUNK + 16 * h) >> c.page_shift, last_entry)];
+        return p;
+    }
+    __device__ __forceinline__ Where where_of(int32_t ch, const Pages& p) const {
+        Where w;
+        w.there = 0;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int32_t x = ch * CHUNK + 16 * h;
+            const bool fine = p.page[h] >= 0 && p.page[h] < c.pages;
+            const size_t page = fine ? p.page[h] : 0;  // (any memory of the pool)
+            w.base[h] = (((page * c.kv_heads + head) << c.page_shift) + (x & ((1 << c.page_shift) - 1))) * row_bytes;
+            const int32_t m = min(max(n_keys - x, 0), 16);
+            w.there |= (fine ? (1u << m) - 1u : 0u) << (16 * h);
+        }
+        return w;
+    }
+};
+
+// ---- where the parts of a tile meet ----------------------------------------------------------------
+// A part's averages and its rows' maxima and sums, written through to memory: the reader may be on another die.
+__device__ __forceinline__ void store_average(const __amdgpu_buffer_rsrc_t& averages, int32_t at, f4 y) {
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, y), averages, at * 4, 0, THROUGH);
+}
+__device__ __forceinline__ void store_stats(const Args& a, size_t row, float m, float l) {
+    const uint64_t both = __builtin_bit_cast(uint32_t, m) | static_cast<uint64_t>(__builtin_bit_cast(uint32_t, l)) << 32;
+    __hip_atomic_store(reinterpret_cast<uint64_t*>(a.stats) + row, both, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+}
+template <int HD, int R>
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t averages_of(const Args& a, size_t slot, int32_t slots) {
+    return __builtin_amdgcn_make_buffer_rsrc(a.averages + slot * R * HD, 0, slots * R * HD * 4, 0x00020000);
+}
+constexpr size_t merge_lds(int R, int NW) { return sizeof(float) * (R * (MAX_SPLITS + 1) + 4 * 64 * NW); }
+
+// Called by all threads of a workgroup once its part is stored. The last workgroup of the tile to arrive merges the
+// parts, in their order, into the context; row_at: where a row of the tile lies there.
+template <int HD, int R, int NW, typename ROW>
+__device__ __forceinline__ void meet(const Args& a, const Part& part, int32_t splits, int32_t held, float* lds, ROW row_at) {
+    const int32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    __shared__ uint32_t arrived;
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if (tid == 0) {
+        uint32_t* counter = a.counters + part.slot;
+        arrived = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+        if (arrived == static_cast<uint32_t>(splits) - 1) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+    }
+    __syncthreads();
+    if (arrived != static_cast<uint32_t>(splits) - 1) return;
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
+    const size_t slot0 = static_cast<size_t>(part.slot) * R;
+    float* weight = lds;                       // [R][MAX_SPLITS]
+    float* total = weight + R * MAX_SPLITS;    // [R]
+    f4* shares = reinterpret_cast<f4*>(total + R);  // [64 NW]
+    // thread (four dims of a row, phase): every phases-th part, eight loads in flight together, the first eight with the
+    // maxima and sums
+    constexpr int BATCH = 8;
+    const __amdgpu_buffer_rsrc_t all = averages_of<HD, R>(a, part.slot, splits);
+    const int32_t items = held * (HD / 4), phases = max(1, 64 * NW / items);
+    const int32_t phase = phases > 1 ? tid / items : 0;
+    u4 v[BATCH];
+    auto load_batch = [&](int32_t item, int32_t s0) {
+        const int32_t at = (min(item, items - 1) / (HD / 4)) * HD + 4 * (min(item, items - 1) % (HD / 4));
+#pragma unroll
+        for (int u = 0; u < BATCH; ++u) v[u] = __builtin_amdgcn_raw_buffer_load_b128(all, (min(s0 + u * phases, splits - 1) * R * HD + at) * 4, 0, THROUGH);
+    };
+    load_batch(phases > 1 ? tid % items : tid, phase);
+    for (int32_t r = wave; r < held; r += NW) {  // a row's weights: lane = part
+        float ml[MAX_SPLITS / 64], ll[MAX_SPLITS / 64], mx = -INFINITY, sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < MAX_SPLITS / 64; ++i) {
+            const int32_t s = lane + 64 * i;
+            const uint64_t both = __hip_atomic_load(reinterpret_cast<uint64_t*>(a.stats) + slot0 + static_cast<size_t>(min(s, splits - 1)) * R + r, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+            ml[i] = s < splits ? __builtin_bit_cast(float, static_cast<uint32_t>(both)) : -INFINITY;
+            ll[i] = s < splits ? __builtin_bit_cast(float, static_cast<uint32_t>(both >> 32)) : 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < MAX_SPLITS / 64; ++i) mx = fmaxf(mx, wave_max_dpp(ml[i]));
+#pragma unroll
+        for (int i = 0; i < MAX_SPLITS / 64; ++i) {
+            const float by = share_of(ml[i], ll[i], mx);
+            weight[r * MAX_SPLITS + lane + 64 * i] = by;
+            sum += wave_sum_dpp(by);
+        }
+        if (lane == 0) total[r] = sum;
+    }
+    __syncthreads();
+    for (int32_t i0 = 0; i0 < items; i0 += 64 * NW) {
+        const int32_t item = phases > 1 ? tid % items : i0 + tid;
+        const bool mine = item < items && phase < phases;
+        const int32_t r = min(item, items - 1) / (HD / 4), d = 4 * (min(item, items - 1) % (HD / 4));
+        f4 y = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int32_t s0 = phase; mine && s0 < splits; s0 += BATCH * phases) {
+            if (i0 > 0 || s0 > phase) load_batch(item, s0);
+#pragma unroll
+            for (int u = 0; u < BATCH; ++u) {
+                const int32_t s = s0 + u * phases;
+                const float by = s < splits ? weight[r * MAX_SPLITS + s] : 0.0f;
+                const f4 z = __builtin_bit_cast(f4, v[u]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) y[i] = s < splits ? fmaf(by, z[i], y[i]) : y[i];
+            }
+        }
+        if (phases > 1) {
+            shares[tid] = y;
+            __syncthreads();
+        }
+        if (mine && phase == 0) {
+            for (int32_t p = 1; p < phases; ++p)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) y[i] += shares[item + p * items][i];
+            const float inv = total[r] == 0.0f ? 0.0f : 1.0f / total[r];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y[i] *= inv;
+            *reinterpret_cast<f4*>(a.p.context + row_at(r) + d) = y;
+        }
+    }
 }
 
 // ---- the kernel ----------------------------------------------------------------------------------
@@ -371,50 +592,11 @@ __global__ void __launch_bounds__(64 * NW, HD == 256 || (FMT == KT_PAGED_F32 && 
         }
     }
 
-    // The tile's keys: tokens below n_keys that some row sees, below n_all that all see.
-    const int32_t t_first = row0 / G, t_last = (row0 + held - 1) / G;
+    const Keys keys = keys_of<R>(a, part, held);
+    if (part.split >= keys.splits) return;
+    const int32_t splits = keys.splits, c0 = keys.c0, c1 = keys.c1, n_all = keys.n_all;
     const int64_t new_first = part.length;
-    const bool tree = b.masks != nullptr;
-    const int32_t n_keys = tree ? part.keys : static_cast<int32_t>(min(static_cast<int64_t>(part.keys), max(new_first + t_last + 1, int64_t{0})));
-    const int32_t n_all = static_cast<int32_t>(min(static_cast<int64_t>(n_keys), max(new_first + (tree ? 0 : t_first + 1), int64_t{0})));
-    const int32_t chunks = (n_keys + CHUNK - 1) / CHUNK;
-    const int32_t splits = max(1, min(part.splits, (chunks + part.per - 1) / part.per));
-    if (part.split >= splits) return;
-    const int32_t c0 = static_cast<int32_t>(static_cast<int64_t>(chunks) * part.split / splits);
-    const int32_t c1 = static_cast<int32_t>(static_cast<int64_t>(chunks) * (part.split + 1) / splits);
-
-    // A chunk's halves of 16 tokens, each in one page: where they begin, and which there are.
-    typedef const __attribute__((address_space(4))) int32_t* table_t;  // (read-only, by uniform indexes)
-    const table_t table = (table_t)(b.tables + static_cast<size_t>(part.sequence) * b.table_stride);
-    const int32_t last_entry = n_keys > 0 ? (n_keys - 1) >> c.page_shift : 0;
-    struct Pages {
-        int32_t page[2];
-    };
-    auto pages_of = [&](int32_t ch) {
-        Pages p;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) p.page[h] = table[min((ch * CHUNK + 16 * h) >> c.page_shift, last_entry)];
-        return p;
-    };
-    const int32_t in_page = (1 << c.page_shift) - 1;
-    struct Where {
-        size_t base[2];
-        uint32_t there;  // bit: a token that the sequence holds
-    };
-    auto where_of = [&](int32_t ch, const Pages& p) {
-        Where w;
-        w.there = 0;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int32_t x = ch * CHUNK + 16 * h;
-            const bool fine = p.page[h] >= 0 && p.page[h] < c.pages;
-            const size_t page = fine ? p.page[h] : 0;
-            w.base[h] = (((page * c.kv_heads + g) << c.page_shift) + (x & in_page)) * (HD * F::E);
-            const int32_t m = min(max(n_keys - x, 0), 16);
-            w.there |= (fine ? (1u << m) - 1u : 0u) << (16 * h);
-        }
-        return w;
-    };
+    const PageReader reader(c, b, part, keys.n_keys, F::E);
 
     uint32_t kr[X::KT][X::QS][X::KW], vr[X::VS][8][X::VW];
     auto load_keys = [&](const Where& w) {
@@ -457,10 +639,10 @@ __global__ void __launch_bounds__(64 * NW, HD == 256 || (FMT == KT_PAGED_F32 && 
     Where here{};
     Pages pages{};
     if (ch < c1) {
-        here = where_of(ch, pages_of(ch));
+        here = reader.where_of(ch, reader.pages_of(ch));
         load_keys(here);
         load_values(here);
-        pages = pages_of(min(ch + NW, c1 - 1));
+        pages = reader.pages_of(min(ch + NW, c1 - 1));
     }
     if constexpr (STEP) {
         if (on) {  // cosines by the key's threads, sines by the value's
@@ -568,25 +750,6 @@ __global__ void __launch_bounds__(64 * NW, HD == 256 || (FMT == KT_PAGED_F32 && 
         if (holder && ch < c1 && ch == part.length / CHUNK) patch();
     }
 
-    // the tokens of a chunk that a column's row sees, a bit each
-    auto seen = [&](int ct, int32_t x0, uint32_t there) {
-        const int64_t below = new_first - x0;  // tokens of the chunk before the new ones
-        uint32_t bits = below >= 32 ? 0xFFFFFFFFu : below <= 0 ? 0u : (1u << below) - 1u;
-        if (tree) {
-            const uint32_t* mask = b.masks + static_cast<size_t>(part.first + token[ct]) * b.mask_words;
-            auto word = [&](int64_t w) { return w >= 0 && w < b.mask_words ? mask[w] : 0u; };
-            if (below < 32) {  // the mask's bits from -below on
-                const int64_t from = -below, w = from >> 5;
-                const int32_t by = static_cast<int32_t>(from & 31);
-                bits |= word(w) >> by | (by ? word(w + 1) << (32 - by) : 0u);
-            }
-        } else {
-            const int64_t upto = below + token[ct] + 1;
-            bits = upto >= 32 ? 0xFFFFFFFFu : upto <= 0 ? 0u : (1u << upto) - 1u;
-        }
-        return bits & there;
-    };
-
     typedef typename std::conditional<X::SMALL, f4, f16v>::type acc_t;
     acc_t o[X::CT][X::DB];
     float m[X::CT], l[X::CT];
@@ -643,45 +806,21 @@ __global__ void __launch_bounds__(64 * NW, HD == 256 || (FMT == KT_PAGED_F32 && 
             }
         }
         const int32_t next = min(ch + NW, c1 - 1);  // (past the end the last chunk again, unused)
-        here = where_of(next, pages);
+        here = reader.where_of(next, pages);
         load_keys(here);
-        pages = pages_of(min(ch + 2 * NW, c1 - 1));
+        pages = reader.pages_of(min(ch + 2 * NW, c1 - 1));
         op p[X::CT][X::VS][F::QP];
         float x[X::CT][X::E];
         uint32_t vis[X::CT];
 #pragma unroll
         for (int ct = 0; ct < X::CT; ++ct) {
-            if constexpr (masked) vis[ct] = seen(ct, ch * CHUNK, now.there);
-            auto hidden = [&](int i) { return masked && !(vis[ct] >> token_of(i >> 3, i & 7) & 1); };
-            float most = -INFINITY;
+            if constexpr (masked) vis[ct] = seen_bits(b, part.first, token[ct], new_first, ch * CHUNK, now.there);
 #pragma unroll
-            for (int i = 0; i < X::E; ++i) {
-                x[ct][i] = X::SMALL ? sc[ct][X::SMALL ? i >> 2 : 0][X::SMALL ? i & 3 : i] : sc[ct][0][i];
-                if (hidden(i)) x[ct][i] = -INFINITY;
-                most = fmaxf(most, x[ct][i]);
-            }
-            most = rounded_score(most, fr[ct]);
-            if (__ballot(most - m[ct] > LAZY)) {
-                const float m_new = fmaxf(m[ct], column_max<X::SMALL>(most));
-                const float alpha = m[ct] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[ct] - m_new);
-                l[ct] *= alpha;
+            for (int i = 0; i < X::E; ++i) x[ct][i] = X::SMALL ? sc[ct][X::SMALL ? i >> 2 : 0][X::SMALL ? i & 3 : i] : sc[ct][0][i];
+            to_weights<FMT, X::SMALL, masked>(x[ct], masked ? vis[ct] : 0u, fr[ct], m[ct], l[ct], [&](int i) { return token_of(i >> 3, i & 7); }, [&](float alpha) {
 #pragma unroll
                 for (int db = 0; db < X::DB; ++db) o[ct][db] *= alpha;
-                m[ct] = m_new;
-            }
-            const float at = m[ct] == -INFINITY ? 0.0f : m[ct];
-            if (__ballot(fabsf(at) > HUGE_SCORE)) {  // (one-hot rows)
-#pragma unroll
-                for (int i = 0; i < X::E; ++i) x[ct][i] = weight_of_huge(x[ct][i], fr[ct], at, F::UP);
-            } else {
-#pragma unroll
-                for (int i = 0; i < X::E; ++i) x[ct][i] = __builtin_amdgcn_exp2f(fmaf(x[ct][i], fr[ct], F::UP - at));
-            }
-#pragma unroll
-            for (int i = 0; i < X::E; ++i) {
-                if (hidden(i)) x[ct][i] = 0.0f;  // (of a row with an infinite maximum)
-                l[ct] += x[ct][i];
-            }
+            });
 #pragma unroll
             for (int s = 0; s < X::VS; ++s) {
                 float w[8];
@@ -781,7 +920,7 @@ __global__ void __launch_bounds__(64 * NW, HD == 256 || (FMT == KT_PAGED_F32 && 
     }
     __syncthreads();
     const size_t at_slot = static_cast<size_t>(part.slot + part.split) * R;
-    const __amdgpu_buffer_rsrc_t averages = __builtin_amdgcn_make_buffer_rsrc(a.averages + at_slot * HD, 0, R * HD * 4, 0x00020000);
+    const __amdgpu_buffer_rsrc_t averages = averages_of<HD, R>(a, part.slot + part.split, 1);
     for (int32_t e = tid; e < held * (HD / 4); e += 64 * NW) {  // (every thread weighs its row's parts itself: no further barrier)
         const int32_t r = e / (HD / 4), d = 4 * (e % (HD / 4));
         float mx = -INFINITY, sum = 0.0f;
@@ -799,116 +938,345 @@ __global__ void __launch_bounds__(64 * NW, HD == 256 || (FMT == KT_PAGED_F32 && 
         for (int i = 0; i < 4; ++i) y[i] *= inv;
         if (splits == 1) {
             *reinterpret_cast<f4*>(a.p.context + row_at(r) + d) = y;
-        } else {  // written through to memory: the reader may be on another die
-            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, y), averages, (r * HD + d) * 4, 0, THROUGH);
-            if (d == 0) {
-                const uint64_t both = __builtin_bit_cast(uint32_t, mx) | static_cast<uint64_t>(__builtin_bit_cast(uint32_t, sum)) << 32;
-                __hip_atomic_store(reinterpret_cast<uint64_t*>(a.stats) + at_slot + r, both, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
-            }
+        } else {
+            store_average(averages, r * HD + d, y);
+            if (d == 0) store_stats(a, at_slot + r, mx, sum);
         }
     }
     if (splits == 1) return;
-    // the last workgroup of the tile to arrive merges the parts, in their order
-    __shared__ uint32_t arrived;
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
-    __builtin_amdgcn_s_waitcnt(0);
-    __syncthreads();
-    if (tid == 0) {
-        uint32_t* counter = a.counters + part.slot;
-        arrived = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
-        if (arrived == static_cast<uint32_t>(splits) - 1) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
-    }
-    __syncthreads();
-    if (arrived != static_cast<uint32_t>(splits) - 1) return;
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
-    const size_t slot0 = static_cast<size_t>(part.slot) * R;
-    float* weight = lds;                       // [R][MAX_SPLITS]
-    float* total = weight + R * MAX_SPLITS;    // [R]
-    f4* shares = reinterpret_cast<f4*>(total + R);  // [64 NW]
-    // thread (four dims of a row, phase): every phases-th part, eight loads in flight together, the first eight with the
-    // maxima and sums
-    constexpr int BATCH = 8;
-    const __amdgpu_buffer_rsrc_t all = __builtin_amdgcn_make_buffer_rsrc(a.averages + slot0 * HD, 0, splits * R * HD * 4, 0x00020000);
-    const int32_t items = held * (HD / 4), phases = max(1, 64 * NW / items);
-    const int32_t phase = phases > 1 ? tid / items : 0;
-    u4 v[BATCH];
-    auto load_batch = [&](int32_t item, int32_t s0) {
-        const int32_t at = (min(item, items - 1) / (HD / 4)) * HD + 4 * (min(item, items - 1) % (HD / 4));
-#pragma unroll
-        for (int u = 0; u < BATCH; ++u) v[u] = __builtin_amdgcn_raw_buffer_load_b128(all, (min(s0 + u * phases, splits - 1) * R * HD + at) * 4, 0, THROUGH);
+    meet<HD, R, NW>(a, part, splits, held, lds, row_at);
+}
+
+// ---- many rows ---------------------------------------------------------------------------------------
+// 128 rows a workgroup, 32 a wave, on 32x32x16. The workgroup's threads load a chunk of 32 keys ahead and lay it out in LDS,
+// where all four waves read it: the keys as rows, the values with a dim's tokens in the order of the operands; fp32 ones
+// split into their parts once for all waves. Queries stay in registers.
+template <int FMT, int HD>
+struct Tile {
+    static constexpr int R = 128, NW = 4, THREADS = 256;
+    static constexpr int KP = Format<FMT>::KP, QP = Format<FMT>::QP, E = Format<FMT>::E;
+    static constexpr int QS = HD / 16, DB = HD / 32;
+    static constexpr int KR = HD + 8, VR = CHUNK + 8;  // padded rows: of a key, of a dim (2-byte elements)
+    static constexpr int KSIZE = CHUNK * KR, VSIZE = HD * VR, SIZE = KP * (KSIZE + VSIZE);
+    static constexpr int BUFFERS = 2 * SIZE * 2 <= (80 << 10) ? 2 : 1;
+    static constexpr int PIECES = HD * E / 16;  // 16-byte pieces of a key
+    static constexpr int KN = (CHUNK * PIECES + THREADS - 1) / THREADS;
+    static constexpr int VN = (CHUNK / 4 * (HD / 4) + THREADS - 1) / THREADS;  // 4 tokens x 4 dims
+    static constexpr size_t LDS = std::max(size_t{2} * SIZE * BUFFERS, merge_lds(R, NW));
+    static constexpr int WAVES = HD == 256 ? 1 : 2;  // a SIMD
+    static constexpr int LEAST = 4;
+};
+
+template <int FMT, int HD>
+__global__ void __launch_bounds__(256, (Tile<FMT, HD>::WAVES)) tile_kernel(Args a) {
+    using F = Format<FMT>;
+    using X = Tile<FMT, HD>;
+    using op = typename F::op;
+    constexpr int R = X::R, NW = X::NW, E = F::E;
+    typedef typename std::conditional<FMT == KT_PAGED_F16, _Float16, __bf16>::type element;
+    extern __shared__ __attribute__((aligned(16))) float lds[];
+    __shared__ int32_t odd_chunk[2];  // the chunk in a buffer if some of its values are not finite
+    const PagedView& c = a.p.c;
+    const BatchView& b = a.p.b;
+    const int32_t tid = threadIdx.x, lane = tid & 63;
+    const int32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int32_t col = lane & 31, grp = lane >> 5;
+    const int32_t H = a.p.num_heads, G = H / c.kv_heads;
+    Part part;
+    if (!find_part<R, X::LEAST>(a, blockIdx.x, part)) return;
+    const int32_t g = part.head, row0 = part.tile * R, held = min(R, part.n * G - row0);
+    auto row_at = [&](int32_t r) {
+        const int32_t t = (row0 + r) / G;
+        return (static_cast<size_t>(part.first + t) * H + g * G + (row0 + r - t * G)) * HD;
     };
-    load_batch(phases > 1 ? tid % items : tid, phase);
-    for (int32_t r = wave; r < held; r += NW) {  // a row's weights: lane = part
-        float ml[MAX_SPLITS / 64], ll[MAX_SPLITS / 64], mx = -INFINITY, sum = 0.0f;
+    const Keys keys = keys_of<R>(a, part, held);
+    if (part.split >= keys.splits) return;
+    const int32_t c0 = keys.c0, c1 = keys.c1;
+    const PageReader reader(c, b, part, keys.n_keys, E);
+    if (tid < 2) odd_chunk[tid] = -1;
+
+    // the chunk ahead: a thread's pieces of keys, and its four tokens of four dims
+    u4 kr[X::KN];
+    uint32_t vr[X::VN][4][E];
+    auto key_item = [&](int i, int32_t& key, int32_t& piece) {
+        const int32_t e = tid + i * X::THREADS;
+        key = e / X::PIECES;
+        piece = e % X::PIECES;
+        return e < CHUNK * X::PIECES;
+    };
+    auto value_item = [&](int i, int32_t& quad, int32_t& dims) {
+        const int32_t e = tid + i * X::THREADS;
+        quad = e / (HD / 4);
+        dims = 4 * (e % (HD / 4));
+        return e < CHUNK / 4 * (HD / 4);
+    };
+    auto load_chunk = [&](const Where& w) {
 #pragma unroll
-        for (int i = 0; i < MAX_SPLITS / 64; ++i) {
-            const int32_t s = lane + 64 * i;
-            const uint64_t both = __hip_atomic_load(reinterpret_cast<uint64_t*>(a.stats) + slot0 + static_cast<size_t>(min(s, splits - 1)) * R + r, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
-            ml[i] = s < splits ? __builtin_bit_cast(float, static_cast<uint32_t>(both)) : -INFINITY;
-            ll[i] = s < splits ? __builtin_bit_cast(float, static_cast<uint32_t>(both >> 32)) : 0.0f;
+        for (int i = 0; i < X::KN; ++i) {
+            int32_t key, piece;
+            if (!key_item(i, key, piece)) break;
+            kr[i] = *reinterpret_cast<const u4*>(c.keys + (key < 16 ? w.base[0] : w.base[1]) + ((key & 15) * HD * E + 16 * piece));
         }
 #pragma unroll
-        for (int i = 0; i < MAX_SPLITS / 64; ++i) mx = fmaxf(mx, wave_max_dpp(ml[i]));
+        for (int i = 0; i < X::VN; ++i) {
+            int32_t quad, dims;
+            if (!value_item(i, quad, dims)) break;
+            const uint8_t* p = c.values + (quad < 4 ? w.base[0] : w.base[1]) + ((4 * quad & 15) * HD + dims) * E;
 #pragma unroll
-        for (int i = 0; i < MAX_SPLITS / 64; ++i) {
-            const float by = share_of(ml[i], ll[i], mx);
-            weight[r * MAX_SPLITS + lane + 64 * i] = by;
-            sum += wave_sum_dpp(by);
+            for (int j = 0; j < 4; ++j) load_words(p + j * HD * E, vr[i][j]);
         }
-        if (lane == 0) total[r] = sum;
-    }
-    __syncthreads();
-    for (int32_t i0 = 0; i0 < items; i0 += 64 * NW) {
-        const int32_t item = phases > 1 ? tid % items : i0 + tid;
-        const bool mine = item < items && phase < phases;
-        const int32_t r = min(item, items - 1) / (HD / 4), d = 4 * (min(item, items - 1) % (HD / 4));
-        f4 y = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int32_t s0 = phase; mine && s0 < splits; s0 += BATCH * phases) {
-            if (i0 > 0 || s0 > phase) load_batch(item, s0);
+    };
+    // whether every row of the tile sees the chunk whole
+    auto whole = [&](int32_t ch, uint32_t there) { return ch * CHUNK + CHUNK <= keys.n_all && there == 0xFFFFFFFFu; };
+    auto store_chunk = [&](int32_t ch, uint32_t there) {
+        element* kl = reinterpret_cast<element*>(lds) + (X::BUFFERS == 2 ? (ch & 1) * X::SIZE : 0);
+        element* vl = kl + X::KP * X::KSIZE;
 #pragma unroll
-            for (int u = 0; u < BATCH; ++u) {
-                const int32_t s = s0 + u * phases;
-                const float by = s < splits ? weight[r * MAX_SPLITS + s] : 0.0f;
-                const f4 z = __builtin_bit_cast(f4, v[u]);
+        for (int i = 0; i < X::KN; ++i) {
+            int32_t key, piece;
+            if (!key_item(i, key, piece)) break;
+            if constexpr (FMT == KT_PAGED_F32) {
+                float rest[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) y[i] = s < splits ? fmaf(by, z[i], y[i]) : y[i];
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t w = kr[i][e];
+                    rest[e] = __builtin_bit_cast(float, w);
+                }
+#pragma unroll
+                for (int w = 0; w < 3; ++w) {
+                    const uint32_t low = nearest_halves(rest[0], rest[1]), high = nearest_halves(rest[2], rest[3]);
+                    *reinterpret_cast<uint2*>(kl + w * X::KSIZE + key * X::KR + 4 * piece) = make_uint2(low, high);
+                    rest[0] -= __builtin_bit_cast(float, low << 16);
+                    rest[1] -= __builtin_bit_cast(float, low & 0xFFFF0000u);
+                    rest[2] -= __builtin_bit_cast(float, high << 16);
+                    rest[3] -= __builtin_bit_cast(float, high & 0xFFFF0000u);
+                }
+            } else {
+                *reinterpret_cast<u4*>(kl + key * X::KR + 8 * piece) = kr[i];
             }
         }
-        if (phases > 1) {
-            shares[tid] = y;
-            __syncthreads();
-        }
-        if (mine && phase == 0) {
-            for (int32_t p = 1; p < phases; ++p)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) y[i] += shares[item + p * items][i];
-            const float inv = total[r] == 0.0f ? 0.0f : 1.0f / total[r];
+        for (int i = 0; i < X::VN; ++i) {
+            int32_t quad, dims;
+            if (!value_item(i, quad, dims)) break;
+            if (!whole(ch, there)) {  // tokens that are not there count for nothing; what is not finite goes to the rows that see it alone
+                bool odd = false;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) y[i] *= inv;
-            *reinterpret_cast<f4*>(a.p.context + row_at(r) + d) = y;
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int w = 0; w < E; ++w) {
+                        if (!(there >> (4 * quad + j) & 1)) vr[i][j][w] = 0;
+                        odd |= any_not_finite<FMT>(vr[i][j][w]);
+                        vr[i][j][w] = finite_only<FMT>(vr[i][j][w]);
+                    }
+                if (odd) odd_chunk[ch & 1] = ch;
+            }
+            const int32_t at = 16 * (quad >> 2) + 8 * (quad & 1) + 4 * (quad >> 1 & 1);  // where the quad's tokens lie among a dim's
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {
+                element* to = vl + (dims + d) * X::VR + at;
+                if constexpr (FMT == KT_PAGED_F32) {
+                    float rest[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) rest[j] = __builtin_bit_cast(float, vr[i][j][d]);
+#pragma unroll
+                    for (int w = 0; w < 3; ++w) {
+                        const uint32_t low = nearest_halves(rest[0], rest[1]), high = nearest_halves(rest[2], rest[3]);
+                        *reinterpret_cast<uint2*>(to + w * X::VSIZE) = make_uint2(low, high);
+                        rest[0] -= __builtin_bit_cast(float, low << 16);
+                        rest[1] -= __builtin_bit_cast(float, low & 0xFFFF0000u);
+                        rest[2] -= __builtin_bit_cast(float, high << 16);
+                        rest[3] -= __builtin_bit_cast(float, high & 0xFFFF0000u);
+                    }
+                } else {
+                    const uint32_t pick = d % 2 ? 0x07060302u : 0x05040100u;
+                    *reinterpret_cast<uint2*>(to) = make_uint2(__builtin_amdgcn_perm(vr[i][1][d / 2], vr[i][0][d / 2], pick), __builtin_amdgcn_perm(vr[i][3][d / 2], vr[i][2][d / 2], pick));
+                }
+            }
         }
+    };
+
+    Where next{};
+    Pages pages{};
+    if (c0 < c1) {
+        next = reader.where_of(c0, reader.pages_of(c0));
+        load_chunk(next);
+        pages = reader.pages_of(min(c0 + 1, c1 - 1));
     }
+    // the wave's queries: a lane's dims of its row, as operands
+    const bool active = 32 * wave < held;  // waves with rows
+    const int32_t r = min(32 * wave + col, held - 1), token = (row0 + r) / G;
+    op q[X::QS][F::QP];
+    float f = a.p.scale * 1.4426950408889634f;
+    if (active) {
+        const float* src = a.p.q + row_at(r) + 8 * grp;
+        float x[X::QS][8];
+#pragma unroll
+        for (int s = 0; s < X::QS; ++s) {
+            const f4 low = *reinterpret_cast<const f4*>(src + 16 * s), high = *reinterpret_cast<const f4*>(src + 16 * s + 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                x[s][e] = low[e];
+                x[s][4 + e] = high[e];
+            }
+        }
+        if constexpr (FMT == KT_PAGED_F16) {
+            // the row scaled by a power of two to 2^13 .. 2^14 (bits below an infinity's, whose order is the floats')
+            uint32_t top = 0;
+#pragma unroll
+            for (int s = 0; s < X::QS; ++s)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) top = max(top, magnitude(x[s][e]));
+            const float most = column_max<false>(__builtin_bit_cast(float, min(top, 0x7F7FFFFFu)));
+            const int32_t up = 13 - max(static_cast<int32_t>(magnitude(most) >> 23) - 127, -100);
+#pragma unroll
+            for (int s = 0; s < X::QS; ++s)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[s][e] = ldexpf(x[s][e], up);
+            f = ldexpf(f, -up);
+        }
+#pragma unroll
+        for (int s = 0; s < X::QS; ++s) split_query(x[s], q[s]);
+    }
+    __syncthreads();  // (odd_chunk)
+    if (c0 < c1) store_chunk(c0, next.there);
+
+    f16v o[X::DB];
+    float m = -INFINITY, l = 0.0f;
+#pragma unroll
+    for (int db = 0; db < X::DB; ++db)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[db][e] = 0.0f;
+    auto token_of = [&](int i) { return 8 * (i >> 2) + 4 * grp + (i & 3); };
+    auto row_token = [&](int32_t at) { return (row0 + at) / G; };
+    const int32_t first_token = row_token(32 * wave), last_token = row_token(min(32 * wave + 31, held - 1));
+    // what the wave's rows see: below all of them, from none on nothing
+    const int64_t see_all = b.masks ? static_cast<int64_t>(part.length) : static_cast<int64_t>(part.length) + first_token + 1;
+    const int64_t see_none = b.masks ? INT64_MAX : static_cast<int64_t>(part.length) + last_token + 1;
+    auto attend_chunk = [&](auto masked_form, int32_t ch, uint32_t there, const Where& where) {
+        constexpr bool masked = decltype(masked_form)::value;
+        const element* kl = reinterpret_cast<const element*>(lds) + (X::BUFFERS == 2 ? (ch & 1) * X::SIZE : 0);
+        const element* vl = kl + X::KP * X::KSIZE;
+        f16v sc;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sc[e] = 0.0f;
+#pragma unroll
+        for (int s = 0; s < X::QS; ++s) {
+            op k[F::KP];
+#pragma unroll
+            for (int w = 0; w < F::KP; ++w) k[w] = *reinterpret_cast<const op*>(kl + w * X::KSIZE + col * X::KR + 16 * s + 8 * grp);
+            sc = products<false>(k, q[s], sc);
+        }
+        float x[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] = sc[i];
+        const uint32_t vis = masked ? seen_bits(b, part.first, token, part.length, ch * CHUNK, there) : 0u;
+        to_weights<FMT, false, masked>(x, vis, f, m, l, token_of, [&](float alpha) {
+#pragma unroll
+            for (int db = 0; db < X::DB; ++db) o[db] *= alpha;
+        });
+        if (masked || !whole(ch, there)) {
+            if (odd_chunk[ch & 1] == ch) {
+                const uint32_t mine = seen_bits(b, part.first, token, part.length, ch * CHUNK, there);
+                for (int32_t tok = 0; tok < CHUNK; ++tok) {
+                    if (!(there >> tok & 1)) continue;
+                    const int32_t from = tok >> 2 & 1, i = 4 * (tok >> 3) + (tok & 3);
+                    const uint8_t* row = c.values + (tok < 16 ? where.base[0] : where.base[1]) + (tok & 15) * HD * E;
+                    float weight = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        if (e == i) weight = x[e];
+                    weight = __shfl(weight, from * 32 + col);
+                    if (!(mine >> tok & 1)) continue;
+#pragma unroll
+                    for (int db = 0; db < X::DB; ++db)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            const float v = load_element<FMT>(row, 32 * db + token_of(e));
+                            if (!(fabsf(v) < INFINITY)) o[db][e] += weight * v;
+                        }
+                }
+            }
+        }
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            float w8[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w8[e] = x[8 * s + e];
+            op p[F::QP];
+            split_weights(w8, p);
+#pragma unroll
+            for (int db = 0; db < X::DB; ++db) {
+                op v[F::KP];
+#pragma unroll
+                for (int w = 0; w < F::KP; ++w) v[w] = *reinterpret_cast<const op*>(vl + w * X::VSIZE + (32 * db + col) * X::VR + 16 * s + 8 * grp);
+                o[db] = products<false>(v, p, o[db]);
+            }
+        }
+    };
+    for (int32_t ch = c0; ch < c1; ++ch) {
+        const Where now = next;
+        if (ch + 1 < c1) {
+            next = reader.where_of(ch + 1, pages);
+            load_chunk(next);
+            pages = reader.pages_of(min(ch + 2, c1 - 1));
+        }
+        __syncthreads();  // the chunk is in LDS
+        if (active && static_cast<int64_t>(ch) * CHUNK < see_none) {
+            if (static_cast<int64_t>(ch) * CHUNK + CHUNK <= see_all && now.there == 0xFFFFFFFFu) attend_chunk(std::false_type{}, ch, now.there, now);
+            else attend_chunk(std::true_type{}, ch, now.there, now);
+        }
+        if constexpr (X::BUFFERS == 1) __syncthreads();  // (and read by all)
+        if (ch + 1 < c1) store_chunk(ch + 1, next.there);
+    }
+
+    l = column_sum<false>(l);
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const size_t at_slot = static_cast<size_t>(part.slot + part.split) * R;
+    const __amdgpu_buffer_rsrc_t averages = averages_of<HD, R>(a, part.slot + part.split, 1);
+    if (32 * wave + col < held) {
+        float* out = a.p.context + row_at(r);
+#pragma unroll
+        for (int db = 0; db < X::DB; ++db)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                const int32_t d = 32 * db + token_of(e);
+                const f4 y = {o[db][e] * inv, o[db][e + 1] * inv, o[db][e + 2] * inv, o[db][e + 3] * inv};
+                if (keys.splits == 1) *reinterpret_cast<f4*>(out + d) = y;
+                else store_average(averages, r * HD + d, y);
+            }
+        if (keys.splits > 1 && grp == 0) store_stats(a, at_slot + r, m, l);
+    }
+    if (keys.splits == 1) return;
+    meet<HD, R, NW>(a, part, keys.splits, held, lds, row_at);
 }
 
 // ---- launches ---------------------------------------------------------------------------------------
-template <int FMT, int HD, int R, int NW, bool STEP>
-int32_t launch_rows(Args a, hipStream_t st) {
+// The grid and the workspace of a launch of tiles of R rows whose parts have at least LEAST chunks.
+template <int HD, int R, int LEAST>
+int32_t prepare(Args& a, int32_t target, int64_t* grid, hipStream_t st) {
     const BatchView& b = a.p.b;
     const int64_t G = a.p.num_heads / a.p.c.kv_heads;
     const int64_t tiles = std::min(b.sequences * ((b.most_rows * G + R - 1) / R), b.rows * G / R + b.sequences) * a.p.c.kv_heads;
-    const int64_t chunks = (static_cast<int64_t>(b.key_bound) + CHUNK - 1) / CHUNK, most_splits = std::min<int64_t>(MAX_SPLITS, (chunks + NW - 1) / NW);
-    a.target = 2 * cu_count();
-    const int64_t grid = std::min(tiles + a.target, tiles * most_splits);
-    if (grid > INT32_MAX / 64) return fail(KT_ERR_SHAPE, "too many rows and heads in one call");
-    if (most_splits > 1) {
-        const size_t slots = static_cast<size_t>(std::min<int64_t>(2 * a.target, grid));
-        void* ws = nullptr;
-        if (const int32_t status = workspace_counters(st, slots * R * (HD + 2) * sizeof(float) + 16, slots, &ws, &a.counters)) return status;
-        ws = reinterpret_cast<void*>((reinterpret_cast<uintptr_t>(ws) + 15) & ~uintptr_t{15});  // (it begins at any dword)
-        a.averages = static_cast<float*>(ws);
-        a.stats = a.averages + slots * R * HD;
-    }
-    constexpr size_t lds = std::max(std::max(sizeof(float) * NW * R * (HD + 6), size_t{2} * Format<FMT>::QP * R * (HD + 8)), sizeof(float) * (R * (MAX_SPLITS + 1) + 4 * 64 * NW));
+    const int64_t chunks = (static_cast<int64_t>(b.key_bound) + CHUNK - 1) / CHUNK, most_splits = std::min<int64_t>(MAX_SPLITS, (chunks + LEAST - 1) / LEAST);
+    a.target = target;
+    *grid = std::min(tiles + target, tiles * most_splits);
+    if (*grid > INT32_MAX / 64) return fail(KT_ERR_SHAPE, "too many rows and heads in one call");
+    if (most_splits <= 1) return KT_OK;
+    const size_t slots = static_cast<size_t>(std::min<int64_t>(2 * target, *grid));
+    void* ws = nullptr;
+    if (const int32_t status = workspace_counters(st, slots * R * (HD + 2) * sizeof(float) + 16, slots, &ws, &a.counters)) return status;
+    ws = reinterpret_cast<void*>((reinterpret_cast<uintptr_t>(ws) + 15) & ~uintptr_t{15});  // (it begins at any dword)
+    a.averages = static_cast<float*>(ws);
+    a.stats = a.averages + slots * R * HD;
+    return KT_OK;
+}
+
+template <int FMT, int HD, int R, int NW, bool STEP>
+int32_t launch_rows(Args a, hipStream_t st) {
+    int64_t grid = 0;
+    if (const int32_t status = prepare<HD, R, NW>(a, 2 * cu_count(), &grid, st)) return status;
+    constexpr size_t lds = std::max(std::max(sizeof(float) * NW * R * (HD + 6), size_t{2} * Format<FMT>::QP * R * (HD + 8)), merge_lds(R, NW));
     if (const int32_t ls = allow_lds<&attention_kernel<FMT, HD, R, NW, STEP>, lds>(lds)) return ls;
     attention_kernel<FMT, HD, R, NW, STEP><<<static_cast<uint32_t>(grid), 64 * NW, lds, st>>>(a);
     KT_LAUNCHED("paged attention kernel");
@@ -916,11 +1284,25 @@ int32_t launch_rows(Args a, hipStream_t st) {
 }
 
 template <int FMT, int HD>
+int32_t launch_tiles(Args a, hipStream_t st) {
+    using X = Tile<FMT, HD>;
+    int64_t grid = 0;
+    if (const int32_t status = prepare<HD, X::R, X::LEAST>(a, X::WAVES * cu_count(), &grid, st)) return status;
+    if (const int32_t ls = allow_lds<&tile_kernel<FMT, HD>, X::LDS>(X::LDS)) return ls;
+    tile_kernel<FMT, HD><<<static_cast<uint32_t>(grid), X::THREADS, X::LDS, st>>>(a);
+    KT_LAUNCHED("paged attention kernel");
+    return KT_OK;
+}
+
+template <int FMT, int HD>
 int32_t launch_dims(const Args& a, hipStream_t st) {
-    const int64_t G = a.p.num_heads / a.p.c.kv_heads;
+    const int64_t rows = static_cast<int64_t>(a.p.b.most_rows) * (a.p.num_heads / a.p.c.kv_heads);
     if constexpr (HD < 256) {
         if (a.k_new) return launch_rows<FMT, HD, 16, 4, true>(a, st);
-        if (a.p.b.most_rows * G > 16) return launch_rows<FMT, HD, 32, 4, false>(a, st);
+    }
+    if (rows > 64) return launch_tiles<FMT, HD>(a, st);
+    if constexpr (HD < 256) {
+        if (rows > 16) return launch_rows<FMT, HD, 32, 4, false>(a, st);
     }
     return launch_rows<FMT, HD, 16, 4, false>(a, st);
 }
