@@ -37,7 +37,6 @@ typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 
 constexpr int CHUNK = 32;        // keys a wave takes at a time
 constexpr float LAZY = 8.0f;     // how far a score may pass the maximum, in powers of two
-constexpr int MAX_SPLITS = 128;  // parts of a tile
 constexpr int THROUGH = 1 | 16;  // buffer cache bits sc0 sc1: past the caches
 
 // ---- operands ------------------------------------------------------------------------------
@@ -64,6 +63,17 @@ template <bool SMALL, typename A>
 __device__ __forceinline__ A product(half8 a, half8 b, A c) {
     if constexpr (SMALL) return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
     else return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+// Several sums at once, product by product: neighbours do not wait for each other.
+template <bool SMALL, int N, int KP, int QP, typename OP, typename A>
+__device__ __forceinline__ void products_of(const OP (&k)[N][KP], const OP (&q)[QP], A (&c)[N]) {
+#pragma unroll
+    for (int w = QP - 1; w >= 0; --w)
+#pragma unroll
+        for (int i = KP - 1; i >= 0; --i)
+#pragma unroll
+            for (int t = 0; t < N; ++t)
+                if (w - i >= 0) c[t] = product<SMALL>(k[t][i], q[w - i], c[t]);
 }
 // The sum of the parts' products down to 2^-17 of the largest, the small ones first.
 template <bool SMALL, int KP, int QP, typename OP, typename A>
@@ -168,11 +178,11 @@ __device__ __forceinline__ float share_of(float m, float l, float mx) {
 }
 
 // A chunk's scores x of one row (a lane's share of them) into weights; m and l: the row's running maximum and the sum of this
-// lane's weights; rescale: what the maximum's move does to the sums. vis: the tokens that the row sees, a bit each.
-template <int FMT, bool SMALL, bool masked, int E, typename TOKEN, typename RESCALE>
-__device__ __forceinline__ void to_weights(float (&x)[E], uint32_t vis, float f, float& m, float& l, TOKEN token_of, RESCALE rescale) {
+// lane's weights; rescale: what the maximum's move does to the sums; is_hidden: whether the row does not see score i's token.
+template <int FMT, bool SMALL, bool masked, int E, typename HIDDEN, typename RESCALE>
+__device__ __forceinline__ void to_weights(float (&x)[E], float f, float& m, float& l, HIDDEN is_hidden, RESCALE rescale) {
     constexpr float UP = Format<FMT>::UP;
-    auto hidden = [&](int i) { return masked && !(vis >> token_of(i) & 1); };
+    auto hidden = [&](int i) { return masked && is_hidden(i); };
     float most = -INFINITY;
 #pragma unroll
     for (int i = 0; i < E; ++i) {
@@ -222,6 +232,8 @@ __device__ __forceinline__ uint32_t seen_bits(const BatchView& b, int32_t first,
 }
 
 // ---- the parts of a launch ---------------------------------------------------------------------
+// Parts of a tile of R rows at most: what a merge holds of their rows' maxima and sums.
+constexpr int most_parts(int R) { return R <= 32 ? 128 : 4096 / R; }
 struct Args {
     PagedAttnArgs p;
     const float* k_new;  // STEP: the step's projections before RoPE
@@ -230,14 +242,6 @@ struct Args {
     float* averages;     // [slots][R][head_dim]: the parts' averages
     float* stats;        // [slots][R][2]: their maxima and sums
     uint32_t* counters;  // [slots], zero between launches
-};
-
-struct Part {
-    int32_t sequence, first, n, length;  // its rows and tokens
-    int32_t tile, head, split, splits;
-    int32_t keys;   // tokens that rows of the sequence may see
-    int32_t per;    // chunks a part may have
-    int32_t slot;   // of the tile's first part
 };
 
 __device__ __forceinline__ int32_t held_keys(const PagedView& c, const BatchView& b, int32_t length, int32_t n) {
@@ -250,10 +254,27 @@ __device__ __forceinline__ int64_t wave_total(int64_t v) {
     return v;
 }
 __device__ __forceinline__ int32_t lane_int(int32_t v, int32_t lane) { return __builtin_amdgcn_readlane(v, lane); }
+// A number that every lane has, as a scalar (divisions leave it in vector registers, and what follows from it too).
+__device__ __forceinline__ int32_t uniform(int32_t v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int32_t>(v))); }
+__device__ __forceinline__ int64_t uniform(int64_t v) {
+    return static_cast<int64_t>(static_cast<uint64_t>(uniform(static_cast<uint32_t>(v >> 32))) << 32 | uniform(static_cast<uint32_t>(v)));
+}
+
+struct Part {
+    int32_t sequence, first, n, length;  // its rows and tokens
+    int32_t tile, head, split, splits;
+    int32_t keys;   // tokens that rows of the sequence may see
+    int32_t per;    // chunks a part may have
+    int32_t slot;   // of the tile's first part
+    __device__ __forceinline__ void make_uniform() {  // (they meet behind branches that look divergent)
+        for (int32_t* v : {&sequence, &first, &n, &length, &tile, &head, &split, &splits, &keys, &per, &slot}) *v = uniform(*v);
+    }
+};
 
 // Which part of the launch workgroup `at` has; false: none. Every lane is a sequence. A launch has at most target + (its tiles
 // of all kv heads) parts, and at most 2 target that share a tile: a part's size is at least the chunks over target.
-template <int R, int LEAST>
+template <int R, int LEAST, int CHUNK>
 __device__ __forceinline__ bool find_part(const Args& a, int32_t at, Part& out) {
     const PagedView& c = a.p.c;
     const BatchView& b = a.p.b;
@@ -275,15 +296,15 @@ __device__ __forceinline__ bool find_part(const Args& a, int32_t at, Part& out) 
         total += static_cast<int64_t>(tiles_of()) * c.kv_heads * max(chunks_of(), 1);
         rows += n;
     }
-    total = wave_total(total);
-    if (wave_total(rows) > b.rows) return false;  // starts that do not ascend
+    total = uniform(wave_total(total));
+    if (uniform(wave_total(rows)) > b.rows) return false;  // starts that do not ascend
     int64_t per = (total + a.target - 1) / a.target;
     per = (max(per, int64_t{1}) + LEAST - 1) / LEAST * LEAST;
     int32_t before = 0, slots = 0;
     for (int32_t s0 = 0; s0 < b.sequences; s0 += 64) {
         if (b.sequences > 64) load(s0);
         const int32_t tiles = tiles_of(), chunks = chunks_of();
-        const int32_t size = static_cast<int32_t>(max(per, static_cast<int64_t>((chunks + MAX_SPLITS - 1) / MAX_SPLITS)));
+        const int32_t size = static_cast<int32_t>(max(per, static_cast<int64_t>((chunks + most_parts(R) - 1) / most_parts(R))));
         const int32_t splits = max((chunks + size - 1) / size, 1), parts = tiles * c.kv_heads * splits;
         const int32_t mine = splits > 1 ? parts : 0;
         int32_t upto = parts, slots_upto = mine;
@@ -295,21 +316,21 @@ __device__ __forceinline__ bool find_part(const Args& a, int32_t at, Part& out) 
                 slots_upto += y;
             }
         }
-        const int32_t passed = __popcll(__ballot(before + upto <= at));
+        const int32_t passed = uniform(static_cast<int32_t>(__popcll(__ballot(before + upto <= at))));
         if (passed < 64) {
             const int32_t local = at - before - (lane_int(upto, passed) - lane_int(parts, passed));
-            out.sequence = s0 + passed;
+            out.sequence = uniform(s0 + passed);
             out.first = lane_int(first, passed);
             out.n = lane_int(n, passed);
             out.length = lane_int(length, passed);
             out.splits = lane_int(splits, passed);
             out.per = lane_int(size, passed);
-            out.head = local % c.kv_heads;  // (workgroups go round the eight dies: a head's stay on few of them)
-            const int32_t rest = local / c.kv_heads;
-            out.split = rest % out.splits;
-            out.tile = lane_int(tiles, passed) - 1 - rest / out.splits;  // (a text's last tiles see the most)
-            out.keys = held_keys(c, b, out.length, out.n);
-            out.slot = slots + lane_int(slots_upto, passed) - lane_int(mine, passed) + (out.tile * c.kv_heads + out.head) * out.splits;
+            out.head = uniform(local % c.kv_heads);  // (workgroups go round the eight dies: a head's stay on few of them)
+            const int32_t rest = uniform(local / c.kv_heads);
+            out.split = uniform(rest % out.splits);
+            out.tile = lane_int(tiles, passed) - 1 - uniform(rest / out.splits);  // (a text's last tiles see the most)
+            out.keys = uniform(held_keys(c, b, out.length, out.n));
+            out.slot = uniform(slots) + lane_int(slots_upto, passed) - lane_int(mine, passed) + (out.tile * c.kv_heads + out.head) * out.splits;
             return true;
         }
         before += lane_int(upto, 63);
@@ -322,55 +343,71 @@ __device__ __forceinline__ bool find_part(const Args& a, int32_t at, Part& out) 
 struct Keys {
     int32_t n_keys, n_all, splits, c0, c1;
 };
-template <int R>
+template <int R, int CHUNK>
 __device__ __forceinline__ Keys keys_of(const Args& a, const Part& part, int32_t held) {
-    const int32_t G = a.p.num_heads / a.p.c.kv_heads, t_first = part.tile * R / G, t_last = (part.tile * R + held - 1) / G;
+    const int32_t G = a.p.num_heads / a.p.c.kv_heads, t_first = uniform(part.tile * R / G), t_last = uniform((part.tile * R + held - 1) / G);
     const int64_t length = part.length;
     const bool tree = a.p.b.masks != nullptr;
     Keys k;
-    k.n_keys = tree ? part.keys : static_cast<int32_t>(min(static_cast<int64_t>(part.keys), max(length + t_last + 1, int64_t{0})));
-    k.n_all = static_cast<int32_t>(min(static_cast<int64_t>(k.n_keys), max(length + (tree ? 0 : t_first + 1), int64_t{0})));
+    k.n_keys = tree ? part.keys : uniform(static_cast<int32_t>(min(static_cast<int64_t>(part.keys), max(length + t_last + 1, int64_t{0}))));
+    k.n_all = uniform(static_cast<int32_t>(min(static_cast<int64_t>(k.n_keys), max(length + (tree ? 0 : t_first + 1), int64_t{0}))));
     const int32_t chunks = (k.n_keys + CHUNK - 1) / CHUNK;
-    k.splits = max(1, min(part.splits, (chunks + part.per - 1) / part.per));
-    k.c0 = static_cast<int32_t>(static_cast<int64_t>(chunks) * part.split / k.splits);
-    k.c1 = static_cast<int32_t>(static_cast<int64_t>(chunks) * (part.split + 1) / k.splits);
+    k.splits = uniform(max(1, min(part.splits, (chunks + part.per - 1) / part.per)));
+    k.c0 = uniform(static_cast<int32_t>(static_cast<int64_t>(chunks) * part.split / k.splits));
+    k.c1 = uniform(static_cast<int32_t>(static_cast<int64_t>(chunks) * (part.split + 1) / k.splits));
     return k;
 }
 
-// A chunk's halves of 16 tokens, each in one page: their pages, then where they begin (bytes from the layer's keys or values)
+// A chunk's runs of 16 tokens, each in one page: their pages, then where they begin (bytes from the layer's keys or values)
 // and which tokens there are, a bit each.
+template <int CHUNK>
 struct Pages {
-    int32_t page[2];
+    int32_t page[CHUNK / 16];
 };
+template <int CHUNK>
 struct Where {
-    size_t base[2];
-    uint32_t there;
+    size_t base[CHUNK / 16];
+    uint32_t there[CHUNK / 32];
+    // where run `run` begins (selects between the scalars: an index would go through scratch memory)
+    __device__ __forceinline__ size_t of_run(int32_t run) const {
+        const size_t low = pick(run & 1, base[0], base[1]);
+        if constexpr (CHUNK == 32) return low;
+        else return pick(run & 2, low, pick(run & 1, base[2], base[3]));
+    }
+    static __device__ __forceinline__ size_t pick(int32_t second, size_t a, size_t b) {
+        const uint32_t low = second ? static_cast<uint32_t>(b) : static_cast<uint32_t>(a), high = second ? static_cast<uint32_t>(b >> 32) : static_cast<uint32_t>(a >> 32);
+        return static_cast<size_t>(high) << 32 | low;
+    }
 };
+template <int CHUNK>
 struct PageReader {
     typedef const __attribute__((address_space(4))) int32_t* table_t;  // (read-only, by uniform indexes)
-    const PagedView& c;
     table_t table;
-    int32_t head, n_keys, last_entry, row_bytes;
-    __device__ __forceinline__ PageReader(const PagedView& view, const BatchView& b, const Part& part, int32_t keys, int32_t element)
-        : c(view), table((table_t)(b.tables + static_cast<size_t>(part.sequence) * b.table_stride)), head(part.head), n_keys(keys),
-          last_entry(keys > 0 ? (keys - 1) >> view.page_shift : 0), row_bytes(view.head_dim * element) {}
-    __device__ __forceinline__ Pages pages_of(int32_t ch) const {
-        Pages p;
+    size_t page_bytes, head_bytes;
+    int32_t pages, page_shift, n_keys, last_entry, row_bytes;
+    __device__ __forceinline__ PageReader(const PagedView& c, const BatchView& b, const Part& part, int32_t keys, int32_t element)
+        : table((table_t)(b.tables + static_cast<size_t>(part.sequence) * b.table_stride)), pages(c.pages), page_shift(c.page_shift), n_keys(keys),
+          last_entry(keys > 0 ? (keys - 1) >> c.page_shift : 0), row_bytes(c.head_dim * element) {
+        head_bytes = (static_cast<size_t>(part.head) << page_shift) * row_bytes;
+        page_bytes = (static_cast<size_t>(c.kv_heads) << page_shift) * row_bytes;
+    }
+    __device__ __forceinline__ Pages<CHUNK> pages_of(int32_t ch) const {
+        Pages<CHUNK> p;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) p.page[h] = table[min((ch * CHUNK + 16 * h) >> c.page_shift, last_entry)];
+        for (int h = 0; h < CHUNK / 16; ++h) p.page[h] = table[min((ch * CHUNK + 16 * h) >> page_shift, last_entry)];
         return p;
     }
-    __device__ __forceinline__ Where where_of(int32_t ch, const Pages& p) const {
-        Where w;
-        w.there = 0;
+    __device__ __forceinline__ Where<CHUNK> where_of(int32_t ch, const Pages<CHUNK>& p) const {
+        Where<CHUNK> w;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < CHUNK / 16; ++h) {
             const int32_t x = ch * CHUNK + 16 * h;
-            const bool fine = p.page[h] >= 0 && p.page[h] < c.pages;
+            const bool fine = static_cast<uint32_t>(p.page[h]) < static_cast<uint32_t>(pages);
             const size_t page = fine ? p.page[h] : 0;  // (any memory of the pool)
-            w.base[h] = (((page * c.kv_heads + head) << c.page_shift) + (x & ((1 << c.page_shift) - 1))) * row_bytes;
+            w.base[h] = page * page_bytes + head_bytes + static_cast<uint32_t>((x & ((1 << page_shift) - 1)) * row_bytes);
             const int32_t m = min(max(n_keys - x, 0), 16);
-            w.there |= (fine ? (1u << m) - 1u : 0u) << (16 * h);
+            if (h % 2 == 0) w.there[h / 2] = 0;
+            w.there[h / 2] |= (fine ? (1u << m) - 1u : 0u) << (16 * (h % 2));
         }
         return w;
     }
@@ -389,12 +426,13 @@ template <int HD, int R>
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t averages_of(const Args& a, size_t slot, int32_t slots) {
     return __builtin_amdgcn_make_buffer_rsrc(a.averages + slot * R * HD, 0, slots * R * HD * 4, 0x00020000);
 }
-constexpr size_t merge_lds(int R, int NW) { return sizeof(float) * (R * (MAX_SPLITS + 1) + 4 * 64 * NW); }
+constexpr size_t merge_lds(int R, int NW) { return sizeof(float) * (2 * R * most_parts(R) + R + 4 * 64 * NW); }
 
 // Called by all threads of a workgroup once its part is stored. The last workgroup of the tile to arrive merges the
 // parts, in their order, into the context; row_at: where a row of the tile lies there.
 template <int HD, int R, int NW, typename ROW>
 __device__ __forceinline__ void meet(const Args& a, const Part& part, int32_t splits, int32_t held, float* lds, ROW row_at) {
+    constexpr int T = 64 * NW, BATCH = 8;
     const int32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     __shared__ uint32_t arrived;
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
@@ -406,73 +444,110 @@ __device__ __forceinline__ void meet(const Args& a, const Part& part, int32_t sp
         if (arrived == static_cast<uint32_t>(splits) - 1) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
     }
     __syncthreads();
-    if (arrived != static_cast<uint32_t>(splits) - 1) return;
+    if (uniform(arrived) != static_cast<uint32_t>(splits) - 1) return;
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
     const size_t slot0 = static_cast<size_t>(part.slot) * R;
-    float* weight = lds;                       // [R][MAX_SPLITS]
-    float* total = weight + R * MAX_SPLITS;    // [R]
-    f4* shares = reinterpret_cast<f4*>(total + R);  // [64 NW]
-    // thread (four dims of a row, phase): every phases-th part, eight loads in flight together, the first eight with the
-    // maxima and sums
-    constexpr int BATCH = 8;
+    float* maxima = lds;                          // [R][splits]: then the parts' weights
+    float* sums = maxima + R * most_parts(R);     // [R][splits]
+    float* total = sums + R * most_parts(R);      // [R]
+    f4* shares = reinterpret_cast<f4*>(total + R);  // [T]
     const __amdgpu_buffer_rsrc_t all = averages_of<HD, R>(a, part.slot, splits);
-    const int32_t items = held * (HD / 4), phases = max(1, 64 * NW / items);
-    const int32_t phase = phases > 1 ? tid / items : 0;
-    u4 v[BATCH];
-    auto load_batch = [&](int32_t item, int32_t s0) {
-        const int32_t at = (min(item, items - 1) / (HD / 4)) * HD + 4 * (min(item, items - 1) % (HD / 4));
-#pragma unroll
-        for (int u = 0; u < BATCH; ++u) v[u] = __builtin_amdgcn_raw_buffer_load_b128(all, (min(s0 + u * phases, splits - 1) * R * HD + at) * 4, 0, THROUGH);
+    // A thread sums its items (four dims of a row) over the parts; where there are fewer items than threads, phases of
+    // threads share an item's parts. Eight loads are in flight while eight others are summed.
+    const int32_t items = held * (HD / 4), phases = uniform(max(1, T / items));
+    const int32_t phase = phases > 1 ? tid / items : 0, step = phases > 1 ? items : T;
+    struct Cursor {
+        int32_t item, part;
     };
-    load_batch(phases > 1 ? tid % items : tid, phase);
-    for (int32_t r = wave; r < held; r += NW) {  // a row's weights: lane = part
-        float ml[MAX_SPLITS / 64], ll[MAX_SPLITS / 64], mx = -INFINITY, sum = 0.0f;
+    Cursor ahead{phases > 1 ? tid % items : tid, phase}, now = ahead;
+    u4 v[2][BATCH];
+    auto load = [&](u4 (&to)[BATCH]) {  // (past the last item or part: the last, unused)
 #pragma unroll
-        for (int i = 0; i < MAX_SPLITS / 64; ++i) {
-            const int32_t s = lane + 64 * i;
-            const uint64_t both = __hip_atomic_load(reinterpret_cast<uint64_t*>(a.stats) + slot0 + static_cast<size_t>(min(s, splits - 1)) * R + r, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
-            ml[i] = s < splits ? __builtin_bit_cast(float, static_cast<uint32_t>(both)) : -INFINITY;
-            ll[i] = s < splits ? __builtin_bit_cast(float, static_cast<uint32_t>(both >> 32)) : 0.0f;
-        }
-#pragma unroll
-        for (int i = 0; i < MAX_SPLITS / 64; ++i) mx = fmaxf(mx, wave_max_dpp(ml[i]));
-#pragma unroll
-        for (int i = 0; i < MAX_SPLITS / 64; ++i) {
-            const float by = share_of(ml[i], ll[i], mx);
-            weight[r * MAX_SPLITS + lane + 64 * i] = by;
-            sum += wave_sum_dpp(by);
-        }
-        if (lane == 0) total[r] = sum;
-    }
-    __syncthreads();
-    for (int32_t i0 = 0; i0 < items; i0 += 64 * NW) {
-        const int32_t item = phases > 1 ? tid % items : i0 + tid;
-        const bool mine = item < items && phase < phases;
-        const int32_t r = min(item, items - 1) / (HD / 4), d = 4 * (min(item, items - 1) % (HD / 4));
-        f4 y = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int32_t s0 = phase; mine && s0 < splits; s0 += BATCH * phases) {
-            if (i0 > 0 || s0 > phase) load_batch(item, s0);
-#pragma unroll
-            for (int u = 0; u < BATCH; ++u) {
-                const int32_t s = s0 + u * phases;
-                const float by = s < splits ? weight[r * MAX_SPLITS + s] : 0.0f;
-                const f4 z = __builtin_bit_cast(f4, v[u]);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) y[i] = s < splits ? fmaf(by, z[i], y[i]) : y[i];
+        for (int u = 0; u < BATCH; ++u) {
+            to[u] = __builtin_amdgcn_raw_buffer_load_b128(all, (min(ahead.part, splits - 1) * (R * HD) + 4 * min(ahead.item, items - 1)) * 4, 0, THROUGH);
+            ahead.part += phases;
+            if (ahead.part >= splits) {
+                ahead.item += step;
+                ahead.part = phase;
             }
         }
-        if (phases > 1) {
-            shares[tid] = y;
-            __syncthreads();
+    };
+    load(v[0]);
+    for (int32_t e = tid; e < held * splits; e += T) {
+        const int32_t s = e / held, r = e % held;
+        const uint64_t both = __hip_atomic_load(reinterpret_cast<uint64_t*>(a.stats) + slot0 + static_cast<size_t>(s) * R + r, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+        maxima[r * splits + s] = __builtin_bit_cast(float, static_cast<uint32_t>(both));
+        sums[r * splits + s] = __builtin_bit_cast(float, static_cast<uint32_t>(both >> 32));
+    }
+    __syncthreads();
+    // a row's weights: as many lanes as hold its parts (128 parts: two a lane)
+    int32_t width = 1;
+    while (width < splits && width < 64) width <<= 1;
+    for (int32_t r0 = wave * (64 / width); r0 < held; r0 += NW * (64 / width)) {
+        const int32_t r = r0 + lane / width, at = min(r, held - 1) * splits;
+        constexpr int PER = (most_parts(R) + 63) / 64;
+        float ml[PER], ll[PER], mx = -INFINITY, sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int32_t s = lane % width + 64 * i;
+            ml[i] = s < splits ? maxima[at + s] : -INFINITY;
+            ll[i] = s < splits ? sums[at + s] : 0.0f;
+            mx = fmaxf(mx, ml[i]);
         }
-        if (mine && phase == 0) {
-            for (int32_t p = 1; p < phases; ++p)
+        for (int32_t o = 1; o < width; o <<= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
 #pragma unroll
-                for (int i = 0; i < 4; ++i) y[i] += shares[item + p * items][i];
-            const float inv = total[r] == 0.0f ? 0.0f : 1.0f / total[r];
+        for (int i = 0; i < PER; ++i) {
+            ll[i] = share_of(ml[i], ll[i], mx);
+            sum += ll[i];
+        }
+        for (int32_t o = 1; o < width; o <<= 1) sum += __shfl_xor(sum, o);
+        if (r < held) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) y[i] *= inv;
-            *reinterpret_cast<f4*>(a.p.context + row_at(r) + d) = y;
+            for (int i = 0; i < PER; ++i)
+                if (lane % width + 64 * i < splits) maxima[at + lane % width + 64 * i] = ll[i];
+            if (lane % width == 0) total[r] = sum;
+        }
+    }
+    __syncthreads();
+    f4 y = {0.0f, 0.0f, 0.0f, 0.0f};
+    auto write = [&](int32_t item, const f4& z) {
+        const int32_t r = item / (HD / 4), d = 4 * (item % (HD / 4));
+        const float inv = total[r] == 0.0f ? 0.0f : 1.0f / total[r];
+        *reinterpret_cast<f4*>(a.p.context + row_at(r) + d) = z * inv;
+    };
+    const int32_t mine = (splits - phase + phases - 1) / phases;  // parts of an item that this thread sums
+    const int32_t entries = phases > 1 ? (phase < phases ? mine : 0) : (items - tid + T - 1) / T * splits;
+    auto sum_batch = [&](const u4 (&from)[BATCH], int32_t e0) {
+#pragma unroll
+        for (int u = 0; u < BATCH; ++u) {
+            if (e0 + u >= entries) break;
+            const float by = maxima[now.item / (HD / 4) * splits + now.part];
+            const f4 z = __builtin_bit_cast(f4, from[u]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y[i] = fmaf(by, z[i], y[i]);
+            now.part += phases;
+            if (now.part >= splits) {
+                if (phases == 1) {
+                    write(now.item, y);
+                    y = f4{0.0f, 0.0f, 0.0f, 0.0f};
+                }
+                now.item += step;
+                now.part = phase;
+            }
+        }
+    };
+    for (int32_t e0 = 0; e0 < entries; e0 += 2 * BATCH) {
+        load(v[1]);
+        sum_batch(v[0], e0);
+        if (e0 + 2 * BATCH < entries) load(v[0]);
+        sum_batch(v[1], e0 + BATCH);
+    }
+    if (phases > 1) {
+        shares[tid] = y;
+        __syncthreads();
+        if (tid < items) {
+            for (int32_t p = 1; p < phases; ++p) y += shares[tid + p * items];
+            write(tid, y);
         }
     }
 }
@@ -555,7 +630,8 @@ __global__ void __launch_bounds__(64 * NW, HD == 256 || (FMT == KT_PAGED_F32 && 
     const int32_t col = lane % X::LANES, grp = lane / X::LANES;
     const int32_t H = a.p.num_heads, G = H / c.kv_heads;
     Part part;
-    if (!find_part<R, NW>(a, blockIdx.x, part)) return;
+    if (!find_part<R, NW, CHUNK>(a, blockIdx.x, part)) return;
+    part.make_uniform();
     const int32_t g = part.head, row0 = part.tile * R, held = min(R, part.n * G - row0);  // rows of this tile
     // where row r of the tile lies in q and context
     auto row_at = [&](int32_t r) {
@@ -592,14 +668,14 @@ __global__ void __launch_bounds__(64 * NW, HD == 256 || (FMT == KT_PAGED_F32 && 
         }
     }
 
-    const Keys keys = keys_of<R>(a, part, held);
+    const Keys keys = keys_of<R, CHUNK>(a, part, held);
     if (part.split >= keys.splits) return;
     const int32_t splits = keys.splits, c0 = keys.c0, c1 = keys.c1, n_all = keys.n_all;
     const int64_t new_first = part.length;
-    const PageReader reader(c, b, part, keys.n_keys, F::E);
+    const PageReader<CHUNK> reader(c, b, part, keys.n_keys, F::E);
 
     uint32_t kr[X::KT][X::QS][X::KW], vr[X::VS][8][X::VW];
-    auto load_keys = [&](const Where& w) {
+    auto load_keys = [&](const Where<CHUNK>& w) {
 #pragma unroll
         for (int t = 0; t < X::KT; ++t) {
             const size_t base = X::SMALL ? w.base[t] : col < 16 ? w.base[0] : w.base[1];
@@ -610,7 +686,7 @@ __global__ void __launch_bounds__(64 * NW, HD == 256 || (FMT == KT_PAGED_F32 && 
     };
     // the token of a lane's value (or weight) e of step s
     auto token_of = [&](int s, int e) { return X::SMALL ? 16 * (e >> 2) + 4 * grp + (e & 3) : 16 * s + 8 * (e >> 2) + 4 * grp + (e & 3); };
-    auto load_values = [&](const Where& w) {
+    auto load_values = [&](const Where<CHUNK>& w) {
 #pragma unroll
         for (int s = 0; s < X::VS; ++s)
 #pragma unroll
@@ -636,8 +712,8 @@ __global__ void __launch_bounds__(64 * NW, HD == 256 || (FMT == KT_PAGED_F32 && 
         }
     };
     int32_t ch = c0 + wave;
-    Where here{};
-    Pages pages{};
+    Where<CHUNK> here{};
+    Pages<CHUNK> pages{};
     if (ch < c1) {
         here = reader.where_of(ch, reader.pages_of(ch));
         load_keys(here);
@@ -779,7 +855,7 @@ __global__ void __launch_bounds__(64 * NW, HD == 256 || (FMT == KT_PAGED_F32 && 
     // (two forms of the loop's body: only chunks that not every row sees whole compare keys with rows)
     auto attend_chunk = [&](auto masked_form) {
         constexpr bool masked = decltype(masked_form)::value;
-        const Where now = here;
+        const Where<CHUNK> now = here;
         acc_t sc[X::CT][X::KT];
 #pragma unroll
         for (int ct = 0; ct < X::CT; ++ct)
@@ -805,19 +881,21 @@ __global__ void __launch_bounds__(64 * NW, HD == 256 || (FMT == KT_PAGED_F32 && 
                 }
             }
         }
+        __builtin_amdgcn_sched_barrier(0);  // (loads ahead of their registers' last use would cost others)
         const int32_t next = min(ch + NW, c1 - 1);  // (past the end the last chunk again, unused)
         here = reader.where_of(next, pages);
         load_keys(here);
         pages = reader.pages_of(min(ch + 2 * NW, c1 - 1));
+        __builtin_amdgcn_sched_barrier(0);
         op p[X::CT][X::VS][F::QP];
         float x[X::CT][X::E];
         uint32_t vis[X::CT];
 #pragma unroll
         for (int ct = 0; ct < X::CT; ++ct) {
-            if constexpr (masked) vis[ct] = seen_bits(b, part.first, token[ct], new_first, ch * CHUNK, now.there);
+            if constexpr (masked) vis[ct] = seen_bits(b, part.first, token[ct], new_first, ch * CHUNK, now.there[0]);
 #pragma unroll
             for (int i = 0; i < X::E; ++i) x[ct][i] = X::SMALL ? sc[ct][X::SMALL ? i >> 2 : 0][X::SMALL ? i & 3 : i] : sc[ct][0][i];
-            to_weights<FMT, X::SMALL, masked>(x[ct], masked ? vis[ct] : 0u, fr[ct], m[ct], l[ct], [&](int i) { return token_of(i >> 3, i & 7); }, [&](float alpha) {
+            to_weights<FMT, X::SMALL, masked>(x[ct], fr[ct], m[ct], l[ct], [&](int i) { return !(vis[ct] >> token_of(i >> 3, i & 7) & 1); }, [&](float alpha) {
 #pragma unroll
                 for (int db = 0; db < X::DB; ++db) o[ct][db] *= alpha;
             });
@@ -838,13 +916,13 @@ __global__ void __launch_bounds__(64 * NW, HD == 256 || (FMT == KT_PAGED_F32 && 
                 for (int e = 0; e < 8; ++e)
 #pragma unroll
                     for (int w = 0; w < X::VW; ++w) {
-                        if (!(now.there >> token_of(s, e) & 1)) vr[s][e][w] = 0;
+                        if (!(now.there[0] >> token_of(s, e) & 1)) vr[s][e][w] = 0;
                         odd |= any_not_finite<FMT>(vr[s][e][w]);
                     }
             if (__ballot(odd)) {
                 const bool own = STEP && holder && ch == part.length / CHUNK;  // (the new token is in LDS)
                 for (int32_t tok = 0; tok < CHUNK; ++tok) {
-                    if (!(now.there >> tok & 1)) continue;
+                    if (!(now.there[0] >> tok & 1)) continue;
                     const int32_t from = X::SMALL ? tok >> 2 & 3 : tok >> 2 & 1, i = X::SMALL ? 4 * (tok >> 4) + (tok & 3) : 4 * (tok >> 3) + (tok & 3);
                     const uint8_t* row = c.values + (tok < 16 ? now.base[0] : now.base[1]) + (tok & 15) * HD * F::E;
                     if constexpr (STEP) {
@@ -865,6 +943,7 @@ __global__ void __launch_bounds__(64 * NW, HD == 256 || (FMT == KT_PAGED_F32 && 
                             for (int db = 0; db < X::DB; ++db) {
                                 const float v = load_element<FMT>(row, d + db);
                                 if (!(fabsf(v) < INFINITY)) o[ct][db][e] += weight * v;
+                                __builtin_amdgcn_sched_barrier(0);  // (rare: one load at a time, few registers)
                             }
                         }
                     }
@@ -886,13 +965,14 @@ __global__ void __launch_bounds__(64 * NW, HD == 256 || (FMT == KT_PAGED_F32 && 
 #pragma unroll
                 for (int ct = 0; ct < X::CT; ++ct) o[ct][db] = products<X::SMALL>(v, p[ct][s], o[ct][db]);
             }
+        __builtin_amdgcn_sched_barrier(0);
         load_values(here);
         if constexpr (STEP) {
             if (holder && next == part.length / CHUNK) patch();
         }
     };
     for (; ch < c1; ch += NW) {
-        if (ch * CHUNK + CHUNK <= n_all && here.there == 0xFFFFFFFFu) attend_chunk(std::false_type{});
+        if (ch * CHUNK + CHUNK <= n_all && here.there[0] == 0xFFFFFFFFu) attend_chunk(std::false_type{});
         else attend_chunk(std::true_type{});
     }
 
@@ -948,31 +1028,39 @@ __global__ void __launch_bounds__(64 * NW, HD == 256 || (FMT == KT_PAGED_F32 && 
 }
 
 // ---- many rows ---------------------------------------------------------------------------------------
-// 128 rows a workgroup, 32 a wave, on 32x32x16. The workgroup's threads load a chunk of 32 keys ahead and lay it out in LDS,
-// where all four waves read it: the keys as rows, the values with a dim's tokens in the order of the operands; fp32 ones
-// split into their parts once for all waves. Queries stay in registers.
+// 128 rows a workgroup, 16 a wave, on 16x16x32. The workgroup's threads load a chunk of keys ahead and lay it out in LDS,
+// where all eight waves read it: the keys as rows, the values as dims with their tokens in the order of the operands; fp32
+// ones split into their parts once for all waves. Queries stay in registers.
+#ifndef XNW
+#define XNW(F, H) 8
+#define XMW(F, H) 2
+#define XCH(F, H) (F == 0 ? 32 : 64)
+#define XT(F, H) 1
+#define XD 4
+#endif
 template <int FMT, int HD>
 struct Tile {
-    static constexpr int R = 128, NW = 4, THREADS = 256;
+    static constexpr int NW = XNW(FMT, HD), MW = XMW(FMT, HD), R = 16 * NW, THREADS = 64 * NW;
     static constexpr int KP = Format<FMT>::KP, QP = Format<FMT>::QP, E = Format<FMT>::E;
-    static constexpr int QS = HD / 16, DB = HD / 32;
-    static constexpr int KR = HD + 8, VR = CHUNK + 8;  // padded rows: of a key, of a dim (2-byte elements)
-    static constexpr int KSIZE = CHUNK * KR, VSIZE = HD * VR, SIZE = KP * (KSIZE + VSIZE);
-    static constexpr int BUFFERS = 2 * SIZE * 2 <= (80 << 10) ? 2 : 1;
+    static constexpr int CH = XCH(FMT, HD), SETS = CH / 32;
+    static constexpr int QS = HD / 32, DB = HD / 16;
+    static constexpr int KR = HD + 8, VR = CH + 8;  // padded rows: of a key, of a dim (2-byte elements)
+    static constexpr int KSIZE = CH * KR, VSIZE = HD * VR, SIZE = KP * (KSIZE + VSIZE);
+    static constexpr int BUFFERS = 2 * SIZE * 2 <= (150 << 10) / (4 * MW / NW) ? 2 : 1;
     static constexpr int PIECES = HD * E / 16;  // 16-byte pieces of a key
-    static constexpr int KN = (CHUNK * PIECES + THREADS - 1) / THREADS;
-    static constexpr int VN = (CHUNK / 4 * (HD / 4) + THREADS - 1) / THREADS;  // 4 tokens x 4 dims
+    static constexpr int KN = (CH * PIECES + THREADS - 1) / THREADS;
+    static constexpr int VN = (CH / 4 * (HD / 4) + THREADS - 1) / THREADS;  // 4 tokens x 4 dims
     static constexpr size_t LDS = std::max(size_t{2} * SIZE * BUFFERS, merge_lds(R, NW));
-    static constexpr int WAVES = HD == 256 ? 1 : 2;  // a SIMD
-    static constexpr int LEAST = 4;
+    static constexpr int LEAST = 128 / CH;
+    static constexpr int VGROUP = FMT == KT_PAGED_F32 ? 2 : 4;
 };
 
 template <int FMT, int HD>
-__global__ void __launch_bounds__(256, (Tile<FMT, HD>::WAVES)) tile_kernel(Args a) {
+__global__ void __launch_bounds__((Tile<FMT, HD>::THREADS), (Tile<FMT, HD>::MW)) tile_kernel(Args a) {
     using F = Format<FMT>;
     using X = Tile<FMT, HD>;
     using op = typename F::op;
-    constexpr int R = X::R, NW = X::NW, E = F::E;
+    constexpr int R = X::R, NW = X::NW, E = F::E, CH = X::CH;
     typedef typename std::conditional<FMT == KT_PAGED_F16, _Float16, __bf16>::type element;
     extern __shared__ __attribute__((aligned(16))) float lds[];
     __shared__ int32_t odd_chunk[2];  // the chunk in a buffer if some of its values are not finite
@@ -980,19 +1068,20 @@ __global__ void __launch_bounds__(256, (Tile<FMT, HD>::WAVES)) tile_kernel(Args 
     const BatchView& b = a.p.b;
     const int32_t tid = threadIdx.x, lane = tid & 63;
     const int32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int32_t col = lane & 31, grp = lane >> 5;
+    const int32_t col = lane & 15, grp = lane >> 4;
     const int32_t H = a.p.num_heads, G = H / c.kv_heads;
     Part part;
-    if (!find_part<R, X::LEAST>(a, blockIdx.x, part)) return;
+    if (!find_part<R, X::LEAST, CH>(a, blockIdx.x, part)) return;
+    part.make_uniform();
     const int32_t g = part.head, row0 = part.tile * R, held = min(R, part.n * G - row0);
     auto row_at = [&](int32_t r) {
         const int32_t t = (row0 + r) / G;
         return (static_cast<size_t>(part.first + t) * H + g * G + (row0 + r - t * G)) * HD;
     };
-    const Keys keys = keys_of<R>(a, part, held);
+    const Keys keys = keys_of<R, CH>(a, part, held);
     if (part.split >= keys.splits) return;
     const int32_t c0 = keys.c0, c1 = keys.c1;
-    const PageReader reader(c, b, part, keys.n_keys, E);
+    const PageReader<CH> reader(c, b, part, keys.n_keys, E);
     if (tid < 2) odd_chunk[tid] = -1;
 
     // the chunk ahead: a thread's pieces of keys, and its four tokens of four dims
@@ -1002,35 +1091,51 @@ __global__ void __launch_bounds__(256, (Tile<FMT, HD>::WAVES)) tile_kernel(Args 
         const int32_t e = tid + i * X::THREADS;
         key = e / X::PIECES;
         piece = e % X::PIECES;
-        return e < CHUNK * X::PIECES;
+        return e < CH * X::PIECES;
     };
     auto value_item = [&](int i, int32_t& quad, int32_t& dims) {
         const int32_t e = tid + i * X::THREADS;
         quad = e / (HD / 4);
         dims = 4 * (e % (HD / 4));
-        return e < CHUNK / 4 * (HD / 4);
+        return e < CH / 4 * (HD / 4);
     };
-    auto load_chunk = [&](const Where& w) {
+    auto load_chunk = [&](const Where<CH>& w) {
 #pragma unroll
         for (int i = 0; i < X::KN; ++i) {
             int32_t key, piece;
             if (!key_item(i, key, piece)) break;
-            kr[i] = *reinterpret_cast<const u4*>(c.keys + (key < 16 ? w.base[0] : w.base[1]) + ((key & 15) * HD * E + 16 * piece));
+            kr[i] = *reinterpret_cast<const u4*>(c.keys + w.of_run(uniform(key >> 4)) + ((key & 15) * HD * E + 16 * piece));
         }
 #pragma unroll
         for (int i = 0; i < X::VN; ++i) {
             int32_t quad, dims;
             if (!value_item(i, quad, dims)) break;
-            const uint8_t* p = c.values + (quad < 4 ? w.base[0] : w.base[1]) + ((4 * quad & 15) * HD + dims) * E;
+            const uint8_t* p = c.values + w.of_run(HD >= 64 ? uniform(quad >> 2) : quad >> 2) + ((4 * quad & 15) * HD + dims) * E;
 #pragma unroll
             for (int j = 0; j < 4; ++j) load_words(p + j * HD * E, vr[i][j]);
         }
     };
+    auto all_there = [&](const Where<CH>& w) { return w.there[0] == 0xFFFFFFFFu && w.there[X::SETS - 1] == 0xFFFFFFFFu; };
     // whether every row of the tile sees the chunk whole
-    auto whole = [&](int32_t ch, uint32_t there) { return ch * CHUNK + CHUNK <= keys.n_all && there == 0xFFFFFFFFu; };
-    auto store_chunk = [&](int32_t ch, uint32_t there) {
+    auto whole = [&](int32_t ch, const Where<CH>& w) { return ch * CH + CH <= keys.n_all && all_there(w); };
+    // where the 8 tokens of (set of 32, lane group) lie among a dim's: blocks turned by the dim, so that the lanes that write
+    // neighbouring dims meet different banks
+    auto block_of = [&](int32_t block, int32_t dim) { return 8 * (block ^ ((dim >> 2) & (CH / 8 - 1))); };
+    auto store_chunk = [&](int32_t ch, const Where<CH>& where) {
         element* kl = reinterpret_cast<element*>(lds) + (X::BUFFERS == 2 ? (ch & 1) * X::SIZE : 0);
         element* vl = kl + X::KP * X::KSIZE;
+        // four numbers' parts
+        auto store_parts = [&](float (&rest)[4], element* to, int32_t size) {
+#pragma unroll
+            for (int w = 0; w < 3; ++w) {
+                const uint32_t low = nearest_halves(rest[0], rest[1]), high = nearest_halves(rest[2], rest[3]);
+                *reinterpret_cast<uint2*>(to + w * size) = make_uint2(low, high);
+                rest[0] -= __builtin_bit_cast(float, low << 16);
+                rest[1] -= __builtin_bit_cast(float, low & 0xFFFF0000u);
+                rest[2] -= __builtin_bit_cast(float, high << 16);
+                rest[3] -= __builtin_bit_cast(float, high & 0xFFFF0000u);
+            }
+        };
 #pragma unroll
         for (int i = 0; i < X::KN; ++i) {
             int32_t key, piece;
@@ -1042,15 +1147,7 @@ __global__ void __launch_bounds__(256, (Tile<FMT, HD>::WAVES)) tile_kernel(Args 
                     const uint32_t w = kr[i][e];
                     rest[e] = __builtin_bit_cast(float, w);
                 }
-#pragma unroll
-                for (int w = 0; w < 3; ++w) {
-                    const uint32_t low = nearest_halves(rest[0], rest[1]), high = nearest_halves(rest[2], rest[3]);
-                    *reinterpret_cast<uint2*>(kl + w * X::KSIZE + key * X::KR + 4 * piece) = make_uint2(low, high);
-                    rest[0] -= __builtin_bit_cast(float, low << 16);
-                    rest[1] -= __builtin_bit_cast(float, low & 0xFFFF0000u);
-                    rest[2] -= __builtin_bit_cast(float, high << 16);
-                    rest[3] -= __builtin_bit_cast(float, high & 0xFFFF0000u);
-                }
+                store_parts(rest, kl + key * X::KR + 4 * piece, X::KSIZE);
             } else {
                 *reinterpret_cast<u4*>(kl + key * X::KR + 8 * piece) = kr[i];
             }
@@ -1059,19 +1156,20 @@ __global__ void __launch_bounds__(256, (Tile<FMT, HD>::WAVES)) tile_kernel(Args 
         for (int i = 0; i < X::VN; ++i) {
             int32_t quad, dims;
             if (!value_item(i, quad, dims)) break;
-            if (!whole(ch, there)) {  // tokens that are not there count for nothing; what is not finite goes to the rows that see it alone
+            if (!whole(ch, where)) {  // tokens that are not there count for nothing; what is not finite goes to the rows that see it alone
+                const uint32_t there = (quad < 8 ? where.there[0] : where.there[X::SETS - 1]) >> (4 * quad & 31);
                 bool odd = false;
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
 #pragma unroll
                     for (int w = 0; w < E; ++w) {
-                        if (!(there >> (4 * quad + j) & 1)) vr[i][j][w] = 0;
+                        if (!(there >> j & 1)) vr[i][j][w] = 0;
                         odd |= any_not_finite<FMT>(vr[i][j][w]);
                         vr[i][j][w] = finite_only<FMT>(vr[i][j][w]);
                     }
                 if (odd) odd_chunk[ch & 1] = ch;
             }
-            const int32_t at = 16 * (quad >> 2) + 8 * (quad & 1) + 4 * (quad >> 1 & 1);  // where the quad's tokens lie among a dim's
+            const int32_t block = quad >> 3 << 2 | (quad & 3), at = block_of(block, dims) + (quad & 4);  // (tokens 16 t + 4 grp + i of a set: 8 grp + 4 t + i)
 #pragma unroll
             for (int d = 0; d < 4; ++d) {
                 element* to = vl + (dims + d) * X::VR + at;
@@ -1079,15 +1177,7 @@ __global__ void __launch_bounds__(256, (Tile<FMT, HD>::WAVES)) tile_kernel(Args 
                     float rest[4];
 #pragma unroll
                     for (int j = 0; j < 4; ++j) rest[j] = __builtin_bit_cast(float, vr[i][j][d]);
-#pragma unroll
-                    for (int w = 0; w < 3; ++w) {
-                        const uint32_t low = nearest_halves(rest[0], rest[1]), high = nearest_halves(rest[2], rest[3]);
-                        *reinterpret_cast<uint2*>(to + w * X::VSIZE) = make_uint2(low, high);
-                        rest[0] -= __builtin_bit_cast(float, low << 16);
-                        rest[1] -= __builtin_bit_cast(float, low & 0xFFFF0000u);
-                        rest[2] -= __builtin_bit_cast(float, high << 16);
-                        rest[3] -= __builtin_bit_cast(float, high & 0xFFFF0000u);
-                    }
+                    store_parts(rest, to, X::VSIZE);
                 } else {
                     const uint32_t pick = d % 2 ? 0x07060302u : 0x05040100u;
                     *reinterpret_cast<uint2*>(to) = make_uint2(__builtin_amdgcn_perm(vr[i][1][d / 2], vr[i][0][d / 2], pick), __builtin_amdgcn_perm(vr[i][3][d / 2], vr[i][2][d / 2], pick));
@@ -1096,16 +1186,16 @@ __global__ void __launch_bounds__(256, (Tile<FMT, HD>::WAVES)) tile_kernel(Args 
         }
     };
 
-    Where next{};
-    Pages pages{};
+    Where<CH> next{};
+    Pages<CH> pages{};
     if (c0 < c1) {
         next = reader.where_of(c0, reader.pages_of(c0));
         load_chunk(next);
         pages = reader.pages_of(min(c0 + 1, c1 - 1));
     }
     // the wave's queries: a lane's dims of its row, as operands
-    const bool active = 32 * wave < held;  // waves with rows
-    const int32_t r = min(32 * wave + col, held - 1), token = (row0 + r) / G;
+    const bool active = 16 * wave < held;  // waves with rows
+    const int32_t r = min(16 * wave + col, held - 1), token = (row0 + r) / G;
     op q[X::QS][F::QP];
     float f = a.p.scale * 1.4426950408889634f;
     if (active) {
@@ -1113,7 +1203,7 @@ __global__ void __launch_bounds__(256, (Tile<FMT, HD>::WAVES)) tile_kernel(Args 
         float x[X::QS][8];
 #pragma unroll
         for (int s = 0; s < X::QS; ++s) {
-            const f4 low = *reinterpret_cast<const f4*>(src + 16 * s), high = *reinterpret_cast<const f4*>(src + 16 * s + 4);
+            const f4 low = *reinterpret_cast<const f4*>(src + 32 * s), high = *reinterpret_cast<const f4*>(src + 32 * s + 4);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 x[s][e] = low[e];
@@ -1127,7 +1217,7 @@ __global__ void __launch_bounds__(256, (Tile<FMT, HD>::WAVES)) tile_kernel(Args 
             for (int s = 0; s < X::QS; ++s)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) top = max(top, magnitude(x[s][e]));
-            const float most = column_max<false>(__builtin_bit_cast(float, min(top, 0x7F7FFFFFu)));
+            const float most = column_max<true>(__builtin_bit_cast(float, min(top, 0x7F7FFFFFu)));
             const int32_t up = 13 - max(static_cast<int32_t>(magnitude(most) >> 23) - 127, -100);
 #pragma unroll
             for (int s = 0; s < X::QS; ++s)
@@ -1139,112 +1229,137 @@ __global__ void __launch_bounds__(256, (Tile<FMT, HD>::WAVES)) tile_kernel(Args 
         for (int s = 0; s < X::QS; ++s) split_query(x[s], q[s]);
     }
     __syncthreads();  // (odd_chunk)
-    if (c0 < c1) store_chunk(c0, next.there);
+    if (c0 < c1) store_chunk(c0, next);
 
-    f16v o[X::DB];
+    constexpr int VG = X::DB < X::VGROUP ? X::DB : X::VGROUP, GROUPS = X::DB / VG;  // dim blocks whose operands are loaded together
+    f4 o[GROUPS][VG];
     float m = -INFINITY, l = 0.0f;
 #pragma unroll
     for (int db = 0; db < X::DB; ++db)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) o[db][e] = 0.0f;
-    auto token_of = [&](int i) { return 8 * (i >> 2) + 4 * grp + (i & 3); };
-    auto row_token = [&](int32_t at) { return (row0 + at) / G; };
-    const int32_t first_token = row_token(32 * wave), last_token = row_token(min(32 * wave + 31, held - 1));
-    // what the wave's rows see: below all of them, from none on nothing
+        for (int e = 0; e < 4; ++e) o[db / VG][db % VG][e] = 0.0f;
+    // the token of a lane's score i in its set of 32
+    auto token_of = [&](int i) { return 16 * (i >> 2) + 4 * grp + (i & 3); };
+    const int32_t first_token = uniform((row0 + 16 * wave) / G), last_token = uniform((row0 + min(16 * wave + 15, held - 1)) / G);
+    // what the wave's rows see: tokens below all of them, from none on nothing
     const int64_t see_all = b.masks ? static_cast<int64_t>(part.length) : static_cast<int64_t>(part.length) + first_token + 1;
     const int64_t see_none = b.masks ? INT64_MAX : static_cast<int64_t>(part.length) + last_token + 1;
-    auto attend_chunk = [&](auto masked_form, int32_t ch, uint32_t there, const Where& where) {
+    auto attend_chunk = [&](auto masked_form, int32_t ch, const Where<CH>& where) {
         constexpr bool masked = decltype(masked_form)::value;
         const element* kl = reinterpret_cast<const element*>(lds) + (X::BUFFERS == 2 ? (ch & 1) * X::SIZE : 0);
         const element* vl = kl + X::KP * X::KSIZE;
-        f16v sc;
+        // (operands of the next step are on their way from LDS while a step's products run)
+        constexpr int T = 2 * X::SETS;
+        op k[2][T][F::KP];
+        auto load_keys = [&](int s) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) sc[e] = 0.0f;
+            for (int t = 0; t < T; ++t)
+#pragma unroll
+                for (int w = 0; w < F::KP; ++w) k[s & 1][t][w] = *reinterpret_cast<const op*>(kl + w * X::KSIZE + (16 * t + col) * X::KR + 32 * s + 8 * grp);
+        };
+        load_keys(0);
+        f4 sc[T];
+#pragma unroll
+        for (int t = 0; t < T; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sc[t][e] = 0.0f;
 #pragma unroll
         for (int s = 0; s < X::QS; ++s) {
-            op k[F::KP];
-#pragma unroll
-            for (int w = 0; w < F::KP; ++w) k[w] = *reinterpret_cast<const op*>(kl + w * X::KSIZE + col * X::KR + 16 * s + 8 * grp);
-            sc = products<false>(k, q[s], sc);
+            if (s + 1 < X::QS) load_keys(s + 1);
+            __builtin_amdgcn_sched_barrier(0);
+            products_of<true>(k[s & 1], q[s], sc);
+            __builtin_amdgcn_sched_barrier(0);
         }
-        float x[16];
+        op v[2][VG][F::KP];
+        auto load_values = [&](int i) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] = sc[i];
-        const uint32_t vis = masked ? seen_bits(b, part.first, token, part.length, ch * CHUNK, there) : 0u;
-        to_weights<FMT, false, masked>(x, vis, f, m, l, token_of, [&](float alpha) {
+            for (int u = 0; u < VG; ++u) {
+                const int32_t dim = 16 * (i % GROUPS * VG + u) + col;
 #pragma unroll
-            for (int db = 0; db < X::DB; ++db) o[db] *= alpha;
+                for (int w = 0; w < F::KP; ++w) v[i & 1][u][w] = *reinterpret_cast<const op*>(vl + w * X::VSIZE + dim * X::VR + block_of(4 * (i / GROUPS) + grp, dim));
+            }
+        };
+        load_values(0);
+        float x[8 * X::SETS];
+#pragma unroll
+        for (int i = 0; i < 8 * X::SETS; ++i) x[i] = sc[i >> 2][i & 3];
+        uint32_t vis[X::SETS] = {};
+        if constexpr (masked)
+#pragma unroll
+            for (int h = 0; h < X::SETS; ++h) vis[h] = seen_bits(b, part.first, token, part.length, ch * CH + 32 * h, where.there[h]);
+        to_weights<FMT, true, masked>(x, f, m, l, [&](int i) { return !(vis[i >> 3] >> token_of(i & 7) & 1); }, [&](float alpha) {
+#pragma unroll
+            for (int db = 0; db < X::DB; ++db) o[db / VG][db % VG] *= alpha;
         });
-        if (masked || !whole(ch, there)) {
+        if (masked || !whole(ch, where)) {
             if (odd_chunk[ch & 1] == ch) {
-                const uint32_t mine = seen_bits(b, part.first, token, part.length, ch * CHUNK, there);
-                for (int32_t tok = 0; tok < CHUNK; ++tok) {
-                    if (!(there >> tok & 1)) continue;
-                    const int32_t from = tok >> 2 & 1, i = 4 * (tok >> 3) + (tok & 3);
-                    const uint8_t* row = c.values + (tok < 16 ? where.base[0] : where.base[1]) + (tok & 15) * HD * E;
+                for (int32_t tok = 0; tok < CH; ++tok) {
+                    const uint32_t there = tok < 32 ? where.there[0] : where.there[X::SETS - 1];
+                    if (!(there >> (tok & 31) & 1)) continue;
+                    const uint32_t mine = seen_bits(b, part.first, token, part.length, ch * CH + (tok & ~31), there);
+                    const int32_t from = tok >> 2 & 3, i = 8 * (tok >> 5) + 4 * (tok >> 4 & 1) + (tok & 3);
+                    const uint8_t* row = c.values + where.of_run(tok >> 4) + (tok & 15) * HD * E;
                     float weight = 0.0f;
 #pragma unroll
-                    for (int e = 0; e < 16; ++e)
+                    for (int e = 0; e < 8 * X::SETS; ++e)
                         if (e == i) weight = x[e];
-                    weight = __shfl(weight, from * 32 + col);
-                    if (!(mine >> tok & 1)) continue;
+                    weight = __shfl(weight, from * 16 + col);
+                    if (!(mine >> (tok & 31) & 1)) continue;
 #pragma unroll
                     for (int db = 0; db < X::DB; ++db)
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) {
-                            const float v = load_element<FMT>(row, 32 * db + token_of(e));
-                            if (!(fabsf(v) < INFINITY)) o[db][e] += weight * v;
+                        for (int e = 0; e < 4; ++e) {
+                            const float v = load_element<FMT>(row, 16 * db + 4 * grp + e);
+                            if (!(fabsf(v) < INFINITY)) o[db / VG][db % VG][e] += weight * v;
+                            __builtin_amdgcn_sched_barrier(0);  // (rare: one load at a time, few registers)
                         }
                 }
             }
         }
+        op p[F::QP];
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            float w8[8];
+        for (int i = 0; i < X::SETS * GROUPS; ++i) {
+            if (i % GROUPS == 0) {
+                float w8[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) w8[e] = x[8 * s + e];
-            op p[F::QP];
-            split_weights(w8, p);
-#pragma unroll
-            for (int db = 0; db < X::DB; ++db) {
-                op v[F::KP];
-#pragma unroll
-                for (int w = 0; w < F::KP; ++w) v[w] = *reinterpret_cast<const op*>(vl + w * X::VSIZE + (32 * db + col) * X::VR + 16 * s + 8 * grp);
-                o[db] = products<false>(v, p, o[db]);
+                for (int e = 0; e < 8; ++e) w8[e] = x[8 * (i / GROUPS) + e];
+                split_weights(w8, p);
             }
+            if (i + 1 < X::SETS * GROUPS) load_values(i + 1);
+            __builtin_amdgcn_sched_barrier(0);
+            products_of<true>(v[i & 1], p, o[i % GROUPS]);
+            __builtin_amdgcn_sched_barrier(0);
         }
     };
     for (int32_t ch = c0; ch < c1; ++ch) {
-        const Where now = next;
+        const Where<CH> now = next;
         if (ch + 1 < c1) {
             next = reader.where_of(ch + 1, pages);
             load_chunk(next);
             pages = reader.pages_of(min(ch + 2, c1 - 1));
         }
         __syncthreads();  // the chunk is in LDS
-        if (active && static_cast<int64_t>(ch) * CHUNK < see_none) {
-            if (static_cast<int64_t>(ch) * CHUNK + CHUNK <= see_all && now.there == 0xFFFFFFFFu) attend_chunk(std::false_type{}, ch, now.there, now);
-            else attend_chunk(std::true_type{}, ch, now.there, now);
+        if (active && static_cast<int64_t>(ch) * CH < see_none) {
+            if (static_cast<int64_t>(ch) * CH + CH <= see_all && all_there(now)) attend_chunk(std::false_type{}, ch, now);
+            else attend_chunk(std::true_type{}, ch, now);
         }
         if constexpr (X::BUFFERS == 1) __syncthreads();  // (and read by all)
-        if (ch + 1 < c1) store_chunk(ch + 1, next.there);
+        if (ch + 1 < c1) store_chunk(ch + 1, next);
     }
 
-    l = column_sum<false>(l);
+    l = column_sum<true>(l);
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     const size_t at_slot = static_cast<size_t>(part.slot + part.split) * R;
     const __amdgpu_buffer_rsrc_t averages = averages_of<HD, R>(a, part.slot + part.split, 1);
-    if (32 * wave + col < held) {
+    if (16 * wave + col < held) {
         float* out = a.p.context + row_at(r);
 #pragma unroll
-        for (int db = 0; db < X::DB; ++db)
-#pragma unroll
-            for (int e = 0; e < 16; e += 4) {
-                const int32_t d = 32 * db + token_of(e);
-                const f4 y = {o[db][e] * inv, o[db][e + 1] * inv, o[db][e + 2] * inv, o[db][e + 3] * inv};
-                if (keys.splits == 1) *reinterpret_cast<f4*>(out + d) = y;
-                else store_average(averages, r * HD + d, y);
-            }
+        for (int db = 0; db < X::DB; ++db) {
+            const int32_t d = 16 * db + 4 * grp;
+            const f4 y = o[db / VG][db % VG] * inv;
+            if (keys.splits == 1) *reinterpret_cast<f4*>(out + d) = y;
+            else store_average(averages, r * HD + d, y);
+        }
         if (keys.splits > 1 && grp == 0) store_stats(a, at_slot + r, m, l);
     }
     if (keys.splits == 1) return;
@@ -1252,13 +1367,13 @@ __global__ void __launch_bounds__(256, (Tile<FMT, HD>::WAVES)) tile_kernel(Args 
 }
 
 // ---- launches ---------------------------------------------------------------------------------------
-// The grid and the workspace of a launch of tiles of R rows whose parts have at least LEAST chunks.
-template <int HD, int R, int LEAST>
+// The grid and the workspace of a launch of tiles of R rows whose parts have at least LEAST chunks of CHUNK keys.
+template <int HD, int R, int LEAST, int CHUNK>
 int32_t prepare(Args& a, int32_t target, int64_t* grid, hipStream_t st) {
     const BatchView& b = a.p.b;
     const int64_t G = a.p.num_heads / a.p.c.kv_heads;
     const int64_t tiles = std::min(b.sequences * ((b.most_rows * G + R - 1) / R), b.rows * G / R + b.sequences) * a.p.c.kv_heads;
-    const int64_t chunks = (static_cast<int64_t>(b.key_bound) + CHUNK - 1) / CHUNK, most_splits = std::min<int64_t>(MAX_SPLITS, (chunks + LEAST - 1) / LEAST);
+    const int64_t chunks = (static_cast<int64_t>(b.key_bound) + CHUNK - 1) / CHUNK, most_splits = std::min<int64_t>(most_parts(R), (chunks + LEAST - 1) / LEAST);
     a.target = target;
     *grid = std::min(tiles + target, tiles * most_splits);
     if (*grid > INT32_MAX / 64) return fail(KT_ERR_SHAPE, "too many rows and heads in one call");
@@ -1275,7 +1390,7 @@ int32_t prepare(Args& a, int32_t target, int64_t* grid, hipStream_t st) {
 template <int FMT, int HD, int R, int NW, bool STEP>
 int32_t launch_rows(Args a, hipStream_t st) {
     int64_t grid = 0;
-    if (const int32_t status = prepare<HD, R, NW>(a, 2 * cu_count(), &grid, st)) return status;
+    if (const int32_t status = prepare<HD, R, NW, CHUNK>(a, XD * cu_count(), &grid, st)) return status;
     constexpr size_t lds = std::max(std::max(sizeof(float) * NW * R * (HD + 6), size_t{2} * Format<FMT>::QP * R * (HD + 8)), merge_lds(R, NW));
     if (const int32_t ls = allow_lds<&attention_kernel<FMT, HD, R, NW, STEP>, lds>(lds)) return ls;
     attention_kernel<FMT, HD, R, NW, STEP><<<static_cast<uint32_t>(grid), 64 * NW, lds, st>>>(a);
@@ -1287,7 +1402,7 @@ template <int FMT, int HD>
 int32_t launch_tiles(Args a, hipStream_t st) {
     using X = Tile<FMT, HD>;
     int64_t grid = 0;
-    if (const int32_t status = prepare<HD, X::R, X::LEAST>(a, X::WAVES * cu_count(), &grid, st)) return status;
+    if (const int32_t status = prepare<HD, X::R, X::LEAST, X::CH>(a, XT(FMT, HD) * cu_count(), &grid, st)) return status;
     if (const int32_t ls = allow_lds<&tile_kernel<FMT, HD>, X::LDS>(X::LDS)) return ls;
     tile_kernel<FMT, HD><<<static_cast<uint32_t>(grid), X::THREADS, X::LDS, st>>>(a);
     KT_LAUNCHED("paged attention kernel");
