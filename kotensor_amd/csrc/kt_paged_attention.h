@@ -86,6 +86,16 @@ __device__ __forceinline__ A products(const OP (&k)[KP], const OP (&q)[QP], A c)
     return c;
 }
 
+// Wait states behind products whose sums the code after a branch reads (20 for 32x32x16, 12 for 16x16x32): the compiler
+// was seen to leave them out where a branch followed at once.
+template <bool SMALL>
+__device__ __forceinline__ void settle() {
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (SMALL) asm volatile("s_nop 11");
+    else asm volatile("s_nop 11\n\ts_nop 7");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
 __device__ __forceinline__ void split_weights(const float (&v)[8], bf16x8 (&part)[3]) { split3_nearest(v, part); }
 __device__ __forceinline__ void split_weights(const float (&v)[8], half8 (&part)[2]) {
 #pragma unroll
@@ -965,7 +975,7 @@ __global__ void __launch_bounds__(64 * NW, HD == 256 || (FMT == KT_PAGED_F32 && 
 #pragma unroll
                 for (int ct = 0; ct < X::CT; ++ct) o[ct][db] = products<X::SMALL>(v, p[ct][s], o[ct][db]);
             }
-        __builtin_amdgcn_sched_barrier(0);
+        settle<X::SMALL>();
         load_values(here);
         if constexpr (STEP) {
             if (holder && next == part.length / CHUNK) patch();
@@ -1034,7 +1044,7 @@ __global__ void __launch_bounds__(64 * NW, HD == 256 || (FMT == KT_PAGED_F32 && 
 #ifndef XNW
 #define XNW(F, H) 8
 #define XMW(F, H) 2
-#define XCH(F, H) (F == 0 ? 32 : 64)
+#define XCH(F, H) (F == 0 || H == 256 ? 32 : 64)
 #define XT(F, H) 1
 #define XD 4
 #endif
@@ -1330,6 +1340,7 @@ __global__ void __launch_bounds__((Tile<FMT, HD>::THREADS), (Tile<FMT, HD>::MW))
             products_of<true>(v[i & 1], p, o[i % GROUPS]);
             __builtin_amdgcn_sched_barrier(0);
         }
+        settle<true>();
     };
     for (int32_t ch = c0; ch < c1; ++ch) {
         const Where<CH> now = next;
@@ -1415,7 +1426,9 @@ int32_t launch_dims(const Args& a, hipStream_t st) {
     if constexpr (HD < 256) {
         if (a.k_new) return launch_rows<FMT, HD, 16, 4, true>(a, st);
     }
-    if (rows > 64) return launch_tiles<FMT, HD>(a, st);
+    if constexpr (HD < 256 || FMT != KT_PAGED_F32) {
+        if (rows > 64) return launch_tiles<FMT, HD>(a, st);
+    }
     if constexpr (HD < 256) {
         if (rows > 16) return launch_rows<FMT, HD, 32, 4, false>(a, st);
     }
