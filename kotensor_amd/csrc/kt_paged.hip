@@ -278,6 +278,7 @@ int32_t view_batch(const kt_paged_batch* b, const kt_paged_cache* cache, BatchVi
     if (b->sequences < 0 || b->sequences > 65535) return fail(KT_ERR_ARGUMENT, "%d sequences: 0 to 65535", b->sequences);
     if (b->rows < 0 || b->most_rows < 0 || b->most_rows > b->rows)
         return fail(KT_ERR_ARGUMENT, "at most %d rows a sequence of %d rows in all", b->most_rows, b->rows);
+    if (b->rows >= 1 << 24) return fail(KT_ERR_SHAPE, "%d rows in one call: at most %d", b->rows, (1 << 24) - 1);
     if (!b->masks != !b->depths) return fail(KT_ERR_ARGUMENT, "a tree has masks and depths, a text neither");
     if (b->masks && (b->mask_words <= 0 || b->mask_words > INT32_MAX / 32 || 32 * static_cast<int64_t>(b->mask_words) < b->most_rows))
         return fail(KT_ERR_SHAPE, "%d mask words do not hold %d rows", b->mask_words, b->most_rows);

@@ -242,8 +242,8 @@ __device__ __forceinline__ uint32_t seen_bits(const BatchView& b, int32_t first,
 }
 
 // ---- the parts of a launch ---------------------------------------------------------------------
-// Parts of a tile of R rows at most: what a merge holds of their rows' maxima and sums.
-constexpr int most_parts(int R) { return R <= 32 ? 128 : 4096 / R; }
+// Parts of a tile at most.
+constexpr int MOST_PARTS = 128;
 struct Args {
     PagedAttnArgs p;
     const float* k_new;  // STEP: the step's projections before RoPE
@@ -252,16 +252,25 @@ struct Args {
     float* averages;     // [slots][R][head_dim]: the parts' averages
     float* stats;        // [slots][R][2]: their maxima and sums
     uint32_t* counters;  // [slots], zero between launches
+    int32_t slots;
 };
 
 __device__ __forceinline__ int32_t held_keys(const PagedView& c, const BatchView& b, int32_t length, int32_t n) {
     const int64_t most = min(room_of(c, b), static_cast<int64_t>(b.key_bound));
     return static_cast<int32_t>(min(max(static_cast<int64_t>(length) + n, int64_t{0}), most));
 }
-__device__ __forceinline__ int64_t wave_total(int64_t v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-    return v;
+// Sums over the lanes up to each lane, without LDS: by DPP inside rows of 16 lanes, then the rows' totals passed on.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int32_t dpp_add(int32_t v) {
+    return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false);
+}
+__device__ __forceinline__ int32_t lanes_upto(int32_t v) {
+    v = dpp_add<0x111, 0xF>(v);  // row_shr 1, 2, 4, 8
+    v = dpp_add<0x112, 0xF>(v);
+    v = dpp_add<0x114, 0xF>(v);
+    v = dpp_add<0x118, 0xF>(v);
+    v = dpp_add<0x142, 0xA>(v);  // lane 15 of a row to the next one (rows 1 and 3), lane 31 to rows 2 and 3
+    return dpp_add<0x143, 0xC>(v);
 }
 __device__ __forceinline__ int32_t lane_int(int32_t v, int32_t lane) { return __builtin_amdgcn_readlane(v, lane); }
 // A number that every lane has, as a scalar (divisions leave it in vector registers, and what follows from it too).
@@ -282,9 +291,9 @@ struct Part {
     }
 };
 
-// Which part of the launch workgroup `at` has; false: none. Every lane is a sequence. A launch has at most target + (its tiles
+// Which part of the launch workgroup `at` has (BY_SLOT: whose slot `at` is); false: none. Every lane is a sequence. A launch has at most target + (its tiles
 // of all kv heads) parts, and at most 2 target that share a tile: a part's size is at least the chunks over target.
-template <int R, int LEAST, int CHUNK>
+template <int R, int LEAST, int CHUNK, bool BY_SLOT = false>
 __device__ __forceinline__ bool find_part(const Args& a, int32_t at, Part& out) {
     const PagedView& c = a.p.c;
     const BatchView& b = a.p.b;
@@ -300,47 +309,51 @@ __device__ __forceinline__ bool find_part(const Args& a, int32_t at, Part& out) 
     };
     auto tiles_of = [&]() { return static_cast<int32_t>((static_cast<int64_t>(n) * G + R - 1) / R); };
     auto chunks_of = [&]() { return (held_keys(c, b, length, n) + CHUNK - 1) / CHUNK; };
-    int64_t total = 0, rows = 0;
+    // (whole numbers up to 2^24 are exact in fp32; of larger totals a little more)
+    float total = 0.0f, rows = 0.0f;
     for (int32_t s0 = 0; s0 < b.sequences; s0 += 64) {
         load(s0);
-        total += static_cast<int64_t>(tiles_of()) * c.kv_heads * max(chunks_of(), 1);
-        rows += n;
+        total += static_cast<float>(tiles_of()) * static_cast<float>(c.kv_heads) * static_cast<float>(max(chunks_of(), 1));
+        rows += static_cast<float>(n);
     }
-    total = uniform(wave_total(total));
-    if (uniform(wave_total(rows)) > b.rows) return false;  // starts that do not ascend
-    int64_t per = (total + a.target - 1) / a.target;
-    per = (max(per, int64_t{1}) + LEAST - 1) / LEAST * LEAST;
+    total = wave_sum_dpp(total);
+    if (wave_sum_dpp(rows) > static_cast<float>(b.rows)) return false;  // starts that do not ascend
+    if (total >= 0x1p24f) total *= 1.0f + 0x1p-16f;
+    const float target = static_cast<float>(a.target);
+    int32_t per = static_cast<int32_t>(fminf(total / target, 0x1p30f));
+    if (static_cast<float>(per) * target < total) ++per;
+    per = uniform((max(per, 1) + LEAST - 1) / LEAST * LEAST);
     int32_t before = 0, slots = 0;
     for (int32_t s0 = 0; s0 < b.sequences; s0 += 64) {
         if (b.sequences > 64) load(s0);
         const int32_t tiles = tiles_of(), chunks = chunks_of();
-        const int32_t size = static_cast<int32_t>(max(per, static_cast<int64_t>((chunks + most_parts(R) - 1) / most_parts(R))));
+        const int32_t size = max(per, (chunks + MOST_PARTS - 1) / MOST_PARTS);
         const int32_t splits = max((chunks + size - 1) / size, 1), parts = tiles * c.kv_heads * splits;
         const int32_t mine = splits > 1 ? parts : 0;
-        int32_t upto = parts, slots_upto = mine;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int32_t x = __shfl_up(upto, o), y = __shfl_up(slots_upto, o);
-            if (lane >= o) {
-                upto += x;
-                slots_upto += y;
-            }
-        }
-        const int32_t passed = uniform(static_cast<int32_t>(__popcll(__ballot(before + upto <= at))));
+        const int32_t upto = lanes_upto(parts), slots_upto = lanes_upto(mine);
+        const int32_t passed = uniform(static_cast<int32_t>(__popcll(__ballot((BY_SLOT ? slots + slots_upto : before + upto) <= at))));
         if (passed < 64) {
-            const int32_t local = at - before - (lane_int(upto, passed) - lane_int(parts, passed));
+            const int32_t slot0 = uniform(slots) + lane_int(slots_upto, passed) - lane_int(mine, passed);
+            const int32_t local = BY_SLOT ? at - slot0 : at - before - (lane_int(upto, passed) - lane_int(parts, passed));
             out.sequence = uniform(s0 + passed);
             out.first = lane_int(first, passed);
             out.n = lane_int(n, passed);
             out.length = lane_int(length, passed);
             out.splits = lane_int(splits, passed);
             out.per = lane_int(size, passed);
-            out.head = uniform(local % c.kv_heads);  // (workgroups go round the eight dies: a head's stay on few of them)
-            const int32_t rest = uniform(local / c.kv_heads);
-            out.split = uniform(rest % out.splits);
-            out.tile = lane_int(tiles, passed) - 1 - uniform(rest / out.splits);  // (a text's last tiles see the most)
+            if constexpr (BY_SLOT) {
+                const int32_t rest = uniform(local / out.splits);
+                out.split = uniform(local % out.splits);
+                out.head = uniform(rest % c.kv_heads);
+                out.tile = uniform(rest / c.kv_heads);
+            } else {
+                out.head = uniform(local % c.kv_heads);  // (workgroups go round the eight dies: a head's stay on few of them)
+                const int32_t rest = uniform(local / c.kv_heads);
+                out.split = uniform(rest % out.splits);
+                out.tile = lane_int(tiles, passed) - 1 - uniform(rest / out.splits);  // (a text's last tiles see the most)
+            }
             out.keys = uniform(held_keys(c, b, out.length, out.n));
-            out.slot = uniform(slots) + lane_int(slots_upto, passed) - lane_int(mine, passed) + (out.tile * c.kv_heads + out.head) * out.splits;
+            out.slot = slot0 + (out.tile * c.kv_heads + out.head) * out.splits;
             return true;
         }
         before += lane_int(upto, 63);
@@ -363,8 +376,9 @@ __device__ __forceinline__ Keys keys_of(const Args& a, const Part& part, int32_t
     k.n_all = uniform(static_cast<int32_t>(min(static_cast<int64_t>(k.n_keys), max(length + (tree ? 0 : t_first + 1), int64_t{0}))));
     const int32_t chunks = (k.n_keys + CHUNK - 1) / CHUNK;
     k.splits = uniform(max(1, min(part.splits, (chunks + part.per - 1) / part.per)));
-    k.c0 = uniform(static_cast<int32_t>(static_cast<int64_t>(chunks) * part.split / k.splits));
-    k.c1 = uniform(static_cast<int32_t>(static_cast<int64_t>(chunks) * (part.split + 1) / k.splits));
+    const uint32_t whole = static_cast<uint32_t>(chunks) / static_cast<uint32_t>(k.splits), rest = static_cast<uint32_t>(chunks) - whole * k.splits;
+    k.c0 = uniform(static_cast<int32_t>(whole * part.split + rest * part.split / static_cast<uint32_t>(k.splits)));
+    k.c1 = uniform(static_cast<int32_t>(whole * (part.split + 1) + rest * (part.split + 1) / static_cast<uint32_t>(k.splits)));
     return k;
 }
 
@@ -436,7 +450,7 @@ template <int HD, int R>
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t averages_of(const Args& a, size_t slot, int32_t slots) {
     return __builtin_amdgcn_make_buffer_rsrc(a.averages + slot * R * HD, 0, slots * R * HD * 4, 0x00020000);
 }
-constexpr size_t merge_lds(int R, int NW) { return sizeof(float) * (2 * R * most_parts(R) + R + 4 * 64 * NW); }
+constexpr size_t merge_lds(int R, int NW) { return sizeof(float) * (2 * R * MOST_PARTS + R + 4 * 64 * NW); }
 
 // Called by all threads of a workgroup once its part is stored. The last workgroup of the tile to arrive merges the
 // parts, in their order, into the context; row_at: where a row of the tile lies there.
@@ -458,8 +472,8 @@ __device__ __forceinline__ void meet(const Args& a, const Part& part, int32_t sp
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
     const size_t slot0 = static_cast<size_t>(part.slot) * R;
     float* maxima = lds;                          // [R][splits]: then the parts' weights
-    float* sums = maxima + R * most_parts(R);     // [R][splits]
-    float* total = sums + R * most_parts(R);      // [R]
+    float* sums = maxima + R * MOST_PARTS;     // [R][splits]
+    float* total = sums + R * MOST_PARTS;      // [R]
     f4* shares = reinterpret_cast<f4*>(total + R);  // [T]
     const __amdgpu_buffer_rsrc_t all = averages_of<HD, R>(a, part.slot, splits);
     // A thread sums its items (four dims of a row) over the parts; where there are fewer items than threads, phases of
@@ -495,7 +509,7 @@ __device__ __forceinline__ void meet(const Args& a, const Part& part, int32_t sp
     while (width < splits && width < 64) width <<= 1;
     for (int32_t r0 = wave * (64 / width); r0 < held; r0 += NW * (64 / width)) {
         const int32_t r = r0 + lane / width, at = min(r, held - 1) * splits;
-        constexpr int PER = (most_parts(R) + 63) / 64;
+        constexpr int PER = (MOST_PARTS + 63) / 64;
         float ml[PER], ll[PER], mx = -INFINITY, sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
@@ -559,6 +573,60 @@ __device__ __forceinline__ void meet(const Args& a, const Part& part, int32_t sp
             for (int32_t p = 1; p < phases; ++p) y += shares[tid + p * items];
             write(tid, y);
         }
+    }
+}
+
+// The same as a launch of its own, for tiles of many rows, whose merge is more than one workgroup's work: the workgroups of a
+// slot take their shares of the tile's rows.
+constexpr int merge_shares(int R) { return R / 32; }
+template <int HD, int R, int LEAST, int CHUNK>
+__global__ void __launch_bounds__(256) merge_kernel(Args a) {
+    __shared__ float maxima[R + MOST_PARTS], sums[R + MOST_PARTS], weights[R + MOST_PARTS];
+    Part part;
+    if (!find_part<R, LEAST, CHUNK, true>(a, blockIdx.x, part)) return;
+    part.make_uniform();
+    const int32_t H = a.p.num_heads, G = H / a.p.c.kv_heads, row0 = part.tile * R, held = min(R, part.n * G - row0);
+    const Keys keys = keys_of<R, CHUNK>(a, part, held);
+    const int32_t splits = keys.splits, tid = threadIdx.x;
+    if (splits == 1) return;
+    const int32_t shares = part.splits * merge_shares(R), share = part.split * merge_shares(R) + blockIdx.y;
+    const int32_t r0 = uniform(held * share / shares), rows = uniform(held * (share + 1) / shares) - r0;
+    if (rows == 0) return;
+    const size_t slot0 = static_cast<size_t>(part.slot) * R;
+    // (fewer than held / part.splits + 1 rows, of at most part.splits parts)
+    for (int32_t e = tid; e < rows * splits; e += 256) {
+        const int32_t s = e / rows, r = e % rows;
+        const float2 both = reinterpret_cast<const float2*>(a.stats)[slot0 + static_cast<size_t>(s) * R + r0 + r];
+        maxima[r * splits + s] = both.x;
+        sums[r * splits + s] = both.y;
+    }
+    __syncthreads();
+    for (int32_t e = tid; e < rows * splits; e += 256) {  // a part's share of its row, over all of them
+        const int32_t r = e / splits;
+        float mx = -INFINITY, sum = 0.0f;
+        for (int32_t s = 0; s < splits; ++s) mx = fmaxf(mx, maxima[r * splits + s]);
+        for (int32_t s = 0; s < splits; ++s) sum += share_of(maxima[r * splits + s], sums[r * splits + s], mx);
+        weights[e] = sum == 0.0f ? 0.0f : share_of(maxima[e], sums[e], mx) / sum;
+    }
+    __syncthreads();
+    constexpr int BATCH = 8;
+    for (int32_t item = tid; item < rows * (HD / 4); item += 256) {
+        const int32_t r = item / (HD / 4), d = 4 * (item % (HD / 4));
+        const float* from = a.averages + (slot0 + r0 + r) * HD + d;
+        f4 y = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int32_t s0 = 0; s0 < splits; s0 += BATCH) {
+            f4 v[BATCH];
+#pragma unroll
+            for (int u = 0; u < BATCH; ++u) v[u] = *reinterpret_cast<const f4*>(from + static_cast<size_t>(min(s0 + u, splits - 1)) * (R * HD));
+#pragma unroll
+            for (int u = 0; u < BATCH; ++u) {
+                const float by = s0 + u < splits ? weights[r * splits + s0 + u] : 0.0f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) y[i] = s0 + u < splits ? fmaf(by, v[u][i], y[i]) : y[i];
+            }
+        }
+        const int32_t t = (row0 + r0 + r) / G;
+        *reinterpret_cast<f4*>(a.p.context + (static_cast<size_t>(part.first + t) * H + part.head * G + (row0 + r0 + r - t * G)) * HD + d) = y;
     }
 }
 
@@ -1034,7 +1102,7 @@ __global__ void __launch_bounds__(64 * NW, HD == 256 || (FMT == KT_PAGED_F32 && 
         }
     }
     if (splits == 1) return;
-    meet<HD, R, NW>(a, part, splits, held, lds, row_at);
+    if constexpr (R == 16) meet<HD, R, NW>(a, part, splits, held, lds, row_at);
 }
 
 // ---- many rows ---------------------------------------------------------------------------------------
@@ -1042,11 +1110,13 @@ __global__ void __launch_bounds__(64 * NW, HD == 256 || (FMT == KT_PAGED_F32 && 
 // where all eight waves read it: the keys as rows, the values as dims with their tokens in the order of the operands; fp32
 // ones split into their parts once for all waves. Queries stay in registers.
 #ifndef XNW
-#define XNW(F, H) 8
-#define XMW(F, H) 2
-#define XCH(F, H) (F == 0 || H == 256 ? 32 : 64)
+#define XNW(F, H) ((F && H <= 64) ? 4 : 8)
+#define XMW(F, H) ((F && H <= 64) ? 3 : 2)
+#define XCH(F, H) (F == 0 || H != 128 ? 32 : 64)
 #define XT(F, H) 1
 #define XD 4
+#define XTILE 64
+#define XR32(F, H) 1
 #endif
 template <int FMT, int HD>
 struct Tile {
@@ -1060,7 +1130,7 @@ struct Tile {
     static constexpr int PIECES = HD * E / 16;  // 16-byte pieces of a key
     static constexpr int KN = (CH * PIECES + THREADS - 1) / THREADS;
     static constexpr int VN = (CH / 4 * (HD / 4) + THREADS - 1) / THREADS;  // 4 tokens x 4 dims
-    static constexpr size_t LDS = std::max(size_t{2} * SIZE * BUFFERS, merge_lds(R, NW));
+    static constexpr size_t LDS = size_t{2} * SIZE * BUFFERS;
     static constexpr int LEAST = 128 / CH;
     static constexpr int VGROUP = FMT == KT_PAGED_F32 ? 2 : 4;
 };
@@ -1070,7 +1140,7 @@ __global__ void __launch_bounds__((Tile<FMT, HD>::THREADS), (Tile<FMT, HD>::MW))
     using F = Format<FMT>;
     using X = Tile<FMT, HD>;
     using op = typename F::op;
-    constexpr int R = X::R, NW = X::NW, E = F::E, CH = X::CH;
+    constexpr int R = X::R, E = F::E, CH = X::CH;
     typedef typename std::conditional<FMT == KT_PAGED_F16, _Float16, __bf16>::type element;
     extern __shared__ __attribute__((aligned(16))) float lds[];
     __shared__ int32_t odd_chunk[2];  // the chunk in a buffer if some of its values are not finite
@@ -1360,21 +1430,13 @@ __global__ void __launch_bounds__((Tile<FMT, HD>::THREADS), (Tile<FMT, HD>::MW))
 
     l = column_sum<true>(l);
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    const size_t at_slot = static_cast<size_t>(part.slot + part.split) * R;
-    const __amdgpu_buffer_rsrc_t averages = averages_of<HD, R>(a, part.slot + part.split, 1);
     if (16 * wave + col < held) {
-        float* out = a.p.context + row_at(r);
+        const size_t at_slot = static_cast<size_t>(part.slot + part.split) * R + r;
+        float* out = keys.splits == 1 ? a.p.context + row_at(r) : a.averages + at_slot * HD;
 #pragma unroll
-        for (int db = 0; db < X::DB; ++db) {
-            const int32_t d = 16 * db + 4 * grp;
-            const f4 y = o[db / VG][db % VG] * inv;
-            if (keys.splits == 1) *reinterpret_cast<f4*>(out + d) = y;
-            else store_average(averages, r * HD + d, y);
-        }
-        if (keys.splits > 1 && grp == 0) store_stats(a, at_slot + r, m, l);
+        for (int db = 0; db < X::DB; ++db) *reinterpret_cast<f4*>(out + 16 * db + 4 * grp) = o[db / VG][db % VG] * inv;
+        if (keys.splits > 1 && grp == 0) reinterpret_cast<float2*>(a.stats)[at_slot] = make_float2(m, l);
     }
-    if (keys.splits == 1) return;
-    meet<HD, R, NW>(a, part, keys.splits, held, lds, row_at);
 }
 
 // ---- launches ---------------------------------------------------------------------------------------
@@ -1384,17 +1446,26 @@ int32_t prepare(Args& a, int32_t target, int64_t* grid, hipStream_t st) {
     const BatchView& b = a.p.b;
     const int64_t G = a.p.num_heads / a.p.c.kv_heads;
     const int64_t tiles = std::min(b.sequences * ((b.most_rows * G + R - 1) / R), b.rows * G / R + b.sequences) * a.p.c.kv_heads;
-    const int64_t chunks = (static_cast<int64_t>(b.key_bound) + CHUNK - 1) / CHUNK, most_splits = std::min<int64_t>(most_parts(R), (chunks + LEAST - 1) / LEAST);
+    const int64_t chunks = (static_cast<int64_t>(b.key_bound) + CHUNK - 1) / CHUNK, most_splits = std::min<int64_t>(MOST_PARTS, (chunks + LEAST - 1) / LEAST);
     a.target = target;
     *grid = std::min(tiles + target, tiles * most_splits);
     if (*grid > INT32_MAX / 64) return fail(KT_ERR_SHAPE, "too many rows and heads in one call");
     if (most_splits <= 1) return KT_OK;
     const size_t slots = static_cast<size_t>(std::min<int64_t>(2 * target, *grid));
+    a.slots = static_cast<int32_t>(slots);
     void* ws = nullptr;
-    if (const int32_t status = workspace_counters(st, slots * R * (HD + 2) * sizeof(float) + 16, slots, &ws, &a.counters)) return status;
+    if (const int32_t status = workspace_counters(st, slots * R * (HD + 2) * sizeof(float) + 16, R == 16 ? slots : 0, &ws, &a.counters)) return status;
     ws = reinterpret_cast<void*>((reinterpret_cast<uintptr_t>(ws) + 15) & ~uintptr_t{15});  // (it begins at any dword)
     a.averages = static_cast<float*>(ws);
     a.stats = a.averages + slots * R * HD;
+    return KT_OK;
+}
+
+template <int HD, int R, int LEAST, int CHUNK>
+int32_t launch_merge(const Args& a, hipStream_t st) {
+    if (a.slots == 0) return KT_OK;
+    merge_kernel<HD, R, LEAST, CHUNK><<<dim3(static_cast<uint32_t>(a.slots), merge_shares(R)), 256, 0, st>>>(a);
+    KT_LAUNCHED("paged attention merge kernel");
     return KT_OK;
 }
 
@@ -1406,6 +1477,7 @@ int32_t launch_rows(Args a, hipStream_t st) {
     if (const int32_t ls = allow_lds<&attention_kernel<FMT, HD, R, NW, STEP>, lds>(lds)) return ls;
     attention_kernel<FMT, HD, R, NW, STEP><<<static_cast<uint32_t>(grid), 64 * NW, lds, st>>>(a);
     KT_LAUNCHED("paged attention kernel");
+    if constexpr (R > 16) return launch_merge<HD, R, NW, CHUNK>(a, st);
     return KT_OK;
 }
 
@@ -1417,7 +1489,7 @@ int32_t launch_tiles(Args a, hipStream_t st) {
     if (const int32_t ls = allow_lds<&tile_kernel<FMT, HD>, X::LDS>(X::LDS)) return ls;
     tile_kernel<FMT, HD><<<static_cast<uint32_t>(grid), X::THREADS, X::LDS, st>>>(a);
     KT_LAUNCHED("paged attention kernel");
-    return KT_OK;
+    return launch_merge<HD, X::R, X::LEAST, X::CH>(a, st);
 }
 
 template <int FMT, int HD>
@@ -1427,10 +1499,10 @@ int32_t launch_dims(const Args& a, hipStream_t st) {
         if (a.k_new) return launch_rows<FMT, HD, 16, 4, true>(a, st);
     }
     if constexpr (HD < 256 || FMT != KT_PAGED_F32) {
-        if (rows > 64) return launch_tiles<FMT, HD>(a, st);
+        if (rows > XTILE) return launch_tiles<FMT, HD>(a, st);
     }
     if constexpr (HD < 256) {
-        if (rows > 16) return launch_rows<FMT, HD, 32, 4, false>(a, st);
+        if (rows > 16 && XR32(FMT, HD)) return launch_rows<FMT, HD, 32, 4, false>(a, st);
     }
     return launch_rows<FMT, HD, 16, 4, false>(a, st);
 }
