@@ -30,7 +30,6 @@ namespace kt {
 namespace paged {
 
 typedef float f4 __attribute__((ext_vector_type(4)));
-typedef float f16v __attribute__((ext_vector_type(16)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
@@ -54,45 +53,35 @@ struct Format<KT_PAGED_F16> {
     static constexpr float UP = 6.0f;  // (so that their second parts are normal numbers down to 2^-20)
 };
 
-template <bool SMALL, typename A>
-__device__ __forceinline__ A product(bf16x8 a, bf16x8 b, A c) {
-    if constexpr (SMALL) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
-    else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
-}
-template <bool SMALL, typename A>
-__device__ __forceinline__ A product(half8 a, half8 b, A c) {
-    if constexpr (SMALL) return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
-    else return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
-}
+__device__ __forceinline__ f4 product(bf16x8 a, bf16x8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f4 product(half8 a, half8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 // Several sums at once, product by product: neighbours do not wait for each other.
-template <bool SMALL, int N, int KP, int QP, typename OP, typename A>
-__device__ __forceinline__ void products_of(const OP (&k)[N][KP], const OP (&q)[QP], A (&c)[N]) {
+template <int N, int KP, int QP, typename OP>
+__device__ __forceinline__ void products_of(const OP (&k)[N][KP], const OP (&q)[QP], f4 (&c)[N]) {
 #pragma unroll
     for (int w = QP - 1; w >= 0; --w)
 #pragma unroll
         for (int i = KP - 1; i >= 0; --i)
 #pragma unroll
             for (int t = 0; t < N; ++t)
-                if (w - i >= 0) c[t] = product<SMALL>(k[t][i], q[w - i], c[t]);
+                if (w - i >= 0) c[t] = product(k[t][i], q[w - i], c[t]);
 }
 // The sum of the parts' products down to 2^-17 of the largest, the small ones first.
-template <bool SMALL, int KP, int QP, typename OP, typename A>
-__device__ __forceinline__ A products(const OP (&k)[KP], const OP (&q)[QP], A c) {
+template <int KP, int QP, typename OP>
+__device__ __forceinline__ f4 products(const OP (&k)[KP], const OP (&q)[QP], f4 c) {
 #pragma unroll
     for (int w = QP - 1; w >= 0; --w)
 #pragma unroll
         for (int i = KP - 1; i >= 0; --i)
-            if (w - i >= 0) c = product<SMALL>(k[i], q[w - i], c);
+            if (w - i >= 0) c = product(k[i], q[w - i], c);
     return c;
 }
 
-// Wait states behind products whose sums the code after a branch reads (20 for 32x32x16, 12 for 16x16x32): the compiler
-// was seen to leave them out where a branch followed at once.
-template <bool SMALL>
+// Wait states behind products whose sums the code after a branch reads: the compiler was seen to leave them out where a
+// branch followed at once.
 __device__ __forceinline__ void settle() {
     __builtin_amdgcn_sched_barrier(0);
-    if constexpr (SMALL) asm volatile("s_nop 11");
-    else asm volatile("s_nop 11\n\ts_nop 7");
+    asm volatile("s_nop 11");
     __builtin_amdgcn_sched_barrier(0);
 }
 
@@ -149,23 +138,13 @@ __device__ __forceinline__ Swapped swap32(float v) {
     asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(s.a), "+v"(s.b));
     return s;
 }
-template <bool SMALL>
 __device__ __forceinline__ float column_max(float v) {
-    if constexpr (SMALL) {
-        const Swapped s = swap16(v);
-        v = fmaxf(s.a, s.b);
-    }
-    const Swapped s = swap32(v);
-    return fmaxf(s.a, s.b);
+    const Swapped near = swap16(v), far = swap32(fmaxf(near.a, near.b));
+    return fmaxf(far.a, far.b);
 }
-template <bool SMALL>
 __device__ __forceinline__ float column_sum(float v) {
-    if constexpr (SMALL) {
-        const Swapped s = swap16(v);
-        v = s.a + s.b;
-    }
-    const Swapped s = swap32(v);
-    return s.a + s.b;
+    const Swapped near = swap16(v), far = swap32(near.a + near.b);
+    return far.a + far.b;
 }
 
 // The maximum is a rounded product; at sizes where its rounding is a power of two and more, the
@@ -189,7 +168,7 @@ __device__ __forceinline__ float share_of(float m, float l, float mx) {
 
 // A chunk's scores x of one row (a lane's share of them) into weights; m and l: the row's running maximum and the sum of this
 // lane's weights; rescale: what the maximum's move does to the sums; is_hidden: whether the row does not see score i's token.
-template <int FMT, bool SMALL, bool masked, int E, typename HIDDEN, typename RESCALE>
+template <int FMT, bool masked, int E, typename HIDDEN, typename RESCALE>
 __device__ __forceinline__ void to_weights(float (&x)[E], float f, float& m, float& l, HIDDEN is_hidden, RESCALE rescale) {
     constexpr float UP = Format<FMT>::UP;
     auto hidden = [&](int i) { return masked && is_hidden(i); };
@@ -201,7 +180,7 @@ __device__ __forceinline__ void to_weights(float (&x)[E], float f, float& m, flo
     }
     most = rounded_score(most, f);
     if (__ballot(most - m > LAZY)) {
-        const float m_new = fmaxf(m, column_max<SMALL>(most));
+        const float m_new = fmaxf(m, column_max(most));
         const float alpha = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - m_new);
         l *= alpha;
         rescale(alpha);
@@ -630,22 +609,16 @@ __global__ void __launch_bounds__(256) merge_kernel(Args a) {
     }
 }
 
-// ---- the kernel ----------------------------------------------------------------------------------
-// R = 16 rows on 16x16x32, or R = 32 CT on 32x32x16.
-template <int FMT, int HD, int R>
+// ---- few rows, and few keys --------------------------------------------------------------------------
+// R = 16 rows a workgroup on 16x16x32.
+template <int FMT, int HD>
 struct Shape {
-    static constexpr bool SMALL = R == 16;
-    static constexpr int CT = SMALL ? 1 : R / 32;         // column tiles
-    static constexpr int LANES = SMALL ? 16 : 32;         // columns of a tile
-    static constexpr int KT = SMALL ? 2 : 1;              // key tiles of a chunk
-    static constexpr int QS = SMALL ? HD / 32 : HD / 16;  // steps of a score
-    static constexpr int E = SMALL ? 8 : 16;              // scores of a lane
-    static constexpr int VS = SMALL ? 1 : 2;              // steps of an output
-    static constexpr int DB = HD / LANES;                 // dim blocks of the output: consecutive dims of a lane
-    static constexpr int OE = SMALL ? 4 : 16;
-    static constexpr int KW = 8 * Format<FMT>::E / 4;     // dwords of a key tile's step
-    static constexpr int VW = (DB * Format<FMT>::E + 3) / 4;  // dwords of a token's dims (of one dim in 16 bits: half of one)
-    static constexpr bool QREG = SMALL && HD < 256;       // a row's operands stay in registers
+    static constexpr int R = 16, NW = 4, LEAST = NW;          // a part has a chunk for each wave
+    static constexpr int QS = HD / 32;                        // steps of a score
+    static constexpr int DB = HD / 16;                        // dim blocks of the output: consecutive dims of a lane
+    static constexpr int KW = 8 * Format<FMT>::E / 4;         // dwords of a key tile's step
+    static constexpr int VW = DB * Format<FMT>::E / 4;        // dwords of a token's dims
+    static constexpr bool QREG = HD < 256;                    // a row's operands stay in registers
 };
 
 // What a step's workgroups share: the rotation, and the new token as the cache holds it.
@@ -688,11 +661,12 @@ __device__ __forceinline__ uint32_t finite_only(uint32_t w) {
     return ((w & x) == x ? 0u : w & 0xFFFFu) | ((w >> 16 & x) == x ? 0u : w & 0xFFFF0000u);
 }
 
-template <int FMT, int HD, int R, int NW, bool STEP>
-__global__ void __launch_bounds__(64 * NW, HD == 256 || (FMT == KT_PAGED_F32 && HD == 128) ? 1 : 2) attention_kernel(Args a) {
+template <int FMT, int HD, bool STEP>
+__global__ void __launch_bounds__((64 * Shape<FMT, HD>::NW), (HD == 256 || (FMT == KT_PAGED_F32 && HD == 128) ? 1 : 2)) attention_kernel(Args a) {
     using F = Format<FMT>;
-    using X = Shape<FMT, HD, R>;
+    using X = Shape<FMT, HD>;
     using op = typename F::op;
+    constexpr int R = X::R, NW = X::NW;
     constexpr int LR = HD + 4;  // padded row of the waves' averages
     constexpr int QR = HD + 8;  // padded row of a query's parts
     extern __shared__ __attribute__((aligned(16))) float lds[];
@@ -705,10 +679,10 @@ __global__ void __launch_bounds__(64 * NW, HD == 256 || (FMT == KT_PAGED_F32 && 
     const BatchView& b = a.p.b;
     const int32_t tid = threadIdx.x, lane = tid & 63;
     const int32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int32_t col = lane % X::LANES, grp = lane / X::LANES;
+    const int32_t col = lane & 15, grp = lane >> 4;
     const int32_t H = a.p.num_heads, G = H / c.kv_heads;
     Part part;
-    if (!find_part<R, NW, CHUNK>(a, blockIdx.x, part)) return;
+    if (!find_part<R, X::LEAST, CHUNK>(a, blockIdx.x, part)) return;
     part.make_uniform();
     const int32_t g = part.head, row0 = part.tile * R, held = min(R, part.n * G - row0);  // rows of this tile
     // where row r of the tile lies in q and context
@@ -719,17 +693,17 @@ __global__ void __launch_bounds__(64 * NW, HD == 256 || (FMT == KT_PAGED_F32 && 
 
     // The rows' queries, sixteen lanes to a row (four dims each, or 64 apart; for the rotation those of the dims'
     // pairs, too).
-    constexpr int RW = R / (4 * NW) > 0 ? R / (4 * NW) : 1, DL = HD / 64 > 0 ? HD / 64 : 1, HALF = HD / 2;
+    constexpr int DL = HD / 64 > 0 ? HD / 64 : 1, HALF = HD / 2;
     const int32_t lr = lane >> 4, lc = lane & 15;
-    f4 qv[RW][DL], qo[STEP ? RW : 1][STEP ? DL : 1];
-#pragma unroll
-    for (int i = 0; i < RW; ++i) {
-        const float* src = a.p.q + row_at(min(4 * (wave + i * NW) + lr, held - 1));
+    static_assert(R == 4 * NW, "a wave brings four rows");
+    f4 qv[DL], qo[STEP ? DL : 1];
+    {
+        const float* src = a.p.q + row_at(min(4 * wave + lr, held - 1));
 #pragma unroll
         for (int u = 0; u < DL; ++u) {
             const int32_t d = (4 * lc + 64 * u) % HD;
-            qv[i][u] = *reinterpret_cast<const f4*>(src + d);
-            if constexpr (STEP) qo[i][u] = *reinterpret_cast<const f4*>(src + (d + HALF) % HD);
+            qv[u] = *reinterpret_cast<const f4*>(src + d);
+            if constexpr (STEP) qo[u] = *reinterpret_cast<const f4*>(src + (d + HALF) % HD);
         }
     }
     // a step: the new token's pairs, those of the key in threads 0 .. 127, of the value in the next 128
@@ -752,27 +726,20 @@ __global__ void __launch_bounds__(64 * NW, HD == 256 || (FMT == KT_PAGED_F32 && 
     const int64_t new_first = part.length;
     const PageReader<CHUNK> reader(c, b, part, keys.n_keys, F::E);
 
-    uint32_t kr[X::KT][X::QS][X::KW], vr[X::VS][8][X::VW];
+    uint32_t kr[2][X::QS][X::KW], vr[8][X::VW];
     auto load_keys = [&](const Where<CHUNK>& w) {
 #pragma unroll
-        for (int t = 0; t < X::KT; ++t) {
-            const size_t base = X::SMALL ? w.base[t] : col < 16 ? w.base[0] : w.base[1];
-            const uint8_t* p = c.keys + base + ((col & 15) * HD + 8 * grp) * F::E;
+        for (int t = 0; t < 2; ++t) {
+            const uint8_t* p = c.keys + w.base[t] + (col * HD + 8 * grp) * F::E;
 #pragma unroll
-            for (int s = 0; s < X::QS; ++s) load_words(p + (X::SMALL ? 32 : 16) * s * F::E, kr[t][s]);
+            for (int s = 0; s < X::QS; ++s) load_words(p + 32 * s * F::E, kr[t][s]);
         }
     };
-    // the token of a lane's value (or weight) e of step s
-    auto token_of = [&](int s, int e) { return X::SMALL ? 16 * (e >> 2) + 4 * grp + (e & 3) : 16 * s + 8 * (e >> 2) + 4 * grp + (e & 3); };
+    // the token of a lane's value (or weight) e
+    auto token_of = [&](int e) { return 16 * (e >> 2) + 4 * grp + (e & 3); };
     auto load_values = [&](const Where<CHUNK>& w) {
 #pragma unroll
-        for (int s = 0; s < X::VS; ++s)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const uint8_t* p = c.values + w.base[X::SMALL ? e >> 2 : s] + ((token_of(s, e) & 15) * HD + col * X::DB) * F::E;
-                if constexpr (X::DB * F::E == 2) vr[s][e][0] = *reinterpret_cast<const uint16_t*>(p);
-                else load_words(p, vr[s][e]);
-            }
+        for (int e = 0; e < 8; ++e) load_words(c.values + w.base[e >> 2] + ((token_of(e) & 15) * HD + col * X::DB) * F::E, vr[e]);
     };
     // a step's token in its chunk's registers, whatever the loads saw
     const bool holder = STEP && part.split == splits - 1;
@@ -780,13 +747,13 @@ __global__ void __launch_bounds__(64 * NW, HD == 256 || (FMT == KT_PAGED_F32 && 
         if constexpr (STEP) {
             const int32_t at = part.length & (CHUNK - 1);
 #pragma unroll
-            for (int t = 0; t < X::KT; ++t)
+            for (int t = 0; t < 2; ++t)
                 if (16 * t + col == at)
 #pragma unroll
                     for (int s = 0; s < X::QS; ++s) load_words(sh.key + (32 * s + 8 * grp) * F::E, kr[t][s]);
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-                if (token_of(0, e) == at) load_words(sh.value + col * X::DB * F::E, vr[0][e]);
+                if (token_of(e) == at) load_words(sh.value + col * X::DB * F::E, vr[e]);
         }
     };
     int32_t ch = c0 + wave;
@@ -809,10 +776,8 @@ __global__ void __launch_bounds__(64 * NW, HD == 256 || (FMT == KT_PAGED_F32 && 
     // the rows' parts through LDS
     typedef typename std::conditional<FMT == KT_PAGED_F16, _Float16, __bf16>::type element;
     element* qs = reinterpret_cast<element*>(lds);  // [QP][R][QR]
-#pragma unroll
-    for (int i = 0; i < RW; ++i) {
-        if (4 * (wave + i * NW) >= held) break;
-        const int32_t r = 4 * (wave + i * NW) + lr;
+    if (4 * wave < held) {
+        const int32_t r = 4 * wave + lr;
         uint32_t top = 0;
 #pragma unroll
         for (int u = 0; u < DL; ++u) {
@@ -823,12 +788,12 @@ __global__ void __launch_bounds__(64 * NW, HD == 256 || (FMT == KT_PAGED_F32 && 
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     float y1, y2;
-                    rope_apply(upper ? qo[i][u][e] : qv[i][u][e], upper ? qv[i][u][e] : qo[i][u][e], cf[e], sf[e], y1, y2);
-                    qv[i][u][e] = upper ? y2 : y1;
+                    rope_apply(upper ? qo[u][e] : qv[u][e], upper ? qv[u][e] : qo[u][e], cf[e], sf[e], y1, y2);
+                    qv[u][e] = upper ? y2 : y1;
                 }
             }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) top = max(top, magnitude(qv[i][u][e]));
+            for (int e = 0; e < 4; ++e) top = max(top, magnitude(qv[u][e]));
         }
         int32_t up = 0;
         if constexpr (FMT == KT_PAGED_F16) {
@@ -846,7 +811,7 @@ __global__ void __launch_bounds__(64 * NW, HD == 256 || (FMT == KT_PAGED_F32 && 
                 if (4 * lc + 64 * u >= HD) continue;
                 float rest[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) rest[e] = FMT == KT_PAGED_F16 ? ldexpf(qv[i][u][e], up) : qv[i][u][e];
+                for (int e = 0; e < 4; ++e) rest[e] = FMT == KT_PAGED_F16 ? ldexpf(qv[u][e], up) : qv[u][e];
 #pragma unroll
                 for (int w = 0; w < F::QP; ++w) {
                     element part4[4];
@@ -882,51 +847,35 @@ __global__ void __launch_bounds__(64 * NW, HD == 256 || (FMT == KT_PAGED_F32 && 
     }
     __syncthreads();
     op qreg[X::QREG ? X::QS : 1][F::QP];
-    const element* qrow[X::CT];
-    float fr[X::CT];
-    int32_t token[X::CT];  // of the column's row, among the sequence's new ones
+    const int32_t own_row = min(col, held - 1), token = (row0 + own_row) / G;  // (columns past the rows repeat the last)
+    const float fr = fr_s[own_row];
+    auto query = [&](int s, op (&q)[F::QP]) {
 #pragma unroll
-    for (int ct = 0; ct < X::CT; ++ct) {
-        const int32_t r = min(32 * ct + col, held - 1);  // (columns past the rows repeat the last)
-        fr[ct] = fr_s[r];
-        token[ct] = (row0 + r) / G;
-        qrow[ct] = qs + r * QR + 8 * grp;
-    }
-    auto query = [&](int ct, int s, op (&q)[F::QP]) {  // step s of column tile ct's operands
-#pragma unroll
-        for (int w = 0; w < F::QP; ++w) q[w] = *reinterpret_cast<const op*>(qrow[ct] + w * R * QR + (X::SMALL ? 32 : 16) * s);
+        for (int w = 0; w < F::QP; ++w) q[w] = *reinterpret_cast<const op*>(qs + (w * R + own_row) * QR + 8 * grp + 32 * s);
     };
     if constexpr (X::QREG) {
 #pragma unroll
-        for (int s = 0; s < X::QS; ++s) query(0, s, qreg[s]);
+        for (int s = 0; s < X::QS; ++s) query(s, qreg[s]);
     }
     if constexpr (STEP) {
         if (holder && ch < c1 && ch == part.length / CHUNK) patch();
     }
 
-    typedef typename std::conditional<X::SMALL, f4, f16v>::type acc_t;
-    acc_t o[X::CT][X::DB];
-    float m[X::CT], l[X::CT];
+    f4 o[X::DB];
+    float m = -INFINITY, l = 0.0f;
 #pragma unroll
-    for (int ct = 0; ct < X::CT; ++ct) {
-        m[ct] = -INFINITY;
-        l[ct] = 0.0f;
-#pragma unroll
-        for (int db = 0; db < X::DB; ++db)
-#pragma unroll
-            for (int e = 0; e < X::OE; ++e) o[ct][db][e] = 0.0f;
-    }
-    // the operands of dim block db, step s: the tokens' elements of the lane's dim
-    auto value_operand = [&](int s, int db, op (&v)[F::KP]) {
+    for (int db = 0; db < X::DB; ++db) o[db] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    // the operands of dim block db: the tokens' elements of the lane's dim
+    auto value_operand = [&](int db, op (&v)[F::KP]) {
         if constexpr (FMT == KT_PAGED_F32) {
             uint32_t w[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) w[e] = vr[s][e][db];
+            for (int e = 0; e < 8; ++e) w[e] = vr[e][db];
             to_operands<FMT>(w, v);
         } else {
             uint32_t w[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = __builtin_amdgcn_perm(vr[s][2 * i + 1][db / 2], vr[s][2 * i][db / 2], db % 2 ? 0x07060302u : 0x05040100u);
+            for (int i = 0; i < 4; ++i) w[i] = __builtin_amdgcn_perm(vr[2 * i + 1][db / 2], vr[2 * i][db / 2], db % 2 ? 0x07060302u : 0x05040100u);
             to_operands<FMT>(w, v);
         }
     };
@@ -934,29 +883,20 @@ __global__ void __launch_bounds__(64 * NW, HD == 256 || (FMT == KT_PAGED_F32 && 
     auto attend_chunk = [&](auto masked_form) {
         constexpr bool masked = decltype(masked_form)::value;
         const Where<CHUNK> now = here;
-        acc_t sc[X::CT][X::KT];
-#pragma unroll
-        for (int ct = 0; ct < X::CT; ++ct)
-#pragma unroll
-            for (int t = 0; t < X::KT; ++t)
-#pragma unroll
-                for (int e = 0; e < X::OE; ++e) sc[ct][t][e] = 0.0f;
+        f4 sc[2] = {f4{0.0f, 0.0f, 0.0f, 0.0f}, f4{0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
         for (int s = 0; s < X::QS; ++s) {
-            op k[X::KT][F::KP];
+            op k[2][F::KP];
 #pragma unroll
-            for (int t = 0; t < X::KT; ++t) to_operands<FMT>(kr[t][s], k[t]);
+            for (int t = 0; t < 2; ++t) to_operands<FMT>(kr[t][s], k[t]);
+            if constexpr (X::QREG) {
 #pragma unroll
-            for (int ct = 0; ct < X::CT; ++ct) {
-                if constexpr (X::QREG) {
+                for (int t = 0; t < 2; ++t) sc[t] = products(k[t], qreg[s], sc[t]);
+            } else {
+                op q[F::QP];
+                query(s, q);
 #pragma unroll
-                    for (int t = 0; t < X::KT; ++t) sc[ct][t] = products<X::SMALL>(k[t], qreg[s], sc[ct][t]);
-                } else {
-                    op q[F::QP];
-                    query(ct, s, q);
-#pragma unroll
-                    for (int t = 0; t < X::KT; ++t) sc[ct][t] = products<X::SMALL>(k[t], q, sc[ct][t]);
-                }
+                for (int t = 0; t < 2; ++t) sc[t] = products(k[t], q, sc[t]);
             }
         }
         __builtin_amdgcn_sched_barrier(0);  // (loads ahead of their registers' last use would cost others)
@@ -965,85 +905,64 @@ __global__ void __launch_bounds__(64 * NW, HD == 256 || (FMT == KT_PAGED_F32 && 
         load_keys(here);
         pages = reader.pages_of(min(ch + 2 * NW, c1 - 1));
         __builtin_amdgcn_sched_barrier(0);
-        op p[X::CT][X::VS][F::QP];
-        float x[X::CT][X::E];
-        uint32_t vis[X::CT];
+        op p[F::QP];
+        float x[8];
+        uint32_t vis = 0;
+        if constexpr (masked) vis = seen_bits(b, part.first, token, new_first, ch * CHUNK, now.there[0]);
 #pragma unroll
-        for (int ct = 0; ct < X::CT; ++ct) {
-            if constexpr (masked) vis[ct] = seen_bits(b, part.first, token[ct], new_first, ch * CHUNK, now.there[0]);
+        for (int i = 0; i < 8; ++i) x[i] = sc[i >> 2][i & 3];
+        to_weights<FMT, masked>(x, fr, m, l, [&](int i) { return !(vis >> token_of(i) & 1); }, [&](float alpha) {
 #pragma unroll
-            for (int i = 0; i < X::E; ++i) x[ct][i] = X::SMALL ? sc[ct][X::SMALL ? i >> 2 : 0][X::SMALL ? i & 3 : i] : sc[ct][0][i];
-            to_weights<FMT, X::SMALL, masked>(x[ct], fr[ct], m[ct], l[ct], [&](int i) { return !(vis[ct] >> token_of(i >> 3, i & 7) & 1); }, [&](float alpha) {
-#pragma unroll
-                for (int db = 0; db < X::DB; ++db) o[ct][db] *= alpha;
-            });
-#pragma unroll
-            for (int s = 0; s < X::VS; ++s) {
-                float w[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) w[e] = x[ct][8 * s + e];
-                split_weights(w, p[ct][s]);
-            }
-        }
+            for (int db = 0; db < X::DB; ++db) o[db] *= alpha;
+        });
+        split_weights(x, p);
         if constexpr (masked) {
             // values of tokens that are not there count for nothing; what is not finite goes to the rows that see it alone
             bool odd = false;
 #pragma unroll
-            for (int s = 0; s < X::VS; ++s)
+            for (int e = 0; e < 8; ++e)
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-#pragma unroll
-                    for (int w = 0; w < X::VW; ++w) {
-                        if (!(now.there[0] >> token_of(s, e) & 1)) vr[s][e][w] = 0;
-                        odd |= any_not_finite<FMT>(vr[s][e][w]);
-                    }
+                for (int w = 0; w < X::VW; ++w) {
+                    if (!(now.there[0] >> token_of(e) & 1)) vr[e][w] = 0;
+                    odd |= any_not_finite<FMT>(vr[e][w]);
+                }
             if (__ballot(odd)) {
                 const bool own = STEP && holder && ch == part.length / CHUNK;  // (the new token is in LDS)
                 for (int32_t tok = 0; tok < CHUNK; ++tok) {
                     if (!(now.there[0] >> tok & 1)) continue;
-                    const int32_t from = X::SMALL ? tok >> 2 & 3 : tok >> 2 & 1, i = X::SMALL ? 4 * (tok >> 4) + (tok & 3) : 4 * (tok >> 3) + (tok & 3);
+                    const int32_t from = tok >> 2 & 3, i = 4 * (tok >> 4) + (tok & 3);
                     const uint8_t* row = c.values + (tok < 16 ? now.base[0] : now.base[1]) + (tok & 15) * HD * F::E;
                     if constexpr (STEP) {
                         if (own && tok == (part.length & (CHUNK - 1))) row = sh.value;
                     }
-#pragma unroll
-                    for (int ct = 0; ct < X::CT; ++ct) {
-                        float weight = 0.0f;
-#pragma unroll
-                        for (int e = 0; e < X::E; ++e)
-                            if (e == i) weight = x[ct][e];
-                        weight = __shfl(weight, from * X::LANES + col);
-                        if (!(vis[ct] >> tok & 1)) continue;
-#pragma unroll
-                        for (int e = 0; e < X::OE; ++e) {
-                            const int32_t d = (X::SMALL ? 4 * grp + e : 8 * (e >> 2) + 4 * grp + (e & 3)) * X::DB;
-#pragma unroll
-                            for (int db = 0; db < X::DB; ++db) {
-                                const float v = load_element<FMT>(row, d + db);
-                                if (!(fabsf(v) < INFINITY)) o[ct][db][e] += weight * v;
-                                __builtin_amdgcn_sched_barrier(0);  // (rare: one load at a time, few registers)
-                            }
-                        }
-                    }
-                }
-#pragma unroll
-                for (int s = 0; s < X::VS; ++s)
+                    float weight = 0.0f;
 #pragma unroll
                     for (int e = 0; e < 8; ++e)
+                        if (e == i) weight = x[e];
+                    weight = __shfl(weight, from * 16 + col);
+                    if (!(vis >> tok & 1)) continue;
 #pragma unroll
-                        for (int w = 0; w < X::VW; ++w) vr[s][e][w] = finite_only<FMT>(vr[s][e][w]);
+                    for (int e = 0; e < 4; ++e)
+#pragma unroll
+                        for (int db = 0; db < X::DB; ++db) {
+                            const float v = load_element<FMT>(row, (4 * grp + e) * X::DB + db);
+                            if (!(fabsf(v) < INFINITY)) o[db][e] += weight * v;
+                            __builtin_amdgcn_sched_barrier(0);  // (rare: one load at a time, few registers)
+                        }
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+#pragma unroll
+                    for (int w = 0; w < X::VW; ++w) vr[e][w] = finite_only<FMT>(vr[e][w]);
             }
         }
 #pragma unroll
-        for (int db = 0; db < X::DB; ++db)
-#pragma unroll
-            for (int s = 0; s < X::VS; ++s) {
-                op v[F::KP];
-                value_operand(s, db, v);
-#pragma unroll
-                for (int ct = 0; ct < X::CT; ++ct) o[ct][db] = products<X::SMALL>(v, p[ct][s], o[ct][db]);
-            }
-        settle<X::SMALL>();
+        for (int db = 0; db < X::DB; ++db) {
+            op v[F::KP];
+            value_operand(db, v);
+            o[db] = products(v, p, o[db]);
+        }
+        settle();
         load_values(here);
         if constexpr (STEP) {
             if (holder && next == part.length / CHUNK) patch();
@@ -1058,21 +977,17 @@ __global__ void __launch_bounds__(64 * NW, HD == 256 || (FMT == KT_PAGED_F32 && 
     const int32_t used = min(NW, c1 - c0);  // waves with keys
     __syncthreads();                        // (the queries' parts are read)
     if (wave < used) {
+        l = column_sum(l);
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        if (col < held) {
+            float* row = avg + (wave * R + col) * LR;
 #pragma unroll
-        for (int ct = 0; ct < X::CT; ++ct) {
-            l[ct] = column_sum<X::SMALL>(l[ct]);
-            const float inv = l[ct] == 0.0f ? 0.0f : 1.0f / l[ct];
-            if (32 * ct + col >= held) continue;
-            float* row = avg + (wave * R + 32 * ct + col) * LR;
+            for (int e = 0; e < 4; ++e)
 #pragma unroll
-            for (int e = 0; e < X::OE; ++e) {
-                const int32_t d = (X::SMALL ? 4 * grp + e : 8 * (e >> 2) + 4 * grp + (e & 3)) * X::DB;
-#pragma unroll
-                for (int db = 0; db < X::DB; ++db) row[d + db] = o[ct][db][e] * inv;
-            }
+                for (int db = 0; db < X::DB; ++db) row[(4 * grp + e) * X::DB + db] = o[db][e] * inv;
             if (grp == 0) {
-                ms[wave * R + 32 * ct + col] = m[ct];
-                ls[wave * R + 32 * ct + col] = l[ct];
+                ms[wave * R + col] = m;
+                ls[wave * R + col] = l;
             }
         }
     }
@@ -1102,27 +1017,20 @@ __global__ void __launch_bounds__(64 * NW, HD == 256 || (FMT == KT_PAGED_F32 && 
         }
     }
     if (splits == 1) return;
-    if constexpr (R == 16) meet<HD, R, NW>(a, part, splits, held, lds, row_at);
+    meet<HD, R, NW>(a, part, splits, held, lds, row_at);
 }
 
 // ---- many rows ---------------------------------------------------------------------------------------
-// 128 rows a workgroup, 16 a wave, on 16x16x32. The workgroup's threads load a chunk of keys ahead and lay it out in LDS,
-// where all eight waves read it: the keys as rows, the values as dims with their tokens in the order of the operands; fp32
-// ones split into their parts once for all waves. Queries stay in registers.
-#ifndef XNW
-#define XNW(F, H) ((F && H <= 64) ? 4 : 8)
-#define XMW(F, H) ((F && H <= 64) ? 3 : 2)
-#define XCH(F, H) (F == 0 || H != 128 ? 32 : 64)
-#define XT(F, H) 1
-#define XD 4
-#define XTILE 64
-#define XR32(F, H) 1
-#endif
-template <int FMT, int HD>
+// 16 rows a wave on 16x16x32. The workgroup's threads load a chunk of keys ahead and lay it out in LDS, where all its waves
+// read it: the keys as rows, the values as dims with their tokens in the order of the operands; fp32 ones split into their
+// parts once for all waves. Queries stay in registers.
+template <int FMT, int HD, int WAVES>
 struct Tile {
-    static constexpr int NW = XNW(FMT, HD), MW = XMW(FMT, HD), R = 16 * NW, THREADS = 64 * NW;
+    static constexpr int NW = WAVES, R = 16 * NW, THREADS = 64 * NW;
+    // waves a SIMD that leave a wave the registers it needs (of 256 dims with two: 352 bytes and more in scratch memory)
+    static constexpr int MW = NW == 8 ? 2 : HD == 256 ? 1 : HD <= 64 && FMT != KT_PAGED_F32 ? 3 : 2;
     static constexpr int KP = Format<FMT>::KP, QP = Format<FMT>::QP, E = Format<FMT>::E;
-    static constexpr int CH = XCH(FMT, HD), SETS = CH / 32;
+    static constexpr int CH = FMT == KT_PAGED_F32 || HD != 128 ? 32 : 64, SETS = CH / 32;
     static constexpr int QS = HD / 32, DB = HD / 16;
     static constexpr int KR = HD + 8, VR = CH + 8;  // padded rows: of a key, of a dim (2-byte elements)
     static constexpr int KSIZE = CH * KR, VSIZE = HD * VR, SIZE = KP * (KSIZE + VSIZE);
@@ -1132,13 +1040,14 @@ struct Tile {
     static constexpr int VN = (CH / 4 * (HD / 4) + THREADS - 1) / THREADS;  // 4 tokens x 4 dims
     static constexpr size_t LDS = size_t{2} * SIZE * BUFFERS;
     static constexpr int LEAST = 128 / CH;
+    static constexpr int TARGET = NW == 4 && HD < 256 ? 2 : 1;  // workgroups a CU among which the launch's chunks are shared out
     static constexpr int VGROUP = FMT == KT_PAGED_F32 ? 2 : 4;
 };
 
-template <int FMT, int HD>
-__global__ void __launch_bounds__((Tile<FMT, HD>::THREADS), (Tile<FMT, HD>::MW)) tile_kernel(Args a) {
+template <int FMT, int HD, int WAVES>
+__global__ void __launch_bounds__((Tile<FMT, HD, WAVES>::THREADS), (Tile<FMT, HD, WAVES>::MW)) tile_kernel(Args a) {
     using F = Format<FMT>;
-    using X = Tile<FMT, HD>;
+    using X = Tile<FMT, HD, WAVES>;
     using op = typename F::op;
     constexpr int R = X::R, E = F::E, CH = X::CH;
     typedef typename std::conditional<FMT == KT_PAGED_F16, _Float16, __bf16>::type element;
@@ -1297,7 +1206,7 @@ __global__ void __launch_bounds__((Tile<FMT, HD>::THREADS), (Tile<FMT, HD>::MW))
             for (int s = 0; s < X::QS; ++s)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) top = max(top, magnitude(x[s][e]));
-            const float most = column_max<true>(__builtin_bit_cast(float, min(top, 0x7F7FFFFFu)));
+            const float most = column_max(__builtin_bit_cast(float, min(top, 0x7F7FFFFFu)));
             const int32_t up = 13 - max(static_cast<int32_t>(magnitude(most) >> 23) - 127, -100);
 #pragma unroll
             for (int s = 0; s < X::QS; ++s)
@@ -1347,7 +1256,7 @@ __global__ void __launch_bounds__((Tile<FMT, HD>::THREADS), (Tile<FMT, HD>::MW))
         for (int s = 0; s < X::QS; ++s) {
             if (s + 1 < X::QS) load_keys(s + 1);
             __builtin_amdgcn_sched_barrier(0);
-            products_of<true>(k[s & 1], q[s], sc);
+            products_of(k[s & 1], q[s], sc);
             __builtin_amdgcn_sched_barrier(0);
         }
         op v[2][VG][F::KP];
@@ -1367,7 +1276,7 @@ __global__ void __launch_bounds__((Tile<FMT, HD>::THREADS), (Tile<FMT, HD>::MW))
         if constexpr (masked)
 #pragma unroll
             for (int h = 0; h < X::SETS; ++h) vis[h] = seen_bits(b, part.first, token, part.length, ch * CH + 32 * h, where.there[h]);
-        to_weights<FMT, true, masked>(x, f, m, l, [&](int i) { return !(vis[i >> 3] >> token_of(i & 7) & 1); }, [&](float alpha) {
+        to_weights<FMT, masked>(x, f, m, l, [&](int i) { return !(vis[i >> 3] >> token_of(i & 7) & 1); }, [&](float alpha) {
 #pragma unroll
             for (int db = 0; db < X::DB; ++db) o[db / VG][db % VG] *= alpha;
         });
@@ -1407,10 +1316,10 @@ __global__ void __launch_bounds__((Tile<FMT, HD>::THREADS), (Tile<FMT, HD>::MW))
             }
             if (i + 1 < X::SETS * GROUPS) load_values(i + 1);
             __builtin_amdgcn_sched_barrier(0);
-            products_of<true>(v[i & 1], p, o[i % GROUPS]);
+            products_of(v[i & 1], p, o[i % GROUPS]);
             __builtin_amdgcn_sched_barrier(0);
         }
-        settle<true>();
+        settle();
     };
     for (int32_t ch = c0; ch < c1; ++ch) {
         const Where<CH> now = next;
@@ -1428,7 +1337,7 @@ __global__ void __launch_bounds__((Tile<FMT, HD>::THREADS), (Tile<FMT, HD>::MW))
         if (ch + 1 < c1) store_chunk(ch + 1, next);
     }
 
-    l = column_sum<true>(l);
+    l = column_sum(l);
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     if (16 * wave + col < held) {
         const size_t at_slot = static_cast<size_t>(part.slot + part.split) * R + r;
@@ -1469,42 +1378,57 @@ int32_t launch_merge(const Args& a, hipStream_t st) {
     return KT_OK;
 }
 
-template <int FMT, int HD, int R, int NW, bool STEP>
+template <int FMT, int HD, bool STEP>
 int32_t launch_rows(Args a, hipStream_t st) {
+    using X = Shape<FMT, HD>;
     int64_t grid = 0;
-    if (const int32_t status = prepare<HD, R, NW, CHUNK>(a, XD * cu_count(), &grid, st)) return status;
-    constexpr size_t lds = std::max(std::max(sizeof(float) * NW * R * (HD + 6), size_t{2} * Format<FMT>::QP * R * (HD + 8)), merge_lds(R, NW));
-    if (const int32_t ls = allow_lds<&attention_kernel<FMT, HD, R, NW, STEP>, lds>(lds)) return ls;
-    attention_kernel<FMT, HD, R, NW, STEP><<<static_cast<uint32_t>(grid), 64 * NW, lds, st>>>(a);
+    if (const int32_t status = prepare<HD, X::R, X::LEAST, CHUNK>(a, 4 * cu_count(), &grid, st)) return status;
+    constexpr size_t lds = std::max(std::max(sizeof(float) * X::NW * X::R * (HD + 6), size_t{2} * Format<FMT>::QP * X::R * (HD + 8)), merge_lds(X::R, X::NW));
+    if (const int32_t ls = allow_lds<&attention_kernel<FMT, HD, STEP>, lds>(lds)) return ls;
+    attention_kernel<FMT, HD, STEP><<<static_cast<uint32_t>(grid), 64 * X::NW, lds, st>>>(a);
     KT_LAUNCHED("paged attention kernel");
-    if constexpr (R > 16) return launch_merge<HD, R, NW, CHUNK>(a, st);
     return KT_OK;
 }
 
-template <int FMT, int HD>
+template <int FMT, int HD, int WAVES>
 int32_t launch_tiles(Args a, hipStream_t st) {
-    using X = Tile<FMT, HD>;
+    using X = Tile<FMT, HD, WAVES>;
     int64_t grid = 0;
-    if (const int32_t status = prepare<HD, X::R, X::LEAST, X::CH>(a, XT(FMT, HD) * cu_count(), &grid, st)) return status;
-    if (const int32_t ls = allow_lds<&tile_kernel<FMT, HD>, X::LDS>(X::LDS)) return ls;
-    tile_kernel<FMT, HD><<<static_cast<uint32_t>(grid), X::THREADS, X::LDS, st>>>(a);
+    if (const int32_t status = prepare<HD, X::R, X::LEAST, X::CH>(a, X::TARGET * cu_count(), &grid, st)) return status;
+    if (const int32_t ls = allow_lds<&tile_kernel<FMT, HD, WAVES>, X::LDS>(X::LDS)) return ls;
+    tile_kernel<FMT, HD, WAVES><<<static_cast<uint32_t>(grid), X::THREADS, X::LDS, st>>>(a);
     KT_LAUNCHED("paged attention kernel");
-    return launch_merge<HD, X::R, X::LEAST, X::CH>(a, st);
+    if (a.slots == 0) return KT_OK;
+    merge_kernel<HD, X::R, X::LEAST, X::CH><<<dim3(static_cast<uint32_t>(a.slots), merge_shares(X::R)), 256, 0, st>>>(a);
+    KT_LAUNCHED("paged attention merge kernel");
+    return KT_OK;
 }
 
+// Which kernel (us here: head dims of 128 unless said, 32 heads on 8 kv heads, one sequence unless said; the kernel taken first):
+//   up to 16 rows of a kv head: tiles of 16, keys straight into registers. A tree of 4 tokens has no use for more.
+//   up to 128 keys: the same for any number of rows, as its waves have a chunk each: no parts to merge, and four
+//     times the workgroups. A prompt of 128: fp16 11.0 against 12.9, fp32 12.6 against 21.7, fp16 at 64 dims 6.7 against 8.6
+//     (fp32 at 256 dims, which spills: 54.8 against 35.9, so not there).
+//   up to 64 rows: tiles of 64, so that no wave is idle, two workgroups a CU: 16 sequences with trees of 15 after 2000 tokens 41
+//     against 54 with tiles of 128 (fp32 76 against 95); one tree of 15 after 4000 30 and 30.
+//   up to 64 dims in 16 bits: tiles of 64 for any number of rows, of which three workgroups share a CU (a prompt of 2048: 74.8).
+//   else: tiles of 128, as the chunk that eight waves share is half the loads and LDS writes a row: a prompt of 2048 102 (fp16),
+//     115 (bf16), 210 (fp32); a tree of 60 in fp32 53 against 63.
+//   256 dims: tiles of 64 whose waves have a SIMD's registers each: a prompt of 512 44 against 50 with tiles of
+//     128 (bf16 48 against 69, fp32 120 against 169).
 template <int FMT, int HD>
 int32_t launch_dims(const Args& a, hipStream_t st) {
     const int64_t rows = static_cast<int64_t>(a.p.b.most_rows) * (a.p.num_heads / a.p.c.kv_heads);
     if constexpr (HD < 256) {
-        if (a.k_new) return launch_rows<FMT, HD, 16, 4, true>(a, st);
+        if (a.k_new) return launch_rows<FMT, HD, true>(a, st);
     }
-    if constexpr (HD < 256 || FMT != KT_PAGED_F32) {
-        if (rows > XTILE) return launch_tiles<FMT, HD>(a, st);
+    if (rows <= 16 || (a.p.b.key_bound <= 128 && (HD < 256 || FMT != KT_PAGED_F32))) return launch_rows<FMT, HD, false>(a, st);
+    if constexpr (HD == 256 || (HD <= 64 && FMT != KT_PAGED_F32)) {
+        return launch_tiles<FMT, HD, 4>(a, st);
+    } else {
+        if (rows <= 64) return launch_tiles<FMT, HD, 4>(a, st);
+        return launch_tiles<FMT, HD, 8>(a, st);
     }
-    if constexpr (HD < 256) {
-        if (rows > 16 && XR32(FMT, HD)) return launch_rows<FMT, HD, 32, 4, false>(a, st);
-    }
-    return launch_rows<FMT, HD, 16, 4, false>(a, st);
 }
 
 template <int FMT>
