@@ -9,7 +9,8 @@ file format (``SafeTensorsFile``, ``save_quantized``, ``load_quantized``) and th
 device-resident decoder around the projections (``Transformer``, ``KVCache``,
 ``InferenceBuffers``, ``RoPEScaling``) and the fused projection + cross-entropy with a
 quantized head (``fused_cross_entropy_loss``). Beside the reference's API: a KV cache held in 8 bits
-(``QuantizedKVCache``) and penalties, biases and masks on logits (``LogitsControls``).
+(``QuantizedKVCache``), one in pages that several sequences share, with trees of drafted tokens (``PagedKVCache``,
+``Transformer.generate_batch``), and penalties, biases and masks on logits (``LogitsControls``).
 """
 from ._lib import IllegalArgumentException, IllegalStateException, LibraryMissingError, LIBRARY_PATH
 from .device import DeviceBuffer, Stream, synchronize, device_count, release_scratch
@@ -17,8 +18,9 @@ from .quantization import Quantization, QuantizedTensor
 from .matmul import MatMul, DeviceTensor
 from .linear import QuantizedLinear, projection, forward_into_group
 from .safetensors import SafeTensorsFile, save_entries, save_quantized, load_quantized
-from .transformer import Transformer, KVCache, InferenceBuffers, RoPEScaling
+from .transformer import Transformer, KVCache, InferenceBuffers, BatchBuffers, RoPEScaling
 from .kv8 import QuantizedKVCache
+from .paged import PagedKVCache, PagedBatch, TextDraft
 from .logits import LogitsControls, process_logits
 from .loss import fused_cross_entropy_loss, FusedLoss, IGNORE_INDEX
 
@@ -46,8 +48,12 @@ __all__ = [
     "Transformer",
     "KVCache",
     "InferenceBuffers",
+    "BatchBuffers",
     "RoPEScaling",
     "QuantizedKVCache",
+    "PagedKVCache",
+    "PagedBatch",
+    "TextDraft",
     "LogitsControls",
     "process_logits",
     "fused_cross_entropy_loss",

@@ -219,6 +219,7 @@ SIGNATURES = {
     "kt_rmsnorm_swiglu_gate": [_P, _P, _F, _P, _I, ctypes.POINTER(_QWeight), ctypes.POINTER(_QWeight), _P, _P, _P, _P, _P],
     "kt_qmatmul_chain": [ctypes.POINTER(QMatmulStep), _I, _P],
     "kt_argmax": [_P, _I, _P, _P],
+    "kt_argmax_rows": [_P, _I, _I, _P, _P, _P, _I, _P],
     "kt_argmax_advance": [_P, _I, _P, _P, _P, _I, _P],
     "kt_process_logits": [_P, _I, _I, ctypes.c_int64, ctypes.POINTER(LogitsControls), _P, ctypes.c_int64, _P],
     "kt_position_add": [_P, _I, _P],

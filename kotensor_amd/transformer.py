@@ -23,6 +23,7 @@ from . import _lib
 from .device import DeviceBuffer, Stream, default_stream
 from .kv8 import QuantizedKVCache
 from .logits import LogitsControls
+from .paged import PagedBatch, PagedKVCache
 from .quantization import Quantization, QuantizedTensor
 
 TILE_M = 32  # MatMul.TILE_M (MatMul.kt:16), the reference's prefill chunk
@@ -223,6 +224,30 @@ class InferenceBuffers(_Rows):
     @property
     def size_in_bytes(self) -> int:
         return (6 * self.dimension + 2 * self.kv_dimension + 2 * self.hidden_dimension + self.vocabulary_size) * 4
+
+
+class BatchBuffers(_Rows):
+    """The activations of up to ``rows`` tokens of several sequences in a call on a ``PagedKVCache``, their logits, the trees
+    they may form, and what is chosen after them. No counterpart in the reference."""
+
+    def __init__(self, dimension: int, hidden_dimension: int, vocabulary_size: int, sequences: int, max_sequence_length: int, rows: int,
+                 kv_dimension: int):
+        if min(dimension, hidden_dimension, vocabulary_size, sequences, max_sequence_length, rows, kv_dimension) <= 0:
+            raise _lib.IllegalArgumentException("BatchBuffers dimensions must be positive")
+        if rows < sequences:
+            raise _lib.IllegalArgumentException(f"BatchBuffers of {rows} rows for {sequences} sequences: at least one each")
+        super().__init__(rows, dimension, hidden_dimension, kv_dimension)
+        self.dimension, self.hidden_dimension, self.kv_dimension = dimension, hidden_dimension, kv_dimension
+        self.vocabulary_size, self.sequences, self.max_sequence_length = vocabulary_size, sequences, max_sequence_length
+        self.last = DeviceBuffer(sequences * dimension * 4)   # the sequences' last rows
+        self.logits = DeviceBuffer(rows * vocabulary_size * 4)
+        self.chosen = DeviceBuffer(4 * rows)                  # the tokens chosen after rows
+        self.generated = DeviceBuffer(4 * sequences * max_sequence_length)  # greedy tokens by sequence and position
+        self.starts = DeviceBuffer(4 * (sequences + 1))
+        self.parents, self.depths = DeviceBuffer(4 * rows), DeviceBuffer(4 * rows)
+        self.masks = DeviceBuffer(4 * rows * -(-rows // 32))
+        self.kept = DeviceBuffer(4 * sequences * rows)
+        self.counts, self.next = DeviceBuffer(4 * sequences), DeviceBuffer(4 * sequences)
 
 
 def _group(weights: list[QuantizedTensor], outs: list[int], biases: list[int | None]):
@@ -427,6 +452,17 @@ class Transformer:
         return InferenceBuffers(self.dimension, self.hidden_dimension, self.vocabulary_size, max_sequence_length,
                                 self.kv_dimension)
 
+    def new_paged_cache(self, sequences: int, max_sequence_length: int, cache_format: str = "float32", page_tokens: int = 64,
+                        pages: int | None = None, stream: Stream | None = None) -> PagedKVCache:
+        """A cache for several sequences of this model (PagedKVCache)."""
+        return PagedKVCache(self.num_layers, self.num_key_value_heads, sequences, max_sequence_length, self.head_dim, cache_format,
+                            page_tokens, pages, stream)
+
+    def new_batch_buffers(self, cache: PagedKVCache, rows: int = 512) -> BatchBuffers:
+        """Buffers for calls of up to ``rows`` tokens on ``cache``; longer texts go through in parts."""
+        return BatchBuffers(self.dimension, self.hidden_dimension, self.vocabulary_size, cache.sequences, cache.max_sequence_length,
+                            max(rows, cache.sequences), self.kv_dimension)
+
     def _check(self, cache: KVCache, buffers: InferenceBuffers, count: int) -> None:
         if cache.num_layers != self.num_layers:
             raise _lib.IllegalArgumentException(f"Cache built for {cache.num_layers} layers, model has {self.num_layers}")
@@ -463,7 +499,7 @@ class Transformer:
     def _bias(self, name: str):
         return None if self._zero_bias.get(name, True) else self.parameters[name + ".bias"].ptr
 
-    def _layers(self, rows: _Rows, count: int, cache: KVCache, key_bound: int, st,
+    def _layers(self, rows: _Rows, count: int, cache: KVCache | QuantizedKVCache | PagedBatch, key_bound: int, st,
                 head: InferenceBuffers | None = None) -> bool:
         """The layers over `count` rows. For one row the projections between two attention
         calls (wOut, norm2 and the gate pair, wDown, and the next layer's norm1 and q/k/v)
@@ -479,7 +515,10 @@ class Transformer:
                 _lib.call("kt_rmsnorm_qmatmul_group", rows.x.ptr, self.parameters[p + "norm1.weight"].ptr,
                           ctypes.c_float(self.norm_eps), rows.normed.ptr, count, ws, n, os_, bs, 0, ctypes.c_float(1.0),
                           st)
-            if isinstance(cache, QuantizedKVCache):
+            if isinstance(cache, PagedBatch):
+                _lib.call("kt_rope_attention_paged", rows.q.ptr, rows.k.ptr, rows.v.ptr, self.inv_freq.ptr, self.num_heads,
+                          ctypes.byref(cache.cache), l, ctypes.byref(cache.batch), rows.context.ptr, st)
+            elif isinstance(cache, QuantizedKVCache):
                 _lib.call("kt_rope_attention_kv8", rows.q.ptr, rows.k.ptr, rows.v.ptr, self.inv_freq.ptr, count,
                           cache.position.ptr, key_bound, ctypes.byref(cache.cache), l, self.num_heads, rows.context.ptr, st)
             else:
@@ -541,12 +580,12 @@ class Transformer:
             s.accumulate, s.alpha, s.swiglu_gate = acc, 1.0, swiglu
         _lib.call("kt_qmatmul_chain", arr, len(steps), st)
 
-    def _head(self, x_row_ptr: int, buffers: InferenceBuffers, st) -> None:
-        """finalNorm and lmHead of one row into buffers.logits (one launch with the norm
+    def _head(self, x_row_ptr: int, buffers: InferenceBuffers | BatchBuffers, st, count: int = 1) -> None:
+        """finalNorm and lmHead of `count` rows, one as a rule, into buffers.logits (one launch with the norm
         inside the product where the one-row kernels take it)."""
         n, ws, os_, bs = _group([self.weights["lmHead"]], [buffers.logits.ptr], [self._bias("lmHead")])
         _lib.call("kt_rmsnorm_qmatmul_group", x_row_ptr, self.parameters["finalNorm.weight"].ptr,
-                  ctypes.c_float(self.norm_eps), buffers.normed.ptr, 1, ws, n, os_, bs, 0, ctypes.c_float(1.0), st)
+                  ctypes.c_float(self.norm_eps), buffers.normed.ptr, count, ws, n, os_, bs, 0, ctypes.c_float(1.0), st)
 
     def _controlled(self, controls: LogitsControls | None, cache: KVCache, buffers: InferenceBuffers, offset: int, st) -> DeviceBuffer:
         """The logits of which the next token is the argmax: buffers.logits, or with controls what they make of
@@ -701,19 +740,25 @@ class Transformer:
         """decode_step recorded once as a HIP graph on `stream` (a created stream; run one
         decode_step first so the library's workspaces already have their sizes)."""
         st = _stream(stream)
+        graph = self._record(st, lambda: self._decode_step(cache, buffers, st, argmax=True, controls=controls))
+        return DecodeGraph(graph, cache, stream, buffers, controls)
+
+    @staticmethod
+    def _record(st, step) -> ctypes.c_void_p:
+        """What `step` calls on the stream, as a HIP graph."""
         if not st:
             raise _lib.IllegalArgumentException("the null stream cannot be captured; create a stream")
         _lib.call("kt_graph_begin", st)
         graph = ctypes.c_void_p()
         try:
-            self._decode_step(cache, buffers, st, argmax=True, controls=controls)
+            step()
         except BaseException:
             # end the capture so the stream is usable again, and drop the partial graph
             if _lib.lib().kt_graph_end(st, ctypes.byref(graph)) == _lib.KT_OK and graph:
                 _lib.lib().kt_graph_destroy(graph)
             raise
         _lib.call("kt_graph_end", st, ctypes.byref(graph))
-        return DecodeGraph(graph, cache, stream, buffers, controls)
+        return graph
 
     def generate(self, prompt, max_tokens: int, stop_tokens=(), stream: Stream | None = None,
                  use_graph: bool = True, cache_format: str | None = None, block_tokens: int = 64,
@@ -743,6 +788,197 @@ class Transformer:
                     break
                 tokens.append(int(t))
             return tokens
+        finally:
+            if own:
+                stream.destroy()
+
+    # -- several sequences (no counterpart in the reference, which decodes one) ----------------
+    def _check_batch(self, cache: PagedKVCache, buffers: BatchBuffers, tokens: dict[int, list[int]]) -> None:
+        if (cache.num_layers, cache.num_heads, cache.head_dim) != (self.num_layers, self.num_key_value_heads, self.head_dim):
+            raise _lib.IllegalArgumentException(
+                f"Cache built for {cache.num_layers} layers of {cache.num_heads} heads of {cache.head_dim} dims, model has "
+                f"{self.num_layers} of {self.num_key_value_heads} of {self.head_dim}")
+        if (buffers.dimension, buffers.hidden_dimension, buffers.vocabulary_size, buffers.kv_dimension) != \
+                (self.dimension, self.hidden_dimension, self.vocabulary_size, self.kv_dimension):
+            raise _lib.IllegalArgumentException("BatchBuffers built for another model configuration")
+        if (buffers.sequences, buffers.max_sequence_length) != (cache.sequences, cache.max_sequence_length):
+            raise _lib.IllegalArgumentException("BatchBuffers built for another cache")
+        if not tokens:
+            raise _lib.IllegalArgumentException("no sequence given")
+        for sequence, text in tokens.items():
+            cache.check_sequence(sequence)
+            if not text:
+                raise _lib.IllegalArgumentException("Prompt cannot be empty")
+            for t in text:
+                if not 0 <= t < self.vocabulary_size:
+                    raise _lib.IllegalArgumentException(f"{t} out of vocab bounds {self.vocabulary_size}")
+
+    def extend(self, texts: dict[int, list[int]], cache: PagedKVCache, buffers: BatchBuffers, stream: Stream | None = None) -> dict[int, int]:
+        """prefill and decode of several sequences at once: appends ``texts[s]`` to each sequence s given, whatever their
+        lengths (prompts beside single tokens), in calls of up to ``buffers.rows`` tokens. Leaves the logits
+        after each one's last token in ``buffers.logits``, a row a sequence in their order, and returns the greedy next
+        tokens."""
+        texts = {int(s): [int(t) for t in texts[s]] for s in sorted(texts)}
+        self._check_batch(cache, buffers, texts)
+        cache.reserve({s: len(t) for s, t in texts.items()}, stream)
+        st = _stream(stream)
+        done = dict.fromkeys(texts, 0)
+        order = {s: i for i, s in enumerate(texts)}
+        while any(done[s] < len(t) for s, t in texts.items()):
+            counts, tokens = [0] * cache.sequences, []
+            for s, t in texts.items():
+                counts[s] = min(len(t) - done[s], buffers.rows - len(tokens))
+                tokens += t[done[s]:done[s] + counts[s]]
+            batch = PagedBatch(cache, counts, buffers.starts, stream=stream)
+            buffers.tokens.upload(np.array(tokens, np.int32), stream)
+            self._embed(buffers, len(tokens), st)
+            self._layers(buffers, len(tokens), batch, 0, st)
+            _lib.call("kt_paged_advance", cache.device_lengths.ptr, ctypes.byref(batch.batch), st)
+            for s, t in texts.items():
+                done[s] += counts[s]
+                cache.lengths[s] += counts[s]
+                if counts[s] and done[s] == len(t):
+                    row = 4 * self.dimension
+                    _lib.call("kt_memcpy_d2d", ctypes.c_void_p(buffers.last.ptr + order[s] * row),
+                              ctypes.c_void_p(buffers.x.ptr + (int(batch.starts[s + 1]) - 1) * row), ctypes.c_size_t(row), st)
+        n = len(texts)
+        self._head(buffers.last.ptr, buffers, st, n)
+        _lib.call("kt_argmax_rows", buffers.logits.ptr, n, self.vocabulary_size, buffers.chosen.ptr, None, None, 0, st)
+        return dict(zip(texts, buffers.chosen.download(np.int32, count=n, stream=stream).tolist()))
+
+    def greedy_decode_batch(self, tokens: list[int], cache: PagedKVCache, buffers: BatchBuffers, steps: int, stream: Stream | None = None,
+                            use_graph: bool = True) -> list[list[int]]:
+        """``steps`` greedy steps of all the cache's sequences at once, from tokens[s], the last chosen one of sequence s
+        (``extend``): each step appends a token to every sequence and chooses its next one, on the device. Returns each
+        sequence's ``steps`` further tokens. With use_graph (on a created, non-null stream) one step is recorded as a HIP graph
+        and replayed. (Of some of the sequences, or where the host looks at each token: ``extend``.)"""
+        tokens = [int(t) for t in tokens]
+        if len(tokens) != cache.sequences:
+            raise _lib.IllegalArgumentException(f"{len(tokens)} tokens for {cache.sequences} sequences")
+        if steps < 0:
+            raise _lib.IllegalArgumentException("steps must not be negative")
+        self._check_batch(cache, buffers, {s: [t] for s, t in enumerate(tokens)})
+        if steps == 0:
+            return [[] for _ in tokens]
+        n = cache.sequences
+        cache.reserve(dict.fromkeys(range(n), steps), stream)
+        st = _stream(stream)
+        batch = PagedBatch(cache, [1] * n, buffers.starts, key_bound=cache.max_sequence_length, stream=stream)
+        buffers.tokens.upload(np.array(tokens, np.int32), stream)
+
+        def step():
+            self._embed(buffers, n, st)
+            self._layers(buffers, n, batch, 0, st)
+            # recorded by the position of the token that the step appended, ahead of the advance
+            self._head(buffers.x.ptr, buffers, st, n)
+            _lib.call("kt_argmax_rows", buffers.logits.ptr, n, self.vocabulary_size, buffers.tokens.ptr, cache.device_lengths.ptr,
+                      buffers.generated.ptr, buffers.max_sequence_length, st)
+            _lib.call("kt_paged_advance", cache.device_lengths.ptr, ctypes.byref(batch.batch), st)
+
+        step()  # (this one also sizes the workspaces)
+        if use_graph and steps > 2 and st:
+            graph = self._record(st, step)
+            try:
+                for _ in range(steps - 1):
+                    _lib.call("kt_graph_launch", graph, st)
+            finally:
+                (stream or default_stream()).synchronize()
+                _lib.call("kt_graph_destroy", graph)
+        else:
+            for _ in range(steps - 1):
+                step()
+        made = buffers.generated.download(np.int32, stream=stream).reshape(n, buffers.max_sequence_length)
+        out = [made[s, first:first + steps].tolist() for s, first in enumerate(cache.lengths)]
+        cache.lengths = [length + steps for length in cache.lengths]
+        return out
+
+    def draft_step(self, drafts: dict[int, tuple[list[int], list[int]]], cache: PagedKVCache, buffers: BatchBuffers,
+                   stream: Stream | None = None) -> dict[int, list[int]]:
+        """One step of each sequence s given, over a tree of drafted tokens: drafts[s] = (tokens, parents), where tokens[0] is the
+        last chosen token (its parent -1) and each other one is a draft of what follows tokens[parents[i]], parents[i] < i. The
+        model runs over all trees at once; of each it keeps the root and, one after another, the drafts it would have
+        chosen. Returns the tokens chosen: the drafts kept and the one after them, at least one, those that as many
+        single greedy steps would have chosen (up to the rounding of products of several rows)."""
+        drafts = {int(s): ([int(t) for t in drafts[s][0]], [int(p) for p in drafts[s][1]]) for s in sorted(drafts)}
+        self._check_batch(cache, buffers, {s: t for s, (t, _) in drafts.items()})
+        for s, (t, p) in drafts.items():
+            if len(t) != len(p) or p[0] != -1 or any(not 0 <= at < i for i, at in enumerate(p[1:], 1)):
+                raise _lib.IllegalArgumentException(f"the draft of sequence {s} is no tree: a root with parent -1, then tokens below earlier ones")
+        counts, tokens, parents = [0] * cache.sequences, [], []
+        for s, (t, p) in drafts.items():
+            counts[s] = len(t)
+            tokens += t
+            parents += p
+        rows = len(tokens)
+        if rows > buffers.rows:
+            raise _lib.IllegalArgumentException(f"{rows} tokens exceed the buffers' {buffers.rows} rows")
+        cache.reserve({s: len(t) for s, (t, _) in drafts.items()}, stream)
+        st = _stream(stream)
+        batch = PagedBatch(cache, counts, buffers.starts, buffers=buffers, stream=stream)
+        ref = ctypes.byref(batch.batch)
+        buffers.tokens.upload(np.array(tokens, np.int32), stream)
+        buffers.parents.upload(np.array(parents, np.int32), stream)
+        _lib.call("kt_tree_masks", buffers.parents.ptr, ref, buffers.depths.ptr, buffers.masks.ptr, st)
+        self._embed(buffers, rows, st)
+        self._layers(buffers, rows, batch, 0, st)
+        self._head(buffers.x.ptr, buffers, st, rows)
+        _lib.call("kt_argmax_rows", buffers.logits.ptr, rows, self.vocabulary_size, buffers.chosen.ptr, None, None, 0, st)
+        stride = batch.batch.most_rows
+        _lib.call("kt_tree_accept", buffers.tokens.ptr, buffers.chosen.ptr, buffers.parents.ptr, ref, buffers.kept.ptr, stride,
+                  buffers.counts.ptr, buffers.next.ptr, st)
+        _lib.call("kt_paged_keep", ctypes.byref(cache.cache), ref, buffers.kept.ptr, stride, buffers.counts.ptr, cache.device_lengths.ptr, st)
+        kept = buffers.kept.download(np.int32, count=cache.sequences * stride, stream=stream).reshape(cache.sequences, stride)
+        number = buffers.counts.download(np.int32, stream=stream).tolist()
+        following = buffers.next.download(np.int32, stream=stream).tolist()
+        out = {}
+        for s, (t, _) in drafts.items():
+            cache.lengths[s] += number[s]
+            out[s] = [t[i] for i in kept[s, 1:number[s]].tolist()] + [following[s]]
+        return out
+
+    def generate_batch(self, prompts, max_tokens: int, stop_tokens=(), stream: Stream | None = None, use_graph: bool = True,
+                       cache_format: str = "float32", page_tokens: int = 64, draft=None, rows: int = 512) -> list[list[int]]:
+        """generate for several prompts at once, over a cache in pages (new_paged_cache). With ``draft``, a function of a
+        text's tokens so far that gives (tokens, parents) of a tree that may follow them (TextDraft; an empty one is none), each
+        step checks the trees of all texts that are not done and takes as many of their tokens as the model would have
+        chosen (draft_step)."""
+        prompts = [[int(t) for t in prompt] for prompt in prompts]
+        if not prompts or not all(prompts):
+            raise _lib.IllegalArgumentException("Prompt cannot be empty")
+        if max_tokens <= 0:
+            return prompts
+        own = stream is None and use_graph
+        stream = Stream.create() if own else stream
+        try:
+            share = max(rows // len(prompts), 1) if draft is not None else 0  # tokens of a text's tree, which has room past the last one wanted
+            cache = self.new_paged_cache(len(prompts), max(map(len, prompts)) + max_tokens + share, cache_format, page_tokens, stream=stream)
+            buffers = self.new_batch_buffers(cache, rows)
+            first = self.extend(dict(enumerate(prompts)), cache, buffers, stream)
+            stops = set(int(s) for s in stop_tokens)
+            if draft is None:
+                rest = self.greedy_decode_batch([first[s] for s in range(len(prompts))], cache, buffers, max_tokens - 1, stream, use_graph)
+                made = {s: [first[s]] + rest[s] for s in first}
+            else:
+                made = {s: [first[s]] for s in first}
+                while True:
+                    going = [s for s, out in made.items() if len(out) < max_tokens and not stops.intersection(out)]
+                    if not going:
+                        break
+                    drafts = {}
+                    for s in going:
+                        tokens, parents = draft(prompts[s] + made[s])
+                        drafts[s] = (made[s][-1:] + list(tokens[:share - 1]), [-1] + [int(p) + 1 for p in parents[:share - 1]])
+                    for s, chosen in self.draft_step(drafts, cache, buffers, stream).items():
+                        made[s] += chosen
+            out = []
+            for s, prompt in enumerate(prompts):
+                tokens = list(prompt)
+                for t in made[s][:max_tokens]:
+                    if t in stops:
+                        break
+                    tokens.append(int(t))
+                out.append(tokens)
+            return out
         finally:
             if own:
                 stream.destroy()

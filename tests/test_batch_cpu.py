@@ -1,0 +1,127 @@
+"""PagedKVCache's pages and TextDraft's trees without a device."""
+import numpy as np
+import pytest
+
+import kotensor_amd as kt
+from kotensor_amd import paged
+
+
+class HostBuffer:
+    """DeviceBuffer's calls on host memory."""
+
+    def __init__(self, nbytes):
+        self.nbytes, self.ptr = nbytes, 4096
+        self.bytes = np.zeros(nbytes, np.uint8)
+
+    @classmethod
+    def from_numpy(cls, array, stream=None):
+        buffer = cls(array.nbytes)
+        buffer.upload(array)
+        return buffer
+
+    def upload(self, array, stream=None, offset=0):
+        raw = np.ascontiguousarray(array).view(np.uint8).reshape(-1)
+        assert offset + raw.size <= self.nbytes
+        self.bytes[offset:offset + raw.size] = raw
+
+
+@pytest.fixture
+def cache(monkeypatch):
+    monkeypatch.setattr(paged, "DeviceBuffer", HostBuffer)
+    return kt.PagedKVCache(2, 2, 4, 100, 32, "float16", 16, pages=12)
+
+
+def tables(cache):
+    return cache.tables.bytes.view(np.int32).reshape(cache.sequences, cache.table_stride)
+
+
+def lengths(cache):
+    return cache.device_lengths.bytes.view(np.int32).tolist()
+
+
+def grow(cache, counts):
+    cache.reserve(counts)
+    for s, n in counts.items():
+        cache.lengths[s] += n
+
+
+def test_pages_go_to_sequences_and_back(cache):
+    assert cache.size_in_bytes == 2 * 2 * 2 * 12 * 2 * 16 * 32 and cache.table_stride == 7
+    grow(cache, {0: 1, 1: 16, 2: 17})
+    assert cache.free_pages == 8
+    grow(cache, {0: 15, 1: 1})
+    assert cache.free_pages == 7
+    held = [row[row >= 0].tolist() for row in tables(cache)]
+    assert [len(h) for h in held] == [1, 2, 2, 0] and len({p for h in held for p in h}) == 5
+    cache.release(1)
+    assert cache.free_pages == 9 and cache.lengths[1] == 0 and lengths(cache)[1] == 0
+    grow(cache, {3: 100})
+    assert cache.free_pages == 2
+    mine = tables(cache)[3].tolist()
+    assert len(set(mine)) == 7 and not set(mine) & set(held[0] + held[2])
+
+
+def test_a_reservation_is_whole_or_none(cache):
+    grow(cache, {0: 90})
+    with pytest.raises(kt.IllegalArgumentException, match="8 pages needed, 6 of 12 free"):
+        cache.reserve({1: 64, 2: 64})
+    with pytest.raises(kt.IllegalArgumentException, match="exceed maxSequenceLength 100"):
+        cache.reserve({1: 1, 0: 11})
+    assert cache.free_pages == 6
+    cache.reserve({1: 64, 2: 32, 0: 0})
+    assert cache.free_pages == 0
+
+
+def test_shared_pages_are_freed_by_the_last_holder(cache):
+    grow(cache, {0: 50})
+    assert cache.share(0, 1, 50) == 48 and cache.share(1, 2, 40) == 32
+    assert cache.free_pages == 8 and lengths(cache) == [0, 48, 32, 0]
+    assert tables(cache)[1, :3].tolist() == tables(cache)[0, :3].tolist()
+    grow(cache, {1: 1, 2: 1})
+    assert cache.free_pages == 6 and tables(cache)[1, 3] != tables(cache)[0, 3]
+    for keep, fine in ((50, True), (48, True), (47, False), (0, False)):
+        if fine:
+            cache.set_length(0, keep)
+        else:
+            with pytest.raises(kt.IllegalArgumentException, match="shared"):
+                cache.set_length(0, keep)
+    cache.release(0)
+    assert cache.free_pages == 7  # its own last page
+    cache.release(2)
+    assert cache.free_pages == 8
+    cache.set_length(1, 0)
+    cache.release(1)
+    assert cache.free_pages == 12 and sorted(cache._free) == list(range(12))
+
+
+def test_refusals(cache):
+    E = kt.IllegalArgumentException
+    for change in ({"num_layers": 0}, {"num_heads": 0}, {"sequences": 0}, {"max_sequence_length": 0}, {"head_dim": 0}, {"page_tokens": 0},
+                   {"format": "int8"}, {"head_dim": 48}, {"page_tokens": 24}, {"pages": -1}):
+        with pytest.raises(E):
+            kt.PagedKVCache(**{**dict(num_layers=1, num_heads=1, sequences=1, max_sequence_length=10, head_dim=32), **change})
+    for call in (lambda: cache.reserve({4: 1}), lambda: cache.reserve({-1: 1}), lambda: cache.reserve({0: -1}), lambda: cache.release(4),
+                 lambda: cache.set_length(0, 1), lambda: cache.set_length(0, -1), lambda: cache.share(0, 4, 0), lambda: cache.share(0, 1, 1),
+                 lambda: kt.TextDraft(0), lambda: kt.TextDraft(1, 0), lambda: kt.TextDraft(1, 1, 0)):
+        with pytest.raises(E):
+            call()
+    with pytest.raises(E):
+        kt.BatchBuffers(8, 8, 8, 4, 10, 3, 8)
+
+
+def test_drafts_from_the_text():
+    draft = kt.TextDraft(tokens=3, branches=2, match=2)
+    assert draft([1]) == ([], []) and draft([]) == ([], [])
+    assert draft([1, 2, 3]) == ([], [])
+    # the last two tokens occur twice before: the later place first; both go on with 9
+    text = [5, 6, 9, 1, 2, 5, 6, 9, 4, 5, 6]
+    tokens, parents = draft(text)
+    assert tokens == [9, 4, 5, 1, 2] and parents == [-1, 0, 1, 0, 3]
+    # only the last one occurs
+    assert draft([7, 8, 3, 8]) == ([3, 8], [-1, 0])
+    assert kt.TextDraft(4, 1, 3)([1, 1, 1]) == ([1], [-1])
+    for run in range(50):
+        rng = np.random.default_rng(run)
+        text = rng.integers(0, 4, 40).tolist()
+        tokens, parents = kt.TextDraft(5, 3, 3)(text)
+        assert len(tokens) == len(parents) <= 15 and all(-1 <= p < i for i, p in enumerate(parents))
