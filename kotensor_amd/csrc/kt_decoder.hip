@@ -1411,6 +1411,7 @@ __global__ void __launch_bounds__(THREADS) argmax_kernel(const float* __restrict
     partials += row * gridDim.x;
     counter += row;
     uint64_t best = 0;
+#pragma unroll 4
     for (int32_t i = blockIdx.x * THREADS + threadIdx.x; i < n; i += gridDim.x * THREADS)
         best = max_u64(best, argmax_key(logits[i], i));
     best = wave_max_u64(best);
@@ -1888,7 +1889,9 @@ static int32_t launch_argmax(const float* logits, int32_t rows, int32_t n, int32
                              int32_t* generated, int32_t capacity, hipStream_t st) {
     int32_t blocks = ceil_div(n, 4 * THREADS);
     if (blocks > ARGMAX_BLOCKS) blocks = ARGMAX_BLOCKS;
-    if (rows > 1) blocks = std::min(blocks, std::max(1, 8 * cu_count() / rows));  // (the card full: 8 workgroups a CU)
+    // Of several rows as many workgroups as fill the CUs twice, two of a row at least: 64 rows of 32000 8.6 us (8 a CU: 17, as
+    // their counters' atomics wait for each other), 960 rows 30 (one workgroup a row: 52).
+    if (rows > 1) blocks = std::min(blocks, std::max(2, 2 * cu_count() / rows));
     void* ws = nullptr;
     uint32_t* counters = nullptr;
     const size_t partials = rows > 1 ? static_cast<size_t>(rows) * blocks : ARGMAX_BLOCKS;
@@ -1915,7 +1918,7 @@ int32_t kt_argmax_advance(const float* logits, int32_t n, int32_t* token, int32_
 
 int32_t kt_argmax_rows(const float* logits, int32_t rows, int32_t n, int32_t* tokens, const int32_t* positions, int32_t* generated,
                        int32_t capacity, void* stream) {
-    if (rows < 0 || rows > 65535) return fail(KT_ERR_SHAPE, "argmax of %d rows: 0 to 65535", rows);
+    if (rows < 0 || rows > static_cast<int32_t>(MAX_COUNTERS)) return fail(KT_ERR_SHAPE, "argmax of %d rows: 0 to %d", rows, static_cast<int32_t>(MAX_COUNTERS));
     if (rows == 0) return KT_OK;
     if (!logits || !tokens) return fail(KT_ERR_ARGUMENT, "logits or tokens is NULL");
     if (n <= 0) return fail(KT_ERR_SHAPE, "argmax needs at least one logit");

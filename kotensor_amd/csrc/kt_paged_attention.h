@@ -270,8 +270,13 @@ struct Part {
     }
 };
 
-// Which part of the launch workgroup `at` has (BY_SLOT: whose slot `at` is); false: none. Every lane is a sequence. A launch has at most target + (its tiles
-// of all kv heads) parts, and at most 2 target that share a tile: a part's size is at least the chunks over target.
+// Which part of the launch workgroup `at` has (BY_SLOT: whose slot `at` is); false: none. Every lane is a sequence. A part's size is at least
+// the chunks over target, so a launch has at most target + (its tiles of all kv heads) parts, and at most 2 target that share a
+// tile. Tiles of many rows (FINE): where that size is above LONG tokens and tiles are fewer than 2 target, whose rounds would leave
+// workgroups idle, the chunks over 2 target: at most 4 target parts that share a tile. (16 sequences with trees of 64 after 3000, bf16, 128
+// dims: 149 -> 141 us; everywhere, a tree of 60 after 4000 would take 49 for 42, a prompt of 2048 122 for 117.)
+constexpr int LONG = 1024;
+constexpr bool fine(int R) { return R > 16; }
 template <int R, int LEAST, int CHUNK, bool BY_SLOT = false>
 __device__ __forceinline__ bool find_part(const Args& a, int32_t at, Part& out) {
     const PagedView& c = a.p.c;
@@ -289,16 +294,20 @@ __device__ __forceinline__ bool find_part(const Args& a, int32_t at, Part& out) 
     auto tiles_of = [&]() { return static_cast<int32_t>((static_cast<int64_t>(n) * G + R - 1) / R); };
     auto chunks_of = [&]() { return (held_keys(c, b, length, n) + CHUNK - 1) / CHUNK; };
     // (whole numbers up to 2^24 are exact in fp32; of larger totals a little more)
-    float total = 0.0f, rows = 0.0f;
+    float total = 0.0f, rows = 0.0f, all_tiles = 0.0f;
     for (int32_t s0 = 0; s0 < b.sequences; s0 += 64) {
         load(s0);
         total += static_cast<float>(tiles_of()) * static_cast<float>(c.kv_heads) * static_cast<float>(max(chunks_of(), 1));
         rows += static_cast<float>(n);
+        all_tiles += static_cast<float>(tiles_of()) * static_cast<float>(c.kv_heads);
     }
     total = wave_sum_dpp(total);
     if (wave_sum_dpp(rows) > static_cast<float>(b.rows)) return false;  // starts that do not ascend
     if (total >= 0x1p24f) total *= 1.0f + 0x1p-16f;
-    const float target = static_cast<float>(a.target);
+    float target = static_cast<float>(a.target);
+    if constexpr (fine(R)) {
+        if (total > target * (LONG / CHUNK) && wave_sum_dpp(all_tiles) < 2.0f * target) target *= 2.0f;
+    }
     int32_t per = static_cast<int32_t>(fminf(total / target, 0x1p30f));
     if (static_cast<float>(per) * target < total) ++per;
     per = uniform((max(per, 1) + LEAST - 1) / LEAST * LEAST);
@@ -556,11 +565,11 @@ __device__ __forceinline__ void meet(const Args& a, const Part& part, int32_t sp
 }
 
 // The same as a launch of its own, for tiles of many rows, whose merge is more than one workgroup's work: the workgroups of a
-// slot take their shares of the tile's rows.
-constexpr int merge_shares(int R) { return R / 32; }
+// slot take their shares of the tile's rows (two a tile of 128: four, with as many empty ones beside them, cost every call 1 us).
+constexpr int merge_shares(int R) { return R / 64; }
 template <int HD, int R, int LEAST, int CHUNK>
 __global__ void __launch_bounds__(256) merge_kernel(Args a) {
-    __shared__ float maxima[R + MOST_PARTS], sums[R + MOST_PARTS], weights[R + MOST_PARTS];
+    __shared__ float maxima[64 + MOST_PARTS], sums[64 + MOST_PARTS], weights[64 + MOST_PARTS];
     Part part;
     if (!find_part<R, LEAST, CHUNK, true>(a, blockIdx.x, part)) return;
     part.make_uniform();
@@ -572,7 +581,7 @@ __global__ void __launch_bounds__(256) merge_kernel(Args a) {
     const int32_t r0 = uniform(held * share / shares), rows = uniform(held * (share + 1) / shares) - r0;
     if (rows == 0) return;
     const size_t slot0 = static_cast<size_t>(part.slot) * R;
-    // (fewer than held / part.splits + 1 rows, of at most part.splits parts)
+    // (fewer than held / shares + 1 rows, of at most part.splits parts: 64 + MOST_PARTS weights at most)
     for (int32_t e = tid; e < rows * splits; e += 256) {
         const int32_t s = e / rows, r = e % rows;
         const float2 both = reinterpret_cast<const float2*>(a.stats)[slot0 + static_cast<size_t>(s) * R + r0 + r];
@@ -1357,10 +1366,11 @@ int32_t prepare(Args& a, int32_t target, int64_t* grid, hipStream_t st) {
     const int64_t tiles = std::min(b.sequences * ((b.most_rows * G + R - 1) / R), b.rows * G / R + b.sequences) * a.p.c.kv_heads;
     const int64_t chunks = (static_cast<int64_t>(b.key_bound) + CHUNK - 1) / CHUNK, most_splits = std::min<int64_t>(MOST_PARTS, (chunks + LEAST - 1) / LEAST);
     a.target = target;
-    *grid = std::min(tiles + target, tiles * most_splits);
+    const int64_t most = fine(R) ? 2 * target : target;  // (find_part)
+    *grid = std::min(tiles + most, tiles * most_splits);
     if (*grid > INT32_MAX / 64) return fail(KT_ERR_SHAPE, "too many rows and heads in one call");
     if (most_splits <= 1) return KT_OK;
-    const size_t slots = static_cast<size_t>(std::min<int64_t>(2 * target, *grid));
+    const size_t slots = static_cast<size_t>(std::min<int64_t>(2 * most, *grid));
     a.slots = static_cast<int32_t>(slots);
     void* ws = nullptr;
     if (const int32_t status = workspace_counters(st, slots * R * (HD + 2) * sizeof(float) + 16, R == 16 ? slots : 0, &ws, &a.counters)) return status;
