@@ -133,22 +133,36 @@ __global__ void __launch_bounds__(THREADS) masks_kernel(const int32_t* parents, 
     }
 }
 
+constexpr int32_t ACCEPT_LDS = 1024;  // rows whose numbers are held in LDS (a step of the walk reads three, one after another)
 // One wave a sequence: from row 0 to the first row whose parent is the last one kept and whose token is
 // the one chosen after that, as long as there is one.
 __global__ void __launch_bounds__(64) accept_kernel(const int32_t* tokens, const int32_t* chosen, const int32_t* parents, BatchView b,
                                                     int32_t* kept, int32_t kept_stride, int32_t* counts, int32_t* next) {
+    __shared__ int32_t held[3][ACCEPT_LDS];
     const int32_t s = blockIdx.x, lane = threadIdx.x, first = start_of(b, s), n = min(start_of(b, s + 1) - first, kept_stride);
     int32_t* out = kept + static_cast<size_t>(s) * kept_stride;
+    const bool in_lds = n <= ACCEPT_LDS;
+    if (in_lds) {
+        for (int32_t i = lane; i < n; i += 64) {
+            held[0][i] = parents[first + i];
+            held[1][i] = tokens[first + i];
+            held[2][i] = chosen[first + i];
+        }
+        __syncthreads();
+    }
+    auto parent_of = [&](int32_t r) { return in_lds ? held[0][r] : parents[first + r]; };
+    auto token_of = [&](int32_t r) { return in_lds ? held[1][r] : tokens[first + r]; };
+    auto chosen_after = [&](int32_t r) { return in_lds ? held[2][r] : chosen[first + r]; };
     int32_t count = 0, last = 0;
     if (n > 0) {
         count = 1;
         if (lane == 0) out[0] = 0;
         for (int32_t i0 = 1; i0 < n;) {  // rows from i0 on may follow `last`
-            const int32_t want = chosen[first + last];
+            const int32_t want = chosen_after(last);
             int32_t found = -1;
             for (int32_t r0 = i0; r0 < n && found < 0; r0 += 64) {
                 const int32_t r = min(r0 + lane, n - 1);
-                const uint64_t hit = __ballot(r0 + lane < n && parents[first + r] == last && tokens[first + r] == want);
+                const uint64_t hit = __ballot(r0 + lane < n && parent_of(r) == last && token_of(r) == want);
                 if (hit) found = r0 + __builtin_ctzll(hit);
             }
             if (found < 0) break;
@@ -161,20 +175,22 @@ __global__ void __launch_bounds__(64) accept_kernel(const int32_t* tokens, const
     for (int32_t i = count + lane; i < kept_stride; i += 64) out[i] = -1;
     if (lane == 0) {
         counts[s] = count;
-        if (n > 0) next[s] = chosen[first + last];
+        if (n > 0) next[s] = chosen_after(last);
     }
 }
 
 // ---- what is kept ------------------------------------------------------------------------
-// How many of a sequence's kept rows count: up to the first that does not ascend or is none of its rows.
+// How many of a sequence's kept rows count: up to the first that does not ascend or is none of its rows. All lanes of the
+// wave active: each looks at an entry and the one before it.
 __device__ __forceinline__ int32_t kept_count(const int32_t* kept, int32_t count, int32_t n) {
-    int32_t before = -1, m = 0;
-    for (; m < count; ++m) {
-        const int32_t r = kept[m];
-        if (r <= before || r >= n) break;
-        before = r;
+    const int32_t lane = threadIdx.x & 63;
+    for (int32_t m0 = 0; m0 < count; m0 += 64) {
+        const int32_t m = m0 + lane;
+        const int32_t r = m < count ? kept[m] : -1, before = m > 0 && m < count ? kept[m - 1] : -1;
+        const uint64_t odd = __ballot(r <= before || r >= n);  // (past the count too)
+        if (odd) return m0 + __builtin_ctzll(odd);
     }
-    return m;
+    return max(count, 0);
 }
 
 // Thread: 16 bytes of a head's keys or values in one layer, which it moves for every kept row in turn (a row
@@ -211,12 +227,18 @@ __global__ void __launch_bounds__(THREADS) keep_kernel(PagedView c, size_t layer
     }
 }
 
-// lengths += what was kept, or (kept NULL) += the rows of the call
-__global__ void __launch_bounds__(THREADS) advance_kernel(BatchView b, const int32_t* kept, int32_t kept_stride, const int32_t* counts, int32_t* lengths) {
-    const int32_t s = blockIdx.x * THREADS + threadIdx.x;
+// lengths += what was kept: a wave a sequence
+__global__ void __launch_bounds__(THREADS) kept_lengths_kernel(BatchView b, const int32_t* kept, int32_t kept_stride, const int32_t* counts, int32_t* lengths) {
+    const int32_t s = blockIdx.x * (THREADS / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (s >= b.sequences) return;
-    const int32_t n = max(start_of(b, s + 1) - start_of(b, s), 0);
-    lengths[s] += kept ? kept_count(kept + static_cast<size_t>(s) * kept_stride, min(counts[s], kept_stride), n) : n;
+    const int32_t count = kept_count(kept + static_cast<size_t>(s) * kept_stride, min(counts[s], kept_stride), start_of(b, s + 1) - start_of(b, s));
+    if ((threadIdx.x & 63) == 0) lengths[s] += count;
+}
+
+// lengths += the rows of the call
+__global__ void __launch_bounds__(THREADS) advance_kernel(BatchView b, int32_t* lengths) {
+    const int32_t s = blockIdx.x * THREADS + threadIdx.x;
+    if (s < b.sequences) lengths[s] += max(start_of(b, s + 1) - start_of(b, s), 0);
 }
 
 // ---- rows as fp32 --------------------------------------------------------------------------
@@ -428,7 +450,7 @@ int32_t kt_paged_keep(const kt_paged_cache* cache, const kt_paged_batch* batch, 
     kernel<<<grid, THREADS, 0, st>>>(c, static_cast<size_t>(layer_elements(cache)) * bytes, static_cast<int32_t>(pieces), b, kept, kept_stride, counts, new_lengths);
     KT_LAUNCHED("paged cache keep kernel");
     if (new_lengths == b.lengths) {  // (the move reads the lengths from before)
-        advance_kernel<<<static_cast<uint32_t>(ceil_div(b.sequences, THREADS)), THREADS, 0, st>>>(b, kept, kept_stride, counts, new_lengths);
+        kept_lengths_kernel<<<static_cast<uint32_t>(ceil_div(b.sequences, THREADS / 64)), THREADS, 0, st>>>(b, kept, kept_stride, counts, new_lengths);
         KT_LAUNCHED("paged cache lengths kernel");
     }
     return KT_OK;
@@ -439,7 +461,7 @@ int32_t kt_paged_advance(int32_t* lengths, const kt_paged_batch* batch, void* st
     if (const int32_t status = view_batch(batch, nullptr, &b)) return status;
     if (!lengths) return fail(KT_ERR_ARGUMENT, "a pointer argument is NULL");
     if (b.sequences == 0) return KT_OK;
-    advance_kernel<<<static_cast<uint32_t>(ceil_div(b.sequences, THREADS)), THREADS, 0, static_cast<hipStream_t>(stream)>>>(b, nullptr, 0, nullptr, lengths);
+    advance_kernel<<<static_cast<uint32_t>(ceil_div(b.sequences, THREADS)), THREADS, 0, static_cast<hipStream_t>(stream)>>>(b, lengths);
     KT_LAUNCHED("paged cache lengths kernel");
     return KT_OK;
 }
