@@ -1039,7 +1039,9 @@ struct Tile {
     // waves a SIMD that leave a wave the registers it needs (of 256 dims with two: 352 bytes and more in scratch memory)
     static constexpr int MW = NW == 8 ? 2 : HD == 256 ? 1 : HD <= 64 && FMT != KT_PAGED_F32 ? 3 : 2;
     static constexpr int KP = Format<FMT>::KP, QP = Format<FMT>::QP, E = Format<FMT>::E;
-    static constexpr int CH = FMT == KT_PAGED_F32 || HD != 128 ? 32 : 64, SETS = CH / 32;
+    // keys of a chunk: half the barriers with 64 (at 64 dims a prompt of 1024 in fp16 36 us for 39, of 2048 in fp32 124 for 134; bf16 76 for 75),
+    // where the registers and LDS allow it
+    static constexpr int CH = HD == 256 || (FMT == KT_PAGED_F32 && HD == 128) ? 32 : 64, SETS = CH / 32;
     static constexpr int QS = HD / 32, DB = HD / 16;
     static constexpr int KR = HD + 8, VR = CH + 8;  // padded rows: of a key, of a dim (2-byte elements)
     static constexpr int KSIZE = CH * KR, VSIZE = HD * VR, SIZE = KP * (KSIZE + VSIZE);
@@ -1422,7 +1424,7 @@ int32_t launch_tiles(Args a, hipStream_t st) {
 //     after 20000 247 against 169 (only 64 sequences of 2000 tokens would be 848 against 877).
 //   up to 64 rows: tiles of 64, so that no wave is idle, two workgroups a CU: 16 sequences with trees of 15 after 2000 tokens 41
 //     against 54 with tiles of 128 (fp32 76 against 95); one tree of 15 after 4000 30 and 30.
-//   up to 64 dims in 16 bits: tiles of 64 for any number of rows, of which three workgroups share a CU (a prompt of 2048: 74.8).
+//   up to 64 dims in 16 bits: tiles of 64 for any number of rows, of which three workgroups share a CU (a prompt of 2048: 67).
 //   else: tiles of 128, as the chunk that eight waves share is half the loads and LDS writes a row: a prompt of 2048 102 (fp16),
 //     115 (bf16), 210 (fp32); a tree of 60 in fp32 53 against 63.
 //   256 dims: tiles of 64 whose waves have a SIMD's registers each: a prompt of 512 44 against 50 with tiles of
