@@ -231,7 +231,7 @@ struct Args {
     float* averages;     // [slots][R][head_dim]: the parts' averages
     float* stats;        // [slots][R][2]: their maxima and sums
     uint32_t* counters;  // [slots], zero between launches
-    int32_t slots;
+    int32_t slots;       // 0: every tile is one part
 };
 
 __device__ __forceinline__ int32_t held_keys(const PagedView& c, const BatchView& b, int32_t length, int32_t n) {
@@ -310,7 +310,7 @@ __device__ __forceinline__ bool find_part(const Args& a, int32_t at, Part& out) 
     }
     int32_t per = static_cast<int32_t>(fminf(total / target, 0x1p30f));
     if (static_cast<float>(per) * target < total) ++per;
-    per = uniform((max(per, 1) + LEAST - 1) / LEAST * LEAST);
+    per = a.slots == 0 ? 1 << 26 : uniform((max(per, 1) + LEAST - 1) / LEAST * LEAST);
     int32_t before = 0, slots = 0;
     for (int32_t s0 = 0; s0 < b.sequences; s0 += 64) {
         if (b.sequences > 64) load(s0);
@@ -1365,13 +1365,18 @@ template <int HD, int R, int LEAST, int CHUNK>
 int32_t prepare(Args& a, int32_t target, int64_t* grid, hipStream_t st) {
     const BatchView& b = a.p.b;
     const int64_t G = a.p.num_heads / a.p.c.kv_heads;
-    const int64_t tiles = std::min(b.sequences * ((b.most_rows * G + R - 1) / R), b.rows * G / R + b.sequences) * a.p.c.kv_heads;
+    const int64_t tiles = std::min(b.sequences * ((b.most_rows * G + R - 1) / R), b.rows * G / R + b.sequences) * a.p.c.kv_heads;  // at most
     const int64_t chunks = (static_cast<int64_t>(b.key_bound) + CHUNK - 1) / CHUNK, most_splits = std::min<int64_t>(MOST_PARTS, (chunks + LEAST - 1) / LEAST);
     a.target = target;
     const int64_t most = fine(R) ? 2 * target : target;  // (find_part)
     *grid = std::min(tiles + most, tiles * most_splits);
     if (*grid > INT32_MAX / 64) return fail(KT_ERR_SHAPE, "too many rows and heads in one call");
-    if (most_splits <= 1) return KT_OK;
+    // One sequence whose tiles are target and more by themselves is not cut (find_part would not, were its rows fewer than the call says it
+    // could): no merge to launch. A prompt of 1024 (fp16, 64 dims): 33 us, with one 36; of 2048 63 and 67.
+    const bool finer = fine(R) && tiles * chunks > int64_t{target} * (LONG / CHUNK) && tiles < 2 * int64_t{target};
+    const bool whole = b.sequences == 1 && tiles >= target && !finer;
+    if (whole) *grid = tiles;
+    if (most_splits <= 1 || whole) return KT_OK;
     const size_t slots = static_cast<size_t>(std::min<int64_t>(2 * most, *grid));
     a.slots = static_cast<int32_t>(slots);
     void* ws = nullptr;
@@ -1424,7 +1429,7 @@ int32_t launch_tiles(Args a, hipStream_t st) {
 //     after 20000 247 against 169 (only 64 sequences of 2000 tokens would be 848 against 877).
 //   up to 64 rows: tiles of 64, so that no wave is idle, two workgroups a CU: 16 sequences with trees of 15 after 2000 tokens 41
 //     against 54 with tiles of 128 (fp32 76 against 95); one tree of 15 after 4000 30 and 30.
-//   up to 64 dims in 16 bits: tiles of 64 for any number of rows, of which three workgroups share a CU (a prompt of 2048: 67).
+//   up to 64 dims in 16 bits: tiles of 64 for any number of rows, of which three workgroups share a CU (a prompt of 2048: 63).
 //   else: tiles of 128, as the chunk that eight waves share is half the loads and LDS writes a row: a prompt of 2048 102 (fp16),
 //     115 (bf16), 210 (fp32); a tree of 60 in fp32 53 against 63.
 //   256 dims: tiles of 64 whose waves have a SIMD's registers each: a prompt of 512 44 against 50 with tiles of
