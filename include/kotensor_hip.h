@@ -457,7 +457,7 @@ typedef struct kt_paged_batch {
     int32_t sequences;        /* at most 65535 */
     int32_t rows;             /* rows of q, k, v and context, fewer than 2^24 */
     int32_t most_rows;        /* at least every sequence's rows */
-    int32_t key_bound;        /* at least every lengths[s] + its rows: it sizes the launch, and tokens from it on are not seen */
+    int32_t key_bound;        /* at least every lengths[s] + its rows: it sizes the launch, and tokens from it on are not seen; at most 2^30 */
     int32_t mask_words;       /* 32 * mask_words >= most_rows */
 } kt_paged_batch;
 /* Bytes of the keys, and of the values. Reads no pointer of the cache. Host arithmetic. */

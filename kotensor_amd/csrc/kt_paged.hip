@@ -307,6 +307,7 @@ int32_t view_batch(const kt_paged_batch* b, const kt_paged_cache* cache, BatchVi
     if (cache) {
         if (b->table_stride <= 0) return fail(KT_ERR_ARGUMENT, "table_stride must be positive");
         const int64_t room = static_cast<int64_t>(b->table_stride) * cache->page_tokens;
+        if (b->key_bound > 1 << 30) return fail(KT_ERR_SHAPE, "key bound %d: at most %d", b->key_bound, 1 << 30);  // (chunks' ends are 32-bit)
         if (b->key_bound < b->most_rows || b->key_bound > room)
             return fail(KT_ERR_ARGUMENT, "key bound %d must cover the %d rows of a sequence and fit its table's %lld tokens", b->key_bound, b->most_rows, static_cast<long long>(room));
     }

@@ -1,0 +1,67 @@
+"""Attention over the cache in pages at the sizes that choose between its kernels (by rows of a kv head, key bound, head
+dimension and format), and between its ways of cutting tiles into parts."""
+import numpy as np
+import pytest
+
+from paged_helpers import Batch, random_parents
+
+pytestmark = pytest.mark.gpu
+
+FORMATS = ["float32", "float16", "bfloat16"]
+
+
+def check(b):
+    b.rope_attention()
+    first = b.context()
+    b.append()
+    b.check_context(first, *b.attend(b.rotated()))
+    b.rope_attention()
+    assert b.context().tobytes() == first.tobytes()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dim", [32, 64, 128, 256])
+@pytest.mark.parametrize("bound", [128, 129])
+@pytest.mark.parametrize("tree", [False, True])
+def test_few_keys(kt, fmt, dim, bound, tree):
+    """Up to 128 keys a launch has tiles of 16 rows without parts; one more and it may have larger ones."""
+    counts = [bound - 1, 1, 0, 40, 17]
+    parents = random_parents(np.random.default_rng(dim), counts) if tree else None
+    check(Batch(kt, 60, [1, 100, 5, 60, 0], counts, (4, 2, dim), fmt, 16, parents=parents, key_bound=bound, extra=1))
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dim", [32, 64, 128, 256])
+@pytest.mark.parametrize("rows", [16, 17, 64, 65, 128, 129])
+def test_rows_of_a_tile(kt, fmt, dim, rows):
+    """One query head a kv head: as many rows as tokens. Parts of a long text, beside a short one."""
+    check(Batch(kt, 61 + rows, [1500, 200], [rows, 3], (2, 2, dim), fmt, 64))
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("group", [3, 5, 16, 17])
+def test_rows_that_tiles_cut(kt, fmt, dim, group):
+    """Tiles that end inside a token's query heads."""
+    rng = np.random.default_rng(group)
+    counts = [13, 6]
+    check(Batch(kt, 62, [900, 31], counts, (group, 1, dim), fmt, 32, parents=random_parents(rng, counts)))
+
+
+@pytest.mark.parametrize("fmt", ["float32", "bfloat16"])
+def test_long_parts_of_few_tiles(kt, fmt):
+    """More than LONG keys a workgroup: 64 or 128 tiles (fewer than 512) of 6500 tokens and more are cut finer."""
+    check(Batch(kt, 63, [6900, 6500, 7100, 6000], [40, 33, 38, 40], (32, 8, 128), fmt, 64))
+
+
+@pytest.mark.parametrize("fmt,shape,count", [("float16", (32, 8, 64), 1030), ("bfloat16", (32, 8, 64), 1024), ("float32", (32, 8, 64), 1024), ("bfloat16", (32, 8, 128), 1100)])
+@pytest.mark.parametrize("given", [None, 50])
+def test_one_sequence_that_fills_the_card(kt, fmt, shape, count, given):
+    """A prompt whose tiles are not cut; also where the sequence has fewer rows than the call has room for."""
+    n = count if given is None else given
+    b = Batch(kt, 64, [7], [n], shape, fmt, 64, extra=count - n, spare=20)
+    b.most, b.words, b.key_bound = count, -(-count // 32), count + 7
+    b.tables = np.concatenate([b.tables, np.full((1, 20), -7, np.int32)], 1)
+    b.stride += 20
+    b.upload()
+    check(b)

@@ -100,7 +100,7 @@ def test_shapes_refused(change, want, message):
     ({"sequences": 65536}, "arg", "65536 sequences"), ({"rows": -1}, "arg", "rows"), ({"most_rows": 9}, "arg", "at most 9 rows"), ({"most_rows": -1}, "arg", "rows"), ({"rows": 1 << 24}, "shape", "at most 16777215"),
     ({"depths": 16}, "arg", "masks and depths"), ({"masks": 16, "mask_words": 1}, "arg", "masks and depths"), ({**TREE, "mask_words": 0}, "shape", "0 mask words"),
     ({**TREE, "rows": 40, "most_rows": 33}, "shape", "do not hold 33"), ({**TREE, "mask_words": 2**31 - 1}, "shape", "mask words"),
-    ({"table_stride": 0}, "arg", "table_stride"), ({"key_bound": 4}, "arg", "key bound 4"), ({"key_bound": 129}, "arg", "128 tokens"),
+    ({"table_stride": 0}, "arg", "table_stride"), ({"key_bound": 4}, "arg", "key bound 4"), ({"key_bound": 129}, "arg", "128 tokens"), ({"key_bound": (1 << 30) + 1, "table_stride": 1 << 30}, "shape", "key bound 1073741825"),
 ])
 def test_batches_refused(change, want, message):
     from kotensor_amd import _lib
