@@ -14,8 +14,8 @@ constexpr int THREADS = 256;
 // ---- RoPE and the append ---------------------------------------------------------------
 // A wave takes one row and HEADS heads a lane of it: lane (pair i, head of 128 / head_dim side by side); its cosine and
 // sine serve all its heads, whose loads go out together. Waves of query heads write the rotated query, waves of
-// kv heads the key and the value.
-constexpr int HEADS = 8;
+// kv heads the key and the value. Bound by its bytes: five prompts of up to 1001 tokens, 32 and 8 heads of 128, fp32: 200 MB in 45 us,
+// 4.5 TB/s; one token of 16 sequences by its launch and three loads that wait for each other (starts, lengths, table): 4 us.
 struct AppendArgs {
     const float* q;  // NULL: only the append
     const float* k;
@@ -38,7 +38,7 @@ __device__ __forceinline__ int32_t sequence_of(const BatchView& b, int32_t row) 
     return s;
 }
 
-template <int FMT>
+template <int FMT, int HEADS>
 __global__ void __launch_bounds__(THREADS) append_kernel(AppendArgs a) {
     const PagedView& c = a.c;
     const int32_t HD = c.head_dim, half = HD >> 1, lane = threadIdx.x & 63;
@@ -73,7 +73,7 @@ __global__ void __launch_bounds__(THREADS) append_kernel(AppendArgs a) {
 #pragma unroll
         for (int u = 0; u < HEADS; ++u) {
             const int32_t h = h0 + u * side;
-            if (h >= heads) break;
+            if (h >= heads) continue;
             float y1, y2;
             rope_apply(x1[u], x2[u], cf, sf, y1, y2);
             if (is_q) {
@@ -82,7 +82,7 @@ __global__ void __launch_bounds__(THREADS) append_kernel(AppendArgs a) {
                 out[half] = y2;
             } else {
                 const int64_t at = place_of(c, a.b, s, slot, h);
-                if (at < 0) break;
+                if (at < 0) continue;
                 store_element<FMT>(c.keys, at + i, y1);
                 store_element<FMT>(c.keys, at + i + half, y2);
                 store_element<FMT>(c.values, at + i, v1[u]);
@@ -92,21 +92,29 @@ __global__ void __launch_bounds__(THREADS) append_kernel(AppendArgs a) {
     }
 }
 
-int32_t launch_append(AppendArgs a, hipStream_t st) {
-    const int32_t side = a.c.head_dim < 128 ? 128 / a.c.head_dim : 1;
+template <int HEADS>
+int32_t launch_append_of(AppendArgs a, int32_t side, hipStream_t st) {
     a.q_groups = a.q ? ceil_div(a.num_heads, HEADS * side) : 0;
     a.groups = a.q_groups + ceil_div(a.c.kv_heads, HEADS * side);
     const int64_t grid = (static_cast<int64_t>(a.b.rows) * a.groups + THREADS / 64 - 1) / (THREADS / 64);
     if (grid > INT32_MAX) return fail(KT_ERR_SHAPE, "too many rows and heads in one call");
-    const auto kernel = a.c.fmt == KT_PAGED_F32 ? append_kernel<KT_PAGED_F32> : a.c.fmt == KT_PAGED_F16 ? append_kernel<KT_PAGED_F16> : append_kernel<KT_PAGED_BF16>;
+    const auto kernel = a.c.fmt == KT_PAGED_F32 ? append_kernel<KT_PAGED_F32, HEADS> : a.c.fmt == KT_PAGED_F16 ? append_kernel<KT_PAGED_F16, HEADS> : append_kernel<KT_PAGED_BF16, HEADS>;
     kernel<<<static_cast<uint32_t>(grid), THREADS, 0, st>>>(a);
     KT_LAUNCHED("paged cache append kernel");
     return KT_OK;
 }
 
+int32_t launch_append(const AppendArgs& a, hipStream_t st) {
+    const int32_t side = a.c.head_dim < 128 ? 128 / a.c.head_dim : 1;
+    const int64_t waves = static_cast<int64_t>(a.b.rows) * ((a.q ? ceil_div(a.num_heads, 8 * side) : 0) + ceil_div(a.c.kv_heads, 8 * side));
+    // eight heads a wave, whose cosines are made once, where that makes 16 waves a CU; else two (16 trees of up to 64, 8 heads of 128: 5.5 us
+    // for 6.7; a token of 16 sequences 4.0 for 5.0)
+    return waves < 16 * cu_count() ? launch_append_of<2>(a, side, st) : launch_append_of<8>(a, side, st);
+}
+
 // ---- trees -------------------------------------------------------------------------------
 // Workgroup: a sequence; thread: a row of it, which walks from parent to parent. A parent comes before its
-// row (any other is none), so the walk ends, and meets the words of its mask in descending order.
+// row (any other is none), so the walk ends, and meets the words of its mask in descending order. Latencies: 2 to 5 us.
 constexpr int32_t TREE_LDS = 4096;  // parents held in LDS
 __global__ void __launch_bounds__(THREADS) masks_kernel(const int32_t* parents, BatchView b, int32_t* depths, uint32_t* masks) {
     __shared__ int32_t held[TREE_LDS];
@@ -133,7 +141,7 @@ __global__ void __launch_bounds__(THREADS) masks_kernel(const int32_t* parents, 
     }
 }
 
-constexpr int32_t ACCEPT_LDS = 1024;  // rows whose numbers are held in LDS (a step of the walk reads three, one after another)
+constexpr int32_t ACCEPT_LDS = 1024;  // rows whose numbers are held in LDS (a step of the walk reads three, one after another: 2.0 us for 4.0 from memory)
 // One wave a sequence: from row 0 to the first row whose parent is the last one kept and whose token is
 // the one chosen after that, as long as there is one.
 __global__ void __launch_bounds__(64) accept_kernel(const int32_t* tokens, const int32_t* chosen, const int32_t* parents, BatchView b,
@@ -194,7 +202,8 @@ __device__ __forceinline__ int32_t kept_count(const int32_t* kept, int32_t count
 }
 
 // Thread: 16 bytes of a head's keys or values in one layer, which it moves for every kept row in turn (a row
-// moves down or stays, so no row is overwritten before it is read), several loads ahead.
+// moves down or stays, so no row is overwritten before it is read), several loads ahead. Latencies (counts, kept rows, table,
+// rows): 4.6 us for one tree of 15 in two layers, 6.0 for 16 of up to 64 in eight.
 constexpr int AHEAD = 8;
 template <int BYTES>
 __global__ void __launch_bounds__(THREADS) keep_kernel(PagedView c, size_t layer_bytes, int32_t pieces, BatchView b, const int32_t* kept, int32_t kept_stride,

@@ -6,18 +6,22 @@
 // tile's keys are cut into parts of about the same number of chunks for all sequences of the launch, whatever
 // their lengths: every workgroup reads the sequences' rows and lengths, from which follow the parts'
 // size and its own place among them, so that one long sequence beside short ones fills the card. A workgroup holds
-// its rows' queries as matrix operands, its waves take the part's chunks of 32 keys in turn, straight from memory into
-// registers: no LDS and no barrier in the loop.
+// its rows' queries as matrix operands and goes through its part's chunks of keys:
 //   S^T = K Q^T: a lane ends with scores of one row (its column), so that the running maximum and sum of a
 //     row stay inside the lanes of a column.
-//   O^T += V^T P^T: a lane loads its dims of the tokens whose weights it holds, and turns them in registers.
+//   O^T += V^T P^T: the weights are operands where they are.
 // Products in fp32 precision: numbers held in fp16 are one operand and queries and weights two fp16 ones (to
 // 2^-22 of a row's largest query, 2^-30 of its largest weight); held in bf16 one operand and three bf16 ones (exact);
 // fp32 three each, of whose nine products the six down to 2^-17 are formed (kt_split.h).
-// A wave's maximum follows a row's lazily: a larger score moves it only once it is 2^8 above, so that the sums are
-// seldom rescaled. Waves' sums meet in LDS; parts' through memory, where the last workgroup of a tile to
-// arrive (a counter, which it returns to zero) merges all in their order: no workgroup waits for
-// another, and the bits do not depend on who is last.
+// A row's maximum follows its scores lazily: a larger one moves it only once it is 2^8 above, so that the sums are
+// seldom rescaled. Parts meet through memory: of tiles of 16 rows the last workgroup of a tile to arrive (a counter, which it
+// returns to zero) merges all in their order, so that no workgroup waits for another and the bits do not depend on who
+// is last; of larger tiles a launch of its own does.
+// Two kernels: attention_kernel for few rows, bound by the cache's bytes (64 steps over 2048 tokens on average, 128 dims, bf16: 111 us,
+// 4.9 TB/s; one of 131000 beside seven shorter, fp16: 86 us, 5.1 TB/s; a large copy runs at 4.8), with short texts by the chain of loads from
+// the lengths to the merge (12 us); tile_kernel for many, bound by the vector and matrix instructions of two waves a SIMD that wait for
+// each other's chunks (a prompt of 2048, 128 dims, bf16: 110 us, 312 TFLOP/s of attention, 936 of matrix products, of which a
+// large library product reaches 1112), with few chunks by a part's beginning, 7 to 10 us.
 #pragma once
 
 #include <algorithm>
@@ -619,7 +623,11 @@ __global__ void __launch_bounds__(256) merge_kernel(Args a) {
 }
 
 // ---- few rows, and few keys --------------------------------------------------------------------------
-// R = 16 rows a workgroup on 16x16x32.
+// R = 16 rows a workgroup on 16x16x32. Its four waves take the part's chunks of 32 keys in turn, straight from memory into registers,
+// no LDS and no barrier in the loop: a lane loads its dims of the tokens whose weights it will hold, and turns them there. The
+// next chunk's keys are on their way while a chunk's weights and output are formed, its values while the next scores are.
+// STEP: the tokens are rotated, appended and attended to in this launch: every workgroup makes its own rotated query, key and
+// value, the last part's also writes them to the cache, and its wave with the token's chunk takes them from LDS.
 template <int FMT, int HD>
 struct Shape {
     static constexpr int R = 16, NW = 4, LEAST = NW;          // a part has a chunk for each wave
@@ -1032,15 +1040,15 @@ __global__ void __launch_bounds__((64 * Shape<FMT, HD>::NW), (HD == 256 || (FMT 
 // ---- many rows ---------------------------------------------------------------------------------------
 // 16 rows a wave on 16x16x32. The workgroup's threads load a chunk of keys ahead and lay it out in LDS, where all its waves
 // read it: the keys as rows, the values as dims with their tokens in the order of the operands; fp32 ones split into their
-// parts once for all waves. Queries stay in registers.
+// parts once for all waves. Queries stay in registers; operands of the next step are on their way from LDS while a step's products run.
 template <int FMT, int HD, int WAVES>
 struct Tile {
     static constexpr int NW = WAVES, R = 16 * NW, THREADS = 64 * NW;
     // waves a SIMD that leave a wave the registers it needs (of 256 dims with two: 352 bytes and more in scratch memory)
     static constexpr int MW = NW == 8 ? 2 : HD == 256 ? 1 : HD <= 64 && FMT != KT_PAGED_F32 ? 3 : 2;
     static constexpr int KP = Format<FMT>::KP, QP = Format<FMT>::QP, E = Format<FMT>::E;
-    // keys of a chunk: half the barriers with 64 (at 64 dims a prompt of 1024 in fp16 36 us for 39, of 2048 in fp32 124 for 134; bf16 76 for 75),
-    // where the registers and LDS allow it
+    // keys of a chunk: half the barriers with 64 (against 32 at 64 dims: a prompt of 1024 in fp16 36 us for 39, of 2048 in fp32 124 for 134, in
+    // bf16 76 for 75), where the registers and LDS allow it
     static constexpr int CH = HD == 256 || (FMT == KT_PAGED_F32 && HD == 128) ? 32 : 64, SETS = CH / 32;
     static constexpr int QS = HD / 32, DB = HD / 16;
     static constexpr int KR = HD + 8, VR = CH + 8;  // padded rows: of a key, of a dim (2-byte elements)
@@ -1399,6 +1407,8 @@ template <int FMT, int HD, bool STEP>
 int32_t launch_rows(Args a, hipStream_t st) {
     using X = Shape<FMT, HD>;
     int64_t grid = 0;
+    // four parts a CU (64 steps over 2048 tokens on average / one of 131000 beside seven: 2 parts 117 / 97 us, 3 112 / 92, 4 113 / 87,
+    // 6 115 / 88, 8 115 / 90)
     if (const int32_t status = prepare<HD, X::R, X::LEAST, CHUNK>(a, 4 * cu_count(), &grid, st)) return status;
     constexpr size_t lds = std::max(std::max(sizeof(float) * X::NW * X::R * (HD + 6), size_t{2} * Format<FMT>::QP * X::R * (HD + 8)), merge_lds(X::R, X::NW));
     if (const int32_t ls = allow_lds<&attention_kernel<FMT, HD, STEP>, lds>(lds)) return ls;
@@ -1422,18 +1432,18 @@ int32_t launch_tiles(Args a, hipStream_t st) {
 }
 
 // Which kernel (us here: head dims of 128 unless said, 32 heads on 8 kv heads, one sequence unless said; the kernel taken first):
-//   up to 16 rows of a kv head: tiles of 16, keys straight into registers. A tree of 4 tokens has no use for more.
+//   up to 16 rows of a kv head: tiles of 16. (A tree of 4 tokens has no use for more.)
 //   up to 128 keys: the same for any number of rows, as its waves have a chunk each: no parts to merge, and four
-//     times the workgroups. A prompt of 128: fp16 11.0 against 12.9, fp32 12.6 against 21.7, fp16 at 64 dims 6.7 against 8.6.
+//     times the workgroups. A prompt of 128: fp16 10.7 against 12.9, fp32 12.4 against 21.7, fp16 at 64 dims 6.7 against 8.6.
 //     Not fp32 at 256 dims, whose operands do not fit the registers: a prompt of 128 54.8 against 35.9 with tiles of 64, a token
 //     after 20000 247 against 169 (only 64 sequences of 2000 tokens would be 848 against 877).
 //   up to 64 rows: tiles of 64, so that no wave is idle, two workgroups a CU: 16 sequences with trees of 15 after 2000 tokens 41
-//     against 54 with tiles of 128 (fp32 76 against 95); one tree of 15 after 4000 30 and 30.
-//   up to 64 dims in 16 bits: tiles of 64 for any number of rows, of which three workgroups share a CU (a prompt of 2048: 63).
-//   else: tiles of 128, as the chunk that eight waves share is half the loads and LDS writes a row: a prompt of 2048 102 (fp16),
-//     115 (bf16), 210 (fp32); a tree of 60 in fp32 53 against 63.
-//   256 dims: tiles of 64 whose waves have a SIMD's registers each: a prompt of 512 44 against 50 with tiles of
-//     128 (bf16 48 against 69, fp32 120 against 169).
+//     against 54 with tiles of 128 (fp32 76 against 95); one tree of 15 after 4000 29 and 30.
+//   up to 64 dims in 16 bits: tiles of 64 for any number of rows, of which three workgroups share a CU: a prompt of 2048 62 (fp16).
+//   else: tiles of 128, as the chunk that eight waves share is half the loads and LDS writes a row: a prompt of 2048 97 (fp16),
+//     110 (bf16), 205 (fp32); a tree of 60 in fp32 53 against 63 with tiles of 64.
+//   256 dims: tiles of 64 whose waves have a SIMD's registers each: a prompt of 512 41 against 50 with tiles of
+//     128 (bf16 44 against 69, fp32 116 against 169).
 template <int FMT, int HD>
 int32_t launch_dims(const Args& a, hipStream_t st) {
     const int64_t rows = static_cast<int64_t>(a.p.b.most_rows) * (a.p.num_heads / a.p.c.kv_heads);
