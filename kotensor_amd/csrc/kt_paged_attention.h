@@ -375,27 +375,31 @@ __device__ __forceinline__ Keys keys_of(const Args& a, const Part& part, int32_t
 }
 
 // A chunk's runs of 16 tokens, each in one page: their pages, then where they begin (bytes from the layer's keys or values)
-// and which tokens there are, a bit each.
-template <int CHUNK>
+// and which tokens there are, a bit each. WHOLE: pages hold whole chunks, so that one look into the table is enough.
+template <int CHUNK, bool WHOLE>
 struct Pages {
-    int32_t page[CHUNK / 16];
+    int32_t page[WHOLE ? 1 : CHUNK / 16];
 };
-template <int CHUNK>
+template <int CHUNK, bool WHOLE>
 struct Where {
-    size_t base[CHUNK / 16];
+    size_t base[WHOLE ? 1 : CHUNK / 16];
     uint32_t there[CHUNK / 32];
     // where run `run` begins (selects between the scalars: an index would go through scratch memory)
-    __device__ __forceinline__ size_t of_run(int32_t run) const {
-        const size_t low = pick(run & 1, base[0], base[1]);
-        if constexpr (CHUNK == 32) return low;
-        else return pick(run & 2, low, pick(run & 1, base[2], base[3]));
+    __device__ __forceinline__ size_t of_run(int32_t run, int32_t row_bytes) const {
+        if constexpr (WHOLE) {
+            return base[0] + static_cast<uint32_t>(16 * run * row_bytes);
+        } else {
+            const size_t low = pick(run & 1, base[0], base[1]);
+            if constexpr (CHUNK == 32) return low;
+            else return pick(run & 2, low, pick(run & 1, base[2], base[3]));
+        }
     }
     static __device__ __forceinline__ size_t pick(int32_t second, size_t a, size_t b) {
         const uint32_t low = second ? static_cast<uint32_t>(b) : static_cast<uint32_t>(a), high = second ? static_cast<uint32_t>(b >> 32) : static_cast<uint32_t>(a >> 32);
         return static_cast<size_t>(high) << 32 | low;
     }
 };
-template <int CHUNK>
+template <int CHUNK, bool WHOLE>
 struct PageReader {
     typedef const __attribute__((address_space(4))) int32_t* table_t;  // (read-only, by uniform indexes)
     table_t table;
@@ -407,23 +411,30 @@ struct PageReader {
         head_bytes = (static_cast<size_t>(part.head) << page_shift) * row_bytes;
         page_bytes = (static_cast<size_t>(c.kv_heads) << page_shift) * row_bytes;
     }
-    __device__ __forceinline__ Pages<CHUNK> pages_of(int32_t ch) const {
-        Pages<CHUNK> p;
+    __device__ __forceinline__ Pages<CHUNK, WHOLE> pages_of(int32_t ch) const {
+        Pages<CHUNK, WHOLE> p;
 #pragma unroll
-        for (int h = 0; h < CHUNK / 16; ++h) p.page[h] = table[min((ch * CHUNK + 16 * h) >> page_shift, last_entry)];
+        for (int h = 0; h < (WHOLE ? 1 : CHUNK / 16); ++h) p.page[h] = table[min((ch * CHUNK + 16 * h) >> page_shift, last_entry)];
         return p;
     }
-    __device__ __forceinline__ Where<CHUNK> where_of(int32_t ch, const Pages<CHUNK>& p) const {
-        Where<CHUNK> w;
+    __device__ __forceinline__ Where<CHUNK, WHOLE> where_of(int32_t ch, const Pages<CHUNK, WHOLE>& p) const {
+        constexpr int RUN = WHOLE ? CHUNK : 16;
+        Where<CHUNK, WHOLE> w;
 #pragma unroll
-        for (int h = 0; h < CHUNK / 16; ++h) {
-            const int32_t x = ch * CHUNK + 16 * h;
+        for (int h = 0; h < CHUNK / RUN; ++h) {
+            const int32_t x = ch * CHUNK + RUN * h;
             const bool fine = static_cast<uint32_t>(p.page[h]) < static_cast<uint32_t>(pages);
             const size_t page = fine ? p.page[h] : 0;  // (any memory of the pool)
             w.base[h] = page * page_bytes + head_bytes + static_cast<uint32_t>((x & ((1 << page_shift) - 1)) * row_bytes);
-            const int32_t m = min(max(n_keys - x, 0), 16);
-            if (h % 2 == 0) w.there[h / 2] = 0;
-            w.there[h / 2] |= (fine ? (1u << m) - 1u : 0u) << (16 * (h % 2));
+            if constexpr (WHOLE) {
+                const int32_t left = fine ? n_keys - x : 0;
+#pragma unroll
+                for (int i = 0; i < CHUNK / 32; ++i) w.there[i] = left >= 32 * i + 32 ? 0xFFFFFFFFu : left <= 32 * i ? 0u : (1u << (left - 32 * i)) - 1u;
+            } else {
+                const int32_t m = min(max(n_keys - x, 0), 16);
+                if (h % 2 == 0) w.there[h / 2] = 0;
+                w.there[h / 2] |= (fine ? (1u << m) - 1u : 0u) << (16 * (h % 2));
+            }
         }
         return w;
     }
@@ -741,10 +752,10 @@ __global__ void __launch_bounds__((64 * Shape<FMT, HD>::NW), (HD == 256 || (FMT 
     if (part.split >= keys.splits) return;
     const int32_t splits = keys.splits, c0 = keys.c0, c1 = keys.c1, n_all = keys.n_all;
     const int64_t new_first = part.length;
-    const PageReader<CHUNK> reader(c, b, part, keys.n_keys, F::E);
+    const PageReader<CHUNK, false> reader(c, b, part, keys.n_keys, F::E);
 
     uint32_t kr[2][X::QS][X::KW], vr[8][X::VW];
-    auto load_keys = [&](const Where<CHUNK>& w) {
+    auto load_keys = [&](const Where<CHUNK, false>& w) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             const uint8_t* p = c.keys + w.base[t] + (col * HD + 8 * grp) * F::E;
@@ -754,7 +765,7 @@ __global__ void __launch_bounds__((64 * Shape<FMT, HD>::NW), (HD == 256 || (FMT 
     };
     // the token of a lane's value (or weight) e
     auto token_of = [&](int e) { return 16 * (e >> 2) + 4 * grp + (e & 3); };
-    auto load_values = [&](const Where<CHUNK>& w) {
+    auto load_values = [&](const Where<CHUNK, false>& w) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) load_words(c.values + w.base[e >> 2] + ((token_of(e) & 15) * HD + col * X::DB) * F::E, vr[e]);
     };
@@ -774,8 +785,8 @@ __global__ void __launch_bounds__((64 * Shape<FMT, HD>::NW), (HD == 256 || (FMT 
         }
     };
     int32_t ch = c0 + wave;
-    Where<CHUNK> here{};
-    Pages<CHUNK> pages{};
+    Where<CHUNK, false> here{};
+    Pages<CHUNK, false> pages{};
     if (ch < c1) {
         here = reader.where_of(ch, reader.pages_of(ch));
         load_keys(here);
@@ -899,7 +910,7 @@ __global__ void __launch_bounds__((64 * Shape<FMT, HD>::NW), (HD == 256 || (FMT 
     // (two forms of the loop's body: only chunks that not every row sees whole compare keys with rows)
     auto attend_chunk = [&](auto masked_form) {
         constexpr bool masked = decltype(masked_form)::value;
-        const Where<CHUNK> now = here;
+        const Where<CHUNK, false> now = here;
         f4 sc[2] = {f4{0.0f, 0.0f, 0.0f, 0.0f}, f4{0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
         for (int s = 0; s < X::QS; ++s) {
@@ -1063,7 +1074,7 @@ struct Tile {
     static constexpr int VGROUP = FMT == KT_PAGED_F32 ? 2 : 4;
 };
 
-template <int FMT, int HD, int WAVES>
+template <int FMT, int HD, int WAVES, bool WHOLE>
 __global__ void __launch_bounds__((Tile<FMT, HD, WAVES>::THREADS), (Tile<FMT, HD, WAVES>::MW)) tile_kernel(Args a) {
     using F = Format<FMT>;
     using X = Tile<FMT, HD, WAVES>;
@@ -1089,7 +1100,7 @@ __global__ void __launch_bounds__((Tile<FMT, HD, WAVES>::THREADS), (Tile<FMT, HD
     const Keys keys = keys_of<R, CH>(a, part, held);
     if (part.split >= keys.splits) return;
     const int32_t c0 = keys.c0, c1 = keys.c1;
-    const PageReader<CH> reader(c, b, part, keys.n_keys, E);
+    const PageReader<CH, WHOLE> reader(c, b, part, keys.n_keys, E);
     if (tid < 2) odd_chunk[tid] = -1;
 
     // the chunk ahead: a thread's pieces of keys, and its four tokens of four dims
@@ -1107,29 +1118,29 @@ __global__ void __launch_bounds__((Tile<FMT, HD, WAVES>::THREADS), (Tile<FMT, HD
         dims = 4 * (e % (HD / 4));
         return e < CH / 4 * (HD / 4);
     };
-    auto load_chunk = [&](const Where<CH>& w) {
+    auto load_chunk = [&](const Where<CH, WHOLE>& w) {
 #pragma unroll
         for (int i = 0; i < X::KN; ++i) {
             int32_t key, piece;
             if (!key_item(i, key, piece)) break;
-            kr[i] = *reinterpret_cast<const u4*>(c.keys + w.of_run(uniform(key >> 4)) + ((key & 15) * HD * E + 16 * piece));
+            kr[i] = *reinterpret_cast<const u4*>(c.keys + w.of_run(uniform(key >> 4), HD * E) + ((key & 15) * HD * E + 16 * piece));
         }
 #pragma unroll
         for (int i = 0; i < X::VN; ++i) {
             int32_t quad, dims;
             if (!value_item(i, quad, dims)) break;
-            const uint8_t* p = c.values + w.of_run(HD >= 64 ? uniform(quad >> 2) : quad >> 2) + ((4 * quad & 15) * HD + dims) * E;
+            const uint8_t* p = c.values + w.of_run(HD >= 64 ? uniform(quad >> 2) : quad >> 2, HD * E) + ((4 * quad & 15) * HD + dims) * E;
 #pragma unroll
             for (int j = 0; j < 4; ++j) load_words(p + j * HD * E, vr[i][j]);
         }
     };
-    auto all_there = [&](const Where<CH>& w) { return w.there[0] == 0xFFFFFFFFu && w.there[X::SETS - 1] == 0xFFFFFFFFu; };
+    auto all_there = [&](const Where<CH, WHOLE>& w) { return w.there[0] == 0xFFFFFFFFu && w.there[X::SETS - 1] == 0xFFFFFFFFu; };
     // whether every row of the tile sees the chunk whole
-    auto whole = [&](int32_t ch, const Where<CH>& w) { return ch * CH + CH <= keys.n_all && all_there(w); };
+    auto whole = [&](int32_t ch, const Where<CH, WHOLE>& w) { return ch * CH + CH <= keys.n_all && all_there(w); };
     // where the 8 tokens of (set of 32, lane group) lie among a dim's: blocks turned by the dim, so that the lanes that write
     // neighbouring dims meet different banks
     auto block_of = [&](int32_t block, int32_t dim) { return 8 * (block ^ ((dim >> 2) & (CH / 8 - 1))); };
-    auto store_chunk = [&](int32_t ch, const Where<CH>& where) {
+    auto store_chunk = [&](int32_t ch, const Where<CH, WHOLE>& where) {
         element* kl = reinterpret_cast<element*>(lds) + (X::BUFFERS == 2 ? (ch & 1) * X::SIZE : 0);
         element* vl = kl + X::KP * X::KSIZE;
         // four numbers' parts
@@ -1194,8 +1205,8 @@ __global__ void __launch_bounds__((Tile<FMT, HD, WAVES>::THREADS), (Tile<FMT, HD
         }
     };
 
-    Where<CH> next{};
-    Pages<CH> pages{};
+    Where<CH, WHOLE> next{};
+    Pages<CH, WHOLE> pages{};
     if (c0 < c1) {
         next = reader.where_of(c0, reader.pages_of(c0));
         load_chunk(next);
@@ -1252,7 +1263,7 @@ __global__ void __launch_bounds__((Tile<FMT, HD, WAVES>::THREADS), (Tile<FMT, HD
     // what the wave's rows see: tokens below all of them, from none on nothing
     const int64_t see_all = b.masks ? static_cast<int64_t>(part.length) : static_cast<int64_t>(part.length) + first_token + 1;
     const int64_t see_none = b.masks ? INT64_MAX : static_cast<int64_t>(part.length) + last_token + 1;
-    auto attend_chunk = [&](auto masked_form, int32_t ch, const Where<CH>& where) {
+    auto attend_chunk = [&](auto masked_form, int32_t ch, const Where<CH, WHOLE>& where) {
         constexpr bool masked = decltype(masked_form)::value;
         const element* kl = reinterpret_cast<const element*>(lds) + (X::BUFFERS == 2 ? (ch & 1) * X::SIZE : 0);
         const element* vl = kl + X::KP * X::KSIZE;
@@ -1306,7 +1317,7 @@ __global__ void __launch_bounds__((Tile<FMT, HD, WAVES>::THREADS), (Tile<FMT, HD
                     if (!(there >> (tok & 31) & 1)) continue;
                     const uint32_t mine = seen_bits(b, part.first, token, part.length, ch * CH + (tok & ~31), there);
                     const int32_t from = tok >> 2 & 3, i = 8 * (tok >> 5) + 4 * (tok >> 4 & 1) + (tok & 3);
-                    const uint8_t* row = c.values + where.of_run(tok >> 4) + (tok & 15) * HD * E;
+                    const uint8_t* row = c.values + where.of_run(tok >> 4, HD * E) + (tok & 15) * HD * E;
                     float weight = 0.0f;
 #pragma unroll
                     for (int e = 0; e < 8 * X::SETS; ++e)
@@ -1341,7 +1352,7 @@ __global__ void __launch_bounds__((Tile<FMT, HD, WAVES>::THREADS), (Tile<FMT, HD
         settle();
     };
     for (int32_t ch = c0; ch < c1; ++ch) {
-        const Where<CH> now = next;
+        const Where<CH, WHOLE> now = next;
         if (ch + 1 < c1) {
             next = reader.where_of(ch + 1, pages);
             load_chunk(next);
@@ -1422,9 +1433,15 @@ int32_t launch_tiles(Args a, hipStream_t st) {
     using X = Tile<FMT, HD, WAVES>;
     int64_t grid = 0;
     if (const int32_t status = prepare<HD, X::R, X::LEAST, X::CH>(a, X::TARGET * cu_count(), &grid, st)) return status;
-    if (const int32_t ls = allow_lds<&tile_kernel<FMT, HD, WAVES>, X::LDS>(X::LDS)) return ls;
-    tile_kernel<FMT, HD, WAVES><<<static_cast<uint32_t>(grid), X::THREADS, X::LDS, st>>>(a);
-    KT_LAUNCHED("paged attention kernel");
+    const auto kernel = [&](auto whole) -> int32_t {
+        constexpr bool WHOLE = decltype(whole)::value;
+        if (const int32_t ls = allow_lds<&tile_kernel<FMT, HD, WAVES, WHOLE>, X::LDS>(X::LDS)) return ls;
+        tile_kernel<FMT, HD, WAVES, WHOLE><<<static_cast<uint32_t>(grid), X::THREADS, X::LDS, st>>>(a);
+        KT_LAUNCHED("paged attention kernel");
+        return KT_OK;
+    };
+    // pages that hold whole chunks have a form of their own (a prompt of 2048, pages of 64 / 16: bf16 at 128 dims 104 us / 111, fp32 at 64 dims 105 / 117)
+    if (const int32_t status = 1 << a.p.c.page_shift >= X::CH ? kernel(std::true_type{}) : kernel(std::false_type{})) return status;
     if (a.slots == 0) return KT_OK;
     merge_kernel<HD, X::R, X::LEAST, X::CH><<<dim3(static_cast<uint32_t>(a.slots), merge_shares(X::R)), 256, 0, st>>>(a);
     KT_LAUNCHED("paged attention merge kernel");
