@@ -385,14 +385,11 @@ struct Where {
     size_t base[WHOLE ? 1 : CHUNK / 16];
     uint32_t there[CHUNK / 32];
     // where run `run` begins (selects between the scalars: an index would go through scratch memory)
-    __device__ __forceinline__ size_t of_run(int32_t run, int32_t row_bytes) const {
-        if constexpr (WHOLE) {
-            return base[0] + static_cast<uint32_t>(16 * run * row_bytes);
-        } else {
-            const size_t low = pick(run & 1, base[0], base[1]);
-            if constexpr (CHUNK == 32) return low;
-            else return pick(run & 2, low, pick(run & 1, base[2], base[3]));
-        }
+    __device__ __forceinline__ size_t of_run(int32_t run) const {
+        static_assert(!WHOLE, "one run");
+        const size_t low = pick(run & 1, base[0], base[1]);
+        if constexpr (CHUNK == 32) return low;
+        else return pick(run & 2, low, pick(run & 1, base[2], base[3]));
     }
     static __device__ __forceinline__ size_t pick(int32_t second, size_t a, size_t b) {
         const uint32_t low = second ? static_cast<uint32_t>(b) : static_cast<uint32_t>(a), high = second ? static_cast<uint32_t>(b >> 32) : static_cast<uint32_t>(a >> 32);
@@ -1110,26 +1107,29 @@ __global__ void __launch_bounds__((Tile<FMT, HD, WAVES>::THREADS), (Tile<FMT, HD
         const int32_t e = tid + i * X::THREADS;
         key = e / X::PIECES;
         piece = e % X::PIECES;
-        return e < CH * X::PIECES;
+        return CH * X::PIECES % X::THREADS == 0 || e < CH * X::PIECES;
     };
     auto value_item = [&](int i, int32_t& quad, int32_t& dims) {
         const int32_t e = tid + i * X::THREADS;
         quad = e / (HD / 4);
         dims = 4 * (e % (HD / 4));
-        return e < CH / 4 * (HD / 4);
+        return CH / 4 * (HD / 4) % X::THREADS == 0 || e < CH / 4 * (HD / 4);
     };
     auto load_chunk = [&](const Where<CH, WHOLE>& w) {
 #pragma unroll
         for (int i = 0; i < X::KN; ++i) {
             int32_t key, piece;
             if (!key_item(i, key, piece)) break;
-            kr[i] = *reinterpret_cast<const u4*>(c.keys + w.of_run(uniform(key >> 4), HD * E) + ((key & 15) * HD * E + 16 * piece));
+            if constexpr (WHOLE) kr[i] = *reinterpret_cast<const u4*>(c.keys + w.base[0] + static_cast<uint32_t>(key * HD * E + 16 * piece));
+            else kr[i] = *reinterpret_cast<const u4*>(c.keys + w.of_run(uniform(key >> 4)) + static_cast<uint32_t>((key & 15) * HD * E + 16 * piece));
         }
 #pragma unroll
         for (int i = 0; i < X::VN; ++i) {
             int32_t quad, dims;
             if (!value_item(i, quad, dims)) break;
-            const uint8_t* p = c.values + w.of_run(HD >= 64 ? uniform(quad >> 2) : quad >> 2, HD * E) + ((4 * quad & 15) * HD + dims) * E;
+            const uint8_t* p;
+            if constexpr (WHOLE) p = c.values + w.base[0] + static_cast<uint32_t>((4 * quad * HD + dims) * E);
+            else p = c.values + w.of_run(HD >= 64 ? uniform(quad >> 2) : quad >> 2) + static_cast<uint32_t>(((4 * quad & 15) * HD + dims) * E);
 #pragma unroll
             for (int j = 0; j < 4; ++j) load_words(p + j * HD * E, vr[i][j]);
         }
@@ -1262,7 +1262,9 @@ __global__ void __launch_bounds__((Tile<FMT, HD, WAVES>::THREADS), (Tile<FMT, HD
     const int32_t first_token = uniform((row0 + 16 * wave) / G), last_token = uniform((row0 + min(16 * wave + 15, held - 1)) / G);
     // what the wave's rows see: tokens below all of them, from none on nothing
     const int64_t see_all = b.masks ? static_cast<int64_t>(part.length) : static_cast<int64_t>(part.length) + first_token + 1;
-    const int64_t see_none = b.masks ? INT64_MAX : static_cast<int64_t>(part.length) + last_token + 1;
+    const int64_t see_none = b.masks ? INT64_MAX - CH : static_cast<int64_t>(part.length) + last_token + 1;
+    const int32_t all_upto = uniform(static_cast<int32_t>(min(max(see_all, int64_t{0}) / CH, int64_t{c1})));              // chunks before which all is seen
+    const int32_t none_from = uniform(active ? static_cast<int32_t>(min((max(see_none, int64_t{0}) + CH - 1) / CH, int64_t{c1})) : 0);  // and from which nothing is
     auto attend_chunk = [&](auto masked_form, int32_t ch, const Where<CH, WHOLE>& where) {
         constexpr bool masked = decltype(masked_form)::value;
         const element* kl = reinterpret_cast<const element*>(lds) + (X::BUFFERS == 2 ? (ch & 1) * X::SIZE : 0);
@@ -1317,7 +1319,9 @@ __global__ void __launch_bounds__((Tile<FMT, HD, WAVES>::THREADS), (Tile<FMT, HD
                     if (!(there >> (tok & 31) & 1)) continue;
                     const uint32_t mine = seen_bits(b, part.first, token, part.length, ch * CH + (tok & ~31), there);
                     const int32_t from = tok >> 2 & 3, i = 8 * (tok >> 5) + 4 * (tok >> 4 & 1) + (tok & 3);
-                    const uint8_t* row = c.values + where.of_run(tok >> 4, HD * E) + (tok & 15) * HD * E;
+                    const uint8_t* row = c.values + tok % (WHOLE ? CH : 16) * HD * E;
+                    if constexpr (WHOLE) row += where.base[0];
+                    else row += where.of_run(tok >> 4);
                     float weight = 0.0f;
 #pragma unroll
                     for (int e = 0; e < 8 * X::SETS; ++e)
@@ -1359,8 +1363,8 @@ __global__ void __launch_bounds__((Tile<FMT, HD, WAVES>::THREADS), (Tile<FMT, HD
             pages = reader.pages_of(min(ch + 2, c1 - 1));
         }
         __syncthreads();  // the chunk is in LDS
-        if (active && static_cast<int64_t>(ch) * CH < see_none) {
-            if (static_cast<int64_t>(ch) * CH + CH <= see_all && all_there(now)) attend_chunk(std::false_type{}, ch, now);
+        if (ch < none_from) {
+            if (ch < all_upto && all_there(now)) attend_chunk(std::false_type{}, ch, now);
             else attend_chunk(std::true_type{}, ch, now);
         }
         if constexpr (X::BUFFERS == 1) __syncthreads();  // (and read by all)
