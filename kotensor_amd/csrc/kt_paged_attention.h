@@ -1068,7 +1068,7 @@ struct Tile {
     static constexpr size_t LDS = size_t{2} * SIZE * BUFFERS;
     static constexpr int LEAST = 128 / CH;
     static constexpr int TARGET = NW == 4 && HD < 256 ? 2 : 1;  // workgroups a CU among which the launch's chunks are shared out
-    static constexpr int VGROUP = FMT == KT_PAGED_F32 ? 2 : 4;
+    static constexpr int VGROUP = FMT != KT_PAGED_F32 ? 4 : HD == 128 ? 1 : 2;  // (fp32 at 128 dims, which spills least with one: a prompt of 2048 211 us for 220)
 };
 
 template <int FMT, int HD, int WAVES, bool WHOLE>
