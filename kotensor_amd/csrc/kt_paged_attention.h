@@ -1137,9 +1137,9 @@ __global__ void __launch_bounds__((Tile<FMT, HD, WAVES>::THREADS), (Tile<FMT, HD
     auto all_there = [&](const Where<CH, WHOLE>& w) { return w.there[0] == 0xFFFFFFFFu && w.there[X::SETS - 1] == 0xFFFFFFFFu; };
     // whether every row of the tile sees the chunk whole
     auto whole = [&](int32_t ch, const Where<CH, WHOLE>& w) { return ch * CH + CH <= keys.n_all && all_there(w); };
-    // where the 8 tokens of (set of 32, lane group) lie among a dim's: blocks turned by the dim, so that the lanes that write
-    // neighbouring dims meet different banks
-    auto block_of = [&](int32_t block, int32_t dim) { return 8 * (block ^ ((dim >> 2) & (CH / 8 - 1))); };
+    // where the 8 tokens of (set of 32, lane group) lie among a dim's: blocks turned by the dim's block of 16, so that the lanes that write
+    // every fourth dim meet different banks, and those that read a block's dims still do
+    auto block_of = [&](int32_t block, int32_t dim) { return 8 * (block ^ ((dim >> 4) & (CH / 8 - 1))); };
     auto store_chunk = [&](int32_t ch, const Where<CH, WHOLE>& where) {
         element* kl = reinterpret_cast<element*>(lds) + (X::BUFFERS == 2 ? (ch & 1) * X::SIZE : 0);
         element* vl = kl + X::KP * X::KSIZE;
