@@ -1265,8 +1265,7 @@ __global__ void __launch_bounds__((Tile<FMT, HD, WAVES>::THREADS), (Tile<FMT, HD
     const int64_t see_none = b.masks ? INT64_MAX - CH : static_cast<int64_t>(part.length) + last_token + 1;
     const int32_t all_upto = uniform(static_cast<int32_t>(min(max(see_all, int64_t{0}) / CH, int64_t{c1})));              // chunks before which all is seen
     const int32_t none_from = uniform(active ? static_cast<int32_t>(min((max(see_none, int64_t{0}) + CH - 1) / CH, int64_t{c1})) : 0);  // and from which nothing is
-    auto attend_chunk = [&](auto masked_form, int32_t ch, const Where<CH, WHOLE>& where) {
-        constexpr bool masked = decltype(masked_form)::value;
+    auto attend_chunk = [&](bool masked, int32_t ch, const Where<CH, WHOLE>& where) {
         const element* kl = reinterpret_cast<const element*>(lds) + (X::BUFFERS == 2 ? (ch & 1) * X::SIZE : 0);
         const element* vl = kl + X::KP * X::KSIZE;
         // (operands of the next step are on their way from LDS while a step's products run)
@@ -1304,11 +1303,16 @@ __global__ void __launch_bounds__((Tile<FMT, HD, WAVES>::THREADS), (Tile<FMT, HD
         float x[8 * X::SETS];
 #pragma unroll
         for (int i = 0; i < 8 * X::SETS; ++i) x[i] = sc[i >> 2][i & 3];
-        uint32_t vis[X::SETS] = {};
-        if constexpr (masked)
+        if (masked) {  // (a score of -infinity has no weight)
 #pragma unroll
-            for (int h = 0; h < X::SETS; ++h) vis[h] = seen_bits(b, part.first, token, part.length, ch * CH + 32 * h, where.there[h]);
-        to_weights<FMT, masked>(x, f, m, l, [&](int i) { return !(vis[i >> 3] >> token_of(i & 7) & 1); }, [&](float alpha) {
+            for (int h = 0; h < X::SETS; ++h) {
+                const uint32_t vis = seen_bits(b, part.first, token, part.length, ch * CH + 32 * h, where.there[h]);
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (!(vis >> token_of(i) & 1)) x[8 * h + i] = -INFINITY;
+            }
+        }
+        to_weights<FMT, false>(x, f, m, l, [](int) { return false; }, [&](float alpha) {
 #pragma unroll
             for (int db = 0; db < X::DB; ++db) o[db / VG][db % VG] *= alpha;
         });
@@ -1364,8 +1368,7 @@ __global__ void __launch_bounds__((Tile<FMT, HD, WAVES>::THREADS), (Tile<FMT, HD
         }
         __syncthreads();  // the chunk is in LDS
         if (ch < none_from) {
-            if (ch < all_upto && all_there(now)) attend_chunk(std::false_type{}, ch, now);
-            else attend_chunk(std::true_type{}, ch, now);
+            attend_chunk(ch >= all_upto || !all_there(now), ch, now);
         }
         if constexpr (X::BUFFERS == 1) __syncthreads();  // (and read by all)
         if (ch + 1 < c1) store_chunk(ch + 1, next);
