@@ -171,17 +171,13 @@ __device__ __forceinline__ float share_of(float m, float l, float mx) {
 }
 
 // A chunk's scores x of one row (a lane's share of them) into weights; m and l: the row's running maximum and the sum of this
-// lane's weights; rescale: what the maximum's move does to the sums; is_hidden: whether the row does not see score i's token.
-template <int FMT, bool masked, int E, typename HIDDEN, typename RESCALE>
-__device__ __forceinline__ void to_weights(float (&x)[E], float f, float& m, float& l, HIDDEN is_hidden, RESCALE rescale) {
+// lane's weights; rescale: what the maximum's move does to the sums. Tokens that the row does not see come with -infinity.
+template <int FMT, int E, typename RESCALE>
+__device__ __forceinline__ void to_weights(float (&x)[E], float f, float& m, float& l, RESCALE rescale) {
     constexpr float UP = Format<FMT>::UP;
-    auto hidden = [&](int i) { return masked && is_hidden(i); };
     float most = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-        if (hidden(i)) x[i] = -INFINITY;
-        most = fmaxf(most, x[i]);
-    }
+    for (int i = 0; i < E; ++i) most = fmaxf(most, x[i]);
     most = rounded_score(most, f);
     if (__ballot(most - m > LAZY)) {
         const float m_new = fmaxf(m, column_max(most));
@@ -199,10 +195,7 @@ __device__ __forceinline__ void to_weights(float (&x)[E], float f, float& m, flo
         for (int i = 0; i < E; ++i) x[i] = __builtin_amdgcn_exp2f(fmaf(x[i], f, UP - at));
     }
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-        if (hidden(i)) x[i] = 0.0f;  // (of a row with an infinite maximum)
-        l += x[i];
-    }
+    for (int i = 0; i < E; ++i) l += x[i];
 }
 
 // The tokens x0 .. x0 + 31 that row `index` of a sequence's rows sees, a bit each.
@@ -904,9 +897,8 @@ __global__ void __launch_bounds__((64 * Shape<FMT, HD>::NW), (HD == 256 || (FMT 
             to_operands<FMT>(w, v);
         }
     };
-    // (two forms of the loop's body: only chunks that not every row sees whole compare keys with rows)
-    auto attend_chunk = [&](auto masked_form) {
-        constexpr bool masked = decltype(masked_form)::value;
+    // (masked: not every row sees the chunk whole)
+    auto attend_chunk = [&](bool masked) {
         const Where<CHUNK, false> now = here;
         f4 sc[2] = {f4{0.0f, 0.0f, 0.0f, 0.0f}, f4{0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
@@ -933,15 +925,20 @@ __global__ void __launch_bounds__((64 * Shape<FMT, HD>::NW), (HD == 256 || (FMT 
         op p[F::QP];
         float x[8];
         uint32_t vis = 0;
-        if constexpr (masked) vis = seen_bits(b, part.first, token, new_first, ch * CHUNK, now.there[0]);
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = sc[i >> 2][i & 3];
-        to_weights<FMT, masked>(x, fr, m, l, [&](int i) { return !(vis >> token_of(i) & 1); }, [&](float alpha) {
+        if (masked) {  // (a score of -infinity has no weight)
+            vis = seen_bits(b, part.first, token, new_first, ch * CHUNK, now.there[0]);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (!(vis >> token_of(i) & 1)) x[i] = -INFINITY;
+        }
+        to_weights<FMT>(x, fr, m, l, [&](float alpha) {
 #pragma unroll
             for (int db = 0; db < X::DB; ++db) o[db] *= alpha;
         });
         split_weights(x, p);
-        if constexpr (masked) {
+        if (masked) {
             // values of tokens that are not there count for nothing; what is not finite goes to the rows that see it alone
             bool odd = false;
 #pragma unroll
@@ -957,9 +954,13 @@ __global__ void __launch_bounds__((64 * Shape<FMT, HD>::NW), (HD == 256 || (FMT 
                     if (!(now.there[0] >> tok & 1)) continue;
                     const int32_t from = tok >> 2 & 3, i = 4 * (tok >> 4) + (tok & 3);
                     const uint8_t* row = c.values + (tok < 16 ? now.base[0] : now.base[1]) + (tok & 15) * HD * F::E;
-                    if constexpr (STEP) {
-                        if (own && tok == (part.length & (CHUNK - 1))) row = sh.value;
-                    }
+                    const bool fresh = STEP && own && tok == (part.length & (CHUNK - 1));
+                    auto element_of = [&](int32_t d) {
+                        if constexpr (STEP) {
+                            if (fresh) return load_element<FMT>(sh.value, d);
+                        }
+                        return load_element<FMT>(row, d);
+                    };
                     float weight = 0.0f;
 #pragma unroll
                     for (int e = 0; e < 8; ++e)
@@ -970,7 +971,7 @@ __global__ void __launch_bounds__((64 * Shape<FMT, HD>::NW), (HD == 256 || (FMT 
                     for (int e = 0; e < 4; ++e)
 #pragma unroll
                         for (int db = 0; db < X::DB; ++db) {
-                            const float v = load_element<FMT>(row, (4 * grp + e) * X::DB + db);
+                            const float v = element_of((4 * grp + e) * X::DB + db);
                             if (!(fabsf(v) < INFINITY)) o[db][e] += weight * v;
                             __builtin_amdgcn_sched_barrier(0);  // (rare: one load at a time, few registers)
                         }
@@ -994,8 +995,7 @@ __global__ void __launch_bounds__((64 * Shape<FMT, HD>::NW), (HD == 256 || (FMT 
         }
     };
     for (; ch < c1; ch += NW) {
-        if (ch * CHUNK + CHUNK <= n_all && here.there[0] == 0xFFFFFFFFu) attend_chunk(std::false_type{});
-        else attend_chunk(std::true_type{});
+        attend_chunk(ch * CHUNK + CHUNK > n_all || here.there[0] != 0xFFFFFFFFu);
     }
 
     // each wave's averages, maxima and sums, then all waves' through LDS
@@ -1312,7 +1312,7 @@ __global__ void __launch_bounds__((Tile<FMT, HD, WAVES>::THREADS), (Tile<FMT, HD
                     if (!(vis >> token_of(i) & 1)) x[8 * h + i] = -INFINITY;
             }
         }
-        to_weights<FMT, false>(x, f, m, l, [](int) { return false; }, [&](float alpha) {
+        to_weights<FMT>(x, f, m, l, [&](float alpha) {
 #pragma unroll
             for (int db = 0; db < X::DB; ++db) o[db / VG][db % VG] *= alpha;
         });
