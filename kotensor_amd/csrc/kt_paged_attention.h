@@ -1471,10 +1471,8 @@ int32_t launch_tiles(Args a, hipStream_t st) {
 template <int FMT, int HD>
 int32_t launch_dims(const Args& a, hipStream_t st) {
     const int64_t rows = static_cast<int64_t>(a.p.b.most_rows) * (a.p.num_heads / a.p.c.kv_heads);
-    if constexpr (HD < 256) {
-        if (a.k_new) return launch_rows<FMT, HD, true>(a, st);
-    }
     if constexpr (HD < 256 || FMT != KT_PAGED_F32) {
+        if (a.k_new) return launch_rows<FMT, HD, true>(a, st);
         if (rows <= 16 || a.p.b.key_bound <= 128) return launch_rows<FMT, HD, false>(a, st);
     }
     if constexpr (HD == 256 || (HD <= 64 && FMT != KT_PAGED_F32)) {
