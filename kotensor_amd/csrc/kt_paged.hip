@@ -407,8 +407,8 @@ int32_t kt_rope_attention_paged(const float* q, const float* k, const float* v, 
     if (const int32_t status = attention_args(q, num_heads, cache, layer, batch, context, &a)) return status;
     if (a.b.rows == 0 || a.b.sequences == 0) return KT_OK;
     hipStream_t st = static_cast<hipStream_t>(stream);
-    // A step of up to 16 query heads a kv head: one launch (in fp32 of 256 dims tiles of 64 rows are faster: launch_dims).
-    if (a.b.most_rows == 1 && num_heads / a.c.kv_heads <= 16 && (a.c.head_dim < 256 || a.c.fmt != KT_PAGED_F32)) {
+    // A step of up to 16 query heads a kv head: one launch.
+    if (a.b.most_rows == 1 && num_heads / a.c.kv_heads <= 16) {
         a.inv_freq = inv_freq;
         return launch_attention(a, st, k, v);
     }

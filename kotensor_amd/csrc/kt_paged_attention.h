@@ -1459,8 +1459,6 @@ int32_t launch_tiles(Args a, hipStream_t st) {
 //   up to 16 rows of a kv head: tiles of 16. (A tree of 4 tokens has no use for more.)
 //   up to 128 keys: the same for any number of rows, as its waves have a chunk each: no parts to merge, and four
 //     times the workgroups. A prompt of 128: fp16 10.7 against 12.9, fp32 12.4 against 21.7, fp16 at 64 dims 6.7 against 8.6.
-//     Not fp32 at 256 dims, whose operands do not fit the registers: a prompt of 128 54.8 against 35.9 with tiles of 64, a token
-//     after 20000 247 against 169 (only 64 sequences of 2000 tokens would be 848 against 877).
 //   up to 64 rows: tiles of 64, so that no wave is idle, two workgroups a CU: 16 sequences with trees of 15 after 2000 tokens 41
 //     against 54 with tiles of 128 (fp32 76 against 95); one tree of 15 after 4000 29 and 30.
 //   up to 64 dims in 16 bits: tiles of 64 for any number of rows, of which three workgroups share a CU: a prompt of 2048 62 (fp16).
@@ -1471,10 +1469,8 @@ int32_t launch_tiles(Args a, hipStream_t st) {
 template <int FMT, int HD>
 int32_t launch_dims(const Args& a, hipStream_t st) {
     const int64_t rows = static_cast<int64_t>(a.p.b.most_rows) * (a.p.num_heads / a.p.c.kv_heads);
-    if constexpr (HD < 256 || FMT != KT_PAGED_F32) {
-        if (a.k_new) return launch_rows<FMT, HD, true>(a, st);
-        if (rows <= 16 || a.p.b.key_bound <= 128) return launch_rows<FMT, HD, false>(a, st);
-    }
+    if (a.k_new) return launch_rows<FMT, HD, true>(a, st);
+    if (rows <= 16 || a.p.b.key_bound <= 128) return launch_rows<FMT, HD, false>(a, st);
     if constexpr (HD == 256 || (HD <= 64 && FMT != KT_PAGED_F32)) {
         return launch_tiles<FMT, HD, 4>(a, st);
     } else {
