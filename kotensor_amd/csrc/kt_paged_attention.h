@@ -17,10 +17,10 @@
 // seldom rescaled. Parts meet through memory: of tiles of 16 rows the last workgroup of a tile to arrive (a counter, which it
 // returns to zero) merges all in their order, so that no workgroup waits for another and the bits do not depend on who
 // is last; of larger tiles a launch of its own does.
-// Two kernels: attention_kernel for few rows, bound by the cache's bytes (64 steps over 2048 tokens on average, 128 dims, bf16: 111 us,
-// 4.9 TB/s; one of 131000 beside seven shorter, fp16: 86 us, 5.1 TB/s; a large copy runs at 4.8), with short texts by the chain of loads from
+// Two kernels: attention_kernel for few rows, bound by the cache's bytes (64 steps over 2048 tokens on average, 128 dims, bf16: 112 us,
+// 4.8 TB/s; one of 131000 beside seven shorter, fp16: 86 us, 5.1 TB/s; a large copy runs at 4.8), with short texts by the chain of loads from
 // the lengths to the merge (12 us); tile_kernel for many, bound by the vector and matrix instructions of two waves a SIMD that wait for
-// each other's chunks (a prompt of 2048, 128 dims, bf16: 110 us, 312 TFLOP/s of attention, 936 of matrix products, of which a
+// each other's chunks (a prompt of 2048, 128 dims, bf16: 97 us, 354 TFLOP/s of attention, 1060 of matrix products, of which a
 // large library product reaches 1112), with few chunks by a part's beginning, 7 to 10 us.
 #pragma once
 
@@ -1455,17 +1455,19 @@ int32_t launch_tiles(Args a, hipStream_t st) {
     return KT_OK;
 }
 
-// Which kernel (us here: head dims of 128 unless said, 32 heads on 8 kv heads, one sequence unless said; the kernel taken first):
+// Which kernel (us here: head dims of 128 unless said, 32 heads on 8 kv heads, one sequence, pages of 32, of trees 64; the kernel taken first):
 //   up to 16 rows of a kv head: tiles of 16. (A tree of 4 tokens has no use for more.)
 //   up to 128 keys: the same for any number of rows, as its waves have a chunk each: no parts to merge, and four
-//     times the workgroups. A prompt of 128: fp16 10.7 against 12.9, fp32 12.4 against 21.7, fp16 at 64 dims 6.7 against 8.6.
-//   up to 64 rows: tiles of 64, so that no wave is idle, two workgroups a CU: 16 sequences with trees of 15 after 2000 tokens 41
-//     against 54 with tiles of 128 (fp32 76 against 95); one tree of 15 after 4000 29 and 30.
-//   up to 64 dims in 16 bits: tiles of 64 for any number of rows, of which three workgroups share a CU: a prompt of 2048 62 (fp16).
-//   else: tiles of 128, as the chunk that eight waves share is half the loads and LDS writes a row: a prompt of 2048 97 (fp16),
-//     110 (bf16), 205 (fp32); a tree of 60 in fp32 53 against 63 with tiles of 64.
-//   256 dims: tiles of 64 whose waves have a SIMD's registers each: a prompt of 512 41 against 50 with tiles of
-//     128 (bf16 44 against 69, fp32 116 against 169).
+//     times the workgroups. A prompt of 128: fp16 8.9 against 12.4, fp32 12.3 against 16.6, fp16 at 64 dims 7.0 against 8.0, fp32
+//     at 256 dims 22 against 42.
+//   up to 64 rows: tiles of 64, so that no wave is idle, two workgroups a CU: 16 sequences with trees of 15 after 2000 tokens 37
+//     against 47 with tiles of 128 (fp32 55 against 80); one tree of 15 after 4000 26 and 26.
+//   up to 64 dims in 16 bits: tiles of 64 for any number of rows, of which three workgroups share a CU: a prompt of 1024 28
+//     against 33, of 2048 61 against 69 (fp16).
+//   else: tiles of 128, as the chunk that eight waves share is half the loads and LDS writes a row: a prompt of 2048 99 against 108 (fp16), 107
+//     against 114 (bf16), 182 against 222 (fp32); a tree of 60 in fp32 43 against 46.
+//   256 dims: tiles of 64 whose waves have a SIMD's registers each: a prompt of 512 36 against 38 with tiles of
+//     128 (bf16 39 against 42, fp32 72 against 101; 16 trees of 15 79 against 68).
 template <int FMT, int HD>
 int32_t launch_dims(const Args& a, hipStream_t st) {
     const int64_t rows = static_cast<int64_t>(a.p.b.most_rows) * (a.p.num_heads / a.p.c.kv_heads);
