@@ -125,3 +125,16 @@ def test_drafts_from_the_text():
         text = rng.integers(0, 4, 40).tolist()
         tokens, parents = kt.TextDraft(5, 3, 3)(text)
         assert len(tokens) == len(parents) <= 15 and all(-1 <= p < i for i, p in enumerate(parents))
+
+
+def test_argmax_of_rows_refused():
+    from kotensor_amd import _lib
+    lib = _lib.lib()
+    call = lambda logits=16, rows=2, n=5, tokens=16, positions=16, generated=16, capacity=4: lib.kt_argmax_rows(
+        logits, rows, n, tokens, positions, generated, capacity, None)
+    for change, want, message in (({"logits": None}, _lib.KT_ERR_ARGUMENT, "NULL"), ({"tokens": None}, _lib.KT_ERR_ARGUMENT, "NULL"),
+                                  ({"rows": -1}, _lib.KT_ERR_SHAPE, "argmax of -1 rows"), ({"rows": 15873}, _lib.KT_ERR_SHAPE, "0 to 15872"),
+                                  ({"n": 0}, _lib.KT_ERR_SHAPE, "at least one logit"), ({"positions": None}, _lib.KT_ERR_ARGUMENT, "without positions"),
+                                  ({"capacity": -1}, _lib.KT_ERR_SHAPE, "negative capacity")):
+        assert call(**change) == want and message in _lib.last_error(), (change, _lib.last_error())
+    assert call(rows=0, logits=None) == _lib.KT_OK
