@@ -12,10 +12,15 @@ namespace {
 constexpr int THREADS = 256;
 
 // ---- RoPE and the append ---------------------------------------------------------------
-// A wave takes one row and HEADS heads a lane of it: lane (pair i, head of 128 / head_dim side by side); its cosine and
-// sine serve all its heads, whose loads go out together. Waves of query heads write the rotated query, waves of
-// kv heads the key and the value. Bound by its bytes: five prompts of up to 1001 tokens, 32 and 8 heads of 128, fp32: 200 MB in 45 us,
-// 4.5 TB/s; one token of 16 sequences by its launch and three loads that wait for each other (starts, lengths, table): 4 us.
+// A wave takes one row and HEADS heads a lane of it: a lane has four pairs of a head, as many heads as fit lie side by side in the wave. Each
+// lane makes one pair's cosine and sine (of 256 dims two), which those that need it take from there; they serve all its heads, whose loads go
+// out together. Waves of query heads write the rotated query, waves of kv heads the key and the value. Bound by its bytes: five prompts
+// of up to 1001 tokens, 32 and 8 heads of 128, fp32: 200 MB in 31 us where the last cache has them, 40 from memory; one token of 16
+// sequences by its launch and three loads that wait for each other (starts, lengths, table): 4 us. (One float of a pair a lane and eight
+// heads: 44 us; four heads of four pairs 32.)
+constexpr int HEADS = 2;
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f4_any __attribute__((ext_vector_type(4), aligned(4)));  // (k, v and q lie at any float)
 struct AppendArgs {
     const float* q;  // NULL: only the append
     const float* k;
@@ -38,78 +43,100 @@ __device__ __forceinline__ int32_t sequence_of(const BatchView& b, int32_t row) 
     return s;
 }
 
-template <int FMT, int HEADS>
+// Four elements as the cache holds them (store_element).
+template <int FMT>
+__device__ __forceinline__ void store_four(uint8_t* p, int64_t at, f4 x) {
+    if constexpr (FMT == KT_PAGED_F32) {
+        *reinterpret_cast<f4*>(p + 4 * at) = x;
+    } else {
+        uint2 both;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) store_element<FMT>(reinterpret_cast<uint8_t*>(&both), e, x[e]);
+        *reinterpret_cast<uint2*>(p + 2 * at) = both;
+    }
+}
+
+template <int FMT>
 __global__ void __launch_bounds__(THREADS) append_kernel(AppendArgs a) {
     const PagedView& c = a.c;
     const int32_t HD = c.head_dim, half = HD >> 1, lane = threadIdx.x & 63;
     const int64_t item = static_cast<int64_t>(blockIdx.x) * (THREADS / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int32_t row = static_cast<int32_t>(item / a.groups), group = static_cast<int32_t>(item % a.groups);
     if (row >= a.b.rows) return;
-    const int32_t side = half < 64 ? 64 / half : 1;  // heads side by side in the lanes
+    const int32_t per_head = half >> 2, side = 64 / per_head, mine = lane % per_head;  // lanes of a head, heads side by side
     const bool is_q = group < a.q_groups;
     const int32_t heads = is_q ? a.num_heads : c.kv_heads;
-    const int32_t h0 = (is_q ? group : group - a.q_groups) * HEADS * side + lane / half;
+    const int32_t h0 = (is_q ? group : group - a.q_groups) * HEADS * side + lane / per_head;
     const int32_t s = sequence_of(a.b, row);
     if (s >= a.b.sequences) return;  // behind the last sequence
     const int32_t index = row - a.b.starts[s];
     if (index < 0) return;
     const int64_t slot = static_cast<int64_t>(a.b.lengths[s]) + index;
-    const int64_t pos = a.b.depths ? static_cast<int64_t>(a.b.lengths[s]) + a.b.depths[row] : slot;
-    for (int32_t i = lane % half; i < half; i += 64) {
-        const float* src = (is_q ? a.q : a.k) + static_cast<size_t>(row) * heads * HD + i;
-        const float* vsrc = a.v + static_cast<size_t>(row) * heads * HD + i;
-        float x1[HEADS], x2[HEADS], v1[HEADS], v2[HEADS], cf, sf;
+    const int32_t pos = static_cast<int32_t>(a.b.depths ? static_cast<int64_t>(a.b.lengths[s]) + a.b.depths[row] : slot);
+    const float* src = (is_q ? a.q : a.k) + static_cast<size_t>(row) * heads * HD + 4 * mine;
+    const float* vsrc = a.v + static_cast<size_t>(row) * heads * HD + 4 * mine;
+    f4 x1[HEADS], x2[HEADS], v1[HEADS], v2[HEADS];
 #pragma unroll
-        for (int u = 0; u < HEADS; ++u) {
-            const size_t at = static_cast<size_t>(min(h0 + u * side, heads - 1)) * HD;
-            x1[u] = src[at];
-            x2[u] = src[at + half];
-            if (!is_q) {
-                v1[u] = vsrc[at];
-                v2[u] = vsrc[at + half];
-            }
+    for (int u = 0; u < HEADS; ++u) {
+        const size_t at = static_cast<size_t>(min(h0 + u * side, heads - 1)) * HD;
+        x1[u] = *reinterpret_cast<const f4_any*>(src + at);
+        x2[u] = *reinterpret_cast<const f4_any*>(src + at + half);
+        if (!is_q) {
+            v1[u] = *reinterpret_cast<const f4_any*>(vsrc + at);
+            v2[u] = *reinterpret_cast<const f4_any*>(vsrc + at + half);
         }
-        rope_sin_cos(static_cast<int32_t>(pos), a.inv_freq[i], cf, sf);
+    }
+    float own_cos, own_sin, far_cos = 0.0f, far_sin = 0.0f, cf[4], sf[4];
+    rope_sin_cos(pos, a.inv_freq[lane % half], own_cos, own_sin);
+    if (half > 64) rope_sin_cos(pos, a.inv_freq[64 + lane], far_cos, far_sin);
 #pragma unroll
-        for (int u = 0; u < HEADS; ++u) {
-            const int32_t h = h0 + u * side;
-            if (h >= heads) continue;
-            float y1, y2;
-            rope_apply(x1[u], x2[u], cf, sf, y1, y2);
-            if (is_q) {
-                float* out = a.q_out + (static_cast<size_t>(row) * heads + h) * HD + i;
-                out[0] = y1;
-                out[half] = y2;
-            } else {
-                const int64_t at = place_of(c, a.b, s, slot, h);
-                if (at < 0) continue;
-                store_element<FMT>(c.keys, at + i, y1);
-                store_element<FMT>(c.keys, at + i + half, y2);
-                store_element<FMT>(c.values, at + i, v1[u]);
-                store_element<FMT>(c.values, at + i + half, v2[u]);
-            }
+    for (int e = 0; e < 4; ++e) {
+        const int32_t pair = 4 * mine + e;
+        cf[e] = __shfl(own_cos, pair & 63);
+        sf[e] = __shfl(own_sin, pair & 63);
+        if (half > 64) {
+            const float other_cos = __shfl(far_cos, pair & 63), other_sin = __shfl(far_sin, pair & 63);
+            cf[e] = pair < 64 ? cf[e] : other_cos;
+            sf[e] = pair < 64 ? sf[e] : other_sin;
+        }
+    }
+    const int64_t place = is_q ? 0 : place_of(c, a.b, s, slot, 0);
+#pragma unroll
+    for (int u = 0; u < HEADS; ++u) {
+        const int32_t h = h0 + u * side;
+        if (h >= heads) continue;
+        f4 y1, y2;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            float low, high;
+            rope_apply(x1[u][e], x2[u][e], cf[e], sf[e], low, high);
+            y1[e] = low;
+            y2[e] = high;
+        }
+        if (is_q) {
+            float* out = a.q_out + (static_cast<size_t>(row) * heads + h) * HD + 4 * mine;
+            *reinterpret_cast<f4_any*>(out) = y1;
+            *reinterpret_cast<f4_any*>(out + half) = y2;
+        } else if (place >= 0) {
+            const int64_t at = place + (static_cast<int64_t>(h) << c.page_shift) * HD + 4 * mine;
+            store_four<FMT>(c.keys, at, y1);
+            store_four<FMT>(c.keys, at + half, y2);
+            store_four<FMT>(c.values, at, v1[u]);
+            store_four<FMT>(c.values, at + half, v2[u]);
         }
     }
 }
 
-template <int HEADS>
-int32_t launch_append_of(AppendArgs a, int32_t side, hipStream_t st) {
-    a.q_groups = a.q ? ceil_div(a.num_heads, HEADS * side) : 0;
-    a.groups = a.q_groups + ceil_div(a.c.kv_heads, HEADS * side);
+int32_t launch_append(AppendArgs a, hipStream_t st) {
+    const int32_t heads = HEADS * (512 / a.c.head_dim);  // of a wave
+    a.q_groups = a.q ? ceil_div(a.num_heads, heads) : 0;
+    a.groups = a.q_groups + ceil_div(a.c.kv_heads, heads);
     const int64_t grid = (static_cast<int64_t>(a.b.rows) * a.groups + THREADS / 64 - 1) / (THREADS / 64);
     if (grid > INT32_MAX) return fail(KT_ERR_SHAPE, "too many rows and heads in one call");
-    const auto kernel = a.c.fmt == KT_PAGED_F32 ? append_kernel<KT_PAGED_F32, HEADS> : a.c.fmt == KT_PAGED_F16 ? append_kernel<KT_PAGED_F16, HEADS> : append_kernel<KT_PAGED_BF16, HEADS>;
+    const auto kernel = a.c.fmt == KT_PAGED_F32 ? append_kernel<KT_PAGED_F32> : a.c.fmt == KT_PAGED_F16 ? append_kernel<KT_PAGED_F16> : append_kernel<KT_PAGED_BF16>;
     kernel<<<static_cast<uint32_t>(grid), THREADS, 0, st>>>(a);
     KT_LAUNCHED("paged cache append kernel");
     return KT_OK;
-}
-
-int32_t launch_append(const AppendArgs& a, hipStream_t st) {
-    const int32_t side = a.c.head_dim < 128 ? 128 / a.c.head_dim : 1;
-    const int64_t waves = static_cast<int64_t>(a.b.rows) * ((a.q ? ceil_div(a.num_heads, 8 * side) : 0) + ceil_div(a.c.kv_heads, 8 * side));
-    // eight heads a wave, whose cosines are made once, where that makes 16 waves a CU; else two (16 trees of up to 64, 8 heads of 128: 5.5 us
-    // for 6.7; a token of 16 sequences 4.0 for 5.0)
-    return waves < 16 * cu_count() ? launch_append_of<2>(a, side, st) : launch_append_of<8>(a, side, st);
 }
 
 // ---- trees -------------------------------------------------------------------------------

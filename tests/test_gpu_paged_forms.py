@@ -1,5 +1,7 @@
 """Attention over the cache in pages at the sizes that choose between its kernels (by rows of a kv head, key bound, head
 dimension and format), and between its ways of cutting tiles into parts."""
+import ctypes
+
 import numpy as np
 import pytest
 
@@ -65,3 +67,22 @@ def test_one_sequence_that_fills_the_card(kt, fmt, shape, count, given):
     b.stride += 20
     b.upload()
     check(b)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dim", [32, 64, 128, 256])
+def test_rows_at_any_float(kt, fmt, dim):
+    """kt_rope_paged takes q, k, v and q_out that begin at any float."""
+    b = Batch(kt, 65, [5, 40], [30, 3], (6, 3, dim), fmt, 16, extra=1)
+    b.rope()
+    want, pool = b.context().tobytes(), [p.tobytes() for p in b.pool_bits()]
+    b.upload()
+    at = {}
+    for name in ("q", "k", "v", "context"):
+        array = b.d["context"].download(np.float32) if name == "context" else getattr(b, name)
+        buffer = at[name] = kt.DeviceBuffer(array.nbytes + 4)
+        buffer.upload(array, offset=4)
+    b.lib.call("kt_rope_paged", at["q"].ptr + 4, at["k"].ptr + 4, at["v"].ptr + 4, b.heads, b.d["inv_freq"].ptr, ctypes.byref(b.cache), 0,
+               ctypes.byref(b.batch), at["context"].ptr + 4, None)
+    assert at["context"].download(np.float32, offset=4).tobytes() == want
+    assert [p.tobytes() for p in b.pool_bits()] == pool
