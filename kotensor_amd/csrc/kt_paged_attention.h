@@ -270,8 +270,9 @@ struct Part {
 // Which part of the launch workgroup `at` has (BY_SLOT: whose slot `at` is); false: none. Every lane is a sequence. A part's size is at least
 // the chunks over target, so a launch has at most target + (its tiles of all kv heads) parts, and at most 2 target that share a
 // tile. Tiles of many rows (FINE): where that size is above LONG tokens and tiles are fewer than 2 target, whose rounds would leave
-// workgroups idle, the chunks over 2 target: at most 4 target parts that share a tile. (16 sequences with trees of 64 after 3000, bf16, 128
-// dims: 149 -> 141 us; everywhere, a tree of 60 after 4000 would take 49 for 42, a prompt of 2048 122 for 117.)
+// workgroups idle, but not a round of whole tiles, the chunks over 2 target: at most 4 target parts that share a tile. (us at target, at 2 target,
+// 128 dims, bf16: 300 rows after 8000 tokens 188, 130; 1300 after 8000 618, 508; 16 sequences with trees of 64 after 3000 123, 118; with 64 rows
+// after 1000 each 60, 75: a round of whole tiles. Everywhere: a tree of 60 after 4000 42, 49.)
 constexpr int LONG = 1024;
 constexpr bool fine(int R) { return R > 16; }
 template <int R, int LEAST, int CHUNK, bool BY_SLOT = false>
@@ -292,22 +293,31 @@ __device__ __forceinline__ bool find_part(const Args& a, int32_t at, Part& out) 
     auto chunks_of = [&]() { return (held_keys(c, b, length, n) + CHUNK - 1) / CHUNK; };
     // (whole numbers up to 2^24 are exact in fp32; of larger totals a little more)
     float total = 0.0f, rows = 0.0f, all_tiles = 0.0f;
+    int32_t most = 0;
     for (int32_t s0 = 0; s0 < b.sequences; s0 += 64) {
         load(s0);
-        total += static_cast<float>(tiles_of()) * static_cast<float>(c.kv_heads) * static_cast<float>(max(chunks_of(), 1));
+        const float tiles = static_cast<float>(tiles_of()) * static_cast<float>(c.kv_heads);
+        total += tiles * static_cast<float>(max(chunks_of(), 1));
+        all_tiles += tiles;
         rows += static_cast<float>(n);
-        all_tiles += static_cast<float>(tiles_of()) * static_cast<float>(c.kv_heads);
+        most = max(most, n > 0 ? chunks_of() : 0);
     }
     total = wave_sum_dpp(total);
     if (wave_sum_dpp(rows) > static_cast<float>(b.rows)) return false;  // starts that do not ascend
     if (total >= 0x1p24f) total *= 1.0f + 0x1p-16f;
-    float target = static_cast<float>(a.target);
+    auto size_for = [&](float target) {
+        int32_t size = static_cast<int32_t>(fminf(total / target, 0x1p30f));
+        if (static_cast<float>(size) * target < total) ++size;
+        return uniform((max(size, 1) + LEAST - 1) / LEAST * LEAST);
+    };
+    const float target = static_cast<float>(a.target);
+    int32_t per = a.slots == 0 ? 1 << 26 : size_for(target);
     if constexpr (fine(R)) {
-        if (total > target * (LONG / CHUNK) && wave_sum_dpp(all_tiles) < 2.0f * target) target *= 2.0f;
+        if (a.slots > 0 && total > target * (LONG / CHUNK)) {
+            all_tiles = wave_sum_dpp(all_tiles);
+            if (all_tiles < 2.0f * target && (all_tiles > target || __ballot(most > per))) per = size_for(2.0f * target);
+        }
     }
-    int32_t per = static_cast<int32_t>(fminf(total / target, 0x1p30f));
-    if (static_cast<float>(per) * target < total) ++per;
-    per = a.slots == 0 ? 1 << 26 : uniform((max(per, 1) + LEAST - 1) / LEAST * LEAST);
     int32_t before = 0, slots = 0;
     for (int32_t s0 = 0; s0 < b.sequences; s0 += 64) {
         if (b.sequences > 64) load(s0);
