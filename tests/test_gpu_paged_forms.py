@@ -86,3 +86,41 @@ def test_rows_at_any_float(kt, fmt, dim):
                ctypes.byref(b.batch), at["context"].ptr + 4, None)
     assert at["context"].download(np.float32, offset=4).tobytes() == want
     assert [p.tobytes() for p in b.pool_bits()] == pool
+
+
+@pytest.mark.parametrize("fmt,dim", [("float16", 64), ("bfloat16", 128), ("float32", 64), ("float32", 256)])
+def test_many_sequences_of_many_rows(kt, fmt, dim):
+    """More sequences than lanes, with tiles of many rows; a long one among the last is cut, one without rows is not there."""
+    rng = np.random.default_rng(dim)
+    lengths = rng.integers(0, 60, 150).tolist()
+    counts = rng.integers(0, 50, 150).tolist()
+    lengths[70], counts[70] = 2500, 0
+    lengths[140], counts[140] = 4000, 45
+    lengths[3], counts[3] = 1500, 33
+    check(Batch(kt, 66, lengths, counts, (2, 1, dim), fmt, 64, extra=3))
+
+
+def test_recorded_trees_of_many_rows(kt):
+    """A recorded call whose tiles are cut and merged, with other lengths and trees from replay to replay, between eager calls."""
+    counts, rng = [60, 0, 33], np.random.default_rng(67)
+    stream = kt.Stream.create()
+    b = Batch(kt, 67, [900, 1500, 40], counts, (8, 2, 64), "float16", 32, parents=random_parents(rng, counts))
+    b.rope_attention(stream=stream.handle)
+    graph = ctypes.c_void_p()
+    b.lib.call("kt_graph_begin", stream.handle)
+    b.masks(stream.handle)
+    b.rope_attention(stream=stream.handle)
+    b.lib.call("kt_graph_end", stream.handle, ctypes.byref(graph))
+    for lengths in ([900, 1500, 40], [3, 1500, 0], [860, 0, 31], [900, 1500, 40]):
+        b.lengths, b.parents = lengths, random_parents(rng, counts)
+        b.d["lengths"].upload(np.array(lengths, np.int32), stream)
+        b.d["parents"].upload(np.concatenate(b.parents), stream)
+        b.append()
+        b.lib.call("kt_graph_launch", graph, stream.handle)
+        replayed = b.context(stream)
+        b.check_context(replayed, *b.attend(b.rotated()))
+        b.masks(stream.handle)
+        b.rope_attention(stream=stream.handle)
+        assert b.context(stream).tobytes() == replayed.tobytes()
+    b.lib.call("kt_graph_destroy", graph)
+    stream.destroy()
