@@ -935,6 +935,7 @@ __global__ void __launch_bounds__((64 * Shape<FMT, HD>::NW), (HD == 256 || (FMT 
         op p[F::QP];
         float x[8];
         uint32_t vis = 0;
+        settle();
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = sc[i >> 2][i & 3];
         if (masked) {  // (a score of -infinity has no weight)
@@ -1310,6 +1311,7 @@ __global__ void __launch_bounds__((Tile<FMT, HD, WAVES>::THREADS), (Tile<FMT, HD
             }
         };
         load_values(0);
+        settle();
         float x[8 * X::SETS];
 #pragma unroll
         for (int i = 0; i < 8 * X::SETS; ++i) x[i] = sc[i >> 2][i & 3];
