@@ -367,6 +367,9 @@ using namespace kt;
 
 namespace {
 
+// Nothing to do for any sequence (rows that belong to none may be there).
+bool no_rows(const BatchView& b) { return b.rows == 0 || b.sequences == 0 || b.most_rows == 0; }
+
 int32_t append_args(const float* q, const float* k, const float* v, int32_t num_heads, const float* inv_freq, const kt_paged_cache* cache, int32_t layer,
                     const kt_paged_batch* batch, float* q_out, AppendArgs* a) {
     if (const int32_t status = view_paged(cache, layer, &a->c)) return status;
@@ -416,14 +419,14 @@ int32_t kt_rope_paged(const float* q, const float* k, const float* v, int32_t nu
                       const kt_paged_batch* batch, float* q_out, void* stream) {
     AppendArgs a{};
     if (const int32_t status = append_args(q, k, v, num_heads, inv_freq, cache, layer, batch, q_out, &a)) return status;
-    return a.b.rows == 0 || a.b.sequences == 0 ? KT_OK : launch_append(a, static_cast<hipStream_t>(stream));
+    return no_rows(a.b) ? KT_OK : launch_append(a, static_cast<hipStream_t>(stream));
 }
 
 int32_t kt_attention_paged(const float* q, int32_t num_heads, const kt_paged_cache* cache, int32_t layer, const kt_paged_batch* batch, float* context,
                            void* stream) {
     PagedAttnArgs a{};
     if (const int32_t status = attention_args(q, num_heads, cache, layer, batch, context, &a)) return status;
-    return a.b.rows == 0 || a.b.sequences == 0 ? KT_OK : launch_attention(a, static_cast<hipStream_t>(stream));
+    return no_rows(a.b) ? KT_OK : launch_attention(a, static_cast<hipStream_t>(stream));
 }
 
 int32_t kt_rope_attention_paged(const float* q, const float* k, const float* v, const float* inv_freq, int32_t num_heads, const kt_paged_cache* cache,
@@ -432,7 +435,7 @@ int32_t kt_rope_attention_paged(const float* q, const float* k, const float* v, 
     PagedAttnArgs a{};
     if (const int32_t status = append_args(q, k, v, num_heads, inv_freq, cache, layer, batch, context, &p)) return status;
     if (const int32_t status = attention_args(q, num_heads, cache, layer, batch, context, &a)) return status;
-    if (a.b.rows == 0 || a.b.sequences == 0) return KT_OK;
+    if (no_rows(a.b)) return KT_OK;
     hipStream_t st = static_cast<hipStream_t>(stream);
     // A step of up to 16 query heads a kv head: one launch.
     if (a.b.most_rows == 1 && num_heads / a.c.kv_heads <= 16) {

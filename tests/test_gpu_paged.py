@@ -416,3 +416,29 @@ def test_offsets_past_32_bits(kt):
         _lib.call("kt_paged_read", ctypes.byref(small.cache), 0, small.d["tables"].ptr + 4 * s * b.stride, b.stride, 0, 3, out[2].ptr, out[3].ptr, None)
         assert out[0].download(np.float32).tobytes() == out[2].download(np.float32).tobytes()
         assert out[1].download(np.float32).tobytes() == out[3].download(np.float32).tobytes()
+
+
+@pytest.mark.parametrize("tree", [False, True])
+def test_rows_of_no_sequence_alone(kt, tree):
+    """A padded batch whose sequences are all empty, eager and recorded: the pool and the context stay as they are."""
+    counts = [0, 0, 0]
+    b = Batch(kt, 52, [40, 0, 7], counts, (8, 2, 64), "float16", 16, parents=random_parents(np.random.default_rng(52), counts) if tree else None, extra=5, lead=2)
+    stream, graph = kt.Stream.create(), ctypes.c_void_p()
+
+    def calls():
+        b.rope(stream=stream.handle)
+        b.attention(stream=stream.handle)
+        b.rope_attention(stream=stream.handle)
+        b.lib.call("kt_paged_advance", b.d["lengths"].ptr, ctypes.byref(b.batch), stream.handle)
+
+    calls()
+    b.lib.call("kt_graph_begin", stream.handle)
+    calls()
+    b.lib.call("kt_graph_end", stream.handle, ctypes.byref(graph))
+    for _ in range(3):
+        b.lib.call("kt_graph_launch", graph, stream.handle)
+        assert np.isnan(b.context(stream)).all()
+        assert b.d["lengths"].download(np.int32)[:3].tolist() == [40, 0, 7]
+        b.check_pool()
+    b.lib.call("kt_graph_destroy", graph)
+    stream.destroy()

@@ -185,3 +185,15 @@ def test_calls_of_nothing():
     assert lib.kt_tree_masks(16, none, 16, 16, None) == _lib.KT_OK and lib.kt_paged_keep(_cache(), none, 16, 5, 16, 16, None) == _lib.KT_OK
     assert lib.kt_tree_accept(16, 16, 16, none, 16, 5, 16, 16, None) == _lib.KT_OK and lib.kt_paged_advance(16, none, None) == _lib.KT_OK
     assert lib.kt_paged_read(_cache(), 0, 16, 4, 128, 0, 16, 16, None) == _lib.KT_OK and lib.kt_paged_read(_cache(), 0, 16, 4, 0, 5, None, None, None) == _lib.KT_OK
+
+
+@pytest.mark.parametrize("tree", [{}, TREE])
+def test_calls_without_a_row_of_a_sequence(tree):
+    """Rows that belong to no sequence alone, as in a padded batch whose sequences are all empty: nothing is enqueued."""
+    from kotensor_amd import _lib
+    lib = _lib.lib()
+    for bound in (0, 100):
+        padding = _batch(most_rows=0, key_bound=bound, **tree)
+        assert lib.kt_rope_paged(16, 16, 16, 4, 16, _cache(), 0, padding, 16, None) == _lib.KT_OK, _lib.last_error()
+        assert lib.kt_attention_paged(16, 4, _cache(), 0, padding, 16, None) == _lib.KT_OK, _lib.last_error()
+        assert lib.kt_rope_attention_paged(16, 16, 16, 16, 4, _cache(), 0, padding, 16, None) == _lib.KT_OK, _lib.last_error()
