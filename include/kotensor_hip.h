@@ -469,8 +469,9 @@ int32_t kt_rope_paged(const float* q, const float* k, const float* v, int32_t nu
                       const kt_paged_cache* cache, int32_t layer, const kt_paged_batch* batch, float* q_out, void* stream);
 /* kt_attention for a batch whose keys and values the pool holds already: softmax(q . k_j / sqrt(head_dim)) over the
  * tokens a row sees, times v, into context [rows x num_heads*head_dim]; products in fp32 precision, sums and softmax
- * in fp32. A row that sees no token gets zeros. Values that are not finite stay with the rows that see them. Scores
- * are taken to lie in fp32's range. q and context are 16-byte aligned and apart. The stream's workspace is sized by one eager call of the
+ * in fp32. A row that sees no token gets zeros. Values that are not finite stay with the rows that see them: an infinity makes
+ * the row's context of that dim infinite, whatever its weight and wherever it lies, infinities of both signs and NaNs make
+ * it NaN. Finite values are taken to be below 2^88, and scores to lie in fp32's range. q and context are 16-byte aligned and apart. The stream's workspace is sized by one eager call of the
  * same bounds before a recording. */
 int32_t kt_attention_paged(const float* q, int32_t num_heads, const kt_paged_cache* cache, int32_t layer,
                            const kt_paged_batch* batch, float* context, void* stream);

@@ -169,6 +169,9 @@ __device__ __forceinline__ float rounded_score(float x, float f) {
 __device__ __forceinline__ float share_of(float m, float l, float mx) {
     return l == 0.0f ? 0.0f : l * __builtin_amdgcn_exp2f((m == -INFINITY ? mx : m) - (mx == -INFINITY ? 0.0f : mx));
 }
+// The weight of a part's average: with keys (l) it is above zero, so that infinities count (2^-149 of a finite average is nothing
+// beside the 2^-30 of the weights' parts).
+__device__ __forceinline__ float weight_of_part(float share, float l) { return share < 0x1p-149f && l != 0.0f ? 0x1p-149f : share; }
 
 // A chunk's scores x of one row (a lane's share of them) into weights; m and l: the row's running maximum and the sum of this
 // lane's weights; rescale: what the maximum's move does to the sums. Tokens that the row does not see come with -infinity.
@@ -524,8 +527,9 @@ __device__ __forceinline__ void meet(const Args& a, const Part& part, int32_t sp
         for (int32_t o = 1; o < width; o <<= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-            ll[i] = share_of(ml[i], ll[i], mx);
-            sum += ll[i];
+            const float share = share_of(ml[i], ll[i], mx);
+            sum += share;
+            ll[i] = weight_of_part(share, ll[i]);
         }
         for (int32_t o = 1; o < width; o <<= 1) sum += __shfl_xor(sum, o);
         if (r < held) {
@@ -609,7 +613,7 @@ __global__ void __launch_bounds__(256) merge_kernel(Args a) {
         float mx = -INFINITY, sum = 0.0f;
         for (int32_t s = 0; s < splits; ++s) mx = fmaxf(mx, maxima[r * splits + s]);
         for (int32_t s = 0; s < splits; ++s) sum += share_of(maxima[r * splits + s], sums[r * splits + s], mx);
-        weights[e] = sum == 0.0f ? 0.0f : share_of(maxima[e], sums[e], mx) / sum;
+        weights[e] = sum == 0.0f ? 0.0f : weight_of_part(share_of(maxima[e], sums[e], mx) / sum, sums[e]);
     }
     __syncthreads();
     constexpr int BATCH = 8;
@@ -687,6 +691,56 @@ __device__ __forceinline__ uint32_t finite_only(uint32_t w) {
     if constexpr (FMT == KT_PAGED_F32) return (w & 0x7F800000u) == 0x7F800000u ? 0u : w;
     constexpr uint32_t x = FMT == KT_PAGED_F16 ? 0x7C00u : 0x7F80u;
     return ((w & x) == x ? 0u : w & 0xFFFFu) | ((w >> 16 & x) == x ? 0u : w & 0xFFFF0000u);
+}
+
+// ---- values that are not finite --------------------------------------------------------------------
+// The weight of a token that a row sees is above zero, so an infinite value makes the row's average of its dim infinite
+// (infinities of both signs and NaNs: NaN), whatever the weight. The products do not give that: a weight's lower parts
+// are zero or of the other sign, fp32 values' parts are NaN, weights and rescaled sums get too small for fp32. So the loops only find
+// out that something is not finite: chunks that not all rows see whole come without such values and leave a flag, other chunks'
+// make sums that are not finite. Then a wave looks at all values that its rows see: 1 bit a number of a lane. (An infinity that all rows
+// see: a prompt of 1024 in fp16 at 64 dims 268 us for 27, a step of eight sequences of 2000 in bf16 at 128 dims 44 for 31.)
+struct Odd {
+    uint64_t up, down;  // infinities above and below zero; of a NaN both
+};
+// Tokens that a lane loads its numbers of together.
+template <int FMT, int DB>
+constexpr int together() {
+    return std::clamp(64 / (DB * element_bytes(FMT)), 1, 8);
+}
+// The lane's numbers of N tokens: DB groups of four, `stride` elements apart, from at(u) on; seen: a bit a token.
+template <int FMT, int DB, int N, typename AT>
+__device__ __forceinline__ void look_at(Odd& odd, uint32_t seen, AT at, int32_t stride) {
+    constexpr int E = element_bytes(FMT);
+    uint32_t w[N][DB][E];
+#pragma unroll
+    for (int u = 0; u < N; ++u)
+#pragma unroll
+        for (int i = 0; i < DB; ++i) load_words(at(u) + i * stride * E, w[u][i]);
+#pragma unroll
+    for (int u = 0; u < N; ++u)
+#pragma unroll
+        for (int i = 0; i < DB; ++i) {
+            bool any = false;
+#pragma unroll
+            for (int j = 0; j < E; ++j) any |= any_not_finite<FMT>(w[u][i][j]);
+            if (!any || !(seen >> u & 1)) continue;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                float v;
+                if constexpr (FMT == KT_PAGED_F32) v = __builtin_bit_cast(float, w[u][i][e]);
+                else if constexpr (FMT == KT_PAGED_F16) v = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(w[u][i][e / 2] >> 16 * (e % 2))));
+                else v = __builtin_bit_cast(float, w[u][i][e / 2] >> 16 * (e % 2) << 16);
+                if (fabsf(v) < INFINITY) continue;
+                odd.up |= static_cast<uint64_t>(!(v < 0.0f)) << (4 * i + e);
+                odd.down |= static_cast<uint64_t>(!(v > 0.0f)) << (4 * i + e);
+            }
+        }
+}
+// What such values make of number i of the lane.
+__device__ __forceinline__ float or_odd(const Odd& odd, int i, float x) {
+    const bool up = odd.up >> i & 1, down = odd.down >> i & 1;
+    return up ? (down ? __builtin_nanf("") : INFINITY) : down ? -INFINITY : x;
 }
 
 template <int FMT, int HD, bool STEP>
@@ -907,6 +961,7 @@ __global__ void __launch_bounds__((64 * Shape<FMT, HD>::NW), (HD == 256 || (FMT 
             to_operands<FMT>(w, v);
         }
     };
+    bool not_finite = false;  // some values were left out
     // (masked: not every row sees the chunk whole)
     auto attend_chunk = [&](bool masked) {
         const Where<CHUNK, false> now = here;
@@ -934,12 +989,11 @@ __global__ void __launch_bounds__((64 * Shape<FMT, HD>::NW), (HD == 256 || (FMT 
         __builtin_amdgcn_sched_barrier(0);
         op p[F::QP];
         float x[8];
-        uint32_t vis = 0;
         settle();
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = sc[i >> 2][i & 3];
         if (masked) {  // (a score of -infinity has no weight)
-            vis = seen_bits(b, part.first, token, new_first, ch * CHUNK, now.there[0]);
+            const uint32_t vis = seen_bits(b, part.first, token, new_first, ch * CHUNK, now.there[0]);
 #pragma unroll
             for (int i = 0; i < 8; ++i)
                 if (!(vis >> token_of(i) & 1)) x[i] = -INFINITY;
@@ -950,7 +1004,7 @@ __global__ void __launch_bounds__((64 * Shape<FMT, HD>::NW), (HD == 256 || (FMT 
         });
         split_weights(x, p);
         if (masked) {
-            // values of tokens that are not there count for nothing; what is not finite goes to the rows that see it alone
+            // values of tokens that are not there count for nothing, nor does here what is not finite
             bool odd = false;
 #pragma unroll
             for (int e = 0; e < 8; ++e)
@@ -960,33 +1014,7 @@ __global__ void __launch_bounds__((64 * Shape<FMT, HD>::NW), (HD == 256 || (FMT 
                     odd |= any_not_finite<FMT>(vr[e][w]);
                 }
             if (__ballot(odd)) {
-                const bool own = STEP && holder && ch == part.length / CHUNK;  // (the new token is in LDS)
-                for (int32_t tok = 0; tok < CHUNK; ++tok) {
-                    if (!(now.there[0] >> tok & 1)) continue;
-                    const int32_t from = tok >> 2 & 3, i = 4 * (tok >> 4) + (tok & 3);
-                    const uint8_t* row = c.values + (tok < 16 ? now.base[0] : now.base[1]) + (tok & 15) * HD * F::E;
-                    const bool fresh = STEP && own && tok == (part.length & (CHUNK - 1));
-                    auto element_of = [&](int32_t d) {
-                        if constexpr (STEP) {
-                            if (fresh) return load_element<FMT>(sh.value, d);
-                        }
-                        return load_element<FMT>(row, d);
-                    };
-                    float weight = 0.0f;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if (e == i) weight = x[e];
-                    weight = __shfl(weight, from * 16 + col);
-                    if (!(vis >> tok & 1)) continue;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-#pragma unroll
-                        for (int db = 0; db < X::DB; ++db) {
-                            const float v = element_of((4 * grp + e) * X::DB + db);
-                            if (!(fabsf(v) < INFINITY)) o[db][e] += weight * v;
-                            __builtin_amdgcn_sched_barrier(0);  // (rare: one load at a time, few registers)
-                        }
-                }
+                not_finite = true;
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
 #pragma unroll
@@ -1007,6 +1035,30 @@ __global__ void __launch_bounds__((64 * Shape<FMT, HD>::NW), (HD == 256 || (FMT 
     };
     for (; ch < c1; ch += NW) {
         attend_chunk(ch * CHUNK + CHUNK > n_all || here.there[0] != 0xFFFFFFFFu);
+    }
+    bool look = not_finite;
+#pragma unroll
+    for (int db = 0; db < X::DB; ++db)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) look |= !(fabsf(o[db][e]) < INFINITY);
+    if (__ballot(look)) {
+        Odd odd{0, 0};
+        for (ch = c0 + wave; ch < c1; ch += NW) {
+            here = reader.where_of(ch, reader.pages_of(ch));
+            uint32_t vis = seen_bits(b, part.first, token, new_first, ch * CHUNK, here.there[0]);
+            if constexpr (STEP) {
+                const uint32_t own = holder && ch == part.length / CHUNK ? 1u << (part.length & (CHUNK - 1)) : 0u;  // (the new token is in LDS)
+                if (vis & own) look_at<FMT, X::DB, 1>(odd, 1, [&](int) { return sh.value + 4 * grp * X::DB * F::E; }, 4);
+                vis &= ~own;
+            }
+            constexpr int N = together<FMT, X::DB>();
+            for (int32_t tok = 0; tok < CHUNK; tok += N) {
+                const uint8_t* rows = c.values + (tok < 16 ? here.base[0] : here.base[1]) + ((tok & 15) * HD + 4 * grp * X::DB) * F::E;
+                look_at<FMT, X::DB, N>(odd, vis >> tok, [&](int u) { return rows + u * HD * F::E; }, 4);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < HD / 4; ++i) o[i % X::DB][i / X::DB] = or_odd(odd, i, o[i % X::DB][i / X::DB]);
     }
 
     // each wave's averages, maxima and sums, then all waves' through LDS
@@ -1036,7 +1088,7 @@ __global__ void __launch_bounds__((64 * Shape<FMT, HD>::NW), (HD == 256 || (FMT 
         f4 y = {0.0f, 0.0f, 0.0f, 0.0f};
         for (int32_t w = 0; w < used; ++w) mx = fmaxf(mx, ms[w * R + r]);
         for (int32_t w = 0; w < used; ++w) {
-            const float by = share_of(ms[w * R + r], ls[w * R + r], mx);
+            const float by = weight_of_part(share_of(ms[w * R + r], ls[w * R + r], mx), ls[w * R + r]);
             const f4 v = *reinterpret_cast<const f4*>(avg + (w * R + r) * LR + d);
             sum += by;
 #pragma unroll
@@ -1090,7 +1142,7 @@ __global__ void __launch_bounds__((Tile<FMT, HD, WAVES>::THREADS), (Tile<FMT, HD
     constexpr int R = X::R, E = F::E, CH = X::CH;
     typedef typename std::conditional<FMT == KT_PAGED_F16, _Float16, __bf16>::type element;
     extern __shared__ __attribute__((aligned(16))) float lds[];
-    __shared__ int32_t odd_chunk[2];  // the chunk in a buffer if some of its values are not finite
+    __shared__ int32_t not_finite;  // some values were left out
     const PagedView& c = a.p.c;
     const BatchView& b = a.p.b;
     const int32_t tid = threadIdx.x, lane = tid & 63;
@@ -1109,7 +1161,7 @@ __global__ void __launch_bounds__((Tile<FMT, HD, WAVES>::THREADS), (Tile<FMT, HD
     if (part.split >= keys.splits) return;
     const int32_t c0 = keys.c0, c1 = keys.c1;
     const PageReader<CH, WHOLE> reader(c, b, part, keys.n_keys, E);
-    if (tid < 2) odd_chunk[tid] = -1;
+    if (tid == 0) not_finite = 0;
 
     // the chunk ahead: a thread's pieces of keys, and its four tokens of four dims
     u4 kr[X::KN];
@@ -1186,7 +1238,7 @@ __global__ void __launch_bounds__((Tile<FMT, HD, WAVES>::THREADS), (Tile<FMT, HD
         for (int i = 0; i < X::VN; ++i) {
             int32_t quad, dims;
             if (!value_item(i, quad, dims)) break;
-            if (!whole(ch, where)) {  // tokens that are not there count for nothing; what is not finite goes to the rows that see it alone
+            if (!whole(ch, where)) {  // values of tokens that are not there count for nothing, nor does here what is not finite
                 const uint32_t there = (quad < 8 ? where.there[0] : where.there[X::SETS - 1]) >> (4 * quad & 31);
                 bool odd = false;
 #pragma unroll
@@ -1197,7 +1249,7 @@ __global__ void __launch_bounds__((Tile<FMT, HD, WAVES>::THREADS), (Tile<FMT, HD
                         odd |= any_not_finite<FMT>(vr[i][j][w]);
                         vr[i][j][w] = finite_only<FMT>(vr[i][j][w]);
                     }
-                if (odd) odd_chunk[ch & 1] = ch;
+                if (odd) not_finite = 1;
             }
             const int32_t block = quad >> 3 << 2 | (quad & 3), at = block_of(block, dims) + (quad & 4);  // (tokens 16 t + 4 grp + i of a set: 8 grp + 4 t + i)
 #pragma unroll
@@ -1258,7 +1310,7 @@ __global__ void __launch_bounds__((Tile<FMT, HD, WAVES>::THREADS), (Tile<FMT, HD
 #pragma unroll
         for (int s = 0; s < X::QS; ++s) split_query(x[s], q[s]);
     }
-    __syncthreads();  // (odd_chunk)
+    __syncthreads();  // (not_finite)
     if (c0 < c1) store_chunk(c0, next);
 
     constexpr int VG = X::DB < X::VGROUP ? X::DB : X::VGROUP, GROUPS = X::DB / VG;  // dim blocks whose operands are loaded together
@@ -1328,33 +1380,6 @@ __global__ void __launch_bounds__((Tile<FMT, HD, WAVES>::THREADS), (Tile<FMT, HD
 #pragma unroll
             for (int db = 0; db < X::DB; ++db) o[db / VG][db % VG] *= alpha;
         });
-        if (masked || !whole(ch, where)) {
-            if (odd_chunk[ch & 1] == ch) {
-                for (int32_t tok = 0; tok < CH; ++tok) {
-                    const uint32_t there = tok < 32 ? where.there[0] : where.there[X::SETS - 1];
-                    if (!(there >> (tok & 31) & 1)) continue;
-                    const uint32_t mine = seen_bits(b, part.first, token, part.length, ch * CH + (tok & ~31), there);
-                    const int32_t from = tok >> 2 & 3, i = 8 * (tok >> 5) + 4 * (tok >> 4 & 1) + (tok & 3);
-                    const uint8_t* row = c.values + tok % (WHOLE ? CH : 16) * HD * E;
-                    if constexpr (WHOLE) row += where.base[0];
-                    else row += where.of_run(tok >> 4);
-                    float weight = 0.0f;
-#pragma unroll
-                    for (int e = 0; e < 8 * X::SETS; ++e)
-                        if (e == i) weight = x[e];
-                    weight = __shfl(weight, from * 16 + col);
-                    if (!(mine >> (tok & 31) & 1)) continue;
-#pragma unroll
-                    for (int db = 0; db < X::DB; ++db)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float v = load_element<FMT>(row, 16 * db + 4 * grp + e);
-                            if (!(fabsf(v) < INFINITY)) o[db / VG][db % VG][e] += weight * v;
-                            __builtin_amdgcn_sched_barrier(0);  // (rare: one load at a time, few registers)
-                        }
-                }
-            }
-        }
         op p[F::QP];
 #pragma unroll
         for (int i = 0; i < X::SETS * GROUPS; ++i) {
@@ -1384,6 +1409,31 @@ __global__ void __launch_bounds__((Tile<FMT, HD, WAVES>::THREADS), (Tile<FMT, HD
         }
         if constexpr (X::BUFFERS == 1) __syncthreads();  // (and read by all)
         if (ch + 1 < c1) store_chunk(ch + 1, next);
+    }
+
+    bool look = not_finite != 0;
+#pragma unroll
+    for (int db = 0; db < X::DB; ++db)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) look |= !(fabsf(o[db / VG][db % VG][e]) < INFINITY);
+    if (active && __ballot(look)) {
+        Odd odd{0, 0};
+        for (int32_t ch = c0; ch < min(c1, none_from); ++ch) {
+            next = reader.where_of(ch, reader.pages_of(ch));
+#pragma unroll
+            for (int h = 0; h < X::SETS; ++h) {
+                const uint32_t vis = seen_bits(b, part.first, token, part.length, ch * CH + 32 * h, next.there[h]);
+                constexpr int N = together<FMT, X::DB>();
+                for (int32_t tok = 0; tok < 32; tok += N) {
+                    const uint8_t* rows = c.values + 4 * grp * E;
+                    if constexpr (WHOLE) rows += next.base[0] + (32 * h + tok) * HD * E;
+                    else rows += next.of_run(2 * h + (tok >> 4)) + (tok & 15) * HD * E;
+                    look_at<FMT, X::DB, N>(odd, vis >> tok, [&](int u) { return rows + u * HD * E; }, 16);
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < HD / 4; ++i) o[i / 4 / VG][i / 4 % VG][i % 4] = or_odd(odd, i, o[i / 4 / VG][i / 4 % VG][i % 4]);
     }
 
     l = column_sum(l);
