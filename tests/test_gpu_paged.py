@@ -442,3 +442,54 @@ def test_rows_of_no_sequence_alone(kt, tree):
         b.check_pool()
     b.lib.call("kt_graph_destroy", graph)
     stream.destroy()
+
+
+@pytest.mark.parametrize("n", [4096, 4097])
+def test_masks_of_large_trees(kt, n):
+    """Trees whose parents fit LDS whole and one that does not: a chain, a star and a random one, beside a small tree."""
+    rng = np.random.default_rng(53)
+    chain = np.arange(-1, n - 1, dtype=np.int32)
+    star = np.where(np.arange(n) == 0, -1, 0).astype(np.int32)
+    for large in (chain, star, *random_parents(rng, [n])):
+        parents = [np.array([-1, 0, 0], np.int32), large]
+        b = Batch(kt, 53, [0, 0], [3, n], (2, 1, 32), "float16", 256, extra=1)
+        d = {"parents": kt.DeviceBuffer.from_numpy(np.concatenate(parents + [np.array([-1], np.int32)])), "depths": kt.DeviceBuffer.from_numpy(np.full(b.rows, 77, np.int32)),
+             "masks": kt.DeviceBuffer.from_numpy(np.full(b.rows * b.words, 0xABABABAB, np.uint32))}
+        b.batch.depths, b.batch.masks = d["depths"].ptr, d["masks"].ptr
+        b.lib.call("kt_tree_masks", d["parents"].ptr, ctypes.byref(b.batch), d["depths"].ptr, d["masks"].ptr, None)
+        depths, bits = d["depths"].download(np.int32), d["masks"].download(np.uint32).reshape(b.rows, b.words)
+        for s in range(2):  # each row's mask is its parent's and itself
+            r = b.sequence_rows(s)
+            want = np.zeros((len(parents[s]), b.words), np.uint32)
+            deep = np.zeros(len(parents[s]), np.int32)
+            for i, p in enumerate(parents[s]):
+                if p >= 0:
+                    want[i], deep[i] = want[p], deep[p] + 1
+                want[i, i // 32] |= np.uint32(1 << (i % 32))
+            assert np.array_equal(depths[r], deep) and np.array_equal(bits[r], want)
+        assert depths[-1] == 77 and (bits[-1] == 0xABABABAB).all()
+
+
+@pytest.mark.parametrize("n", [1024, 1025])
+def test_accept_of_large_trees(kt, n):
+    """Trees whose numbers fit LDS whole and one that does not: a chain that is kept whole, one that breaks at its last row, the last of many children, and a
+    random tree, beside a small one."""
+    rng = np.random.default_rng(54)
+    chain, counting = np.arange(-1, n - 1, dtype=np.int32), np.arange(n, dtype=np.int32)
+    star = np.where(np.arange(n) == 0, -1, 0).astype(np.int32)
+    any_tree, few = random_parents(rng, [n])[0], rng.integers(0, 2, (2, n)).astype(np.int32)
+    broken = counting.copy()
+    broken[-1] = -5
+    for large, tokens, chosen in ((chain, counting, counting + 1), (chain, broken, counting + 1), (star, counting, np.full(n, n - 1, np.int32)), (any_tree, few[0], few[1])):
+        parents = [np.array([-1, 0, 0], np.int32), large]
+        b = Batch(kt, 54, [0, 0], [3, n], (2, 1, 32), "float16", 256)
+        tokens, chosen = [np.array([4, 5, 6], np.int32), tokens], [np.array([6, 0, 9], np.int32), chosen]
+        up = lambda arrays: kt.DeviceBuffer.from_numpy(np.concatenate(arrays).astype(np.int32))
+        d = {"parents": up(parents), "tokens": up(tokens), "chosen": up(chosen), "kept": up([np.full(2 * (n + 3), 55)]), "counts": up([np.full(2, 55)]), "next": up([np.full(2, 55)])}
+        b.lib.call("kt_tree_accept", d["tokens"].ptr, d["chosen"].ptr, d["parents"].ptr, ctypes.byref(b.batch), d["kept"].ptr, n + 3, d["counts"].ptr, d["next"].ptr, None)
+        kept, counts, following = d["kept"].download(np.int32).reshape(2, n + 3), d["counts"].download(np.int32), d["next"].download(np.int32)
+        for s in range(2):
+            path = paged_ref.accept(parents[s], tokens[s], chosen[s])
+            assert counts[s] == len(path) and kept[s].tolist() == path + [-1] * (n + 3 - len(path)) and following[s] == chosen[s][path[-1]]
+        if large is chain:
+            assert counts[1] == (n if tokens[1][-1] != -5 else n - 1)
