@@ -141,20 +141,34 @@ class PagedKVCache:
 
 
 class PagedBatch:
-    """The rows of a call on a ``PagedKVCache``: ``counts[s]`` further tokens of sequence s, in the order of the
-    sequences, as texts, or as trees when ``buffers`` holds their parents."""
+    """The rows of a call on a ``PagedKVCache``: ``counts[s]`` further tokens of sequence s, which have pages (``reserve``), in the
+    order of the sequences, as texts, or as trees when ``buffers`` holds their parents. key_bound: what the sequences' tokens stay below,
+    where the call is recorded and they grow from replay to replay."""
 
     def __init__(self, cache: PagedKVCache, counts: list[int], starts: DeviceBuffer, key_bound: int | None = None,
                  buffers: "BatchBuffers | None" = None, stream: Stream | None = None):
+        counts = [int(n) for n in counts]
+        if len(counts) != cache.sequences:
+            raise _lib.IllegalArgumentException(f"{len(counts)} counts for {cache.sequences} sequences")
+        for sequence, n in enumerate(counts):
+            if n < 0:
+                raise _lib.IllegalArgumentException("counts must not be negative")
+            if n and cache.lengths[sequence] + n > len(cache._held[sequence]) * cache.page_tokens:
+                raise _lib.IllegalArgumentException(f"sequence {sequence} has no pages for {n} tokens after {cache.lengths[sequence]}: reserve them first")
+        tokens = max((length + n for length, n in zip(cache.lengths, counts) if n), default=0)
+        if key_bound is not None and key_bound < tokens:
+            raise _lib.IllegalArgumentException(f"key bound {key_bound} for sequences of up to {tokens} tokens")
+        if buffers is not None and sum(counts) > buffers.rows:
+            raise _lib.IllegalArgumentException(f"{sum(counts)} tokens exceed the buffers' {buffers.rows} rows")
         first = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
         starts.upload(first, stream)
         b = _lib.PagedBatch()
         b.tables, b.lengths, b.starts = cache.tables.ptr, cache.device_lengths.ptr, starts.ptr
         b.table_stride, b.sequences = cache.table_stride, cache.sequences
         b.rows, b.most_rows = int(first[-1]), max(counts)
-        b.key_bound = max(length + n for length, n in zip(cache.lengths, counts) if n) if key_bound is None else key_bound
+        b.key_bound = tokens if key_bound is None else key_bound
         if buffers is not None:
-            b.depths, b.masks, b.mask_words = buffers.depths.ptr, buffers.masks.ptr, -(-b.most_rows // 32)
+            b.depths, b.masks, b.mask_words = buffers.depths.ptr, buffers.masks.ptr, max(1, -(-b.most_rows // 32))
         self.cache, self.counts, self.starts = cache.cache, counts, first
         self.batch = b  # kt_paged_batch
 

@@ -138,3 +138,36 @@ def test_argmax_of_rows_refused():
                                   ({"capacity": -1}, _lib.KT_ERR_SHAPE, "negative capacity")):
         assert call(**change) == want and message in _lib.last_error(), (change, _lib.last_error())
     assert call(rows=0, logits=None) == _lib.KT_OK
+
+
+class Rows:
+    """Of BatchBuffers what a batch of trees takes."""
+
+    def __init__(self, rows):
+        self.rows, self.depths, self.masks = rows, HostBuffer(4 * rows), HostBuffer(4 * rows * -(-rows // 32))
+
+
+def test_batches_of_rows(cache):
+    grow(cache, {0: 20, 2: 5})
+    cache.reserve({0: 12, 1: 3, 2: 1})
+    starts = HostBuffer(4 * 5)
+    batch = kt.PagedBatch(cache, [12, 3, 0, 0], starts)
+    assert starts.bytes.view(np.int32).tolist() == [0, 12, 15, 15, 15]
+    assert (batch.batch.sequences, batch.batch.rows, batch.batch.most_rows, batch.batch.key_bound) == (4, 15, 12, 32)
+    nothing = kt.PagedBatch(cache, [0] * 4, starts).batch
+    assert (nothing.rows, nothing.most_rows, nothing.key_bound) == (0, 0, 0)
+    tree = kt.PagedBatch(cache, [8, 3, 0, 0], starts, buffers=Rows(11)).batch
+    assert tree.mask_words == 1 and tree.masks == tree.depths == 4096
+    assert kt.PagedBatch(cache, np.array([1, 1, 1, 0]), starts, key_bound=100).batch.key_bound == 100
+
+
+def test_batches_of_rows_refused(cache):
+    grow(cache, {0: 20, 2: 5})
+    cache.reserve({0: 12, 1: 3, 2: 1})
+    starts = HostBuffer(4 * 5)
+    for counts, change, message in (([1, 1, 1], {}, "3 counts for 4 sequences"), ([1] * 5, {}, "5 counts for 4 sequences"), ([], {}, "0 counts"),
+                                    ([4, -1, 0, 0], {}, "must not be negative"), ([13, 0, 0, 0], {}, "no pages"), ([0, 0, 0, 1], {}, "no pages"), ([0, 17, 0, 0], {}, "no pages"),
+                                    ([1, 1, 0, 0], {"key_bound": 20}, "key bound 20"), ([8, 3, 1, 0], {"buffers": Rows(11)}, "12 tokens exceed the buffers' 11 rows")):
+        with pytest.raises(kt.IllegalArgumentException, match=message):
+            kt.PagedBatch(cache, counts, starts, **change)
+    assert not starts.bytes.any()
