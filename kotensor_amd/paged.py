@@ -6,6 +6,7 @@ checks and messages are ``KVCache``'s.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 
 import numpy as np
@@ -124,6 +125,18 @@ class PagedKVCache:
         self.device_lengths.upload(np.array([shared], np.int32), stream, offset=4 * target)
         self.lengths[target] = shared
         return shared
+
+    @contextlib.contextmanager
+    def unchanged_on_error(self, stream: Stream | None = None):
+        """An error of what runs inside leaves the sequences as long as they were before, on the host and on the device (they keep
+        the pages that they took)."""
+        lengths = list(self.lengths)
+        try:
+            yield
+        except BaseException:
+            self.lengths = lengths
+            self.device_lengths.upload(np.array(lengths, np.int32), stream)  # (after what is enqueued)
+            raise
 
     @property
     def size_in_bytes(self) -> int:

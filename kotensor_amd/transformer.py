@@ -821,30 +821,31 @@ class Transformer:
         texts = {int(s): [int(t) for t in texts[s]] for s in sorted(texts)}
         self._check_batch(cache, buffers, texts)
         cache.reserve({s: len(t) for s, t in texts.items()}, stream)
-        st = _stream(stream)
-        done = dict.fromkeys(texts, 0)
-        order = {s: i for i, s in enumerate(texts)}
-        while any(done[s] < len(t) for s, t in texts.items()):
-            counts, tokens = [0] * cache.sequences, []
-            for s, t in texts.items():
-                counts[s] = min(len(t) - done[s], buffers.rows - len(tokens))
-                tokens += t[done[s]:done[s] + counts[s]]
-            batch = PagedBatch(cache, counts, buffers.starts, stream=stream)
-            buffers.tokens.upload(np.array(tokens, np.int32), stream)
-            self._embed(buffers, len(tokens), st)
-            self._layers(buffers, len(tokens), batch, 0, st)
-            _lib.call("kt_paged_advance", cache.device_lengths.ptr, ctypes.byref(batch.batch), st)
-            for s, t in texts.items():
-                done[s] += counts[s]
-                cache.lengths[s] += counts[s]
-                if counts[s] and done[s] == len(t):
-                    row = 4 * self.dimension
-                    _lib.call("kt_memcpy_d2d", ctypes.c_void_p(buffers.last.ptr + order[s] * row),
-                              ctypes.c_void_p(buffers.x.ptr + (int(batch.starts[s + 1]) - 1) * row), ctypes.c_size_t(row), st)
-        n = len(texts)
-        self._head(buffers.last.ptr, buffers, st, n)
-        _lib.call("kt_argmax_rows", buffers.logits.ptr, n, self.vocabulary_size, buffers.chosen.ptr, None, None, 0, st)
-        return dict(zip(texts, buffers.chosen.download(np.int32, count=n, stream=stream).tolist()))
+        with cache.unchanged_on_error(stream):
+            st = _stream(stream)
+            done = dict.fromkeys(texts, 0)
+            order = {s: i for i, s in enumerate(texts)}
+            while any(done[s] < len(t) for s, t in texts.items()):
+                counts, tokens = [0] * cache.sequences, []
+                for s, t in texts.items():
+                    counts[s] = min(len(t) - done[s], buffers.rows - len(tokens))
+                    tokens += t[done[s]:done[s] + counts[s]]
+                batch = PagedBatch(cache, counts, buffers.starts, stream=stream)
+                buffers.tokens.upload(np.array(tokens, np.int32), stream)
+                self._embed(buffers, len(tokens), st)
+                self._layers(buffers, len(tokens), batch, 0, st)
+                _lib.call("kt_paged_advance", cache.device_lengths.ptr, ctypes.byref(batch.batch), st)
+                for s, t in texts.items():
+                    done[s] += counts[s]
+                    cache.lengths[s] += counts[s]
+                    if counts[s] and done[s] == len(t):
+                        row = 4 * self.dimension
+                        _lib.call("kt_memcpy_d2d", ctypes.c_void_p(buffers.last.ptr + order[s] * row),
+                                  ctypes.c_void_p(buffers.x.ptr + (int(batch.starts[s + 1]) - 1) * row), ctypes.c_size_t(row), st)
+            n = len(texts)
+            self._head(buffers.last.ptr, buffers, st, n)
+            _lib.call("kt_argmax_rows", buffers.logits.ptr, n, self.vocabulary_size, buffers.chosen.ptr, None, None, 0, st)
+            return dict(zip(texts, buffers.chosen.download(np.int32, count=n, stream=stream).tolist()))
 
     def greedy_decode_batch(self, tokens: list[int], cache: PagedKVCache, buffers: BatchBuffers, steps: int, stream: Stream | None = None,
                             use_graph: bool = True) -> list[list[int]]:
@@ -862,35 +863,36 @@ class Transformer:
             return [[] for _ in tokens]
         n = cache.sequences
         cache.reserve(dict.fromkeys(range(n), steps), stream)
-        st = _stream(stream)
-        batch = PagedBatch(cache, [1] * n, buffers.starts, key_bound=cache.max_sequence_length, stream=stream)
-        buffers.tokens.upload(np.array(tokens, np.int32), stream)
+        with cache.unchanged_on_error(stream):
+            st = _stream(stream)
+            batch = PagedBatch(cache, [1] * n, buffers.starts, key_bound=cache.max_sequence_length, stream=stream)
+            buffers.tokens.upload(np.array(tokens, np.int32), stream)
 
-        def step():
-            self._embed(buffers, n, st)
-            self._layers(buffers, n, batch, 0, st)
-            # recorded by the position of the token that the step appended, ahead of the advance
-            self._head(buffers.x.ptr, buffers, st, n)
-            _lib.call("kt_argmax_rows", buffers.logits.ptr, n, self.vocabulary_size, buffers.tokens.ptr, cache.device_lengths.ptr,
-                      buffers.generated.ptr, buffers.max_sequence_length, st)
-            _lib.call("kt_paged_advance", cache.device_lengths.ptr, ctypes.byref(batch.batch), st)
+            def step():
+                self._embed(buffers, n, st)
+                self._layers(buffers, n, batch, 0, st)
+                # recorded by the position of the token that the step appended, ahead of the advance
+                self._head(buffers.x.ptr, buffers, st, n)
+                _lib.call("kt_argmax_rows", buffers.logits.ptr, n, self.vocabulary_size, buffers.tokens.ptr, cache.device_lengths.ptr,
+                          buffers.generated.ptr, buffers.max_sequence_length, st)
+                _lib.call("kt_paged_advance", cache.device_lengths.ptr, ctypes.byref(batch.batch), st)
 
-        step()  # (this one also sizes the workspaces)
-        if use_graph and steps > 2 and st:
-            graph = self._record(st, step)
-            try:
+            step()  # (this one also sizes the workspaces)
+            if use_graph and steps > 2 and st:
+                graph = self._record(st, step)
+                try:
+                    for _ in range(steps - 1):
+                        _lib.call("kt_graph_launch", graph, st)
+                finally:
+                    (stream or default_stream()).synchronize()
+                    _lib.call("kt_graph_destroy", graph)
+            else:
                 for _ in range(steps - 1):
-                    _lib.call("kt_graph_launch", graph, st)
-            finally:
-                (stream or default_stream()).synchronize()
-                _lib.call("kt_graph_destroy", graph)
-        else:
-            for _ in range(steps - 1):
-                step()
-        made = buffers.generated.download(np.int32, stream=stream).reshape(n, buffers.max_sequence_length)
-        out = [made[s, first:first + steps].tolist() for s, first in enumerate(cache.lengths)]
-        cache.lengths = [length + steps for length in cache.lengths]
-        return out
+                    step()
+            made = buffers.generated.download(np.int32, stream=stream).reshape(n, buffers.max_sequence_length)
+            out = [made[s, first:first + steps].tolist() for s, first in enumerate(cache.lengths)]
+            cache.lengths = [length + steps for length in cache.lengths]
+            return out
 
     def draft_step(self, drafts: dict[int, tuple[list[int], list[int]]], cache: PagedKVCache, buffers: BatchBuffers,
                    stream: Stream | None = None) -> dict[int, list[int]]:
@@ -913,28 +915,29 @@ class Transformer:
         if rows > buffers.rows:
             raise _lib.IllegalArgumentException(f"{rows} tokens exceed the buffers' {buffers.rows} rows")
         cache.reserve({s: len(t) for s, (t, _) in drafts.items()}, stream)
-        st = _stream(stream)
-        batch = PagedBatch(cache, counts, buffers.starts, buffers=buffers, stream=stream)
-        ref = ctypes.byref(batch.batch)
-        buffers.tokens.upload(np.array(tokens, np.int32), stream)
-        buffers.parents.upload(np.array(parents, np.int32), stream)
-        _lib.call("kt_tree_masks", buffers.parents.ptr, ref, buffers.depths.ptr, buffers.masks.ptr, st)
-        self._embed(buffers, rows, st)
-        self._layers(buffers, rows, batch, 0, st)
-        self._head(buffers.x.ptr, buffers, st, rows)
-        _lib.call("kt_argmax_rows", buffers.logits.ptr, rows, self.vocabulary_size, buffers.chosen.ptr, None, None, 0, st)
-        stride = batch.batch.most_rows
-        _lib.call("kt_tree_accept", buffers.tokens.ptr, buffers.chosen.ptr, buffers.parents.ptr, ref, buffers.kept.ptr, stride,
-                  buffers.counts.ptr, buffers.next.ptr, st)
-        _lib.call("kt_paged_keep", ctypes.byref(cache.cache), ref, buffers.kept.ptr, stride, buffers.counts.ptr, cache.device_lengths.ptr, st)
-        kept = buffers.kept.download(np.int32, count=cache.sequences * stride, stream=stream).reshape(cache.sequences, stride)
-        number = buffers.counts.download(np.int32, stream=stream).tolist()
-        following = buffers.next.download(np.int32, stream=stream).tolist()
-        out = {}
-        for s, (t, _) in drafts.items():
-            cache.lengths[s] += number[s]
-            out[s] = [t[i] for i in kept[s, 1:number[s]].tolist()] + [following[s]]
-        return out
+        with cache.unchanged_on_error(stream):
+            st = _stream(stream)
+            batch = PagedBatch(cache, counts, buffers.starts, buffers=buffers, stream=stream)
+            ref = ctypes.byref(batch.batch)
+            buffers.tokens.upload(np.array(tokens, np.int32), stream)
+            buffers.parents.upload(np.array(parents, np.int32), stream)
+            _lib.call("kt_tree_masks", buffers.parents.ptr, ref, buffers.depths.ptr, buffers.masks.ptr, st)
+            self._embed(buffers, rows, st)
+            self._layers(buffers, rows, batch, 0, st)
+            self._head(buffers.x.ptr, buffers, st, rows)
+            _lib.call("kt_argmax_rows", buffers.logits.ptr, rows, self.vocabulary_size, buffers.chosen.ptr, None, None, 0, st)
+            stride = batch.batch.most_rows
+            _lib.call("kt_tree_accept", buffers.tokens.ptr, buffers.chosen.ptr, buffers.parents.ptr, ref, buffers.kept.ptr, stride,
+                      buffers.counts.ptr, buffers.next.ptr, st)
+            _lib.call("kt_paged_keep", ctypes.byref(cache.cache), ref, buffers.kept.ptr, stride, buffers.counts.ptr, cache.device_lengths.ptr, st)
+            kept = buffers.kept.download(np.int32, count=cache.sequences * stride, stream=stream).reshape(cache.sequences, stride)
+            number = buffers.counts.download(np.int32, stream=stream).tolist()
+            following = buffers.next.download(np.int32, stream=stream).tolist()
+            out = {}
+            for s, (t, _) in drafts.items():
+                cache.lengths[s] += number[s]
+                out[s] = [t[i] for i in kept[s, 1:number[s]].tolist()] + [following[s]]
+            return out
 
     def generate_batch(self, prompts, max_tokens: int, stop_tokens=(), stream: Stream | None = None, use_graph: bool = True,
                        cache_format: str = "float32", page_tokens: int = 64, draft=None, rows: int = 512) -> list[list[int]]:

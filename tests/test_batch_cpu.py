@@ -171,3 +171,98 @@ def test_batches_of_rows_refused(cache):
         with pytest.raises(kt.IllegalArgumentException, match=message):
             kt.PagedBatch(cache, counts, starts, **change)
     assert not starts.bytes.any()
+
+
+class Memory(HostBuffer):
+    """Device memory by address, so that calls can find it."""
+    at: dict = {}
+
+    def __init__(self, nbytes):
+        super().__init__(nbytes)
+        self.ptr = 4096 * (len(Memory.at) + 1)
+        Memory.at[self.ptr] = self
+
+    def download(self, dtype, count=None, stream=None, offset=0):
+        return self.bytes.view(dtype)[:count].copy()
+
+
+@pytest.fixture
+def decoder(monkeypatch):
+    """(model, cache, buffers, calls): a decoder whose kernels do nothing but the lengths' advance; calls names what is to raise, and when."""
+    from kotensor_amd import _lib, transformer
+    for module in (paged, transformer):
+        monkeypatch.setattr(module, "DeviceBuffer", Memory)
+    monkeypatch.setattr(Memory, "at", {})
+    model = object.__new__(kt.Transformer)
+    model.num_layers, model.num_key_value_heads, model.head_dim, model.vocabulary_size = 2, 2, 32, 50
+    model.dimension, model.hidden_dimension, model.kv_dimension = 64, 96, 64
+    calls = {"made": [], "raise": None}
+    plain = _lib.call
+
+    def call(name, *args):
+        if name == "kt_paged_layout":
+            return plain(name, *args)
+        calls["made"].append(name)
+        if calls["raise"] and calls["raise"][0] == name and calls["made"].count(name) == calls["raise"][1]:
+            raise kt.IllegalStateException("planted")
+        if name == "kt_paged_advance":
+            lengths = Memory.at[args[0]].bytes.view(np.int32)
+            starts = Memory.at[args[1]._obj.starts].bytes.view(np.int32)
+            lengths += starts[1:] - starts[:-1]
+
+    monkeypatch.setattr(_lib, "call", call)
+    for name in ("_embed", "_layers", "_head"):
+        monkeypatch.setattr(kt.Transformer, name, lambda self, *args, name=name: call(name))
+    cache = model.new_paged_cache(3, 60, "float16", 16)
+    buffers = model.new_batch_buffers(cache, 8)
+    return model, cache, buffers, calls
+
+
+def test_a_call_that_fails_leaves_the_lengths_as_they_were(decoder):
+    """Device and host agree after an error, whichever step of the call it comes from, and the next call goes on from there."""
+    model, cache, buffers, calls = decoder
+
+    def fails(at, call):
+        before = list(cache.lengths)
+        calls["made"], calls["raise"] = [], at
+        with pytest.raises(kt.IllegalStateException, match="planted"):
+            call()
+        calls["raise"] = None
+        assert cache.lengths == before == lengths(cache)
+
+    assert set(model.extend({0: [1] * 5, 2: [2] * 9}, cache, buffers)) == {0, 2}
+    assert cache.lengths == lengths(cache) == [5, 0, 9]
+    texts = {0: [1] * 20, 1: [3] * 3}  # (three parts of eight rows)
+    for at in (("_layers", 1), ("_layers", 3), ("kt_paged_advance", 2), ("kt_memcpy_d2d", 1), ("_head", 1), ("kt_argmax_rows", 1)):
+        fails(at, lambda: model.extend(texts, cache, buffers))
+    for at in (("_layers", 1), ("_layers", 3), ("_head", 2), ("kt_argmax_rows", 4), ("kt_paged_advance", 3)):
+        fails(at, lambda: model.greedy_decode_batch([1, 2, 3], cache, buffers, 5, use_graph=False))
+    drafts = {0: ([4, 5, 6], [-1, 0, 0])}
+    for at in (("_layers", 1), ("kt_tree_accept", 1), ("kt_paged_keep", 1)):
+        fails(at, lambda: model.draft_step(drafts, cache, buffers))
+    model.extend(texts, cache, buffers)
+    assert cache.lengths == lengths(cache) == [25, 3, 9]
+    assert len(model.greedy_decode_batch([1, 2, 3], cache, buffers, 4, use_graph=False)) == 3
+    assert cache.lengths == lengths(cache) == [29, 7, 13]
+
+
+def test_a_recorded_replay_that_fails_leaves_the_lengths_as_they_were(decoder, monkeypatch):
+    model, cache, buffers, calls = decoder
+    from kotensor_amd import transformer
+
+    class Stream:
+        handle = 7
+
+        def synchronize(self):
+            calls["made"].append("synchronize")
+
+    def record(st, step):  # (nothing of a recording runs)
+        return "graph"
+
+    monkeypatch.setattr(kt.Transformer, "_record", staticmethod(record))
+    for at in (("kt_graph_launch", 1), ("kt_graph_launch", 3)):
+        calls["made"], calls["raise"] = [], at
+        with pytest.raises(kt.IllegalStateException, match="planted"):
+            model.greedy_decode_batch([1, 2, 3], cache, buffers, 6, Stream())
+        assert calls["made"].count("kt_graph_destroy") == 1 and "synchronize" in calls["made"]
+        assert cache.lengths == lengths(cache) == [0, 0, 0]
