@@ -566,9 +566,10 @@ int32_t kt_swiglu_qmatmul(float* gate, const float* up, int32_t m, const kt_qwei
 /* Transformer.argmaxOfLastToken (K/Transformer.kt:253-266) of logits[0..n) into the
  * device int32 *index: the first index of the largest logit above -1e9, else 0. */
 int32_t kt_argmax(const float* logits, int32_t n, int32_t* index, void* stream);
+#define KT_ARGMAX_MOST_ROWS 15872
 /* kt_argmax of each row of logits [rows x n] into tokens[row], in one launch: the next tokens of several sequences, or after
  * each row of their trees. generated (NULL: not recorded): generated[row * capacity + positions[row]] = tokens[row] when
- * 0 <= positions[row] < capacity. At most 15872 rows. */
+ * 0 <= positions[row] < capacity. At most KT_ARGMAX_MOST_ROWS rows. */
 int32_t kt_argmax_rows(const float* logits, int32_t rows, int32_t n, int32_t* tokens, const int32_t* positions, int32_t* generated,
                        int32_t capacity, void* stream);
 /* One greedy decode step's bookkeeping in one launch: kt_argmax(logits, n, token), then

@@ -111,6 +111,9 @@ KT_PAGED_F16 = 1
 KT_PAGED_BF16 = 2
 
 
+KT_ARGMAX_MOST_ROWS = 15872  # rows of a kt_argmax_rows call
+
+
 class PagedCache(ctypes.Structure):
     """kt_paged_cache: the memory and shape of a cache in pages."""
     _fields_ = [("keys", ctypes.c_void_p), ("values", ctypes.c_void_p), ("format", ctypes.c_int32), ("layers", ctypes.c_int32),

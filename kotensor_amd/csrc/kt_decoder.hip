@@ -1918,7 +1918,8 @@ int32_t kt_argmax_advance(const float* logits, int32_t n, int32_t* token, int32_
 
 int32_t kt_argmax_rows(const float* logits, int32_t rows, int32_t n, int32_t* tokens, const int32_t* positions, int32_t* generated,
                        int32_t capacity, void* stream) {
-    if (rows < 0 || rows > static_cast<int32_t>(MAX_COUNTERS)) return fail(KT_ERR_SHAPE, "argmax of %d rows: 0 to %d", rows, static_cast<int32_t>(MAX_COUNTERS));
+    static_assert(KT_ARGMAX_MOST_ROWS <= MAX_COUNTERS, "a counter a row");
+    if (rows < 0 || rows > KT_ARGMAX_MOST_ROWS) return fail(KT_ERR_SHAPE, "argmax of %d rows: 0 to %d", rows, KT_ARGMAX_MOST_ROWS);
     if (rows == 0) return KT_OK;
     if (!logits || !tokens) return fail(KT_ERR_ARGUMENT, "logits or tokens is NULL");
     if (n <= 0) return fail(KT_ERR_SHAPE, "argmax needs at least one logit");

@@ -236,6 +236,8 @@ class BatchBuffers(_Rows):
             raise _lib.IllegalArgumentException("BatchBuffers dimensions must be positive")
         if rows < sequences:
             raise _lib.IllegalArgumentException(f"BatchBuffers of {rows} rows for {sequences} sequences: at least one each")
+        if sequences > _lib.KT_ARGMAX_MOST_ROWS:
+            raise _lib.IllegalArgumentException(f"BatchBuffers for {sequences} sequences: at most {_lib.KT_ARGMAX_MOST_ROWS}")
         super().__init__(rows, dimension, hidden_dimension, kv_dimension)
         self.dimension, self.hidden_dimension, self.kv_dimension = dimension, hidden_dimension, kv_dimension
         self.vocabulary_size, self.sequences, self.max_sequence_length = vocabulary_size, sequences, max_sequence_length
@@ -914,6 +916,8 @@ class Transformer:
         rows = len(tokens)
         if rows > buffers.rows:
             raise _lib.IllegalArgumentException(f"{rows} tokens exceed the buffers' {buffers.rows} rows")
+        if rows > _lib.KT_ARGMAX_MOST_ROWS:  # (a token is chosen after each)
+            raise _lib.IllegalArgumentException(f"{rows} drafted tokens in one step: at most {_lib.KT_ARGMAX_MOST_ROWS}")
         cache.reserve({s: len(t) for s, (t, _) in drafts.items()}, stream)
         with cache.unchanged_on_error(stream):
             st = _stream(stream)

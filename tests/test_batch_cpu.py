@@ -266,3 +266,18 @@ def test_a_recorded_replay_that_fails_leaves_the_lengths_as_they_were(decoder, m
             model.greedy_decode_batch([1, 2, 3], cache, buffers, 6, Stream())
         assert calls["made"].count("kt_graph_destroy") == 1 and "synchronize" in calls["made"]
         assert cache.lengths == lengths(cache) == [0, 0, 0]
+
+
+def test_more_rows_than_an_argmax_takes(decoder, monkeypatch):
+    model, cache, buffers, calls = decoder
+    from kotensor_amd import _lib
+    E = kt.IllegalArgumentException
+    assert _lib.lib().kt_argmax_rows(16, _lib.KT_ARGMAX_MOST_ROWS + 1, 5, 16, None, None, 0, None) == _lib.KT_ERR_SHAPE
+    with pytest.raises(E, match="at most 15872"):
+        kt.BatchBuffers(8, 8, 8, 15873, 10, 15873, 8)
+    kt.BatchBuffers(1, 1, 1, 1, 40000, 20000, 1)  # (parts of prompts may be larger)
+    buffers.rows = 20000
+    calls["made"] = []
+    with pytest.raises(E, match="at most 15872"):
+        model.draft_step({0: ([1] * 15873, [-1] + [0] * 15872)}, cache, buffers)
+    assert not calls["made"] and not cache._held[0]
