@@ -414,7 +414,7 @@ int32_t kt_kv8_copy(const kt_kv8_cache* source, int32_t source_length, const kt_
                     void* stream);
 
 /* ---- the cache in pages that several sequences share, and trees of drafted tokens --------
- * (kt_paged.hip, kt_paged_attention.hip). No counterpart in the reference, whose cache holds one
+ * (kt_paged.hip, kt_paged_attention.h). No counterpart in the reference, whose cache holds one
  * sequence (K/KVCache.kt:3-59).
  * The pool: keys and values [layers][pages][kv_heads][page_tokens][head_dim] in fp32, fp16 or bf16
  * (rounded to the nearest, ties to even; fp16 takes magnitudes from 65520 on as infinities), 16-byte
@@ -468,11 +468,12 @@ int32_t kt_paged_layout(const kt_paged_cache* cache, int64_t* bytes);
 int32_t kt_rope_paged(const float* q, const float* k, const float* v, int32_t num_heads, const float* inv_freq,
                       const kt_paged_cache* cache, int32_t layer, const kt_paged_batch* batch, float* q_out, void* stream);
 /* kt_attention for a batch whose keys and values the pool holds already: softmax(q . k_j / sqrt(head_dim)) over the
- * tokens a row sees, times v, into context [rows x num_heads*head_dim]; products in fp32 precision, sums and softmax
- * in fp32. A row that sees no token gets zeros. Values that are not finite stay with the rows that see them: an infinity makes
- * the row's context of that dim infinite, whatever its weight and wherever it lies, infinities of both signs and NaNs make
- * it NaN. Finite values are taken to be below 2^88, and scores to lie in fp32's range. q and context are 16-byte aligned and apart. The stream's workspace is sized by one eager call of the
- * same bounds before a recording. */
+ * tokens a row sees, times v, into context [rows x num_heads*head_dim]; products in fp32 precision (on fp16 pages
+ * queries are taken to 2^-22 of the row's largest, weights to 2^-22 and to 2^-30 of the row's largest), sums and softmax
+ * in fp32. A row that sees no token gets zeros. Values that are not finite stay with the rows that see them: an infinity
+ * makes the row's context of that dim infinite, whatever its weight and wherever it lies, infinities of both signs and
+ * NaNs make it NaN. Finite values are taken to be below 2^88, and scores to lie in fp32's range. q and context are 16-byte
+ * aligned and apart. The stream's workspace is sized by one eager call of the same bounds before a recording. */
 int32_t kt_attention_paged(const float* q, int32_t num_heads, const kt_paged_cache* cache, int32_t layer,
                            const kt_paged_batch* batch, float* context, void* stream);
 /* kt_rope_paged, then kt_attention_paged on the rotated queries. q, k and v stay as they are. */
@@ -481,7 +482,8 @@ int32_t kt_rope_attention_paged(const float* q, const float* k, const float* v, 
                                 void* stream);
 /* The depths (of a root 0) and masks (a row and what is above it) of each sequence's rows as trees: parents[row] is the
  * index of its parent among its sequence's rows; a root's is -1 (as is any that is not below the row's own index).
- * Writes depths and masks, which may be the batch's own; of the batch reads starts, sequences, rows and mask_words. */
+ * Writes depths and masks, which may be the batch's own; of the batch reads starts and takes sequences, rows, most_rows and
+ * mask_words; its depths and masks are not NULL, as for any tree. */
 int32_t kt_tree_masks(const int32_t* parents, const kt_paged_batch* batch, int32_t* depths, uint32_t* masks, void* stream);
 /* The greedy check of each sequence's tree: tokens[row] is its token, chosen[row] the token the model chose after it
  * (kt_argmax of the row's logits). Row 0 is kept; then, as long as there is one, the first row whose parent is the

@@ -1511,10 +1511,7 @@ int32_t launch_tiles(Args a, hipStream_t st) {
     };
     // pages that hold whole chunks have a form of their own (a prompt of 2048, pages of 64 / 16: bf16 at 128 dims 104 us / 111, fp32 at 64 dims 105 / 117)
     if (const int32_t status = 1 << a.p.c.page_shift >= X::CH ? kernel(std::true_type{}) : kernel(std::false_type{})) return status;
-    if (a.slots == 0) return KT_OK;
-    merge_kernel<HD, X::R, X::LEAST, X::CH><<<dim3(static_cast<uint32_t>(a.slots), merge_shares(X::R)), 256, 0, st>>>(a);
-    KT_LAUNCHED("paged attention merge kernel");
-    return KT_OK;
+    return launch_merge<HD, X::R, X::LEAST, X::CH>(a, st);
 }
 
 // Which kernel (us here: head dims of 128 unless said, 32 heads on 8 kv heads, one sequence, pages of 32, of trees 64; the kernel taken first):
