@@ -81,14 +81,6 @@ __device__ __forceinline__ f4 products(const OP (&k)[KP], const OP (&q)[QP], f4 
     return c;
 }
 
-// Wait states behind products whose sums the code after a branch reads: the compiler was seen to leave them out where a
-// branch followed at once.
-__device__ __forceinline__ void settle() {
-    __builtin_amdgcn_sched_barrier(0);
-    asm volatile("s_nop 11");
-    __builtin_amdgcn_sched_barrier(0);
-}
-
 __device__ __forceinline__ void split_weights(const float (&v)[8], bf16x8 (&part)[3]) { split3_nearest(v, part); }
 __device__ __forceinline__ void split_weights(const float (&v)[8], half8 (&part)[2]) {
 #pragma unroll
@@ -989,7 +981,6 @@ __global__ void __launch_bounds__((64 * Shape<FMT, HD>::NW), (HD == 256 || (FMT 
         __builtin_amdgcn_sched_barrier(0);
         op p[F::QP];
         float x[8];
-        settle();
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = sc[i >> 2][i & 3];
         if (masked) {  // (a score of -infinity has no weight)
@@ -1027,7 +1018,7 @@ __global__ void __launch_bounds__((64 * Shape<FMT, HD>::NW), (HD == 256 || (FMT 
             value_operand(db, v);
             o[db] = products(v, p, o[db]);
         }
-        settle();
+        __builtin_amdgcn_sched_barrier(0);  // (loads ahead of their registers' last use would cost others)
         load_values(here);
         if constexpr (STEP) {
             if (holder && next == part.length / CHUNK) patch();
@@ -1363,7 +1354,7 @@ __global__ void __launch_bounds__((Tile<FMT, HD, WAVES>::THREADS), (Tile<FMT, HD
             }
         };
         load_values(0);
-        settle();
+        __builtin_amdgcn_sched_barrier(0);  // (the first values are on their way from LDS while the weights are made)
         float x[8 * X::SETS];
 #pragma unroll
         for (int i = 0; i < 8 * X::SETS; ++i) x[i] = sc[i >> 2][i & 3];
@@ -1394,7 +1385,6 @@ __global__ void __launch_bounds__((Tile<FMT, HD, WAVES>::THREADS), (Tile<FMT, HD
             products_of(v[i & 1], p, o[i % GROUPS]);
             __builtin_amdgcn_sched_barrier(0);
         }
-        settle();
     };
     for (int32_t ch = c0; ch < c1; ++ch) {
         const Where<CH, WHOLE> now = next;
