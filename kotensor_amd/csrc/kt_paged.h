@@ -58,6 +58,9 @@ __device__ __forceinline__ void store_element(uint8_t* p, int64_t at, float x) {
     else reinterpret_cast<__bf16*>(p)[at] = static_cast<__bf16>(x);
 }
 
+// Whether a launch of that many workgroups has 2^32 threads or more, which no launch has.
+constexpr bool too_many(int64_t workgroups, int32_t threads) { return workgroups > UINT32_MAX / threads; }
+
 // The checks of the entry points (kt_paged.hip).
 int32_t view_paged(const kt_paged_cache* cache, int32_t layer, PagedView* v);
 int32_t view_batch(const kt_paged_batch* batch, const kt_paged_cache* cache, BatchView* v);

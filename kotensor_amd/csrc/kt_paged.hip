@@ -132,7 +132,7 @@ int32_t launch_append(AppendArgs a, hipStream_t st) {
     a.q_groups = a.q ? ceil_div(a.num_heads, heads) : 0;
     a.groups = a.q_groups + ceil_div(a.c.kv_heads, heads);
     const int64_t grid = (static_cast<int64_t>(a.b.rows) * a.groups + THREADS / 64 - 1) / (THREADS / 64);
-    if (grid > INT32_MAX) return fail(KT_ERR_SHAPE, "too many rows and heads in one call");
+    if (too_many(grid, THREADS)) return fail(KT_ERR_SHAPE, "too many rows and heads in one call");
     const auto kernel = a.c.fmt == KT_PAGED_F32 ? append_kernel<KT_PAGED_F32> : a.c.fmt == KT_PAGED_F16 ? append_kernel<KT_PAGED_F16> : append_kernel<KT_PAGED_BF16>;
     kernel<<<static_cast<uint32_t>(grid), THREADS, 0, st>>>(a);
     KT_LAUNCHED("paged cache append kernel");
@@ -516,7 +516,7 @@ int32_t kt_paged_read(const kt_paged_cache* cache, int32_t layer, const int32_t*
         return fail(KT_ERR_RANGE, "tokens %d + %d out of bounds %lld", first, count, static_cast<long long>(entries > 0 ? room : 0));
     if (count == 0 || (!keys && !values)) return KT_OK;
     const int64_t grid = (static_cast<int64_t>(count) * c.kv_heads * c.head_dim + THREADS - 1) / THREADS;
-    if (grid > INT32_MAX) return fail(KT_ERR_SHAPE, "too many tokens and heads in one call");
+    if (too_many(grid, THREADS)) return fail(KT_ERR_SHAPE, "too many tokens and heads in one call");
     BatchView b{};
     b.tables = table;
     b.table_stride = entries;

@@ -1438,9 +1438,9 @@ __global__ void __launch_bounds__((Tile<FMT, HD, WAVES>::THREADS), (Tile<FMT, HD
 }
 
 // ---- launches ---------------------------------------------------------------------------------------
-// The grid and the workspace of a launch of tiles of R rows whose parts have at least LEAST chunks of CHUNK keys.
+// The grid (of workgroups of `threads`) and the workspace of a launch of tiles of R rows whose parts have at least LEAST chunks of CHUNK keys.
 template <int HD, int R, int LEAST, int CHUNK>
-int32_t prepare(Args& a, int32_t target, int64_t* grid, hipStream_t st) {
+int32_t prepare(Args& a, int32_t target, int32_t threads, int64_t* grid, hipStream_t st) {
     const BatchView& b = a.p.b;
     const int64_t G = a.p.num_heads / a.p.c.kv_heads;
     const int64_t tiles = std::min(b.sequences * ((b.most_rows * G + R - 1) / R), b.rows * G / R + b.sequences) * a.p.c.kv_heads;  // at most
@@ -1448,7 +1448,7 @@ int32_t prepare(Args& a, int32_t target, int64_t* grid, hipStream_t st) {
     a.target = target;
     const int64_t most = fine(R) ? 2 * target : target;  // (find_part)
     *grid = std::min(tiles + most, tiles * most_splits);
-    if (*grid > INT32_MAX / 64) return fail(KT_ERR_SHAPE, "too many rows and heads in one call");
+    if (too_many(*grid, threads)) return fail(KT_ERR_SHAPE, "too many rows and heads in one call");
     // One sequence whose tiles are target and more by themselves is not cut (find_part would not, were its rows fewer than the call says it
     // could): no merge to launch. A prompt of 1024 (fp16, 64 dims): 33 us, with one 36; of 2048 63 and 67.
     const bool finer = fine(R) && tiles * chunks > int64_t{target} * (LONG / CHUNK) && tiles < 2 * int64_t{target};
@@ -1479,7 +1479,7 @@ int32_t launch_rows(Args a, hipStream_t st) {
     int64_t grid = 0;
     // four parts a CU (64 steps over 2048 tokens on average / one of 131000 beside seven: 2 parts 117 / 97 us, 3 112 / 92, 4 113 / 87,
     // 6 115 / 88, 8 115 / 90)
-    if (const int32_t status = prepare<HD, X::R, X::LEAST, CHUNK>(a, 4 * cu_count(), &grid, st)) return status;
+    if (const int32_t status = prepare<HD, X::R, X::LEAST, CHUNK>(a, 4 * cu_count(), 64 * X::NW, &grid, st)) return status;
     constexpr size_t lds = std::max(std::max(sizeof(float) * X::NW * X::R * (HD + 6), size_t{2} * Format<FMT>::QP * X::R * (HD + 8)), merge_lds(X::R, X::NW));
     if (const int32_t ls = allow_lds<&attention_kernel<FMT, HD, STEP>, lds>(lds)) return ls;
     attention_kernel<FMT, HD, STEP><<<static_cast<uint32_t>(grid), 64 * X::NW, lds, st>>>(a);
@@ -1491,7 +1491,7 @@ template <int FMT, int HD, int WAVES>
 int32_t launch_tiles(Args a, hipStream_t st) {
     using X = Tile<FMT, HD, WAVES>;
     int64_t grid = 0;
-    if (const int32_t status = prepare<HD, X::R, X::LEAST, X::CH>(a, X::TARGET * cu_count(), &grid, st)) return status;
+    if (const int32_t status = prepare<HD, X::R, X::LEAST, X::CH>(a, X::TARGET * cu_count(), X::THREADS, &grid, st)) return status;
     const auto kernel = [&](auto whole) -> int32_t {
         constexpr bool WHOLE = decltype(whole)::value;
         if (const int32_t ls = allow_lds<&tile_kernel<FMT, HD, WAVES, WHOLE>, X::LDS>(X::LDS)) return ls;

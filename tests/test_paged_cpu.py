@@ -197,3 +197,20 @@ def test_calls_without_a_row_of_a_sequence(tree):
         assert lib.kt_rope_paged(16, 16, 16, 4, 16, _cache(), 0, padding, 16, None) == _lib.KT_OK, _lib.last_error()
         assert lib.kt_attention_paged(16, 4, _cache(), 0, padding, 16, None) == _lib.KT_OK, _lib.last_error()
         assert lib.kt_rope_attention_paged(16, 16, 16, 16, 4, _cache(), 0, padding, 16, None) == _lib.KT_OK, _lib.last_error()
+
+
+def test_launches_past_32_bits_of_threads_refused():
+    """A launch has fewer than 2^32 threads: more rows and heads, or tokens to read, are refused as such, not by the device."""
+    from kotensor_amd import _lib
+    lib = _lib.lib()
+    rows = (1 << 24) - 1
+    many = dict(rows=rows, most_rows=rows, sequences=1, table_stride=1 << 20, key_bound=1 << 24)
+    few_keys = dict(rows=1 << 20, most_rows=16, sequences=65535, table_stride=4, key_bound=128)
+    for batch, kv, heads, dim in ((many, 1, 128, 32), (many, 2, 130, 64), (many, 8, 128, 128), (many, 4, 256, 256), (few_keys, 512, 512, 32)):
+        for fmt in range(3):
+            cache = _cache(kv_heads=kv, head_dim=dim, format=fmt)
+            assert lib.kt_attention_paged(16, heads, cache, 0, _batch(**batch), 16, None) == _lib.KT_ERR_SHAPE, (kv, heads, dim, fmt, _lib.last_error())
+            assert "too many rows and heads" in _lib.last_error()
+    wide = _cache(kv_heads=64, head_dim=256)
+    assert lib.kt_rope_paged(16, 16, 16, 256, 16, wide, 0, _batch(**many), 16, None) == _lib.KT_ERR_SHAPE and "too many rows and heads" in _lib.last_error()
+    assert lib.kt_paged_read(wide, 0, 16, 1 << 20, 0, 1 << 18, 16, 16, None) == _lib.KT_ERR_SHAPE and "too many tokens and heads" in _lib.last_error()
