@@ -17,10 +17,10 @@
 // seldom rescaled. Parts meet through memory: of tiles of 16 rows the last workgroup of a tile to arrive (a counter, which it
 // returns to zero) merges all in their order, so that no workgroup waits for another and the bits do not depend on who
 // is last; of larger tiles a launch of its own does.
-// Two kernels: attention_kernel for few rows, bound by the cache's bytes (64 steps over 2048 tokens on average, 128 dims, bf16: 112 us,
-// 4.8 TB/s; one of 131000 beside seven shorter, fp16: 86 us, 5.1 TB/s; a large copy runs at 4.8), with short texts by the chain of loads from
-// the lengths to the merge (12 us); tile_kernel for many, bound by the vector and matrix instructions of two waves a SIMD that wait for
-// each other's chunks (a prompt of 2048, 128 dims, bf16: 97 us, 354 TFLOP/s of attention, 1060 of matrix products, of which a
+// Two kernels: attention_kernel for few rows, bound by the cache's bytes (64 steps over 2048 tokens on average, 128 dims, bf16: 111 us,
+// 4.9 TB/s; one of 131000 beside seven shorter, fp16: 84 us, 5.2 TB/s; a large copy runs at 4.8), with short texts by the chain of loads from
+// the lengths to the merge (11.5 us); tile_kernel for many, bound by the vector and matrix instructions of two waves a SIMD that wait for
+// each other's chunks (a prompt of 2048, 128 dims, bf16, pages of 64: 94 us, 365 TFLOP/s of attention, 1095 of matrix products, of which a
 // large library product reaches 1112), with few chunks by a part's beginning, 7 to 10 us.
 #pragma once
 
@@ -266,8 +266,8 @@ struct Part {
 // the chunks over target, so a launch has at most target + (its tiles of all kv heads) parts, and at most 2 target that share a
 // tile. Tiles of many rows (FINE): where that size is above LONG tokens and tiles are fewer than 2 target, whose rounds would leave
 // workgroups idle, but not a round of whole tiles, the chunks over 2 target: at most 4 target parts that share a tile. (us at target, at 2 target,
-// 128 dims, bf16: 300 rows after 8000 tokens 188, 130; 1300 after 8000 618, 508; 16 sequences with trees of 64 after 3000 123, 118; with 64 rows
-// after 1000 each 60, 75: a round of whole tiles. Everywhere: a tree of 60 after 4000 42, 49.)
+// 128 dims, bf16: 300 rows after 8000 tokens 185, 122; 1300 after 8000 597, 495; 16 sequences with trees of 64 after 3000 120, 117; with 64 rows
+// after 1000 each 58, 75: a round of whole tiles. Everywhere: a tree of 60 after 4000 38, 46.)
 constexpr int LONG = 1024;
 constexpr bool fine(int R) { return R > 16; }
 template <int R, int LEAST, int CHUNK, bool BY_SLOT = false>
@@ -633,6 +633,8 @@ __global__ void __launch_bounds__(256) merge_kernel(Args a) {
 // R = 16 rows a workgroup on 16x16x32. Its four waves take the part's chunks of 32 keys in turn, straight from memory into registers,
 // no LDS and no barrier in the loop: a lane loads its dims of the tokens whose weights it will hold, and turns them there. The
 // next chunk's keys are on their way while a chunk's weights and output are formed, its values while the next scores are.
+// Registers: 106 scalars are too few for what the loop and its surroundings need; 6 to 132 of them (of 256 dims up to 264) wait in vector registers, and
+// a chunk reads up to four back. From 256 dims on (fp32: 128) sums lie in accumulators and move 88 to 263 times a chunk.
 // STEP: the tokens are rotated, appended and attended to in this launch: every workgroup makes its own rotated query, key and
 // value, the last part's also writes them to the cache, and its wave with the token's chunk takes them from LDS.
 template <int FMT, int HD>
@@ -1107,8 +1109,8 @@ struct Tile {
     // waves a SIMD that leave a wave the registers it needs (of 256 dims with two: 352 bytes and more in scratch memory)
     static constexpr int MW = NW == 8 ? 2 : HD == 256 ? 1 : HD <= 64 && FMT != KT_PAGED_F32 ? 3 : 2;
     static constexpr int KP = Format<FMT>::KP, QP = Format<FMT>::QP, E = Format<FMT>::E;
-    // keys of a chunk: half the barriers with 64 (against 32 at 64 dims: a prompt of 1024 in fp16 36 us for 39, of 2048 in fp32 124 for 134, in
-    // bf16 76 for 75), where the registers and LDS allow it
+    // keys of a chunk: half the barriers with 64 (against 32, pages of 64: at 64 dims a prompt of 1024 in fp16 23 us for 28, of 2048 in fp32 98 for
+    // 110, in bf16 58 for 63; at 128 dims in fp16 79 for 86), where the registers and LDS allow it
     static constexpr int CH = HD == 256 || (FMT == KT_PAGED_F32 && HD == 128) ? 32 : 64, SETS = CH / 32;
     static constexpr int QS = HD / 32, DB = HD / 16;
     static constexpr int KR = HD + 8, VR = CH + 8;  // padded rows: of a key, of a dim (2-byte elements)
@@ -1120,7 +1122,7 @@ struct Tile {
     static constexpr size_t LDS = size_t{2} * SIZE * BUFFERS;
     static constexpr int LEAST = 128 / CH;
     static constexpr int TARGET = NW == 4 && HD < 256 ? 2 : 1;  // workgroups a CU among which the launch's chunks are shared out
-    static constexpr int VGROUP = FMT != KT_PAGED_F32 ? 4 : HD == 128 ? 1 : 2;  // (fp32 at 128 dims, which spills least with one: a prompt of 2048 211 us for 220)
+    static constexpr int VGROUP = FMT != KT_PAGED_F32 ? 4 : HD == 128 ? 1 : 2;  // (fp32 at 128 dims: a prompt of 2048 171 us with one, 176 with two)
 };
 
 template <int FMT, int HD, int WAVES, bool WHOLE>
@@ -1473,8 +1475,10 @@ template <int FMT, int HD, bool STEP>
 int32_t launch_rows(Args a, hipStream_t st) {
     using X = Shape<FMT, HD>;
     int64_t grid = 0;
-    // four parts a CU (64 steps over 2048 tokens on average / one of 131000 beside seven: 2 parts 117 / 97 us, 3 112 / 92, 4 113 / 87,
-    // 6 115 / 88, 8 115 / 90)
+    // four parts a CU (64 steps over 2048 tokens on average, 128 dims, bf16 / one of 131000 beside seven, 64 dims, fp16: 2 parts 115 / 95 us,
+    // 3 110 / 91, 4 111 / 84, 6 112 / 86, 8 112 / 87). One to four rounds of them, as registers leave a CU five to one of these workgroups:
+    // of texts of 1000 tokens two or three parts take 5 to 13% less (64 of them, from the last cache, at 2, 3, 4, 6: 64 dims in fp16 30, 30, 34,
+    // 33; 128 54, 52, 59, 59; 256 126, 129, 139, 145; fp32 128 126, 129, 141, 150).
     if (const int32_t status = prepare<HD, X::R, X::LEAST, CHUNK>(a, 4 * cu_count(), 64 * X::NW, &grid, st)) return status;
     constexpr size_t lds = std::max(std::max(sizeof(float) * X::NW * X::R * (HD + 6), size_t{2} * Format<FMT>::QP * X::R * (HD + 8)), merge_lds(X::R, X::NW));
     if (const int32_t ls = allow_lds<&attention_kernel<FMT, HD, STEP>, lds>(lds)) return ls;
@@ -1495,7 +1499,7 @@ int32_t launch_tiles(Args a, hipStream_t st) {
         KT_LAUNCHED("paged attention kernel");
         return KT_OK;
     };
-    // pages that hold whole chunks have a form of their own (a prompt of 2048, pages of 64 / 16: bf16 at 128 dims 104 us / 111, fp32 at 64 dims 105 / 117)
+    // pages that hold whole chunks have a form of their own (a prompt of 2048, pages of 64, with and without it: bf16 at 128 dims 94 and 100 us, fp32 at 64 dims 98 and 108)
     if (const int32_t status = 1 << a.p.c.page_shift >= X::CH ? kernel(std::true_type{}) : kernel(std::false_type{})) return status;
     return launch_merge<HD, X::R, X::LEAST, X::CH>(a, st);
 }
@@ -1503,16 +1507,16 @@ int32_t launch_tiles(Args a, hipStream_t st) {
 // Which kernel (us here: head dims of 128 unless said, 32 heads on 8 kv heads, one sequence, pages of 32, of trees 64; the kernel taken first):
 //   up to 16 rows of a kv head: tiles of 16. (A tree of 4 tokens has no use for more.)
 //   up to 128 keys: the same for any number of rows, as its waves have a chunk each: no parts to merge, and four
-//     times the workgroups. A prompt of 128: fp16 8.9 against 12.4, fp32 12.3 against 16.6, fp16 at 64 dims 7.0 against 8.0, fp32
-//     at 256 dims 22 against 42.
-//   up to 64 rows: tiles of 64, so that no wave is idle, two workgroups a CU: 16 sequences with trees of 15 after 2000 tokens 37
-//     against 47 with tiles of 128 (fp32 55 against 80); one tree of 15 after 4000 26 and 26.
-//   up to 64 dims in 16 bits: tiles of 64 for any number of rows, of which three workgroups share a CU: a prompt of 1024 28
-//     against 33, of 2048 61 against 69 (fp16).
-//   else: tiles of 128, as the chunk that eight waves share is half the loads and LDS writes a row: a prompt of 2048 99 against 108 (fp16), 107
-//     against 114 (bf16), 182 against 222 (fp32); a tree of 60 in fp32 43 against 46.
+//     times the workgroups. A prompt of 128: fp16 9.2 against 12.7, fp32 12.6 against 16.8, fp16 at 64 dims 6.9 against 7.9, fp32
+//     at 256 dims 24 against 26.
+//   up to 64 rows: tiles of 64, so that no wave is idle, two workgroups a CU: 16 sequences with trees of 15 after 2000 tokens 36
+//     against 46 with tiles of 128 (fp32 54 against 79); one tree of 15 after 4000 in fp32 30 and 29.
+//   up to 64 dims in 16 bits: tiles of 64 for any number of rows, of which three workgroups share a CU: a prompt of 1024 26
+//     against 31, of 2048 54 against 64 (fp16).
+//   else: tiles of 128, as the chunk that eight waves share is half the loads and LDS writes a row: a prompt of 2048 86 against 96 (fp16), 100
+//     against 110 (bf16), 171 against 211 (fp32); a tree of 60 in fp32 43 against 46.
 //   256 dims: tiles of 64 whose waves have a SIMD's registers each: a prompt of 512 36 against 38 with tiles of
-//     128 (bf16 39 against 42, fp32 72 against 101; 16 trees of 15 79 against 68).
+//     128 (bf16 40 against 42, fp32 72 against 97; 16 trees of 15 78 against 67).
 template <int FMT, int HD>
 int32_t launch_dims(const Args& a, hipStream_t st) {
     const int64_t rows = static_cast<int64_t>(a.p.b.most_rows) * (a.p.num_heads / a.p.c.kv_heads);
